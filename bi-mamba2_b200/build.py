@@ -18,8 +18,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "ssd", "_lib")
 OUT = os.path.join(OUT_DIR, "libbissd.so")
-SOURCES = ["bissd_api.cu", "bissd_layer.cu", "bissd_simt.cu"]
-TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+SOURCES = ["bissd_api.cu", "bissd_layer.cu", "bissd_simt.cu", "bissd_uni.cu"]
+TORCH_SOURCES = ["torch_ops.cpp", "torch_uni.cpp"]
 TORCH_OUT = os.path.join(OUT_DIR, "_bissd_torch.so")
 
 
@@ -44,23 +44,31 @@ def _run(cmd, verbose, what):
         raise RuntimeError(f"{cmd[0]} failed building {what}")
 
 
+def _compile(sources, cmd, force, verbose):
+    """Objects of the sources, what is out of date compiled anew, side by side."""
+    objs = [os.path.join(OUT_DIR, os.path.splitext(s)[0] + ".o") for s in sources]
+    stale = [(s, o) for s, o in zip(sources, objs) if force or not os.path.exists(o) or os.path.getmtime(o) < _newest_source_mtime(s)]
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        list(pool.map(lambda so: _run([*cmd, "-c", "-o", so[1], os.path.join(CSRC, so[0])], verbose, so[0]), stale))
+    return objs
+
+
 def build_torch(force=False, verbose=False):
-    """The extension depends on its own source and the C header only: libbissd.so may be rebuilt beneath it."""
-    header = os.path.join(os.path.dirname(HERE), "include", "bissd.h")
-    newest = max(os.path.getmtime(TORCH_SRC), os.path.getmtime(header))
-    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= newest:
+    """The extension depends on its own sources and the C header only: libbissd.so may be rebuilt beneath it."""
+    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= max(map(_newest_source_mtime, TORCH_SOURCES)):
         return TORCH_OUT
     import torch
     from torch.utils import cpp_extension
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_bissd_torch"]
+    cxx = os.environ.get("CXX", "g++")
+    flags = ["-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_bissd_torch"]
     for path in cpp_extension.include_paths() + [os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]:
-        cmd += ["-isystem", path]
-    cmd += [TORCH_SRC, "-o", TORCH_OUT, "-L" + OUT_DIR, "-l:libbissd.so", "-Wl,-rpath,$ORIGIN"]
-    cmd += ["-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
-            "-ltorch_python"]
-    _run(cmd, verbose, os.path.basename(TORCH_OUT))
+        flags += ["-isystem", path]
+    objs = _compile(TORCH_SOURCES, [cxx, *flags], force, verbose)
+    _run([cxx, "-shared", "-o", TORCH_OUT, *objs, "-L" + OUT_DIR, "-l:libbissd.so", "-Wl,-rpath,$ORIGIN",
+          "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"],
+         verbose, os.path.basename(TORCH_OUT))
     return TORCH_OUT
 
 
@@ -77,10 +85,7 @@ def build_library(force=False, verbose=False):
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     flags = ["-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a", "--expt-relaxed-constexpr",
              "--extended-lambda", "-Xcompiler", "-fPIC"] + (["-Xptxas", "-v"] if verbose else [])
-    objs = [os.path.join(OUT_DIR, s.replace(".cu", ".o")) for s in SOURCES]
-    stale = [(s, o) for s, o in zip(SOURCES, objs) if force or not os.path.exists(o) or os.path.getmtime(o) < _newest_source_mtime(s)]
-    with concurrent.futures.ThreadPoolExecutor() as pool:                # one nvcc per translation unit, side by side
-        list(pool.map(lambda so: _run([nvcc, *flags, "-c", "-o", so[1], os.path.join(CSRC, so[0])], verbose, so[0]), stale))
+    objs = _compile(SOURCES, [nvcc, *flags], force, verbose)
     _run([nvcc, "-shared", "-o", OUT, *objs], verbose, os.path.basename(OUT))
     return OUT
 

@@ -21,6 +21,9 @@
 #include <string>
 
 #include "../../include/bissd.h"
+#include "torch_errors.h"
+
+void bind_uni(py::module_ &m);                                   // torch_uni.cpp
 
 namespace {
 
@@ -29,26 +32,8 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
-struct BissdError : std::runtime_error {                         // ssd._cabi.BissdError in Python
-    using std::runtime_error::runtime_error;
-};
-
-void check(int rc) {
-    if (rc == BISSD_OK) return;
-    const char *cuda = bissd_last_cuda_error();
-    std::string msg = "libbissd error " + std::to_string(rc) + ": " + bissd_strerror(rc);
-    if (cuda && cuda[0]) msg += std::string(" [") + cuda + "]";
-    throw BissdError(msg);
-}
-
-// Tests and debugging: a synchronising read of the device status word after every pass.
-void check_device_status(bool on, const void *ws, void *stream) {
-    if (!on) return;
-    int st = 0;
-    check(bissd_read_status(ws, stream, &st));
-    if (st != 0)
-        throw BissdError("libbissd device status " + std::to_string(st) + ": a device-side wait ran out; results are invalid");
-}
+constexpr auto &check = bissd_check;
+constexpr auto &check_device_status = bissd_check_device_status;
 
 int dtype_code(at::ScalarType t) {
     switch (t) {
@@ -596,4 +581,5 @@ PYBIND11_MODULE(_bissd_torch, m) {
     });
     m.def("chunk_scan", &chunk_scan);
     m.def("layer", &layer);
+    bind_uni(m);
 }

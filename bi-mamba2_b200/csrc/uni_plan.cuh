@@ -1,0 +1,120 @@
+// Where the sequences of a decay attention call lie, and the segments that their tokens are dealt out in.  A batch's rows are
+// sequences of one length, and a segment's place is arithmetic; packed sequences have theirs on the device, so a small
+// kernel writes a table of their segments, and a launch has as many blocks as there can be at most.
+#pragma once
+#include "common.cuh"
+
+namespace bissd {
+namespace uni {
+
+struct Plan {
+    int packed, L, seg, per_seq, most;                           // most: segments there can be (all of them where not packed)
+    const int4 *table;                                           // packed: first token, tokens, sequence, 2 * index + last
+    const int *first;                                            // packed: (nseq + 1) first segment of each sequence
+};
+struct Segment {
+    int batch, t0, len, seq, idx;                                // len 0: there is no such segment
+    bool last;
+};
+
+__device__ __forceinline__ Segment segment(const Plan &p, int i) {
+    Segment s;
+    if (p.packed) {
+        const int4 e = __ldg(p.table + i);
+        s.batch = 0; s.t0 = e.x; s.len = e.y; s.seq = e.z; s.idx = e.w >> 1; s.last = e.w & 1;
+    } else {
+        s.batch = s.seq = i / p.per_seq;
+        s.idx = i % p.per_seq;
+        s.t0 = s.idx * p.seg;
+        s.len = min(p.seg, p.L - s.t0);
+        s.last = s.idx == p.per_seq - 1;
+    }
+    return s;
+}
+// The segments of a sequence: first and how many.
+__device__ __forceinline__ int2 segments(const Plan &p, int seq) {
+    if (!p.packed) return make_int2(seq * p.per_seq, p.per_seq);
+    return make_int2(p.first[seq], p.first[seq + 1] - p.first[seq]);
+}
+
+struct PlanOut {                                                 // one table for each segment length
+    int seg, most;
+    int4 *table;
+    int *first, *bounds;                                         // bounds (nseq + 1): the boundaries as taken
+};
+
+// Inclusive scan over a block of 1024 threads; `op` max or sum.
+template <class F> __device__ __forceinline__ int block_scan(int v, int *warps, F op, int none) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = op(v, u);
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = v;
+    __syncthreads();
+    int before = none;
+    for (int w = 0; w < warp; ++w) before = op(before, warps[w]);
+    return op(before, v);
+}
+
+// A block for each table.  Boundaries are taken to 0 ... L and never back, so every segment lies inside the tensors whatever the
+// caller's array holds.
+__global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int L, PlanOut a, PlanOut b) {
+    pdl_begin();
+    __shared__ int warps[32], carry[2];
+    const PlanOut o = blockIdx.x ? b : a;
+    const int tid = threadIdx.x;
+    auto most = [](int x, int y) { return max(x, y); };
+    auto sum = [](int x, int y) { return x + y; };
+    auto inside = [&](int i) { return max(0, min(cu[i], L)); };
+    if (tid == 0) {
+        o.first[0] = carry[1] = 0;
+        o.bounds[0] = carry[0] = inside(0);
+    }
+    __syncthreads();
+    for (int s0 = 0; s0 < nseq; s0 += 1024) {
+        const int s = s0 + tid;
+        const int end = max(carry[0], block_scan(s < nseq ? inside(s + 1) : 0, warps, most, 0));
+        const int start = max(carry[0], block_scan(s < nseq ? inside(s) : 0, warps, most, 0));
+        const int upto = carry[1] + block_scan(s < nseq ? (end - start + o.seg - 1) / o.seg : 0, warps, sum, 0);
+        if (s < nseq) {
+            o.first[s + 1] = upto;
+            o.bounds[s + 1] = end;
+        }
+        __syncthreads();
+        if (tid == 1023) {
+            carry[0] = end;
+            carry[1] = upto;
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < o.most; i += 1024) {
+        int lo = 0, hi = nseq;                                   // the sequence that segment i belongs to: first[lo] <= i < first[lo + 1]
+        if (i >= carry[1]) {
+            o.table[i] = make_int4(0, 0, 0, 0);
+            continue;
+        }
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (o.first[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        const int idx = i - o.first[lo], t0 = o.bounds[lo] + idx * o.seg;
+        o.table[i] = make_int4(t0, min(o.seg, o.bounds[lo + 1] - t0), lo, 2 * idx + (t0 + o.seg >= o.bounds[lo + 1]));
+    }
+}
+
+// Zeros in the rows of a packed output that belong to no sequence: those before the first one and behind the last.
+template <class T> __global__ void __launch_bounds__(256) decay_gaps(T *out, long long row_stride, int row_elems, int L, const int *bounds, int nseq) {
+    pdl_begin();
+    const int head = bounds[0], tail = bounds[nseq], rows = head + L - tail;
+    for (int i = blockIdx.x; i < rows; i += gridDim.x) {
+        T *row = out + (long long)(i < head ? i : tail + i - head) * row_stride;
+        for (int e = threadIdx.x; e < row_elems; e += 256) row[e] = from_f<T>(0.f);
+    }
+}
+
+}  // namespace uni
+}  // namespace bissd

@@ -1,0 +1,298 @@
+// The causal decay attention one token after another, on CUDA cores: every type, every size, fp32 throughout.
+//     S_t = e^{g_t} S_{t-1} + a_t b_t^T,    y_t = y_scale S_t^T r_t
+// walked forwards with (a, b, r) = (k, v, q) gives o and, with the roles of S's two sides exchanged (v, k, dout), dq; walked
+// backwards - the decay of the token after t in e^{g_t}'s place - (q, dout, k) gives dv and (dout, q, v) dk, all four from one
+// kernel.  A thread has one column of S and a part of its rows in registers; the lanes that share a column add their
+// products up.  Three multiply-adds per element of S and token, two reads of shared memory (16 bytes) for every 12 of them:
+// bound by the CUDA cores' fp32 rate.
+// A long sequence is walked in segments at once: each segment's own sum of states first (no y), the states that enter the segments
+// from those (decay_chain), then the walk proper from there.
+#pragma once
+#include "uni_plan.cuh"
+
+namespace bissd {
+namespace uni {
+
+constexpr int kWalkThreads = 128;
+
+struct Vector {                                                  // one of a, b, r: (batch, token, head, inner)
+    View v;
+    int of_q;                                                    // its heads are those of q and k
+};
+struct WalkParams {
+    Plan plan;
+    int H, hk, I, J, lanes, reverse;                             // lanes that share a column
+    Vector a, b, r;
+    View g;
+    int g_dtype;
+    float a_scale, y_scale;
+    void *y;                                                     // (tokens, H, J) contiguous, or NULL: states only
+    int y_dtype;
+    long long y_batch;                                           // elements of a batch row of y
+    const float *init;                                           // what enters: (segments, H, ..), or NULL: zeros
+    float *fin;                                                  // what leaves: (segments, H, ..), or NULL
+    float *decay;                                                // (segments, H): the segment's whole decay, or NULL
+    int si, sj;                                                  // strides of S's two sides in init and fin
+    int *status;                                                 // cleared, or NULL
+};
+
+inline int walk_tile(int lanes) { return lanes > 4 ? 16 : 32; }  // tokens staged at a time
+inline size_t walk_smem(int lanes, int ipt) {
+    const int tile = walk_tile(lanes), cols = kWalkThreads / lanes;
+    return sizeof(float) * ((size_t)tile * 2 * lanes * (ipt + 4) + 2 * (size_t)tile * cols + tile);
+}
+
+template <class T, int IPT> __global__ void __launch_bounds__(kWalkThreads) decay_walk(WalkParams a) {
+    pdl_begin();
+    extern __shared__ float dyn[];
+    if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+    const int LI = a.lanes, cols = kWalkThreads / LI, tile = LI > 4 ? 16 : 32, rowlen = LI * (IPT + 4);
+    float *as = dyn, *rs = as + tile * rowlen, *bs = rs + tile * rowlen, *ys = bs + tile * cols, *ds = ys + tile * cols;
+    const int jb = (a.J + cols - 1) / cols;
+    const int cb = blockIdx.x % jb, h = blockIdx.x / jb % a.H, si = blockIdx.x / (jb * a.H);
+    const Segment s = segment(a.plan, si);
+    if (s.len == 0) return;
+    const int tid = threadIdx.x, li = tid % LI, jc = tid / LI, j = cb * cols + jc, hq = h * a.hk / a.H;
+    const long long S = (long long)a.I * a.J;
+    float st_[IPT];
+#pragma unroll
+    for (int e = 0; e < IPT; ++e) {
+        const int i = li * IPT + e;
+        st_[e] = a.init && i < a.I && j < a.J ? a.init[(si * (long long)a.H + h) * S + (long long)i * a.si + (long long)j * a.sj] : 0.f;
+    }
+    auto row = [&](const Vector &x, int t) {
+        return (long long)s.batch * x.v.sb + (long long)t * x.v.sl + (long long)(x.of_q ? hq : h) * x.v.sh;
+    };
+    float total = 0.f;
+    for (int done = 0; done < s.len; done += tile) {
+        const int n = min(tile, s.len - done);
+        const int first = a.reverse ? s.t0 + s.len - done - n : s.t0 + done;   // lowest token of the tile
+        __syncthreads();
+        for (int x = tid; x < n * LI * IPT; x += kWalkThreads) {
+            const int t = x / (LI * IPT), i = x % (LI * IPT), at = t * rowlen + i / IPT * (IPT + 4) + i % IPT;
+            as[at] = i < a.I ? a.a_scale * ld<T>(a.a.v.ptr, row(a.a, first + t) + i) : 0.f;
+            if (a.y) rs[at] = i < a.I ? ld<T>(a.r.v.ptr, row(a.r, first + t) + i) : 0.f;
+        }
+        for (int x = tid; x < n * cols; x += kWalkThreads) {
+            const int t = x / cols, c = cb * cols + x % cols;
+            bs[x] = c < a.J ? ld<T>(a.b.v.ptr, row(a.b, first + t) + c) : 0.f;
+        }
+        if (tid < n) {
+            const int t = first + tid + a.reverse;
+            float g = 0.f;
+            if (!(a.reverse && s.last && t == s.t0 + s.len))
+                g = ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)t * a.g.sl + (long long)h * a.g.sh);
+            ds[tid] = g;
+        }
+        __syncthreads();
+        if (a.decay && tid == 0)
+            for (int t = 0; t < n; ++t) total += ds[t];
+        for (int u = 0; u < n; ++u) {
+            const int t = a.reverse ? n - 1 - u : u;
+            const float d = expf(ds[t]), b = bs[t * cols + jc];
+            const float4 *a4 = reinterpret_cast<const float4 *>(as + t * rowlen + li * (IPT + 4));
+            const float4 *r4 = reinterpret_cast<const float4 *>(rs + t * rowlen + li * (IPT + 4));
+            if (a.y) {
+                float acc = 0.f, acc2 = 0.f;
+#pragma unroll
+                for (int e = 0; e < IPT; e += 4) {
+                    const float4 x = a4[e / 4], r = r4[e / 4];
+                    st_[e] = st_[e] * d + x.x * b;
+                    st_[e + 1] = st_[e + 1] * d + x.y * b;
+                    st_[e + 2] = st_[e + 2] * d + x.z * b;
+                    st_[e + 3] = st_[e + 3] * d + x.w * b;
+                    acc += r.x * st_[e];
+                    acc2 += r.y * st_[e + 1];
+                    acc += r.z * st_[e + 2];
+                    acc2 += r.w * st_[e + 3];
+                }
+                acc += acc2;
+                for (int o = 1; o < LI; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+                if (li == 0) ys[t * cols + jc] = acc * a.y_scale;
+            } else {
+#pragma unroll
+                for (int e = 0; e < IPT; e += 4) {
+                    const float4 x = a4[e / 4];
+                    st_[e] = st_[e] * d + x.x * b;
+                    st_[e + 1] = st_[e + 1] * d + x.y * b;
+                    st_[e + 2] = st_[e + 2] * d + x.z * b;
+                    st_[e + 3] = st_[e + 3] * d + x.w * b;
+                }
+            }
+        }
+        if (a.y) {
+            __syncthreads();
+            for (int x = tid; x < n * cols; x += kWalkThreads) {
+                const int t = x / cols, c = cb * cols + x % cols;
+                if (c < a.J)
+                    st_any(a.y, a.y_dtype, (long long)s.batch * a.y_batch + ((long long)(first + t) * a.H + h) * a.J + c, ys[x]);
+            }
+        }
+    }
+    if (a.fin) {
+#pragma unroll
+        for (int e = 0; e < IPT; ++e) {
+            const int i = li * IPT + e;
+            if (i < a.I && j < a.J) a.fin[(si * (long long)a.H + h) * S + (long long)i * a.si + (long long)j * a.sj] = st_[e];
+        }
+    }
+    if (a.decay && cb == 0 && tid == 0) a.decay[si * (long long)a.H + h] = expf(total);
+}
+
+// The states that enter the segments, from each segment's own sum (in its place): forwards run = D run + own, written before it is
+// added to; backwards the same from the last segment on.  Also the state after the last segment (forwards), or the gradient of
+// the initial state: that of the state after the first token, times the first token's decay (backwards).
+// A thread has an element of one (sequence, head).   `per` elements a state.
+struct ChainParams {
+    Plan plan;
+    int H, per, reverse, nseq;
+    const float *start;                                          // (sequences, H, per), or NULL
+    float *states;                                               // (segments, H, per): own sums in, entering states out
+    const float *decay;                                          // (segments, H)
+    float *end;                                                  // (sequences, H, per), or NULL
+    View g;
+    int g_dtype;
+};
+__global__ void __launch_bounds__(256) decay_chain(ChainParams a) {
+    pdl_begin();
+    const int blocks = (a.per + 255) / 256;
+    const int e = blockIdx.x % blocks * 256 + threadIdx.x, h = blockIdx.x / blocks % a.H, seq = blockIdx.x / (blocks * a.H);
+    if (e >= a.per) return;
+    const long long of_seq = ((long long)seq * a.H + h) * a.per + e;
+    const int2 f = segments(a.plan, seq);
+    float run = a.start ? a.start[of_seq] : 0.f;
+    for (int u0 = 0; u0 < f.y; u0 += 8) {                        // eight segments' values under way at a time
+        float own[8], d[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int u = u0 + k, i = f.x + (a.reverse ? f.y - 1 - u : u);
+            own[k] = u < f.y ? a.states[((long long)i * a.H + h) * a.per + e] : 0.f;
+            d[k] = u < f.y ? a.decay[(long long)i * a.H + h] : 1.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int u = u0 + k, i = f.x + (a.reverse ? f.y - 1 - u : u);
+            if (u < f.y) {
+                a.states[((long long)i * a.H + h) * a.per + e] = run;
+                run = run * d[k] + own[k];
+            }
+        }
+    }
+    if (a.end) {
+        if (a.reverse && f.y > 0) {
+            const Segment s = segment(a.plan, f.x);
+            run *= expf(ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)s.t0 * a.g.sl + (long long)h * a.g.sh));
+        }
+        a.end[of_seq] = run;
+    }
+}
+
+// What the per-head gradients leave: dq and dk summed over the heads that share them, and what a token's decay gets from its own
+// place, flow = q.dq - k.dk (a pair of tokens s < t counts +1 at t and -1 at s).  One warp for a (token, head of q).
+struct FinishParams {
+    int L, H, hk, N;
+    long long tokens;
+    View q, k;
+    const float *dqh, *dkh;                                      // (tokens, H, N)
+    void *dq, *dk;                                               // (tokens, hk, N)
+    float *flow;                                                 // (tokens, H)
+};
+template <class T> __global__ void __launch_bounds__(256) decay_finish(FinishParams a) {
+    pdl_begin();
+    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (w >= a.tokens * a.hk) return;
+    const long long tok = w / a.hk;
+    const int m = (int)(w % a.hk), R = a.H / a.hk;
+    const long long at = tok / a.L * a.q.sb + tok % a.L * a.q.sl + m * a.q.sh, kt = tok / a.L * a.k.sb + tok % a.L * a.k.sl + m * a.k.sh;
+    for (int n0 = 0; n0 < a.N; n0 += 32) {
+        const int n = n0 + lane;
+        float sq = 0.f, sk = 0.f;
+        const float q = n < a.N ? ld<T>(a.q.ptr, at + n) : 0.f, k = n < a.N ? ld<T>(a.k.ptr, kt + n) : 0.f;
+        for (int r = 0; r < R; ++r) {
+            const long long i = (tok * a.H + m * R + r) * a.N + n;
+            const float dq = n < a.N ? a.dqh[i] : 0.f, dk = n < a.N ? a.dkh[i] : 0.f;
+            sq += dq;
+            sk += dk;
+            float f = q * dq - k * dk;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+            if (lane == 0) a.flow[tok * a.H + m * R + r] = (n0 ? a.flow[tok * a.H + m * R + r] : 0.f) + f;
+        }
+        if (n < a.N) {
+            st<T>(a.dq, w * a.N + n, sq);
+            st<T>(a.dk, w * a.N + n, sk);
+        }
+    }
+}
+
+// dg_t: everything that flows from tokens before t (or the initial state) to t and those after (or the final state) = what crosses
+// the segment's right end + flow of the tokens t ... there.  What crosses is a product of two states, so rounding does not pile
+// up over more than one segment.  A block for a (segment, head).
+struct DecayGradParams {
+    Plan plan;
+    int H, per, g_dtype, out_dtype, L;
+    const float *flow, *enter, *denter;                          // states entering each segment from the left, gradients from the right
+    const float *final_, *dfinal;                                // (sequences, H, per); dfinal NULL: zeros
+    View g;
+    void *dg;                                                    // (tokens, H)
+};
+__global__ void __launch_bounds__(256) decay_dg(DecayGradParams a) {
+    pdl_begin();
+    __shared__ double part[8], carry;
+    const int h = blockIdx.x % a.H, si = blockIdx.x / a.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Segment s = segment(a.plan, si);
+    if (s.len == 0) return;
+    const int end = s.t0 + s.len;
+    double cross = 0.0;
+    if (!s.last || a.dfinal) {
+        const long long here = ((long long)si * a.H + h) * a.per;
+        const float *x = s.last ? a.final_ + ((long long)s.seq * a.H + h) * a.per : a.enter + here + (long long)a.H * a.per;
+        const float *y = s.last ? a.dfinal + ((long long)s.seq * a.H + h) * a.per : a.denter + here;
+        for (int e = tid; e < a.per; e += 256) cross += (double)x[e] * y[e];
+        if (!s.last) cross *= expf(ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)end * a.g.sl + (long long)h * a.g.sh));
+    }
+    for (int o = 16; o > 0; o >>= 1) cross += __shfl_xor_sync(0xffffffffu, cross, o);
+    if (lane == 0) part[warp] = cross;
+    __syncthreads();
+    if (tid == 0) {
+        double c = 0.0;
+        for (int w = 0; w < 8; ++w) c += part[w];
+        carry = c;
+    }
+    __syncthreads();
+    for (int hi = end; hi > s.t0; hi -= 256) {                   // from the right, thread 0 the last token
+        const int t = hi - 1 - tid;
+        const long long at = ((long long)s.batch * a.L + t) * a.H + h;
+        double v = t >= s.t0 ? (double)a.flow[at] : 0.0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const double u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (lane == 31) part[warp] = v;
+        __syncthreads();
+        double before = carry;
+        for (int w = 0; w < warp; ++w) before += part[w];
+        if (t >= s.t0) st_any(a.dg, a.out_dtype, at, (float)(before + v));
+        __syncthreads();
+        if (tid == 255) carry = before + v;
+        __syncthreads();
+    }
+}
+
+// One decay for each head: the sum of its tokens' gradients, in a fixed order.
+__global__ void __launch_bounds__(1024) decay_dg_heads(const float *dg, long long tokens, int H, void *out, int dtype) {
+    pdl_begin();
+    __shared__ double part[32];
+    double v = 0.0;
+    for (long long t = threadIdx.x; t < tokens; t += 1024) v += dg[t * H + blockIdx.x];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 32; ++w) v += part[w];
+    st_any(out, dtype, blockIdx.x, (float)v);
+}
+
+}  // namespace uni
+}  // namespace bissd

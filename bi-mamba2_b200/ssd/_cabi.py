@@ -65,11 +65,36 @@ class ConvArgs(C.Structure):
                 ("dout", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p)]
 
 
+class DecayArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "seqlen", "nheads", "nkheads", "kdim", "vdim", "nseq", "dtype", "g_dtype",
+                                         "g_per_head")] + \
+               [("scale", C.c_float), ("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", C.c_void_p), ("g", Tensor),
+                ("cu_seqlens", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p),
+                ("dout", Tensor), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dg", C.c_void_p),
+                ("dfinal_state", C.c_void_p), ("dinitial_state", C.c_void_p)]
+
+
+class DecayStepArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "nheads", "nkheads", "kdim", "vdim", "dtype", "g_dtype", "g_per_head")] + \
+               [("scale", C.c_float), ("q", Tensor), ("k", Tensor), ("v", Tensor), ("g", Tensor), ("o", Tensor),
+                ("state", C.c_void_p), ("slot_stride", C.c_int64), ("nslots", C.c_int32), ("slots", C.c_void_p)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("gate_rows", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32), ("r_dtype", C.c_int32),
+                ("w_dtype", C.c_int32), ("gate_act", C.c_int32), ("scale", C.c_float), ("eps", C.c_float)] + \
+               [(n, C.c_int64) for n in ("stride_x", "stride_residual", "stride_gate", "stride_dr", "stride_dnormed")] + \
+               [(n, C.c_void_p) for n in ("x", "residual", "gate", "scale_vector", "post_weight", "pre_weight", "r", "normed", "rstd",
+                                          "dr", "dnormed", "dx", "dresidual", "dgate", "dscale", "dpost", "dpre")]
+
+
 EXPORTS = ("bissd_abi_version", "bissd_strerror", "bissd_last_cuda_error", "bissd_workspace_bytes", "bissd_workspace_bytes_least", "bissd_forward",
            "bissd_backward", "bissd_kernel_path", "bissd_launch_count", "bissd_trace_enable", "bissd_trace_read", "bissd_selftest_gemm", "bissd_read_status",
            "bissd_forward_static_scratch", "bissd_chain_boundaries", "bissd_rmsnorm_gated_workspace_bytes", "bissd_rmsnorm_gated_forward",
            "bissd_rmsnorm_gated_backward", "bissd_dwconv_silu_workspace_bytes", "bissd_dwconv_silu_forward",
-           "bissd_dwconv_silu_backward", "bissd_backward_into", "bissd_layer_params_in", "bissd_layer_params_out")
+           "bissd_dwconv_silu_backward", "bissd_backward_into", "bissd_layer_params_in", "bissd_layer_params_out",
+           "bissd_decay_workspace_bytes", "bissd_decay_forward", "bissd_decay_backward", "bissd_decay_step",
+           "bissd_block_norm_workspace_bytes", "bissd_block_norm_forward", "bissd_block_norm_backward")
 
 STATIC_SCRATCH_BYTES = 16 << 20      # BISSD_STATIC_SCRATCH_BYTES
 ERR_WORKSPACE, ERR_TOO_LARGE = -5, -9
@@ -124,6 +149,15 @@ def load():
     lib.bissd_dwconv_silu_forward.argtypes = [C.POINTER(ConvArgs), C.c_void_p]
     lib.bissd_dwconv_silu_backward.restype = C.c_int
     lib.bissd_dwconv_silu_backward.argtypes = [C.POINTER(ConvArgs), C.c_void_p, C.c_size_t, C.c_void_p]
+    for name, args in (("bissd_decay_workspace_bytes", [C.POINTER(DecayArgs), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+                       ("bissd_decay_forward", [C.POINTER(DecayArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+                       ("bissd_decay_backward", [C.POINTER(DecayArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+                       ("bissd_decay_step", [C.POINTER(DecayStepArgs), C.c_void_p]),
+                       ("bissd_block_norm_workspace_bytes", [C.POINTER(BlockNormArgs), C.POINTER(C.c_size_t)]),
+                       ("bissd_block_norm_forward", [C.POINTER(BlockNormArgs), C.c_void_p]),
+                       ("bissd_block_norm_backward", [C.POINTER(BlockNormArgs), C.c_void_p, C.c_size_t, C.c_void_p])):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = args
     lib.bissd_chain_boundaries.restype = C.c_int
     lib.bissd_chain_boundaries.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int,
                                            C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]

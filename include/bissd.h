@@ -268,6 +268,87 @@ typedef struct bissd_layer_params {
 int bissd_layer_params_in(const bissd_layer_params *args, void *stream);
 int bissd_layer_params_out(const bissd_layer_params *args, void *stream);
 
+/* ---- causal linear attention with a decay for each head -----------------------------------------------------------
+ * The one-directional sibling of the scan above, as a decoder needs it (the reference keeps a causal path beside its
+ * bidirectional one, src/ssd/uni/):
+ *     S_t = e^{g_t} S_{t-1} + k_t v_t^T,     o_t = scale S_t^T q_t
+ * q, k (batch, seqlen, nkheads, kdim), v, o (batch, seqlen, nheads, vdim), g (batch, seqlen, nheads) the log decays, or
+ * (nheads) with g_per_head; head h of v reads head h * nkheads / nheads of q and k.  S (kdim, vdim) fp32.
+ * Rows of the batch are sequences; with nseq > 0 the batch is one row of packed sequences instead, sequence i the
+ * tokens cu_seqlens[i] ... cu_seqlens[i + 1] - 1 (device memory; what lies outside 0 ... seqlen or runs backwards is
+ * taken as the nearest that does not).  Tokens of no sequence get zeros in o, dq, dk, dv and dg.
+ * Log decays are meant to be <= 0; -inf empties the state.  kdim and vdim from 1 to 256.
+ * The states are fp32 wherever they leave the library, and there as exact as fp32 sums of the inputs' products. */
+typedef struct bissd_decay_args {
+    int32_t batch, seqlen, nheads, nkheads, kdim, vdim;
+    int32_t nseq;                        /* 0: each row of the batch is a sequence */
+    int32_t dtype;                       /* bissd_dtype of q, k, v, o, dout, dq, dk, dv */
+    int32_t g_dtype, g_per_head;
+    float scale;
+    bissd_tensor q, k, v;
+    void *o;                             /* contiguous */
+    bissd_tensor g;                      /* (batch, seqlen, nheads), or ptr alone with g_per_head (contiguous) */
+    const int32_t *cu_seqlens;           /* (nseq + 1) */
+    const float *initial_state;          /* (sequences, nheads, kdim, vdim) contiguous, or NULL: zeros */
+    float *final_state;                  /* the same shape; may be NULL */
+    /* backward: */
+    bissd_tensor dout;
+    void *dq, *dk, *dv;                  /* contiguous, like q, k, v */
+    void *dg;                            /* contiguous, like g and of its dtype; may be NULL */
+    const float *dfinal_state;           /* may be NULL */
+    float *dinitial_state;               /* may be NULL */
+} bissd_decay_args;
+
+/* Scratch of either pass, a multiple of 256; workspace must be 256-byte aligned. */
+int bissd_decay_workspace_bytes(const bissd_decay_args *args, size_t *fwd_bytes, size_t *bwd_bytes);
+int bissd_decay_forward(const bissd_decay_args *args, void *workspace, size_t workspace_bytes, void *stream);
+int bissd_decay_backward(const bissd_decay_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token for each of `batch` requests, states updated in place:
+ *     S = e^{g} S + k v^T,     o = scale S^T q
+ * state: `nslots` states of (nheads, kdim, vdim) fp32 contiguous, slot_stride elements apart.  Request i has the state
+ * slots[i] (device memory), or i with slots == NULL.  A slot outside 0 ... nslots - 1 marks padding: its row of o becomes
+ * zeros and no state changes.  Requests with the same slot are tokens that follow one another, in the order of their
+ * index.  q, k (batch, nkheads, kdim), v, o (batch, nheads, vdim): stride_batch and stride_head count, stride_seq does
+ * not; g (batch, nheads), or (nheads) with g_per_head. */
+typedef struct bissd_decay_step_args {
+    int32_t batch, nheads, nkheads, kdim, vdim;
+    int32_t dtype, g_dtype, g_per_head;
+    float scale;
+    bissd_tensor q, k, v, g, o;
+    float *state;
+    int64_t slot_stride;
+    int32_t nslots;
+    const int32_t *slots;
+} bissd_decay_step_args;
+int bissd_decay_step(const bissd_decay_step_args *args, void *stream);
+
+/* ---- the norms before and after a block, with its gate and residual scale ------------------------------------------
+ *     n = rms(x) post_weight   (n = x where post_weight is NULL),     r = residual + scale * act(gate) * n,
+ *     normed = rms(r) pre_weight                                      rms(t) = t / sqrt(mean(t^2) + eps)
+ * x: the block's output, r: the residual stream after the block, normed: the next block's input.  `rows` rows of `width`
+ * contiguous channels, 1 ... 8192.  gate: NULL, one row for each row of x, or (gate_rows > 0) one for every gate_rows
+ * rows of x, gate_rows dividing rows.  The inputs' rows lie stride_* elements apart, the outputs are contiguous.  scale: the number, or (width) values where scale_vector is not NULL.  Weights
+ * and scale_vector are w_dtype: fp32 or dtype.  residual, r and their gradients are r_dtype: dtype or fp32, and rms(r) is
+ * taken of r before it is rounded.  The backward pass reads what the forward pass wrote to rstd (2 * rows fp32). */
+enum { BISSD_GATE_NONE = 0, BISSD_GATE_SIGMOID = 1, BISSD_GATE_SILU = 2 };
+typedef struct bissd_block_norm_args {
+    int64_t rows, gate_rows;
+    int32_t width, dtype, r_dtype, w_dtype;
+    int32_t gate_act;                    /* BISSD_GATE_* */
+    float scale, eps;
+    int64_t stride_x, stride_residual, stride_gate, stride_dr, stride_dnormed;
+    const void *x, *residual, *gate, *scale_vector, *post_weight, *pre_weight;
+    void *r, *normed;                    /* normed NULL where pre_weight is NULL */
+    float *rstd;                         /* forward: may be NULL */
+    /* backward: dr and dnormed may be NULL (zeros); so may each gradient that is not wanted */
+    const void *dr, *dnormed;
+    void *dx, *dresidual, *dgate, *dscale, *dpost, *dpre;
+} bissd_block_norm_args;
+int bissd_block_norm_workspace_bytes(const bissd_block_norm_args *args, size_t *bwd_bytes);
+int bissd_block_norm_forward(const bissd_block_norm_args *args, void *stream);
+int bissd_block_norm_backward(const bissd_block_norm_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Name of the kernel family the library selects for `p` ("tcgen05" or "simt"); for reports and tests. */
 const char *bissd_kernel_path(const bissd_problem *p);
 
