@@ -8,6 +8,7 @@
 #include "host.cuh"
 #include "uni_plan.cuh"
 #include "uni_step.cuh"
+#include "uni_tc.cuh"
 #include "uni_walk.cuh"
 
 using namespace bissd;
@@ -295,7 +296,7 @@ WalkSpace walk_space(const bissd_decay_args *a, Bump &ws, bool backward) {
 uni::ChainParams chain_params(const Walks &w, bool reverse, const float *start, float *states, const float *decay, float *end) {
     uni::ChainParams c{};
     c.plan = w.plan; c.H = w.z.H; c.per = w.z.N * w.z.P; c.reverse = reverse; c.nseq = w.z.sequences;
-    c.start = start; c.states = states; c.decay = decay; c.end = end; c.g = w.g; c.g_dtype = w.a->g_dtype;
+    c.start = start; c.states = states; c.decay = decay; c.end = end; c.first_decay = reverse; c.g = w.g; c.g_dtype = w.a->g_dtype;
     return c;
 }
 
@@ -379,6 +380,131 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     return BISSD_OK;
 }
 
+using tc::make_map2;
+using tc::make_map4;
+using unitc::bf16;
+
+// ---- on the tensor cores ----------------------------------------------------------------------------------------------
+
+// bf16 with head sizes and rows that 16-byte loads fit, a positive scale (it is added to the decays' logarithms).
+bool tc_sizes(const bissd_decay_args *a) {
+    return a->dtype == BISSD_BF16 && a->kdim % 8 == 0 && a->kdim <= 128 && a->vdim % 8 == 0 && a->scale > 0.f && std::isfinite(a->scale);
+}
+bool tc_tensor(const bissd_tensor &t, long long batch, long long seq, long long heads) {
+    auto fits = [](long long stride, long long n) { return n == 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38)); };
+    return aligned16(t.ptr) && fits(t.stride_batch, batch) && fits(t.stride_seq, seq) && fits(t.stride_head, heads);
+}
+bool tc_forward_ok(const bissd_decay_args *a) {
+    return tc_sizes(a) && tc_tensor(a->q, a->batch, a->seqlen, a->nkheads) && tc_tensor(a->k, a->batch, a->seqlen, a->nkheads) &&
+           tc_tensor(a->v, a->batch, a->seqlen, a->nheads) && aligned16(a->o);
+}
+
+struct TcSpace {
+    int NT, PB;
+    uni::Plan seg, chunk;
+    uni::PlanOut seg_table{}, chunk_table{};
+    bool split;                                                  // sequences in several segments, or packed
+    bf16 *tiles;
+    float *states, *decay;
+};
+
+// Tokens to a segment: the walk over the chunks has a block for each (row, head, 64 columns), two blocks an SM; where that leaves
+// SMs without, rows are cut, into pieces of four chunks at least (a piece is walked twice, the first time without results).
+int tc_segment(const bissd_decay_args *a, int PB) {
+    const int chunks = ceil_div(a->seqlen, unitc::kQ);
+    const long long blocks = (long long)a->batch * a->nheads * PB;
+    const long long parts = std::max<long long>(1, std::min<long long>(2 * 148 / blocks, chunks / 4));
+    return (int)((chunks + parts - 1) / parts) * unitc::kQ;
+}
+TcSpace tc_space(const bissd_decay_args *a, Bump &ws) {
+    TcSpace t{};
+    t.NT = a->kdim <= 64 ? 64 : 128;
+    t.PB = ceil_div(a->vdim, unitc::kP);
+    t.chunk = plan_of(a, unitc::kQ, ws, &t.chunk_table);
+    t.seg = plan_of(a, tc_segment(a, t.PB), ws, &t.seg_table);
+    t.split = t.seg.packed || t.seg.per_seq > 1;
+    t.tiles = ws.take<bf16>((size_t)t.chunk.most * a->nheads * t.PB * t.NT * unitc::kP);
+    if (t.split) {
+        t.states = ws.take<float>((size_t)t.seg.most * a->nheads * a->kdim * a->vdim);
+        t.decay = ws.take<float>((size_t)t.seg.most * a->nheads);
+    }
+    return t;
+}
+unitc::Heads tc_heads(const bissd_decay_args *a, int PB) {
+    unitc::Heads h{};
+    h.H = a->nheads; h.hk = a->nkheads; h.N = a->kdim; h.P = a->vdim; h.PB = PB;
+    h.g = view(a->g); h.g_dtype = a->g_dtype;
+    if (a->g_per_head) { h.g.sb = h.g.sl = 0; h.g.sh = 1; }
+    h.log_scale = std::log2(a->scale);
+    return h;
+}
+bool tc_map(CUtensorMap *m, const bissd_decay_args *a, const bissd_tensor &t, int inner, int heads) {
+    auto bytes = [](long long stride, int n) { return n == 1 ? 16ULL : (unsigned long long)stride * 2; };
+    return make_map4(m, BISSD_BF16, t.ptr, {(unsigned long long)inner, (unsigned long long)heads, (unsigned long long)a->seqlen, (unsigned long long)a->batch},
+                     {bytes(t.stride_head, heads), bytes(t.stride_seq, a->seqlen), bytes(t.stride_batch, a->batch)}, {64, 1, unitc::kQ, 1});
+}
+
+struct TcMaps {
+    CUtensorMap q, k, v;
+};
+// The states that enter the chunks (or the gradients, backwards), as bf16 tiles; those that enter and leave the sequences in fp32.
+int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &cols, bool reverse, const float *start, float *end,
+              float *states, float *decay, bf16 *tiles, int *status, cudaStream_t s) {
+    unitc::StatesParams p{};
+    p.h = tc_heads(a, t.PB);
+    p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.exact = end != nullptr; p.status = status;
+    const auto kernel = t.NT == 64 ? unitc::decay_states<64> : unitc::decay_states<128>;
+    const size_t smem = unitc::states_smem(t.NT);
+    const long long grid = (long long)t.seg.most * a->nheads * t.PB;
+    if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    BISSD_ALLOW(kernel, smem);
+    if (t.split) {
+        p.fin = states; p.decay = decay;
+        BISSD_LAUNCH("decay_states_own", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, cols));
+        uni::ChainParams c{};
+        c.plan = t.seg; c.H = a->nheads; c.per = a->kdim * a->vdim; c.reverse = reverse; c.nseq = a->nseq > 0 ? a->nseq : a->batch;
+        c.start = start; c.states = states; c.decay = decay; c.end = end;
+        BISSD_DO(launch_chain(c, s));
+        p.init = states; p.fin = p.decay = nullptr; p.exact = 0;
+    } else {
+        p.init = start; p.fin = end; p.by_seq = 1;
+    }
+    p.tiles = tiles;
+    BISSD_LAUNCH("decay_states", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, cols));
+    return BISSD_OK;
+}
+bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, const bf16 *tiles) {
+    return make_map2(m, BISSD_BF16, tiles, unitc::kP, (unsigned long long)t.chunk.most * a->nheads * t.PB * t.NT, unitc::kP, t.NT);
+}
+
+int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
+    const TcSpace t = tc_space(a, ws);
+    int *status = reinterpret_cast<int *>(ws.base);
+    if ((long long)t.chunk.most * a->nheads * t.PB * t.NT > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    CUtensorMap q, k, v, tiles;
+    if (!tc_map(&q, a, a->q, a->kdim, a->nkheads) || !tc_map(&k, a, a->k, a->kdim, a->nkheads) || !tc_map(&v, a, a->v, a->vdim, a->nheads) ||
+        !tc_tile_map(&tiles, a, t, t.tiles))
+        return note_cuda(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
+    BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
+    BISSD_DO(launch_gaps(a, a->dtype, a->o, a->nheads * a->vdim, t.chunk_table.bounds, s));
+    BISSD_DO(tc_states(a, t, k, v, false, a->initial_state, a->final_state, t.states, t.decay, t.tiles, status, s));
+    unitc::ChunksParams p{};
+    p.h = tc_heads(a, t.PB);
+    p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
+    const int tiles_v = a->nheads / a->nkheads * t.PB;
+    const long long all = (long long)t.chunk.most * a->nkheads * tiles_v;
+    p.vpc = (int)std::max<long long>(1, std::min<long long>(tiles_v, all / (4 * 2 * 148)));
+    p.parts = ceil_div(tiles_v, p.vpc);
+    const auto kernel = t.NT == 64 ? unitc::decay_chunks<64> : unitc::decay_chunks<128>;
+    const size_t smem = unitc::chunks_smem(t.NT);
+    const long long grid = (long long)t.chunk.most * a->nkheads * p.parts;
+    if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    BISSD_ALLOW(kernel, smem);
+    BISSD_LAUNCH("decay_chunks", launch_pdl(kernel, (int)grid, 256, smem, s, p, q, k, v, tiles));
+    return BISSD_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -387,9 +513,10 @@ int bissd_decay_workspace_bytes(const bissd_decay_args *a, size_t *fwd_bytes, si
     const int rc = decay_check(a, false);
     if (rc != BISSD_OK) return rc;
     if (fwd_bytes) {
-        Bump b{nullptr};
+        Bump b{nullptr}, c{nullptr};                              // which of the two runs is known at the call
         walk_space(a, b, false);
-        *fwd_bytes = b.used;
+        if (tc_sizes(a)) tc_space(a, c);
+        *fwd_bytes = std::max(b.used, c.used);
     }
     if (bwd_bytes) {
         Bump b{nullptr};
@@ -407,7 +534,8 @@ int bissd_decay_forward(const bissd_decay_args *a, void *workspace, size_t works
     if (reinterpret_cast<uintptr_t>(workspace) % 256) return BISSD_ERR_ALIGN;
     BISSD_DO(check_device());
     Bump b{static_cast<char *>(workspace)};
-    return walk_forward(a, b, static_cast<cudaStream_t>(stream));
+    const auto s = static_cast<cudaStream_t>(stream);
+    return tc_forward_ok(a) ? tc_forward(a, b, s) : walk_forward(a, b, s);
 }
 
 int bissd_decay_backward(const bissd_decay_args *a, void *workspace, size_t workspace_bytes, void *stream) {

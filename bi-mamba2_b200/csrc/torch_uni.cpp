@@ -73,7 +73,7 @@ Tensor in_place(const Tensor &t) {
     }
     // a dimension of one element may have any stride, also one that no descriptor holds
     for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && st[i] >= 0;
-    return ok ? t : t.contiguous();
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);       // contiguous() would leave an odd address as it is
 }
 Tensor contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 void once(const char *who) {

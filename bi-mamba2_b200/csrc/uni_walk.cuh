@@ -150,6 +150,7 @@ struct ChainParams {
     float *states;                                               // (segments, H, per): own sums in, entering states out
     const float *decay;                                          // (segments, H)
     float *end;                                                  // (sequences, H, per), or NULL
+    int first_decay;                                             // backwards: `end` is one decay further back
     View g;
     int g_dtype;
 };
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(256) decay_chain(ChainParams a) {
         }
     }
     if (a.end) {
-        if (a.reverse && f.y > 0) {
+        if (a.first_decay && f.y > 0) {
             const Segment s = segment(a.plan, f.x);
             run *= expf(ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)s.t0 * a.g.sl + (long long)h * a.g.sh));
         }
