@@ -444,15 +444,12 @@ bool tc_map(CUtensorMap *m, const bissd_decay_args *a, const bissd_tensor &t, in
                      {bytes(t.stride_head, heads), bytes(t.stride_seq, a->seqlen), bytes(t.stride_batch, a->batch)}, {64, 1, unitc::kQ, 1});
 }
 
-struct TcMaps {
-    CUtensorMap q, k, v;
-};
 // The states that enter the chunks (or the gradients, backwards), as bf16 tiles; those that enter and leave the sequences in fp32.
-int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &cols, bool reverse, const float *start, float *end,
-              float *states, float *decay, bf16 *tiles, int *status, cudaStream_t s) {
+int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const bissd_tensor &cols, const CUtensorMap &tiles, bool reverse,
+              const float *start, float *end, float *states, float *decay, int *status, cudaStream_t s) {
     unitc::StatesParams p{};
     p.h = tc_heads(a, t.PB);
-    p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.exact = end != nullptr; p.status = status;
+    p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.exact = end != nullptr; p.v = view(cols); p.status = status;
     const auto kernel = t.NT == 64 ? unitc::decay_states<64> : unitc::decay_states<128>;
     const size_t smem = unitc::states_smem(t.NT);
     const long long grid = (long long)t.seg.most * a->nheads * t.PB;
@@ -460,7 +457,7 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
     BISSD_ALLOW(kernel, smem);
     if (t.split) {
         p.fin = states; p.decay = decay;
-        BISSD_LAUNCH("decay_states_own", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, cols));
+        BISSD_LAUNCH("decay_states_own", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, tiles));
         uni::ChainParams c{};
         c.plan = t.seg; c.H = a->nheads; c.per = a->kdim * a->vdim; c.reverse = reverse; c.nseq = a->nseq > 0 ? a->nseq : a->batch;
         c.start = start; c.states = states; c.decay = decay; c.end = end;
@@ -469,8 +466,8 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
     } else {
         p.init = start; p.fin = end; p.by_seq = 1;
     }
-    p.tiles = tiles;
-    BISSD_LAUNCH("decay_states", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, cols));
+    p.tiles = 1;
+    BISSD_LAUNCH("decay_states", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, tiles));
     return BISSD_OK;
 }
 bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, const bf16 *tiles) {
@@ -488,7 +485,7 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
     BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
     BISSD_DO(launch_gaps(a, a->dtype, a->o, a->nheads * a->vdim, t.chunk_table.bounds, s));
-    BISSD_DO(tc_states(a, t, k, v, false, a->initial_state, a->final_state, t.states, t.decay, t.tiles, status, s));
+    BISSD_DO(tc_states(a, t, k, a->v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, s));
     unitc::ChunksParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
@@ -502,6 +499,85 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     BISSD_ALLOW(kernel, smem);
     BISSD_LAUNCH("decay_chunks", launch_pdl(kernel, (int)grid, 256, smem, s, p, q, k, v, tiles));
+    return BISSD_OK;
+}
+
+struct TcGradSpace {
+    TcSpace t;
+    bf16 *grads;                                                 // tiles of the states' gradients
+    float *gstates, *gdecay;
+    int vpc, parts;
+    float *part, *dg_tokens;
+};
+TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
+    TcGradSpace g{};
+    g.t = tc_space(a, ws);
+    const long long tokens = (long long)a->batch * a->seqlen;
+    g.grads = ws.take<bf16>((size_t)g.t.chunk.most * a->nheads * g.t.PB * g.t.NT * unitc::kP);
+    if (g.t.split) {
+        g.gstates = ws.take<float>((size_t)g.t.seg.most * a->nheads * a->kdim * a->vdim);
+        g.gdecay = ws.take<float>((size_t)g.t.seg.most * a->nheads);
+    }
+    // heads that share q and k are walked by one block, by several where that leaves SMs without
+    const int R = a->nheads / a->nkheads;
+    const long long items = (long long)g.t.chunk.most * a->nkheads;
+    const int heads = (int)std::max<long long>(1, std::min<long long>(R, R * items / 148));
+    g.vpc = heads * g.t.PB;
+    g.parts = ceil_div(R, heads);
+    if (g.parts > 1) g.part = ws.take<float>((size_t)2 * g.parts * tokens * a->nkheads * a->kdim);
+    if (a->g_per_head) g.dg_tokens = ws.take<float>((size_t)tokens * a->nheads);
+    return g;
+}
+bool tc_backward_ok(const bissd_decay_args *a) {
+    return tc_sizes(a) && tc_tensor(a->q, a->batch, a->seqlen, a->nkheads) && tc_tensor(a->k, a->batch, a->seqlen, a->nkheads) &&
+           tc_tensor(a->v, a->batch, a->seqlen, a->nheads) && tc_tensor(a->dout, a->batch, a->seqlen, a->nheads) && aligned16(a->dq) && aligned16(a->dk) &&
+           aligned16(a->dv);
+}
+
+int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
+    const TcGradSpace g = tc_grad_space(a, ws);
+    const TcSpace &t = g.t;
+    int *status = reinterpret_cast<int *>(ws.base);
+    if ((long long)t.chunk.most * a->nheads * t.PB * t.NT > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    CUtensorMap q, k, v, dout, tiles, grads;
+    if (!tc_map(&q, a, a->q, a->kdim, a->nkheads) || !tc_map(&k, a, a->k, a->kdim, a->nkheads) || !tc_map(&v, a, a->v, a->vdim, a->nheads) ||
+        !tc_map(&dout, a, a->dout, a->vdim, a->nheads) || !tc_tile_map(&tiles, a, t, t.tiles) || !tc_tile_map(&grads, a, t, g.grads))
+        return note_cuda(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
+    BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
+    const int *bounds = t.chunk_table.bounds;
+    BISSD_DO(launch_gaps(a, a->dtype, a->dv, a->nheads * a->vdim, bounds, s));
+    BISSD_DO(launch_gaps(a, a->dtype, a->dq, a->nkheads * a->kdim, bounds, s));
+    BISSD_DO(launch_gaps(a, a->dtype, a->dk, a->nkheads * a->kdim, bounds, s));
+    if (!a->g_per_head) BISSD_DO(launch_gaps(a, a->g_dtype, a->dg, a->nheads, bounds, s));
+    BISSD_DO(launch_gaps(a, BISSD_F32, g.dg_tokens, a->nheads, bounds, s));
+    if (g.part)
+        for (int i = 0; i < 2 * g.parts; ++i)
+            BISSD_DO(launch_gaps(a, BISSD_F32, g.part + (size_t)i * a->seqlen * a->nkheads * a->kdim, a->nkheads * a->kdim, bounds, s));
+    BISSD_DO(tc_states(a, t, k, a->v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
+    BISSD_DO(tc_states(a, t, q, a->dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, s));
+    unitc::GradsParams p{};
+    p.h = tc_heads(a, t.PB);
+    p.chunk = t.chunk; p.vpc = g.vpc; p.parts = g.parts;
+    p.dq = static_cast<bf16 *>(a->dq); p.dk = static_cast<bf16 *>(a->dk); p.dv = static_cast<bf16 *>(a->dv);
+    p.part = g.part; p.tokens = (long long)a->batch * a->seqlen;
+    p.dg = a->dg ? (a->g_per_head ? g.dg_tokens : a->dg) : nullptr;
+    p.dg_dtype = a->g_per_head ? BISSD_F32 : a->g_dtype;
+    p.status = status;
+    const auto kernel = t.NT == 64 ? unitc::decay_grads<64> : unitc::decay_grads<128>;
+    const size_t smem = unitc::grads_smem(t.NT);
+    const long long grid = (long long)t.chunk.most * a->nkheads * p.parts;
+    if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    BISSD_ALLOW(kernel, smem);
+    BISSD_LAUNCH("decay_grads", launch_pdl(kernel, (int)grid, 512, smem, s, p, q, k, v, dout, tiles, grads));
+    if (g.parts > 1) {
+        const long long each = p.tokens * a->nkheads * a->kdim;
+        BISSD_LAUNCH("decay_sum_parts", launch_pdl(unitc::decay_sum_parts, (int)((2 * each / 4 + 255) / 256), 256, 0, s, (const float *)g.part, g.parts, each,
+                                                   p.dq, p.dk));
+    }
+    if (a->dg && a->g_per_head)
+        BISSD_LAUNCH("decay_dg_heads", launch_pdl(uni::decay_dg_heads, (int)a->nheads, 1024, 0, s, (const float *)g.dg_tokens, p.tokens, (int)a->nheads, a->dg,
+                                                  (int)a->g_dtype));
     return BISSD_OK;
 }
 
@@ -519,9 +595,10 @@ int bissd_decay_workspace_bytes(const bissd_decay_args *a, size_t *fwd_bytes, si
         *fwd_bytes = std::max(b.used, c.used);
     }
     if (bwd_bytes) {
-        Bump b{nullptr};
+        Bump b{nullptr}, c{nullptr};
         walk_space(a, b, true);
-        *bwd_bytes = b.used;
+        if (tc_sizes(a)) tc_grad_space(a, c);
+        *bwd_bytes = std::max(b.used, c.used);
     }
     return BISSD_OK;
 }
@@ -546,7 +623,8 @@ int bissd_decay_backward(const bissd_decay_args *a, void *workspace, size_t work
     if (reinterpret_cast<uintptr_t>(workspace) % 256) return BISSD_ERR_ALIGN;
     BISSD_DO(check_device());
     Bump b{static_cast<char *>(workspace)};
-    return walk_backward(a, b, static_cast<cudaStream_t>(stream));
+    const auto s = static_cast<cudaStream_t>(stream);
+    return tc_backward_ok(a) ? tc_backward(a, b, s) : walk_backward(a, b, s);
 }
 
 int bissd_decay_step(const bissd_decay_step_args *a, void *stream) {

@@ -97,73 +97,91 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
 // ---- the states that enter the chunks ------------------------------------------------------------------------------------
 // Forwards S' as above; backwards (v the outputs' gradient, k the queries) the gradient that enters each chunk from its right,
 // G' = e^{c_end} G + sum_t q_t (scale e^{c_t} do_t)^T.  A block walks the chunks of one (segment, head, 64 columns), S or G in
-// registers (a row n and 32 columns a thread) and the next chunk's rows on their way; v's rows are weighted in place.
+// registers (a row n and 32 columns a thread).  k's rows come by TMA a chunk ahead; v's go through registers, a chunk ahead as well,
+// and are weighted on the way to shared memory; S leaves as a bf16 tile through a TMA store.  The weights need the decays alone: the
+// eight warps make those of eight chunks at a time.
 // exact: the weighted row is given to the tensor cores in three bf16 parts, each what is left of those before, so that the states
 // that leave the library are fp32's.  The tiles that the other kernels read are bf16 in any case: they meet bf16 factors.
 struct StatesParams {
     Heads h;
     Plan seg, chunk;
-    int reverse, exact, by_seq;                                  // by_seq: init and fin hold a state a sequence, not a segment
+    int reverse, exact, by_seq, tiles;                           // by_seq: init and fin hold a state a sequence, not a segment
+    View v;                                                      // v or the outputs' gradient
     const float *init;
     float *fin, *decay;                                          // decay: (segments, H) the segment's whole decay, or NULL
-    bf16 *tiles;                                                 // (chunks, H, PB, NT, 64), or NULL
     int *status;
 };
+// The thread's tile stores so far have read their shared memory.
+__device__ __forceinline__ void tma_store_read() {
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+constexpr int kAhead = 8;                                        // chunks whose weights are made at a time
 inline size_t states_smem(int NT) { return 1024 + 2 * (size_t)(NT / 64) * kSlab + 2 * (size_t)kSlab; }
 
 template <int NT> __global__ void __launch_bounds__(256, 2)
-decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV) {
+decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
     constexpr int kSlabs = NT / 64;
     extern __shared__ uint8_t dyn[];
-    __shared__ uint64_t full[2], done, unused;
+    __shared__ uint64_t full[2], done[2], unused;
     __shared__ uint32_t tmem_slot;
-    __shared__ float w[3][kQ], whole[3];                          // of three steps: a warp may be one behind another
-    uint8_t *smK = smem_align1024(dyn), *smV = smK + 2 * kSlabs * kSlab;   // two stages of each
+    __shared__ float w[kAhead][kQ], whole[kAhead];
+    uint8_t *smK = smem_align1024(dyn), *smV = smK + 2 * kSlabs * kSlab, *smS = smV + kSlab;   // two stages of k; weighted rows; S
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pb = blockIdx.x % a.h.PB, h = blockIdx.x / a.h.PB % a.h.H, si = blockIdx.x / (a.h.PB * a.h.H), hq = h * a.h.hk / a.h.H;
     const Segment s = uni::segment(a.seg, si);
     if (s.len == 0) return;                                      // packed: fewer segments than there could be
     const int nc = ceil_div(s.len, kQ), c0 = uni::segments(a.chunk, s.seq).x + s.idx * (a.seg.seg / kQ);
     auto place = [&](int i) { return a.reverse ? nc - 1 - i : i; };        // chunk of the segment at step i
+    auto length = [&](int i) { return min(kQ, s.len - place(i) * kQ); };
     auto load = [&](int i) {
         const int st = i & 1, t = s.t0 + place(i) * kQ;
-        mbar_expect_tx(&full[st], (kSlabs + 1) * kSlab);
+        mbar_expect_tx(&full[st], kSlabs * kSlab);
         for (int j = 0; j < kSlabs; ++j) tma_load4(smK + (st * kSlabs + j) * kSlab, &tmK, j * 64, hq, t, s.batch, &full[st]);
-        tma_load4(smV + st * kSlab, &tmV, pb * kP, h, t, s.batch, &full[st]);
     };
-    auto weights = [&](int i, Decays d) {                        // one warp
-        const int len = min(kQ, s.len - place(i) * kQ);
+    const bool in_cols = pb * kP + (tid & 7) * 8 < a.h.P;
+    const bf16 *vp = static_cast<const bf16 *>(a.v.ptr) + (long long)s.batch * a.v.sb + (long long)h * a.v.sh + pb * kP + (tid & 7) * 8;
+    auto fetch = [&](int i, uint4 (&rows)[4]) {                  // 16 bytes of four rows of v
+        const int t = s.t0 + place(i) * kQ, len = length(i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int row = (tid >> 3) + k * 32;
+            rows[k] = row < len && in_cols ? __ldg(reinterpret_cast<const uint4 *>(vp + (long long)(t + row) * a.v.sl)) : zero8();
+        }
+    };
+    Decays decays;
+    auto ask = [&](int i) {
+        if (i < nc) decays.load(a.h, s.batch, s.t0 + place(i) * kQ, length(i), h, lane);
+    };
+    auto weights = [&](int i) {                                  // this warp's chunk of the next kAhead
+        if (i >= nc) return;
+        const int len = length(i);
         float c[4], p[4];
-        d.log2(a.h);
-        d.prefix(p, lane);
+        decays.log2(a.h);
+        decays.prefix(p, lane);
         if (a.reverse) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) c[k] = p[k] + a.h.log_scale;
         } else {
-            d.suffix(c, lane);
+            decays.suffix(c, lane);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[i % 3][lane * 4 + k] = lane * 4 + k < len ? exp2f(c[k]) : 0.f;
-        if (lane == 31) whole[i % 3] = p[3];
+        for (int k = 0; k < 4; ++k) w[warp][lane * 4 + k] = lane * 4 + k < len ? exp2f(c[k]) : 0.f;
+        if (lane == 31) whole[warp] = p[3];
     };
+    ask(warp);
     if (warp == 0) tmem_alloc(&tmem_slot, 64);
     if (tid == 32) {
         mbar_init(&full[0], 1);
         mbar_init(&full[1], 1);
-        mbar_init(&done, 1);
+        mbar_init(&done[0], 1);
+        mbar_init(&done[1], 1);
         fence_mbar_init();
         load(0);
     }
-    Decays next;                                                 // warp 2: of the step after the one whose weights it writes
-    auto fetch = [&](int i) {
-        if (i < nc) next.load(a.h, s.batch, s.t0 + place(i) * kQ, min(kQ, s.len - place(i) * kQ), h, lane);
-    };
-    if (warp == 2) {
-        fetch(0);
-        weights(0, next);
-        fetch(1);
-    }
+    uint4 rows[4];
+    fetch(0, rows);
     const int n = (warp & 3) * 32 + lane, half = warp >> 2, col = pb * kP + half * 32;
     const long long at = (((long long)(a.by_seq ? s.seq : si) * a.h.H + h) * a.h.N + n) * a.h.P + col;
     float S[32];
@@ -175,26 +193,31 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     const uint32_t tmem = tmem_slot;
     constexpr uint32_t idesc = instr_desc(1, true, true, kP);
     bool ok = true;
-    int loads = 1, waits = 0;                                    // loads asked for, uses of `done`
+    int loads = 1, uses = 0;                                     // loads asked for, commits
     float total = 0.f;
+    // `use` is waited for as the phase use / 2 of barrier use & 1: the parts of an exact step overlap, two at a time
+    auto wait = [&](int use) { return mbar_wait(&done[use & 1], (use >> 1) & 1); };
     for (int i = 0; i < nc; ++i) {
-        const int st = i & 1, len = min(kQ, s.len - place(i) * kQ);
+        const int st = i & 1;
         if (i + 1 < nc) {                                        // the stage was read by the MMAs of the step before, which are done
             if (tid == 32) load(i + 1);
             ++loads;
         }
-        ok = ok && mbar_wait(&full[st], (i >> 1) & 1);
-        uint8_t *v = smV + st * kSlab;
-        uint4 rows[4];                                           // v's as loaded
-        auto weigh = [&](int part) {                             // part 0, 1 or 2 of the weighted rows to where v's were
+        if (i % kAhead == 0) {
+            if (i) __syncthreads();                              // the last weights have been read
+            weights(i + warp);
+            ask(i + kAhead + warp);
+            __syncthreads();
+        }
+        auto weigh = [&](int part, uint8_t *to) {                // part 0, 1 or 2 of the weighted rows
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int x = tid + k * 256, row = x >> 3;
-                const float f = row < len ? w[i % 3][row] : 0.f;
+                const float f = w[i % kAhead][row];
                 float e[8], r[8];
                 unpack8<bf16>(rows[k], e);
 #pragma unroll
-                for (int m = 0; m < 8; ++m) e[m] = row < len ? e[m] * f : 0.f;
+                for (int m = 0; m < 8; ++m) e[m] *= f;
                 uint4 out = pack8<bf16>(e);
                 for (int q = 0; q < part; ++q) {
                     unpack8<bf16>(out, r);
@@ -202,57 +225,61 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                     for (int m = 0; m < 8; ++m) e[m] -= r[m];
                     out = pack8<bf16>(e);
                 }
-                *reinterpret_cast<uint4 *>(v + x * 16) = out;
+                *reinterpret_cast<uint4 *>(to + row * 128 + (((x & 7) ^ (row & 7)) << 4)) = out;
             }
-            fence_async_smem();
         };
-        if (ok) {
-            if (a.seg.packed && len < kQ)
-                for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, len, tid, 256);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) rows[k] = *reinterpret_cast<const uint4 *>(v + (tid + k * 256) * 16);
-            weigh(0);
-        }
-        if (warp == 2 && i + 1 < nc) {
-            weights(i + 1, next);
-            fetch(i + 2);
-        }
-        tc_fence_before();                                       // the last step's loads from tensor memory
-        ok = __syncthreads_and(ok);
-        if (!ok) break;
-        auto issue = [&](uint32_t first) {
-            tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < kQ / 16; ++kk)                 // where NT is 64, rows 64 ... 127 are v's columns: products of no use
-                umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 2 * kSlab : kSlab, 1024),
-                     smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : first);
-            umma_commit(&done);
-        };
-        if (warp == 0 && elect_one()) issue(0u);
+        weigh(0, smV);
         if (a.tiles && n < NT) {                                 // what enters this chunk
-            uint4 *o = reinterpret_cast<uint4 *>(a.tiles + ((((long long)(c0 + place(i)) * a.h.H + h) * a.h.PB + pb) * NT + n) * kP + half * 32);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float e[8] = {S[8 * j], S[8 * j + 1], S[8 * j + 2], S[8 * j + 3], S[8 * j + 4], S[8 * j + 5], S[8 * j + 6], S[8 * j + 7]};
-                o[j] = pack8<bf16>(e);
+                *reinterpret_cast<uint4 *>(smS + n * 128 + (((half * 4 + j) ^ (n & 7)) << 4)) = pack8<bf16>(e);
             }
         }
-        ok = mbar_wait(&done, waits & 1);
-        ++waits;
+        ok = ok && mbar_wait(&full[st], (i >> 1) & 1);
+        if (ok && a.seg.packed && length(i) < kQ)
+            for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, length(i), tid, 256);
+        fence_async_smem();
+        tc_fence_before();                                       // the last step's loads from tensor memory
+        ok = __syncthreads_and(ok);
+        if (!ok) break;
+        auto issue = [&](const uint8_t *v, uint32_t first) {
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < kQ / 16; ++kk)                 // where NT is 64, rows 64 ... 127 are the first 64 again: products of no use
+                umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 0 : kSlab, 1024),
+                     smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : first);
+        };
+        if (warp == 0 && elect_one()) {
+            if (a.tiles) tma_store2(&tmTiles, smS, 0, (((c0 + place(i)) * a.h.H + h) * a.h.PB + pb) * NT);
+            issue(smV, 0u);
+            if (a.tiles) tma_store_read();                       // so whoever has waited for the MMAs may write S's tile again
+            umma_commit(&done[uses & 1]);
+        }
+        ++uses;
         if (a.exact) {
+            uint8_t *second = a.tiles ? smV : smS;               // with a tile under way, one buffer for the parts
 #pragma unroll
             for (int part = 1; part < 3; ++part) {
-                if (ok) weigh(part);
+                uint8_t *to = part == 1 ? second : smV;
+                if (ok && (part == 2 || to == smV)) ok = wait(part == 2 && to != second ? uses - 2 : uses - 1);
+                if (ok) weigh(part, to);
+                fence_async_smem();
                 ok = __syncthreads_and(ok);
-                if (ok && warp == 0 && elect_one()) issue(1u);
-                if (ok) ok = mbar_wait(&done, waits & 1);
-                ++waits;
+                if (ok && warp == 0 && elect_one()) {
+                    issue(to, 1u);
+                    umma_commit(&done[uses & 1]);
+                }
+                ++uses;
             }
         }
+        if (ok && i + 1 < nc) fetch(i + 1, rows);
+        if (ok && a.exact) ok = wait(uses - 2);                  // phases are waited for one by one
+        if (ok) ok = wait(uses - 1);
         if (!ok) continue;                                       // leaves at the next barrier
         tc_fence_after();
-        const float d = exp2f(whole[i % 3]);
-        total += whole[i % 3];
+        const float d = exp2f(whole[i % kAhead]);
+        total += whole[i % kAhead];
         float v32[32];
         tmem_ld32(tmem_lane_base(tmem) + half * 32, v32);
 #pragma unroll
@@ -272,6 +299,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     tc_fence_before();
     __syncthreads();
     if (warp == 0) {
+        if (a.tiles && elect_one()) tma_store_wait();
         if (!ok && elect_one()) {                                // leave nothing in flight
             drain_mmas(&unused);
             drain_loads(full, 2, loads);
@@ -496,6 +524,387 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         __syncwarp();
         tmem_dealloc(tmem, 256);
     }
+}
+
+// ---- the gradients ------------------------------------------------------------------------------------------------------
+// All chunks at once, given what enters each from the left (S) and from the right (G, the gradient of the state behind the chunk).
+// With w_ts = scale e^{c_t - c_s} for s <= t, p = w (q.k) and d = w (do.v):
+//     dv_s = sum_t p_ts do_t + e^{c_end - c_s} G^T k_s        dk_s = sum_t d_ts q_t + G (e^{c_end - c_s} v_s)
+//     dq_t = sum_s d_ts k_s + S (scale e^{c_t} do_t)
+//     dg_t = e^{c_end} S.G  +  sum_{t' >= t} scale e^{c_t'} do_t'.S^T q_t'  +  sum_{s < t} e^{c_end - c_s} v_s.G^T k_s  +  sum_{s < t <= t'} d_t's q_t'.k_s
+// - every pair of places before and from t on: past and future of the chunk, past and its tokens, its tokens and the future, tokens
+// among themselves; the last as sums over rows less sums over columns of the same fp32 products, so that what cancels does so
+// exactly.  Everything is laid out with s along the rows (lanes): p and d then are operands of dv and dk as they lie, and d of dq
+// read the other way.  A block has a chunk and a head of q and k, and walks (its part of) the heads of v that share them, dq and dk
+// adding up in tensor memory; twelve of its sixteen warps have weights to make, four lie above the diagonal.
+struct GradsParams {
+    Heads h;
+    Plan chunk;
+    int vpc, parts;                                              // tiles of v a block (whole heads), blocks a (chunk, head of q)
+    bf16 *dq, *dk, *dv;                                          // contiguous
+    float *part;                                                 // parts > 1: (2, parts, tokens, hk, N), dq and dk
+    long long tokens;
+    void *dg;                                                    // (tokens, H), or NULL
+    int dg_dtype;
+    int *status;
+};
+inline size_t grads_smem(int NT) { return 1024 + 2 * (size_t)(NT / 64) * kSlab + 3 * (size_t)kSlab + 2 * (size_t)NT * 128 + 4 * (size_t)kSlab; }
+
+template <int NT> __global__ void __launch_bounds__(512, 1)
+decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+            const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmG) {
+    pdl_begin();
+    constexpr int kSlabs = NT / 64, kT = 512;
+    extern __shared__ uint8_t dyn[];
+    __shared__ uint64_t bar_qk, bar_v, done, unused;
+    __shared__ uint32_t tmem_slot;
+    __shared__ __align__(16) float c[kQ], ws[kQ], et[kQ];        // c_t; e^{c_end - c_s}; scale e^{c_t}
+    __shared__ __align__(16) float above[64], beside[64];        // weights below the diagonal blocks: e^{c_63 - c_s}, scale e^{c_t - c_63}
+    __shared__ float rowsum[4][kQ], colsum[4][kQ], past[4][kQ], future[4][kQ], cross[16];
+    uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + kSlabs * kSlab, *smD = smV + kSlab, *smE = smD + kSlab,
+            *smP = smE + kSlab, *smN = smP + 2 * kSlab, *smS = smN + 2 * kSlab, *smG = smS + NT * 128;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int part = blockIdx.x % a.parts, m = blockIdx.x / a.parts % a.h.hk, ci = blockIdx.x / (a.parts * a.h.hk);
+    const Segment sg = uni::segment(a.chunk, ci);
+    if (sg.len == 0) return;
+    const int len = sg.len, R = a.h.H / a.h.hk, v0 = part * a.vpc, nv = min(a.vpc, R * a.h.PB - v0);
+    auto head = [&](int i) { return m * R + (v0 + i) / a.h.PB; };
+    auto load_v = [&](int i) {
+        const int h = head(i), pb = (v0 + i) % a.h.PB, row = ((ci * a.h.H + h) * a.h.PB + pb) * NT;
+        mbar_expect_tx(&bar_v, 2 * kSlab + 2 * NT * 128);
+        tma_load4(smV, &tmV, pb * kP, h, sg.t0, sg.batch, &bar_v);
+        tma_load4(smD, &tmD, pb * kP, h, sg.t0, sg.batch, &bar_v);
+        tma_load2(smS, &tmS, 0, row, &bar_v);
+        tma_load2(smG, &tmG, 0, row, &bar_v);
+    };
+    Decays next;                                                 // warp 0: of the head to come
+    float whole = 0.f;                                           // warp 0: c_end
+    auto table = [&]() {                                         // one warp
+        float p[4], q[4];
+        next.log2(a.h);
+        next.prefix(p, lane);
+        next.suffix(q, lane);
+        const float corner = __shfl_sync(0xffffffffu, p[3], 15);
+        whole = __shfl_sync(0xffffffffu, p[3], 31);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int t = lane * 4 + k;
+            c[t] = p[k];
+            et[t] = exp2f(p[k] + a.h.log_scale);
+            ws[t] = exp2f(q[k]);
+            if (lane < 16) above[t] = exp2f(corner - p[k]);
+            else beside[t - 64] = exp2f(p[k] - corner + a.h.log_scale);
+        }
+    };
+    if (warp == 0) tmem_alloc(&tmem_slot, 512);
+    if (tid == 32) {
+        mbar_init(&bar_qk, 1);
+        mbar_init(&bar_v, 1);
+        mbar_init(&done, 1);
+        fence_mbar_init();
+        mbar_expect_tx(&bar_qk, 2 * kSlabs * kSlab);
+        for (int j = 0; j < kSlabs; ++j) {
+            tma_load4(smQ + j * kSlab, &tmQ, j * 64, m, sg.t0, sg.batch, &bar_qk);
+            tma_load4(smK + j * kSlab, &tmK, j * 64, m, sg.t0, sg.batch, &bar_qk);
+        }
+        load_v(0);
+    }
+    if (warp == 0) next.load(a.h, sg.batch, sg.t0, len, head(0), lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot, tl = tmem_lane_base(tmem);
+    constexpr uint32_t cQ = 256, cK = 256 + NT;                  // columns of dq and dk; 0: q.k, then dv; 128: do.v, then S^T q
+    int loads = 1, waits = 0;
+    bool ok = mbar_wait(&bar_qk, 0);
+    const int quad = warp & 3, cg = warp >> 2, s = quad * 32 + lane;   // this thread: row s; columns t of 32 cg ...; 16 of dv's 64
+    const bool diagonal = (quad >> 1) == (cg >> 1), empty = (quad >> 1) > (cg >> 1);
+    if (ok && a.chunk.packed && len < kQ)
+        for (int j = 0; j < kSlabs; ++j) {
+            clear_rows(smQ + j * kSlab, len, tid, kT);
+            clear_rows(smK + j * kSlab, len, tid, kT);
+        }
+    float through = 0.f;                                         // this thread's part of S.G
+    for (int i = 0; i < nv; ++i) {
+        const bool first = (v0 + i) % a.h.PB == 0, last = (v0 + i) % a.h.PB == a.h.PB - 1 || i + 1 == nv;   // tiles of a head
+        if (warp == 0 && first) {
+            table();
+            if (i + a.h.PB < nv) next.load(a.h, sg.batch, sg.t0, len, head(i + a.h.PB), lane);
+        }
+        ok = ok && mbar_wait(&bar_v, i & 1);
+        if (ok && a.chunk.packed && len < kQ) {
+            clear_rows(smV, len, tid, kT);
+            clear_rows(smD, len, tid, kT);
+        }
+        fence_async_smem();
+        tc_fence_before();
+        ok = __syncthreads_and(ok);
+        if (!ok) break;
+        if (warp == 0 && elect_one()) {                          // q.k and do.v of all pairs, rows s
+            tc_fence_after();
+            constexpr uint32_t idesc = instr_desc(1, false, false, kQ);
+#pragma unroll
+            for (int kk = 0; kk < NT / 16; ++kk)
+                umma(tmem, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
+                     smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+                umma(tmem + 128, smem_desc(smem_u32(smV) + kk * 32, 16, 1024), smem_desc(smem_u32(smD) + kk * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+            umma_commit(&done);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {                            // scale e^{c_t} do_t beside do_t
+            const int x = tid + k * kT, row = x >> 3;
+            float e[8];
+            unpack8<bf16>(*reinterpret_cast<const uint4 *>(smD + x * 16), e);
+            const float f = et[row];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] *= f;
+            *reinterpret_cast<uint4 *>(smE + x * 16) = pack8<bf16>(e);
+        }
+        if (first) through = 0.f;
+        for (int x = tid; x < NT * 8; x += kT) {
+            float e[8], f[8];
+            unpack8<bf16>(*reinterpret_cast<const uint4 *>(smS + x * 16), e);
+            unpack8<bf16>(*reinterpret_cast<const uint4 *>(smG + x * 16), f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) through = fmaf(e[j], f[j], through);
+        }
+        ok = mbar_wait(&done, waits & 1);
+        ++waits;
+        tc_fence_after();
+        if (ok) {
+            // rows of 64 t, 16-byte pieces swizzled
+            uint8_t *prow = smP + (cg >> 1) * kSlab + s * 128, *drow = smN + (cg >> 1) * kSlab + s * 128;
+            float x[32], y[32], of_row = 0.f, of_column = 0.f;   // for dg: d (q.k) over this row, over column 32 cg + lane
+            if (!empty) {
+                tmem_ld32(tl + cg * 32, x);
+                tmem_ld32(tl + 128 + cg * 32, y);
+                const float cs = c[s] - a.h.log_scale, fs = above[s & 63];
+#pragma unroll
+                for (int j0 = 0; j0 < 32; j0 += 8) {
+                    float p[8], d[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int t = cg * 32 + j0 + j;
+                        const float w = diagonal ? (t >= s ? ex2_approx(c[t] - cs) : 0.f) : fs * beside[t & 63];
+                        p[j] = w * x[j0 + j];
+                        d[j] = w * y[j0 + j];
+                        x[j0 + j] = t > s ? d[j] * x[j0 + j] : 0.f;   // a token's own pair flows nowhere
+                        of_row += x[j0 + j];
+                    }
+                    const int piece = ((cg & 1) * 4 + j0 / 8) ^ (s & 7);
+                    *reinterpret_cast<uint4 *>(prow + (piece << 4)) = pack8<bf16>(p);
+                    *reinterpret_cast<uint4 *>(drow + (piece << 4)) = pack8<bf16>(d);
+                }
+                auto value = [&](auto k) { return x[decltype(k)::value]; };
+                of_column = warp_sums<32>(value, lane);
+            } else if (i == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int piece = ((cg & 1) * 4 + j) ^ (s & 7);
+                    *reinterpret_cast<uint4 *>(prow + (piece << 4)) = zero8();
+                    *reinterpret_cast<uint4 *>(drow + (piece << 4)) = zero8();
+                }
+            }
+            rowsum[cg][s] = of_row + (first ? 0.f : rowsum[cg][s]);
+            colsum[quad][cg * 32 + lane] = of_column + (first ? 0.f : colsum[quad][cg * 32 + lane]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {                        // e^{c_end - c_s} v_s in v_s' place
+                const int q = tid + k * kT;
+                uint4 *v = reinterpret_cast<uint4 *>(smV + q * 16);
+                float e[8];
+                unpack8<bf16>(*v, e);
+                const float f = ws[q >> 3];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] *= f;
+                *v = pack8<bf16>(e);
+            }
+            fence_async_smem();
+        }
+        tc_fence_before();
+        ok = __syncthreads_and(ok);
+        if (!ok) break;
+        if (warp == 0 && elect_one()) {
+            tc_fence_after();
+            constexpr uint32_t narrow = instr_desc(1, false, true, kP), wide = instr_desc(1, false, false, NT);
+            const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), p0 = smem_u32(smP), n0 = smem_u32(smN);
+            const uint32_t v_ = smem_u32(smV), d_ = smem_u32(smD), e_ = smem_u32(smE), s_ = smem_u32(smS), g_ = smem_u32(smG);
+#pragma unroll
+            for (int kk = 0; kk < kQ / 16; ++kk)                 // dv from the chunk, from the future; S^T q
+                umma(tmem, smem_desc(p0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(d_ + kk * 2048, kSlab, 1024), narrow, kk > 0 ? 1u : 0u);
+#pragma unroll
+            for (int kk = 0; kk < NT / 16; ++kk)
+                umma(tmem + 64, smem_desc(k0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(g_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
+#pragma unroll
+            for (int kk = 0; kk < NT / 16; ++kk)
+                umma(tmem + 128, smem_desc(q0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(s_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
+#pragma unroll
+            for (int kk = 0; kk < kQ / 16; ++kk) {               // dq and dk from the chunk
+                umma(tmem + cQ, smem_desc(n0 + kk * 2048, kSlab, 1024), smem_desc(k0 + kk * 2048, kSlab, 1024), instr_desc(1, true, true, NT),
+                     i > 0 || kk > 0 ? 1u : 0u);
+                umma(tmem + cK, smem_desc(n0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(q0 + kk * 2048, kSlab, 1024),
+                     instr_desc(1, false, true, NT), i > 0 || kk > 0 ? 1u : 0u);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {                     // dq from the past, dk from the future
+                umma(tmem + cQ, smem_desc(e_ + kk * 32, 16, 1024), smem_desc(s_ + kk * 32, 16, 1024), wide, 1u);
+                umma(tmem + cK, smem_desc(v_ + kk * 32, 16, 1024), smem_desc(g_ + kk * 32, 16, 1024), wide, 1u);
+            }
+            umma_commit(&done);
+        }
+        if (last) {
+            float v = through;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == 0) cross[warp] = v;
+        }
+        ok = mbar_wait(&done, waits & 1);
+        ++waits;
+        tc_fence_after();
+        if (ok) {                                                // row s (or t), columns 16 cg ... of v's 64
+            float own[16], far[16], o[16], e[8], f = 0.f, p = 0.f;
+            tmem_ld16(tl + cg * 16, own);
+            tmem_ld16(tl + 64 + cg * 16, far);
+            tmem_ld16(tl + 128 + cg * 16, o);
+            const float w = ws[s];
+#pragma unroll
+            for (int j = 0; j < 16; j += 8) {
+                const int piece = ((cg * 2 + j / 8) ^ (s & 7)) << 4;
+                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smV + s * 128 + piece), e);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f = fmaf(e[k], far[j + k], f);
+                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smE + s * 128 + piece), e);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) p = fmaf(e[k], o[j + k], p);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[k] = fmaf(w, far[j + k], own[j + k]);
+                *reinterpret_cast<uint4 *>(smP + kSlab + s * 128 + piece) = pack8<bf16>(e);   // every row there is written anew
+            }
+            future[cg][s] = f + (first ? 0.f : future[cg][s]);
+            past[cg][s] = p + (first ? 0.f : past[cg][s]);
+        }
+        tc_fence_before();
+        ok = __syncthreads_and(ok);
+        if (!ok) break;
+        if (i + 1 < nv) {
+            if (tid == 32) load_v(i + 1);
+            ++loads;
+        }
+        const int h = head(i), col = (v0 + i) % a.h.PB * kP + (tid & 7) * 8;
+        const long long token = (long long)sg.batch * a.chunk.L + sg.t0;
+        if (col < a.h.P) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = (tid >> 3) + k * 64;
+                if (r < len)
+                    *reinterpret_cast<uint4 *>(a.dv + ((token + r) * a.h.H + h) * a.h.P + col) =
+                        *reinterpret_cast<const uint4 *>(smP + kSlab + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
+            }
+        }
+        if (last && warp == 0 && a.dg) {
+            float all = lane < 16 ? cross[lane] : 0.f, x[4], b[4];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            all *= exp2f(whole);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = lane * 4 + k;
+                x[k] = b[k] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[k] += past[j][t] + (colsum[j][t] - rowsum[j][t]);
+                    b[k] += future[j][t];
+                }
+            }
+            // sums of x from each token on, of b before each
+            float xs = x[0] + x[1] + x[2] + x[3], bs = b[0] + b[1] + b[2] + b[3];
+            const float own_b = bs;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float u = __shfl_down_sync(0xffffffffu, xs, o), v = __shfl_up_sync(0xffffffffu, bs, o);
+                if (lane + o < 32) xs += u;
+                if (lane >= o) bs += v;
+            }
+            bs -= own_b;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = lane * 4 + k;
+                if (t < len) st_any(a.dg, a.dg_dtype, (token + t) * a.h.H + h, all + xs + bs);
+                xs -= x[k];
+                bs += b[k];
+            }
+        }
+    }
+    ok = __syncthreads_and(ok);
+    if (ok) {                                                    // dq and dk: rows s (or t), NT / 4 columns a thread
+        constexpr int kCols = NT / 4;
+        const long long token = (long long)sg.batch * a.chunk.L + sg.t0;
+#pragma unroll
+        for (int what = 0; what < 2; ++what) {
+            const uint32_t at = tl + (what ? cK : cQ) + cg * kCols;
+            uint8_t *to = what ? smN : smP;
+#pragma unroll
+            for (int j0 = 0; j0 < kCols; j0 += 16) {
+                float x[16];
+                tmem_ld16(at + j0, x);
+                const int n = cg * kCols + j0;
+                if (a.parts > 1) {
+                    float *o = a.part + (((long long)(what * a.parts + part) * a.tokens + token + s) * a.h.hk + m) * a.h.N + n;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                        if (s < len && n + j < a.h.N) *reinterpret_cast<float4 *>(o + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 8) {
+                        const float e[8] = {x[j], x[j + 1], x[j + 2], x[j + 3], x[j + 4], x[j + 5], x[j + 6], x[j + 7]};
+                        *reinterpret_cast<uint4 *>(to + (n + j) / 64 * kSlab + s * 128 + ((((n + j) % 64 / 8) ^ (s & 7)) << 4)) = pack8<bf16>(e);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (a.parts == 1) {
+            const int pieces = a.h.N / 8;
+            for (int x = tid; x < 2 * kQ * (NT / 8); x += kT) {
+                const int what = x / (kQ * (NT / 8)), r = x / (NT / 8) % kQ, j = x % (NT / 8);
+                if (r < len && j < pieces)
+                    *reinterpret_cast<uint4 *>((what ? a.dk : a.dq) + ((token + r) * a.h.hk + m) * a.h.N + j * 8) =
+                        *reinterpret_cast<const uint4 *>((what ? smN : smP) + j / 8 * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4));
+            }
+        }
+    } else if (tid == 0) {
+        atomicExch(a.status, kErrDecay + 3);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        if (!ok && elect_one()) {                                // leave nothing in flight
+            drain_mmas(&unused);
+            drain_loads(&bar_qk, 1, 1);
+            drain_loads(&bar_v, 1, loads);
+        }
+        __syncwarp();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// dq and dk of chunks whose heads were walked by several blocks: their parts added up in order.
+__global__ void __launch_bounds__(256) decay_sum_parts(const float *part, int parts, long long each, bf16 *dq, bf16 *dk) {
+    pdl_begin();
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= 2 * each) return;
+    const int what = i >= each;
+    const float *p = part + what * parts * each + (i - what * each);
+    float4 v = *reinterpret_cast<const float4 *>(p);
+    for (int k = 1; k < parts; ++k) {
+        const float4 u = *reinterpret_cast<const float4 *>(p + k * each);
+        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+    }
+    uint2 o;
+    o.x = pack2<bf16>(v.x, v.y);
+    o.y = pack2<bf16>(v.z, v.w);
+    *reinterpret_cast<uint2 *>((what ? dk : dq) + (i - what * each)) = o;
 }
 
 }  // namespace unitc
