@@ -1,0 +1,151 @@
+// C ABI of the norms before and after a block, with its gate and residual scale.
+#include <algorithm>
+
+#include "block_norm.cuh"
+#include "common.cuh"
+#include "host.cuh"
+
+using namespace bissd;
+
+static bool dtype_ok(int t) { return t >= BISSD_F32 && t <= BISSD_F16; }
+static bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+static int block_norm_sizes(const bissd_block_norm_args *a) {
+    if (!a) return BISSD_ERR_NULL;
+    if (a->rows <= 0 || a->width <= 0 || a->width > bnorm::kMaxWidth || a->gate_rows < 0 || (a->gate_rows > 0 && a->rows % a->gate_rows))
+        return BISSD_ERR_SHAPE;
+    if (!dtype_ok(a->dtype) || (a->r_dtype != a->dtype && a->r_dtype != BISSD_F32) || (a->w_dtype != a->dtype && a->w_dtype != BISSD_F32))
+        return BISSD_ERR_DTYPE;
+    if (a->gate_act < BISSD_GATE_NONE || a->gate_act > BISSD_GATE_SILU) return BISSD_ERR_SHAPE;
+    return BISSD_OK;
+}
+static int block_norm_check(const bissd_block_norm_args *a, bool backward) {
+    if (!a || !a->x || !a->residual) return BISSD_ERR_NULL;
+    if (!backward && (!a->r || (a->pre_weight && !a->normed))) return BISSD_ERR_NULL;
+    if (backward && !a->rstd && (a->post_weight || a->dnormed)) return BISSD_ERR_NULL;
+    if (backward && a->dnormed && !a->pre_weight) return BISSD_ERR_NULL;
+    return block_norm_sizes(a);
+}
+// Rows side by side in a block: up to 256 threads.
+static int block_norm_threads(const bnorm::Params &p) { return p.threads_row * std::max(1, 256 / p.threads_row); }
+// 16-byte pieces: every row starts at a multiple of 16 bytes
+static bool block_norm_vec(const bissd_block_norm_args *a) {
+    bool ok = a->width % 8 == 0;
+    for (const void *p : {a->x, a->residual, a->gate, (const void *)a->r, (const void *)a->normed, a->dr, a->dnormed, (const void *)a->dx,
+                          (const void *)a->dresidual, (const void *)a->dgate})
+        ok = ok && aligned16(p);
+    for (const int64_t s : {a->stride_x, a->stride_residual, a->stride_gate, a->stride_dr, a->stride_dnormed}) ok = ok && s % 8 == 0;
+    return ok;
+}
+static long long block_norm_entries(const bnorm::Params &p) { return p.gate && p.gate_rows > 0 ? p.rows / p.gate_rows : 1; }
+static bnorm::Params block_norm_params(const bissd_block_norm_args *a) {
+    bnorm::Params p{};
+    p.rows = a->rows;
+    p.gate_rows = a->gate_rows == 1 ? 0 : a->gate_rows;          // a gate row for each row
+    p.D = a->width;
+    p.threads_row = ceil_div(ceil_div(a->width, bnorm::kCh), 32) * 32;
+    p.w_dtype = a->w_dtype; p.act = a->gate_act;
+    p.scale = a->scale; p.eps = a->eps;
+    p.sx = a->stride_x; p.sres = a->stride_residual; p.sgate = a->stride_gate; p.sdr = a->stride_dr; p.sdu = a->stride_dnormed;
+    p.x = a->x; p.res = a->residual; p.gate = a->gate; p.scale_v = a->scale_vector; p.w2 = a->post_weight; p.w1 = a->pre_weight;
+    p.r = a->r; p.u = a->pre_weight ? a->normed : nullptr; p.rstd = a->rstd;
+    p.dr = a->dr; p.du = a->dnormed; p.dx = a->dx; p.dres = a->dresidual; p.dgate = a->gate ? a->dgate : nullptr;
+    return p;
+}
+// Blocks to an entry: `resident` of them an SM, shared by the entries, and no more than there are rows.
+static int block_norm_blocks(const bnorm::Params &p, int resident) {
+    const long long entries = block_norm_entries(p), per = block_norm_threads(p) / p.threads_row;
+    const long long want = std::max<long long>(1, 148LL * resident / entries);
+    return (int)std::min<long long>(want, (p.rows / entries + per - 1) / per);
+}
+constexpr int kFwd = 3, kBwd = 2;                                // blocks of 256 threads an SM: what the registers allow
+static int block_norm_resident(const bnorm::Params &p, int of_256) { return std::max(1, 256 * of_256 / block_norm_threads(p)); }
+
+// Rows that a thread copies ahead: four, as long as the blocks of an SM have the shared memory.
+static int block_norm_depth(int pieces, int threads, int blocks) {
+    const int room = 216 * 1024 / blocks;
+    return std::max(1, std::min(4, room / (pieces * 16 * threads)));
+}
+template <class T, class R> static int block_norm_forward_impl(const bissd_block_norm_args *a, cudaStream_t s) {
+    bnorm::Params p = block_norm_params(a);
+    const int threads = block_norm_threads(p);
+    const bool vec = block_norm_vec(a);
+    p.blocks = block_norm_blocks(p, block_norm_resident(p, kFwd));
+    const long long grid = block_norm_entries(p) * p.blocks;
+    if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    const int pieces = (int)(sizeof(T) * (a->gate && p.gate_rows == 0 ? 2 : 1) + sizeof(R)) / 2;
+    p.depth = block_norm_depth(pieces, threads, block_norm_resident(p, kFwd));
+    const size_t smem = vec ? (size_t)p.depth * pieces * 16 * threads : 0;
+    const auto kernel = !vec            ? bnorm::block_norm_fwd<T, R, false, 1024, 1>
+                        : threads > 512 ? bnorm::block_norm_fwd<T, R, true, 1024, 1>
+                        : threads > 256 ? bnorm::block_norm_fwd<T, R, true, 512, 1>
+                                        : bnorm::block_norm_fwd<T, R, true, 256, kFwd>;
+    BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
+    BISSD_LAUNCH("block_norm_fwd", launch_pdl(kernel, (int)grid, threads, smem, s, p));
+    return BISSD_OK;
+}
+template <class T, class R> static int block_norm_backward_impl(const bissd_block_norm_args *a, float *part, cudaStream_t s) {
+    bnorm::Params p = block_norm_params(a);
+    const int threads = block_norm_threads(p), per = threads / p.threads_row;
+    const bool vec = block_norm_vec(a);
+    const long long entries = block_norm_entries(p);
+    p.blocks = block_norm_blocks(p, block_norm_resident(p, kBwd));
+    if (entries * p.blocks > 0x7fffffffLL || (entries + 3) * ceil_div(p.D, 32) > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    p.part = part;
+    const int pieces = (int)(sizeof(T) * (1 + (a->gate && p.gate_rows == 0) + (a->dnormed != nullptr)) + sizeof(R) * (1 + (a->dr != nullptr))) / 2;
+    p.depth = block_norm_depth(pieces, threads, block_norm_resident(p, kBwd));
+    const size_t rows = (size_t)(per - 1) * p.threads_row * bnorm::kCh * sizeof(float);
+    const size_t smem = std::max(rows, vec ? (size_t)p.depth * pieces * 16 * threads : 0);
+    const auto kernel = !vec            ? bnorm::block_norm_bwd<T, R, false, 1024, 1>
+                        : threads > 512 ? bnorm::block_norm_bwd<T, R, true, 1024, 1>
+                        : threads > 256 ? bnorm::block_norm_bwd<T, R, true, 512, 1>
+                                        : bnorm::block_norm_bwd<T, R, true, 256, kBwd>;
+    BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
+    BISSD_LAUNCH("block_norm_bwd", launch_pdl(kernel, (int)(entries * p.blocks), threads, smem, s, p));
+    bnorm::SumParams q{};
+    q.part = part; q.D = p.D; q.blocks = p.blocks; q.entries = (int)entries; q.w_dtype = p.w_dtype; q.g_dtype = a->dtype;
+    q.dpre = a->dnormed ? a->dpre : nullptr; q.dpost = a->post_weight ? a->dpost : nullptr;
+    q.dscale = a->scale_vector ? a->dscale : nullptr; q.dgate = p.gate_rows > 0 ? p.dgate : nullptr;
+    if (q.dpre || q.dpost || q.dscale || q.dgate)
+        BISSD_LAUNCH("block_norm_sums", launch_pdl(bnorm::block_norm_sums, (int)((3 + (q.dgate ? entries : 0)) * ceil_div(p.D, 32)),
+                                                   dim3(32, 8), 0, s, q));
+    return BISSD_OK;
+}
+template <class F> static int by_types(const bissd_block_norm_args *a, F f) {
+    if (a->dtype == BISSD_F32) return f(float(), float());
+    if (a->dtype == BISSD_BF16) return a->r_dtype == BISSD_F32 ? f(__nv_bfloat16(), float()) : f(__nv_bfloat16(), __nv_bfloat16());
+    return a->r_dtype == BISSD_F32 ? f(__half(), float()) : f(__half(), __half());
+}
+
+extern "C" {
+
+int bissd_block_norm_workspace_bytes(const bissd_block_norm_args *a, size_t *bwd_bytes) {
+    const int rc = block_norm_sizes(a);
+    if (rc != BISSD_OK) return rc;
+    const bnorm::Params p = block_norm_params(a);
+    if (bwd_bytes) *bwd_bytes = align256((size_t)block_norm_entries(p) * block_norm_blocks(p, block_norm_resident(p, kBwd)) * 4 * p.D * sizeof(float));
+    return BISSD_OK;
+}
+
+int bissd_block_norm_forward(const bissd_block_norm_args *a, void *stream) {
+    int rc = block_norm_check(a, false);
+    if (rc == BISSD_OK) rc = check_device();
+    if (rc != BISSD_OK) return rc;
+    return by_types(a, [&](auto t, auto r) { return block_norm_forward_impl<decltype(t), decltype(r)>(a, static_cast<cudaStream_t>(stream)); });
+}
+
+int bissd_block_norm_backward(const bissd_block_norm_args *a, void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = block_norm_check(a, true);
+    size_t need = 0;
+    if (rc == BISSD_OK) rc = bissd_block_norm_workspace_bytes(a, &need);
+    if (rc != BISSD_OK) return rc;
+    if (!workspace || workspace_bytes < need) return BISSD_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) return BISSD_ERR_ALIGN;
+    rc = check_device();
+    if (rc != BISSD_OK) return rc;
+    return by_types(a, [&](auto t, auto r) {
+        return block_norm_backward_impl<decltype(t), decltype(r)>(a, static_cast<float *>(workspace), static_cast<cudaStream_t>(stream));
+    });
+}
+
+}  // extern "C"

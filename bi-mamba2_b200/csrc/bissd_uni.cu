@@ -1,9 +1,7 @@
-// C ABI of what a decoder built from this library's layers needs: causal linear attention with a decay for each head, its
-// single-token form, and the norms around a residual block.
+// C ABI of the causal linear attention with a decay for each head and of its single-token form.
 #include <algorithm>
 #include <cmath>
 
-#include "block_norm.cuh"
 #include "common.cuh"
 #include "host.cuh"
 #include "uni_plan.cuh"
@@ -53,86 +51,6 @@ static int step_launch(const bissd_decay_step_args *a, cudaStream_t s) {
         BISSD_LAUNCH("decay_step", launch_pdl(kernel, grid, uni::kStepThreads, 0, s, p));
         return BISSD_OK;
     });
-}
-
-// ---- the norms around a block --------------------------------------------------------------------------------------
-static int block_norm_check(const bissd_block_norm_args *a, bool backward) {
-    if (!a || !a->x || !a->residual) return BISSD_ERR_NULL;
-    if (!backward && (!a->r || (a->pre_weight && !a->normed))) return BISSD_ERR_NULL;
-    if (backward && !a->rstd && (a->post_weight || a->dnormed)) return BISSD_ERR_NULL;
-    if (backward && a->dnormed && !a->pre_weight) return BISSD_ERR_NULL;
-    if (a->rows <= 0 || a->width <= 0 || a->width > bnorm::kMaxWidth || a->gate_rows < 0 || (a->gate_rows > 0 && a->rows % a->gate_rows))
-        return BISSD_ERR_SHAPE;
-    if (!dtype_ok(a->dtype) || (a->r_dtype != a->dtype && a->r_dtype != BISSD_F32) || (a->w_dtype != a->dtype && a->w_dtype != BISSD_F32))
-        return BISSD_ERR_DTYPE;
-    if (a->gate_act < BISSD_GATE_NONE || a->gate_act > BISSD_GATE_SILU) return BISSD_ERR_SHAPE;
-    return BISSD_OK;
-}
-static bnorm::Params block_norm_params(const bissd_block_norm_args *a) {
-    bnorm::Params p{};
-    p.rows = a->rows;
-    p.gate_rows = a->gate_rows == 1 ? 0 : a->gate_rows;          // a gate row for each row
-    p.D = a->width;
-    p.threads_row = ceil_div(ceil_div(a->width, bnorm::kCh), 32) * 32;
-    p.w_dtype = a->w_dtype; p.act = a->gate_act;
-    p.scale = a->scale; p.eps = a->eps;
-    p.sx = a->stride_x; p.sres = a->stride_residual; p.sgate = a->stride_gate; p.sdr = a->stride_dr; p.sdu = a->stride_dnormed;
-    p.x = a->x; p.res = a->residual; p.gate = a->gate; p.scale_v = a->scale_vector; p.w2 = a->post_weight; p.w1 = a->pre_weight;
-    p.r = a->r; p.u = a->pre_weight ? a->normed : nullptr; p.rstd = a->rstd;
-    p.dr = a->dr; p.du = a->dnormed; p.dx = a->dx; p.dres = a->dresidual; p.dgate = a->gate ? a->dgate : nullptr;
-    return p;
-}
-// 16-byte pieces: every row starts at a multiple of 16 bytes
-static bool block_norm_vec(const bissd_block_norm_args *a) {
-    bool ok = a->width % 8 == 0;
-    for (const void *p : {a->x, a->residual, a->gate, (const void *)a->r, (const void *)a->normed, a->dr, a->dnormed, (const void *)a->dx,
-                          (const void *)a->dresidual, (const void *)a->dgate})
-        ok = ok && aligned16(p);
-    for (const int64_t s : {a->stride_x, a->stride_residual, a->stride_gate, a->stride_dr, a->stride_dnormed}) ok = ok && s % 8 == 0;
-    return ok;
-}
-// Rows side by side in a block: up to 256 threads.
-static int block_norm_threads(const bnorm::Params &p) { return p.threads_row * std::max(1, 256 / p.threads_row); }
-// Blocks of the backward pass to an entry (rows that share a gate row whose gradient is wanted; else all rows): as many as are
-// resident at two blocks of 256 threads an SM, shared by the entries, and no more than there are rows.
-static void block_norm_split(const bnorm::Params &p, long long *entries, int *blocks) {
-    *entries = p.gate_rows > 0 && p.dgate ? p.rows / p.gate_rows : 1;
-    const long long rows = p.rows / *entries, per = block_norm_threads(p) / p.threads_row;
-    const long long want = std::max<long long>(1, 148LL * std::max(1, 512 / block_norm_threads(p)) / *entries);
-    *blocks = (int)std::min<long long>(want, (rows + per - 1) / per);
-}
-
-template <class T, class R> static int block_norm_forward_impl(const bissd_block_norm_args *a, cudaStream_t s) {
-    const bnorm::Params p = block_norm_params(a);
-    const int threads = block_norm_threads(p), per = threads / p.threads_row;
-    const bool vec = block_norm_vec(a), big = threads > 512;
-    const auto kernel = big ? (vec ? bnorm::block_norm_fwd<T, R, true, 1024> : bnorm::block_norm_fwd<T, R, false, 1024>)
-                            : (vec ? bnorm::block_norm_fwd<T, R, true, 512> : bnorm::block_norm_fwd<T, R, false, 512>);
-    const long long rows = (a->rows + per - 1) / per;
-    const int grid = (int)std::min<long long>(rows, (long long)sm_count() * resident_blocks(kernel, threads, 0));
-    BISSD_LAUNCH("block_norm_fwd", launch_pdl(kernel, grid, threads, 0, s, p));
-    return BISSD_OK;
-}
-template <class T, class R> static int block_norm_backward_impl(const bissd_block_norm_args *a, float *part, cudaStream_t s) {
-    bnorm::Params p = block_norm_params(a);
-    const int threads = block_norm_threads(p), per = threads / p.threads_row;
-    const bool vec = block_norm_vec(a), big = threads > 512;
-    long long entries;
-    block_norm_split(p, &entries, &p.blocks);
-    if (entries * p.blocks > 0x7fffffffLL || (entries + 3) * ceil_div(p.D, 32) > 0x7fffffffLL) return BISSD_ERR_SHAPE;
-    p.part = part;
-    const auto kernel = big ? (vec ? bnorm::block_norm_bwd<T, R, true, 1024> : bnorm::block_norm_bwd<T, R, false, 1024>)
-                            : (vec ? bnorm::block_norm_bwd<T, R, true, 512> : bnorm::block_norm_bwd<T, R, false, 512>);
-    const size_t smem = (size_t)(per - 1) * p.threads_row * bnorm::kCh * sizeof(float);
-    BISSD_LAUNCH("block_norm_bwd", launch_pdl(kernel, (int)(entries * p.blocks), threads, smem, s, p));
-    bnorm::SumParams q{};
-    q.part = part; q.D = p.D; q.blocks = p.blocks; q.entries = (int)entries; q.w_dtype = p.w_dtype; q.g_dtype = a->dtype;
-    q.dpre = a->dnormed ? a->dpre : nullptr; q.dpost = a->post_weight ? a->dpost : nullptr;
-    q.dscale = a->scale_vector ? a->dscale : nullptr; q.dgate = p.gate_rows > 0 ? p.dgate : nullptr;
-    if (q.dpre || q.dpost || q.dscale || q.dgate)
-        BISSD_LAUNCH("block_norm_sums", launch_pdl(bnorm::block_norm_sums, (int)((3 + (q.dgate ? entries : 0)) * ceil_div(p.D, 32)),
-                                                   dim3(32, 8), 0, s, q));
-    return BISSD_OK;
 }
 
 // ---- the decay attention ---------------------------------------------------------------------------------------------
@@ -631,41 +549,6 @@ int bissd_decay_step(const bissd_decay_step_args *a, void *stream) {
     BISSD_DO(step_check(a));
     BISSD_DO(check_device());
     return step_launch(a, static_cast<cudaStream_t>(stream));
-}
-
-int bissd_block_norm_workspace_bytes(const bissd_block_norm_args *a, size_t *bwd_bytes) {
-    BISSD_DO(block_norm_check(a, false) == BISSD_ERR_NULL ? (a ? BISSD_OK : BISSD_ERR_NULL) : block_norm_check(a, false));
-    long long entries;
-    int blocks;
-    const bnorm::Params p = block_norm_params(a);
-    block_norm_split(p, &entries, &blocks);
-    if (bwd_bytes) *bwd_bytes = align256((size_t)entries * blocks * 4 * p.D * sizeof(float));
-    return BISSD_OK;
-}
-
-int bissd_block_norm_forward(const bissd_block_norm_args *a, void *stream) {
-    BISSD_DO(block_norm_check(a, false));
-    BISSD_DO(check_device());
-    const auto s = static_cast<cudaStream_t>(stream);
-    return by_dtype(a->dtype, [&](auto t) -> int {
-        using T = decltype(t);
-        return a->r_dtype == a->dtype ? block_norm_forward_impl<T, T>(a, s) : block_norm_forward_impl<T, float>(a, s);
-    });
-}
-
-int bissd_block_norm_backward(const bissd_block_norm_args *a, void *workspace, size_t workspace_bytes, void *stream) {
-    BISSD_DO(block_norm_check(a, true));
-    size_t need = 0;
-    BISSD_DO(bissd_block_norm_workspace_bytes(a, &need));
-    if (!workspace || workspace_bytes < need) return BISSD_ERR_WORKSPACE;
-    if (reinterpret_cast<uintptr_t>(workspace) % 16) return BISSD_ERR_ALIGN;
-    BISSD_DO(check_device());
-    const auto s = static_cast<cudaStream_t>(stream);
-    return by_dtype(a->dtype, [&](auto t) -> int {
-        using T = decltype(t);
-        float *part = static_cast<float *>(workspace);
-        return a->r_dtype == a->dtype ? block_norm_backward_impl<T, T>(a, part, s) : block_norm_backward_impl<T, float>(a, part, s);
-    });
 }
 
 }  // extern "C"

@@ -4,24 +4,35 @@
 //     dr' = dr + rstd(r) (t - r^ mean(t r^)),   dresidual = dr',   dn = dr' m,   dw1 = sum_rows du r^,   dw2 = sum_rows dn x^,
 //     dx = rstd(x) (dn w2 - x^ mean(dn w2 x^)),   dscale = sum_rows dr' act(gate) n,   dgate = dr' scale n act'(gate)
 // Bound by the rows' bytes: each tensor is read or written once, everything between stays in registers.  A row has
-// width / 8 threads with eight channels each - neighbouring ones (16-byte accesses), or where a width is no multiple of
-// eight, ones a stride apart - and a block walks rows with the weights in registers, the next row's values under way while it
-// sums this one's squares.  r is formed again in the backward pass, from what the forward pass read, so that no rounding of it
-// enters.  Sums over rows: in registers over a block's rows, then over the blocks in a second kernel, always in one order.
+// width / 8 threads with eight channels each - neighbouring ones (16-byte accesses), or where width or addresses do not allow that,
+// ones a stride apart - and a block walks rows with the weights in registers.  With 16-byte accesses a thread's pieces of the
+// next rows come by asynchronous copies into shared memory of its own, several rows ahead: held in registers, one row ahead, they
+// left two blocks an SM waiting.  Arithmetic is on pairs of channels (two multiply-adds an instruction).  r is formed
+// again in the backward pass, from what the forward pass read, so that no rounding of it enters.  Sums over rows: in registers over a
+// block's rows - act, w2 and scale are factors of them that wait until the end, so that dw2, dscale and the gradient of a shared gate row
+// come from one sum of dr' x^ (act) - then over the blocks in a second kernel, always in one order.
 #pragma once
 #include <type_traits>
 
 #include "common.cuh"
+#include "vec.cuh"
 
 namespace bissd {
 namespace bnorm {
 
-constexpr int kCh = 8;                                           // channels a thread
+using vec::add2;
+using vec::f2;
+using vec::fma2;
+using vec::mul2;
+using vec::pack;
+using vec::unpack;
+
+constexpr int kCh = 8, kPairs = kCh / 2;                         // channels a thread
 constexpr int kMaxWidth = 8192;
 
 struct Params {
-    long long rows, gate_rows;                                   // gate_rows: rows of x to a row of the gate
-    int D, threads_row, w_dtype, act, blocks;                    // blocks: backward, of an entry
+    long long rows, gate_rows;                                   // gate_rows: rows of x to a row of the gate, 0 where each has its own
+    int D, threads_row, w_dtype, act, blocks, depth;             // blocks: of an entry; depth: rows copied ahead
     float scale, eps;
     long long sx, sres, sgate, sdr, sdu;                         // row strides
     const void *x, *res, *gate, *scale_v, *w2, *w1;
@@ -32,52 +43,84 @@ struct Params {
     float *part;                                                 // [blocks][4][D]: dw1, dw2, dscale, dgate of a shared row
 };
 
-// Eight channels of a row as they lie in memory.
-template <class T, bool VEC> struct Piece {
-    using Raw = typename std::conditional<VEC, uint4[sizeof(T) / 2], T[kCh]>::type;
-    Raw raw;
-    __device__ __forceinline__ void load(const void *p, long long at, int t, int tr, int D) {
-        const T *base = static_cast<const T *>(p) + at;
+// Channel e of thread t of a row.
+template <bool VEC> __device__ __forceinline__ int channel(int t, int tr, int e) { return VEC ? t * kCh + e : t + e * tr; }
+
+// A thread's eight channels of one tensor: where the next row's lie, and how they get into registers.
+template <class T, bool VEC> struct Column {
+    static constexpr int kPieces = VEC ? kCh * (int)sizeof(T) / 16 : 0;   // 16-byte pieces a row
+    const T *at;                                                 // this row's first channel of the thread (VEC) or of the row
+    int slot;                                                    // first piece's place in the ring's stage
+    __device__ __forceinline__ void start(const void *p, long long row, long long stride, int t, int *slots) {
+        at = static_cast<const T *>(p) + row * stride + (VEC ? t * kCh : 0);
+        slot = *slots;
+        *slots += kPieces;
+    }
+    __device__ __forceinline__ void copy(uint32_t stage, int threads, bool in) const {
         if constexpr (VEC) {
-            const bool in = t * kCh < D;
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-                raw[i] = in ? *(reinterpret_cast<const uint4 *>(base + t * kCh) + i) : make_uint4(0u, 0u, 0u, 0u);
-        } else {
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) raw[e] = t + e * tr < D ? base[t + e * tr] : from_f<T>(0.f);
+            for (int i = 0; i < kPieces; ++i)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + (slot + i) * threads * 16),
+                             "l"(reinterpret_cast<const uint4 *>(at) + i), "r"(in ? 16 : 0) : "memory");
         }
     }
-    __device__ __forceinline__ void get(float (&v)[kCh]) const {
-        const T *e = reinterpret_cast<const T *>(&raw);
+    __device__ __forceinline__ void get(const uint8_t *stage, int threads, int t, int tr, int D, f2 (&v)[kPairs]) const {
+        vec::Row<T, kPairs> row;
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < kCh; ++i) v[i] = to_f<T>(e[i]);
+            for (int i = 0; i < kPieces; ++i) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(stage + (slot + i) * threads * 16);
+                if constexpr (sizeof(T) == 4) {
+                    row.v[2 * i] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+                    row.v[2 * i + 1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
+                } else {
+                    row.v[0] = q.x; row.v[1] = q.y; row.v[2] = q.z; row.v[3] = q.w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) v[i] = vec::widen<T>(row.v[i]);
+        } else {
+            float e[kCh];
+#pragma unroll
+            for (int i = 0; i < kCh; ++i) e[i] = t + i * tr < D ? to_f<T>(at[t + i * tr]) : 0.f;
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) v[i] = pack(e[2 * i], e[2 * i + 1]);
+        }
     }
 };
 template <class T, bool VEC>
-__device__ __forceinline__ void put(void *p, long long row, int t, int tr, int D, const float (&v)[kCh]) {
+__device__ __forceinline__ void put(void *p, long long row, int t, int tr, int D, const f2 (&v)[kPairs]) {
     T *base = static_cast<T *>(p) + row * D;
     if constexpr (VEC) {
         if (t * kCh >= D) return;
-        union { uint4 w[sizeof(T) / 2]; T e[kCh]; } o;
+        vec::Row<T, kPairs> o;
 #pragma unroll
-        for (int i = 0; i < kCh; ++i) o.e[i] = from_f<T>(v[i]);
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) *(reinterpret_cast<uint4 *>(base + t * kCh) + i) = o.w[i];
+        for (int i = 0; i < kPairs; ++i) o.v[i] = vec::narrow<T>(v[i]);
+        vec::store_row<T, kPairs>(base + t * kCh, o);
     } else {
 #pragma unroll
-        for (int e = 0; e < kCh; ++e)
-            if (t + e * tr < D) base[t + e * tr] = from_f<T>(v[e]);
+        for (int i = 0; i < kPairs; ++i) {
+            float a, b;
+            unpack(v[i], a, b);
+            if (t + 2 * i * tr < D) base[t + 2 * i * tr] = from_f<T>(a);
+            if (t + (2 * i + 1) * tr < D) base[t + (2 * i + 1) * tr] = from_f<T>(b);
+        }
     }
 }
-template <bool VEC> __device__ __forceinline__ int channel(int t, int tr, int e) { return VEC ? t * kCh + e : t + e * tr; }
-template <bool VEC>
-__device__ __forceinline__ void weights(const void *p, int dtype, float none, int t, int tr, int D, float (&w)[kCh]) {
+template <bool VEC> __device__ __forceinline__ void weights(const void *p, int dtype, float none, int t, int tr, int D, f2 (&w)[kPairs]) {
+    float e[kCh];
 #pragma unroll
-    for (int e = 0; e < kCh; ++e) {
-        const int c = channel<VEC>(t, tr, e);
-        w[e] = p ? (c < D ? ld_any(p, dtype, c) : 0.f) : none;
+    for (int i = 0; i < kCh; ++i) {
+        const int c = channel<VEC>(t, tr, i);
+        e[i] = p ? (c < D ? ld_any(p, dtype, c) : 0.f) : none;
     }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) w[i] = pack(e[2 * i], e[2 * i + 1]);
+}
+__device__ __forceinline__ float both(f2 v) {
+    float a, b;
+    unpack(v, a, b);
+    return a + b;
 }
 
 // Sum over the threads of a row; every thread of the block calls.  The two buffers take turns: who writes one again has met the
@@ -96,216 +139,319 @@ template <int WARPS> __device__ __forceinline__ float row_sum(float v, float (&b
     return s;
 }
 
-// act(v) and its slope, from the hardware's 2^x and reciprocal (each within 2 ulp); 0 and 1 at the ends.
-__device__ __forceinline__ void activation(int act, float v, float &a, float &slope) {
-    if (act == BISSD_GATE_NONE) {
-        a = v;
-        slope = 1.f;
-        return;
-    }
-    float e = v * -1.44269504f, s;
-    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
-    if (act == BISSD_GATE_SIGMOID) {
-        a = s;
-        slope = s * (1.f - s);
-    } else {
-        a = v * s;
-        slope = s * (1.f + v * (1.f - s));
-    }
-}
-
-template <class T, class R, bool VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1) block_norm_fwd(Params a) {
-    pdl_begin();
-    __shared__ float buf[2][THREADS / 32];
-    int turn = 0;
-    const int tr = a.threads_row, per = blockDim.x / tr, grp = threadIdx.x / tr, t = threadIdx.x % tr, D = a.D;
-    const long long step = (long long)gridDim.x * per;
-    float w2[kCh], w1[kCh], sc[kCh];
-    weights<VEC>(a.w2, a.w_dtype, 1.f, t, tr, D, w2);
-    weights<VEC>(a.w1, a.w_dtype, 0.f, t, tr, D, w1);
-    weights<VEC>(a.scale_v, a.w_dtype, a.scale, t, tr, D, sc);
-    const float inv = 1.f / D;
-    Piece<T, VEC> px, pg;
-    Piece<R, VEC> pr;
-    auto fetch = [&](long long row) {
-        if (row >= a.rows) row = a.rows - 1;
-        px.load(a.x, row * a.sx, t, tr, D);
-        pr.load(a.res, row * a.sres, t, tr, D);
-        if (a.gate) pg.load(a.gate, (a.gate_rows > 0 ? row / a.gate_rows : row) * a.sgate, t, tr, D);
-    };
-    constexpr bool kAhead = VEC && THREADS <= 512;               // else the registers do not hold another row
-    if (kAhead) fetch((long long)blockIdx.x * per + grp);
-    for (long long base = (long long)blockIdx.x * per; base < a.rows; base += step) {
-        const long long row = base + grp;
-        if (!kAhead) fetch(row);
-        float x[kCh], r[kCh];
-        px.get(x);
-        pr.get(r);
-        if (a.gate) {
-            float g[kCh];
-            pg.get(g);
+// act of a gate and its slope.
+__device__ __forceinline__ void activation(int act, f2 (&a)[kPairs], f2 (&slope)[kPairs]) {
 #pragma unroll
-            for (int e = 0; e < kCh; ++e) {
-                float act, slope;
-                activation(a.act, g[e], act, slope);
-                g[e] = act * sc[e] * w2[e];
-            }
-            if (kAhead && base + step < a.rows) fetch(row + step);
-            float sx = 0.f;
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) sx += x[e] * x[e];
-            const float rx = a.w2 ? rsqrtf(row_sum(sx, buf, turn, tr) * inv + a.eps) : 1.f;
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) r[e] += g[e] * (x[e] * rx);
-            if (a.rstd && a.w2 && t == 0 && row < a.rows) a.rstd[row] = rx;
+    for (int i = 0; i < kPairs; ++i) {
+        if (act == BISSD_GATE_NONE) {
+            slope[i] = pack(1.f, 1.f);
         } else {
-            if (kAhead && base + step < a.rows) fetch(row + step);
-            float sx = 0.f;
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) sx += x[e] * x[e];
-            const float rx = a.w2 ? rsqrtf(row_sum(sx, buf, turn, tr) * inv + a.eps) : 1.f;
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) r[e] += sc[e] * w2[e] * (x[e] * rx);
-            if (a.rstd && a.w2 && t == 0 && row < a.rows) a.rstd[row] = rx;
-        }
-        if (row < a.rows) put<R, VEC>(a.r, row, t, tr, D, r);
-        if (a.u) {
-            float sr = 0.f;
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) sr += channel<VEC>(t, tr, e) < D ? r[e] * r[e] : 0.f;
-            const float rr = rsqrtf(row_sum(sr, buf, turn, tr) * inv + a.eps);
-            if (a.rstd && t == 0 && row < a.rows) a.rstd[a.rows + row] = rr;
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) r[e] *= rr * w1[e];
-            if (row < a.rows) put<T, VEC>(a.u, row, t, tr, D, r);
+            const f2 s = vec::sigmoid2(a[i]);
+            if (act == BISSD_GATE_SIGMOID) {
+                slope[i] = fma2(mul2(s, pack(-1.f, -1.f)), s, s);
+                a[i] = s;
+            } else {
+                slope[i] = vec::silu_slope2(a[i], s);
+                a[i] = mul2(a[i], s);
+            }
         }
     }
 }
 
-// entries * blocks blocks: an entry is the rows that share a gate row, where its gradient is wanted, else all of them.
-template <class T, class R, bool VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1) block_norm_bwd(Params a) {
+// The oldest of `depth` groups of copies has landed.
+__device__ __forceinline__ void wait_copies(int depth) {
+    if (depth >= 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// What both kernels walk: rows first + i of an entry (the rows that share a gate row, or all), i = blk per + grp, + step, ...  A row
+// behind the last is the last again, and nothing of it is kept.
+struct Walk {
+    int tr, per, grp, t, D, blk;
+    long long n, first, step;
+    __device__ __forceinline__ Walk(const Params &a) {
+        tr = a.threads_row; per = blockDim.x / tr; grp = threadIdx.x / tr; t = threadIdx.x % tr; D = a.D;
+        blk = blockIdx.x % a.blocks;
+        n = a.gate && a.gate_rows > 0 ? a.gate_rows : a.rows;
+        first = blockIdx.x / a.blocks * n;
+        step = (long long)a.blocks * per;
+    }
+    __device__ __forceinline__ long long row(long long i) const { return first + (i < n ? i : n - 1); }
+};
+
+template <class T, class R, bool VEC, int THREADS, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     pdl_begin();
+    extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ float buf[2][THREADS / 32];
-    int turn = 0;
-    const int tr = a.threads_row, per = blockDim.x / tr, grp = threadIdx.x / tr, t = threadIdx.x % tr, D = a.D;
-    const int blk = blockIdx.x % a.blocks;
-    const long long n_rows = a.rows / (gridDim.x / a.blocks), first = blockIdx.x / a.blocks * n_rows, step = (long long)a.blocks * per;
-    float w2[kCh], w1[kCh], sc[kCh], d1[kCh], d2[kCh], ds[kCh], dg[kCh];
-    weights<VEC>(a.w2, a.w_dtype, 1.f, t, tr, D, w2);
-    weights<VEC>(a.w1, a.w_dtype, 0.f, t, tr, D, w1);
-    weights<VEC>(a.scale_v, a.w_dtype, a.scale, t, tr, D, sc);
+    const Walk k(a);
+    const int t = k.t, tr = k.tr, D = k.D, threads = blockDim.x;
+    const bool full = a.gate && a.gate_rows == 0, in = t * kCh < D;
+    f2 mw[kPairs], w1[kPairs], scw[kPairs];                      // scale act w2; scale w2
+    {
+        f2 w2[kPairs], sc[kPairs];
+        weights<VEC>(a.w2, a.w_dtype, 1.f, t, tr, D, w2);
+        weights<VEC>(a.w1, a.w_dtype, 0.f, t, tr, D, w1);
+        weights<VEC>(a.scale_v, a.w_dtype, a.scale, t, tr, D, sc);
 #pragma unroll
-    for (int e = 0; e < kCh; ++e) d1[e] = d2[e] = ds[e] = dg[e] = 0.f;
-    const float inv = 1.f / D;
-    const bool row_gate = a.gate && a.gate_rows > 0;
-    Piece<T, VEC> px, pg, pu;
-    Piece<R, VEC> pr, pd;
-    auto fetch = [&](long long i) {
-        const long long row = first + (i < n_rows ? i : n_rows - 1);
-        px.load(a.x, row * a.sx, t, tr, D);
-        pr.load(a.res, row * a.sres, t, tr, D);
-        if (a.gate) pg.load(a.gate, (row_gate ? row / a.gate_rows : row) * a.sgate, t, tr, D);
-        if (a.du) pu.load(a.du, row * a.sdu, t, tr, D);
-        if (a.dr) pd.load(a.dr, row * a.sdr, t, tr, D);
+        for (int i = 0; i < kPairs; ++i) mw[i] = scw[i] = mul2(sc[i], w2[i]);
+    }
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
+    int slots = 0, turn = 0, at = 0;
+    long long i = (long long)k.blk * k.per + k.grp;
+    Column<T, VEC> cx, cg;
+    Column<R, VEC> cr;
+    auto aim = [&](long long j) {                                // the columns at row j
+        int s = 0;
+        const long long row = k.row(j);
+        cx.start(a.x, row, a.sx, t, &s);
+        cr.start(a.res, row, a.sres, t, &s);
+        if (full) cg.start(a.gate, row, a.sgate, t, &s);
+        slots = s;
     };
-    constexpr bool kAhead = VEC && THREADS <= 512;
-    if (kAhead) fetch((long long)blk * per + grp);
-    for (long long base = (long long)blk * per; base < n_rows; base += step) {
-        const bool in = base + grp < n_rows;
-        const long long row = first + (in ? base + grp : n_rows - 1);
-        if (!kAhead) fetch(base + grp);
-        float xh[kCh], r[kCh], act[kCh], m[kCh], dr[kCh], slope[kCh];
-        px.get(xh);
-        pr.get(r);
-        const float rx = a.w2 ? a.rstd[row] : 1.f, rr = a.du ? a.rstd[a.rows + row] : 0.f;
-        if (a.gate) {
-            pg.get(act);
+    auto copy = [&](int stage) {
+        const uint32_t to = ring + stage * slots * threads * 16;
+        cx.copy(to, threads, in);
+        cr.copy(to, threads, in);
+        if (full) cg.copy(to, threads, in);
+    };
+    if (a.gate && !full) {
+        f2 slope[kPairs];
+        int s = 0;
+        Column<T, false> c;                                      // once a block: element by element
+        c.start(a.gate, blockIdx.x / a.blocks, a.sgate, t, &s);
+        float e[kCh];
 #pragma unroll
-            for (int e = 0; e < kCh; ++e) activation(a.act, act[e], act[e], slope[e]);
-        } else {
+        for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(c.at[channel<VEC>(t, tr, j)]) : 0.f;
+        f2 g[kPairs];
 #pragma unroll
-            for (int e = 0; e < kCh; ++e) act[e] = 1.f;
+        for (int j = 0; j < kPairs; ++j) g[j] = pack(e[2 * j], e[2 * j + 1]);
+        activation(a.act, g, slope);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) mw[j] = mul2(g[j], scw[j]);
+    }
+    if (VEC)
+        for (int s = 0; s < a.depth; ++s) {
+            aim(i + s * k.step);
+            copy(s);
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
+    const float inv = 1.f / D;
+    for (long long base = (long long)k.blk * k.per; base < k.n; base += k.step, i += k.step) {
+        const bool valid = i < k.n;
+        const long long row = k.row(i);
+        f2 x[kPairs], r[kPairs];
+        const uint8_t *stage = dyn + (at * slots * threads + threadIdx.x) * 16;
+        if (VEC) wait_copies(a.depth);
+        else aim(i);
+        cx.get(stage, threads, t, tr, D, x);
+        cr.get(stage, threads, t, tr, D, r);
+        if (full) {
+            f2 g[kPairs], slope[kPairs];
+            cg.get(stage, threads, t, tr, D, g);
+            activation(a.act, g, slope);
 #pragma unroll
-        for (int e = 0; e < kCh; ++e) {
-            xh[e] *= rx;
-            m[e] = sc[e] * act[e];
-            r[e] = (r[e] + m[e] * w2[e] * xh[e]) * rr;           // rms(r)
-            dr[e] = 0.f;
+            for (int j = 0; j < kPairs; ++j) mw[j] = mul2(g[j], scw[j]);
         }
-        if (a.dr) pd.get(dr);
-        float c = 0.f, du[kCh];
-        if (a.du) {
-            pu.get(du);
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) {
-                if (in) d1[e] += du[e] * r[e];
-                du[e] *= w1[e];
-                c += du[e] * r[e];
-            }
+        if (VEC) {                                               // its values are in registers: the row `depth` on takes its place
+            aim(i + a.depth * k.step);
+            copy(at);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            at = at + 1 == a.depth ? 0 : at + 1;
         }
-        if (kAhead && base + step < n_rows) fetch(base + grp + step);
-        if (a.du) {
-            c = row_sum(c, buf, turn, tr) * inv;
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) dr[e] += rr * (du[e] - r[e] * c);
-        }
-        if (in && a.dres) put<R, VEC>(a.dres, row, t, tr, D, dr);
-        if (a.gate && a.dgate) {
-            float o[kCh];
-#pragma unroll
-            for (int e = 0; e < kCh; ++e) {
-                o[e] = dr[e] * sc[e] * w2[e] * xh[e] * slope[e];
-                if (row_gate && in) dg[e] += o[e];
-            }
-            if (!row_gate && in) put<T, VEC>(a.dgate, row, t, tr, D, o);
-        }
-        float c2 = 0.f;
-#pragma unroll
-        for (int e = 0; e < kCh; ++e) {
-            if (in) {
-                ds[e] += dr[e] * act[e] * w2[e] * xh[e];
-                d2[e] += dr[e] * m[e] * xh[e];
-            }
-            dr[e] *= m[e] * w2[e];
-            c2 += dr[e] * xh[e];
-        }
+        float rx = 1.f;
         if (a.w2) {
-            c2 = row_sum(c2, buf, turn, tr) * inv;
+            f2 q = mul2(x[0], x[0]);
 #pragma unroll
-            for (int e = 0; e < kCh; ++e) dr[e] = rx * (dr[e] - xh[e] * c2);
+            for (int j = 1; j < kPairs; ++j) q = fma2(x[j], x[j], q);
+            rx = rsqrtf(row_sum(both(q), buf, turn, tr) * inv + a.eps);
+            if (a.rstd && t == 0 && valid) a.rstd[row] = rx;
         }
-        if (in && a.dx) put<T, VEC>(a.dx, row, t, tr, D, dr);
+        const f2 rx2 = pack(rx, rx);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) r[j] = fma2(mul2(x[j], rx2), mw[j], r[j]);
+        if (valid) put<R, VEC>(a.r, row, t, tr, D, r);
+        if (a.u) {
+            f2 q = mul2(r[0], r[0]);
+#pragma unroll
+            for (int j = 1; j < kPairs; ++j) q = fma2(r[j], r[j], q);
+            const float rr = rsqrtf(row_sum(both(q), buf, turn, tr) * inv + a.eps);
+            if (a.rstd && t == 0 && valid) a.rstd[a.rows + row] = rr;
+            const f2 rr2 = pack(rr, rr);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) r[j] = mul2(mul2(r[j], rr2), w1[j]);
+            if (valid) put<T, VEC>(a.u, row, t, tr, D, r);
+        }
     }
-    // rows side by side in this block, then one partial row a block
-    extern __shared__ float dyn[];
+    if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <class T, class R, bool VEC, int THREADS, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
+    pdl_begin();
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ float buf[2][THREADS / 32];
+    const Walk k(a);
+    const int t = k.t, tr = k.tr, D = k.D, threads = blockDim.x;
+    const bool full = a.gate && a.gate_rows == 0, in = t * kCh < D;
+    f2 w1[kPairs], scw[kPairs], act[kPairs], slope[kPairs], d1[kPairs], d2[kPairs];   // scw: scale w2; d2: sums of dr' x^ (act)
+    {
+        f2 w2[kPairs], sc[kPairs];
+        weights<VEC>(a.w2, a.w_dtype, 1.f, t, tr, D, w2);
+        weights<VEC>(a.w1, a.w_dtype, 0.f, t, tr, D, w1);
+        weights<VEC>(a.scale_v, a.w_dtype, a.scale, t, tr, D, sc);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            scw[i] = mul2(sc[i], w2[i]);
+            act[i] = slope[i] = pack(1.f, 1.f);
+            d1[i] = d2[i] = pack(0.f, 0.f);
+        }
+    }
+    if (a.gate && !full) {
+        const T *p = static_cast<const T *>(a.gate) + blockIdx.x / a.blocks * a.sgate;
+        float e[kCh];
+#pragma unroll
+        for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(p[channel<VEC>(t, tr, j)]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) act[j] = pack(e[2 * j], e[2 * j + 1]);
+        activation(a.act, act, slope);
+    }
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
+    int slots = 0, turn = 0, at = 0;
+    long long i = (long long)k.blk * k.per + k.grp;
+    Column<T, VEC> cx, cg, cu;
+    Column<R, VEC> cr, cd;
+    auto aim = [&](long long j) {
+        int s = 0;
+        const long long row = k.row(j);
+        cx.start(a.x, row, a.sx, t, &s);
+        cr.start(a.res, row, a.sres, t, &s);
+        if (full) cg.start(a.gate, row, a.sgate, t, &s);
+        if (a.du) cu.start(a.du, row, a.sdu, t, &s);
+        if (a.dr) cd.start(a.dr, row, a.sdr, t, &s);
+        slots = s;
+    };
+    auto copy = [&](int stage) {
+        const uint32_t to = ring + stage * slots * threads * 16;
+        cx.copy(to, threads, in);
+        cr.copy(to, threads, in);
+        if (full) cg.copy(to, threads, in);
+        if (a.du) cu.copy(to, threads, in);
+        if (a.dr) cd.copy(to, threads, in);
+    };
+    if (VEC)
+        for (int s = 0; s < a.depth; ++s) {
+            aim(i + s * k.step);
+            copy(s);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    const float inv = 1.f / D;
+    for (long long base = (long long)k.blk * k.per; base < k.n; base += k.step, i += k.step) {
+        const bool valid = i < k.n;
+        const long long row = k.row(i);
+        const float rx = a.w2 ? a.rstd[row] : 1.f, rr = a.du ? a.rstd[a.rows + row] : 0.f;
+        const uint8_t *stage = dyn + (at * slots * threads + threadIdx.x) * 16;
+        f2 xh[kPairs], r[kPairs], dr[kPairs], du[kPairs];
+        if (VEC) wait_copies(a.depth);
+        else aim(i);
+        cx.get(stage, threads, t, tr, D, xh);
+        cr.get(stage, threads, t, tr, D, r);
+        if (full) cg.get(stage, threads, t, tr, D, act);
+        if (a.du) cu.get(stage, threads, t, tr, D, du);
+        if (a.dr) cd.get(stage, threads, t, tr, D, dr);
+        if (VEC) {
+            aim(i + a.depth * k.step);
+            copy(at);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            at = at + 1 == a.depth ? 0 : at + 1;
+        }
+        if (full) activation(a.act, act, slope);
+        const f2 rx2 = pack(rx, rx), rr2 = pack(rr, rr);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+            xh[j] = mul2(xh[j], rx2);
+            if (!a.dr || !valid) dr[j] = pack(0.f, 0.f);         // a row that is here for the second time adds nothing
+        }
+        if (a.du) {
+            f2 q = pack(0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+                if (!valid) du[j] = pack(0.f, 0.f);
+                r[j] = mul2(fma2(mul2(act[j], scw[j]), xh[j], r[j]), rr2);   // rms(r)
+                d1[j] = fma2(du[j], r[j], d1[j]);
+                du[j] = mul2(du[j], w1[j]);
+                q = fma2(du[j], r[j], q);
+            }
+            const float c = -rr * (row_sum(both(q), buf, turn, tr) * inv);
+            const f2 c2 = pack(c, c);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) dr[j] = fma2(r[j], c2, fma2(du[j], rr2, dr[j]));
+        }
+        if (valid && a.dres) put<R, VEC>(a.dres, row, t, tr, D, dr);
+        f2 q = pack(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+            const f2 z = mul2(dr[j], xh[j]);
+            d2[j] = full ? fma2(z, act[j], d2[j]) : add2(z, d2[j]);
+            du[j] = mul2(mul2(z, scw[j]), slope[j]);             // the gate's
+            dr[j] = mul2(dr[j], mul2(act[j], scw[j]));
+            q = fma2(dr[j], xh[j], q);
+        }
+        if (full && a.dgate && valid) put<T, VEC>(a.dgate, row, t, tr, D, du);
+        if (a.dx) {
+            if (a.w2) {
+                const float c = -rx * (row_sum(both(q), buf, turn, tr) * inv);
+                const f2 c2 = pack(c, c);
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) dr[j] = fma2(xh[j], c2, mul2(dr[j], rx2));
+            }
+            if (valid) put<T, VEC>(a.dx, row, t, tr, D, dr);
+        }
+    }
+    if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // rows side by side in this block added up, then one partial row a block
+    float *sums = reinterpret_cast<float *>(dyn);
     const long long part = (long long)blockIdx.x * 4 * D;
-    float *acc[4] = {d1, d2, ds, dg};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        __syncthreads();
-        if (grp > 0) {
+    for (int what = 0; what < 2; ++what) {
+        f2(&v)[kPairs] = what ? d2 : d1;
+        __syncthreads();                                         // the ring, or the sums before, are no longer read
+        if (k.grp > 0) {
 #pragma unroll
-            for (int e = 0; e < kCh; ++e) dyn[((grp - 1) * tr + t) * kCh + e] = acc[k][e];
+            for (int j = 0; j < kPairs; ++j) unpack(v[j], sums[((k.grp - 1) * tr + t) * kCh + 2 * j], sums[((k.grp - 1) * tr + t) * kCh + 2 * j + 1]);
         }
         __syncthreads();
-        if (grp == 0) {
+        if (k.grp > 0) continue;
+        float s[kCh], ac[kCh], sl[kCh], sw[kCh];
 #pragma unroll
-            for (int e = 0; e < kCh; ++e) {
-                float s = acc[k][e];
-                for (int i = 0; i + 1 < per; ++i) s += dyn[(i * tr + t) * kCh + e];
-                const int ch = channel<VEC>(t, tr, e);
-                if (ch < D) a.part[part + (long long)k * D + ch] = s;
+        for (int j = 0; j < kPairs; ++j) {
+            unpack(v[j], s[2 * j], s[2 * j + 1]);
+            unpack(act[j], ac[2 * j], ac[2 * j + 1]);
+            unpack(slope[j], sl[2 * j], sl[2 * j + 1]);
+            unpack(scw[j], sw[2 * j], sw[2 * j + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < kCh; ++j) {
+            for (int g = 0; g + 1 < k.per; ++g) s[j] += sums[(g * tr + t) * kCh + j];
+            const int ch = channel<VEC>(t, tr, j);
+            if (ch >= D) continue;
+            if (what == 0) {
+                a.part[part + ch] = s[j];
+            } else {
+                const float w = a.w2 ? ld_any(a.w2, a.w_dtype, ch) : 1.f, sc = a.scale_v ? ld_any(a.scale_v, a.w_dtype, ch) : a.scale;
+                const float m = full ? s[j] : s[j] * ac[j];
+                a.part[part + D + ch] = m * sc;
+                a.part[part + 2LL * D + ch] = m * w;
+                if (!full) a.part[part + 3LL * D + ch] = s[j] * sw[j] * sl[j];
             }
         }
     }
 }
 
 // Sums of the blocks' partial rows: what = 0 dw1, 1 dw2, 2 dscale over all blocks; 3 dgate over the blocks of an entry.
-// ceil(D / 32) * (3 + entries) blocks, 32 x 8 threads: a thread adds every eighth partial row, then the eight are added.
+// ceil(D / 32) * (3 + entries) blocks, 32 x 8 threads: a thread adds every eighth partial row, four in flight, then the eight are added.
 struct SumParams {
     const float *part;
     int D, blocks, entries, w_dtype, g_dtype;
@@ -318,14 +464,23 @@ __global__ void __launch_bounds__(256) block_norm_sums(SumParams a) {
     void *out = what == 0 ? a.dpre : what == 1 ? a.dpost : what == 2 ? a.dscale : a.dgate;
     if (!out) return;
     const int c = blockIdx.x % cols * 32 + threadIdx.x, n = what < 3 ? a.blocks * a.entries : a.blocks;
-    float v = 0.f;
-    if (c < a.D)
-        for (int i = threadIdx.y; i < n; i += 8) v += a.part[((long long)(entry * a.blocks + i) * 4 + what) * a.D + c];
-    s[threadIdx.y][threadIdx.x] = v;
+    const long long stride = 4LL * a.D;
+    const float *p = a.part + (long long)entry * a.blocks * stride + (long long)what * a.D + c;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.D) {
+        int i = threadIdx.y;
+        for (; i + 24 < n; i += 32) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += p[(i + 8 * k) * stride];
+        }
+        for (; i < n; i += 8) v[0] += p[i * stride];
+    }
+    float sum = (v[0] + v[1]) + (v[2] + v[3]);
+    s[threadIdx.y][threadIdx.x] = sum;
     __syncthreads();
     if (threadIdx.y || c >= a.D) return;
-    for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
-    st_any(out, what < 3 ? a.w_dtype : a.g_dtype, (long long)entry * a.D + c, v);
+    for (int i = 1; i < 8; ++i) sum += s[i][threadIdx.x];
+    st_any(out, what < 3 ? a.w_dtype : a.g_dtype, (long long)entry * a.D + c, sum);
 }
 
 }  // namespace bnorm
