@@ -61,10 +61,10 @@ static int block_norm_blocks(const bnorm::Params &p, int resident) {
 constexpr int kFwd = 3, kBwd = 2;                                // blocks of 256 threads an SM: what the registers allow
 static int block_norm_resident(const bnorm::Params &p, int of_256) { return std::max(1, 256 * of_256 / block_norm_threads(p)); }
 
-// Rows that a thread copies ahead: four, as long as the blocks of an SM have the shared memory.
-static int block_norm_depth(int pieces, int threads, int blocks) {
-    const int room = 216 * 1024 / blocks;
-    return std::max(1, std::min(4, room / (pieces * 16 * threads)));
+// Bytes of the rows that a block copies ahead.
+template <class T> static size_t block_norm_ring(int pieces, int threads) {
+    const int rows = threads > 512 ? bnorm::Ahead<T, 1024>::rows : threads > 256 ? bnorm::Ahead<T, 512>::rows : bnorm::Ahead<T, 256>::rows;
+    return (size_t)rows * pieces * 16 * threads;
 }
 template <class T, class R> static int block_norm_forward_impl(const bissd_block_norm_args *a, cudaStream_t s) {
     bnorm::Params p = block_norm_params(a);
@@ -74,8 +74,7 @@ template <class T, class R> static int block_norm_forward_impl(const bissd_block
     const long long grid = block_norm_entries(p) * p.blocks;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     const int pieces = (int)(sizeof(T) * (a->gate && p.gate_rows == 0 ? 2 : 1) + sizeof(R)) / 2;
-    p.depth = block_norm_depth(pieces, threads, block_norm_resident(p, kFwd));
-    const size_t smem = vec ? (size_t)p.depth * pieces * 16 * threads : 0;
+    const size_t smem = vec ? block_norm_ring<T>(pieces, threads) : 0;
     const auto kernel = !vec            ? bnorm::block_norm_fwd<T, R, false, 1024, 1>
                         : threads > 512 ? bnorm::block_norm_fwd<T, R, true, 1024, 1>
                         : threads > 256 ? bnorm::block_norm_fwd<T, R, true, 512, 1>
@@ -93,9 +92,8 @@ template <class T, class R> static int block_norm_backward_impl(const bissd_bloc
     if (entries * p.blocks > 0x7fffffffLL || (entries + 3) * ceil_div(p.D, 32) > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     p.part = part;
     const int pieces = (int)(sizeof(T) * (1 + (a->gate && p.gate_rows == 0) + (a->dnormed != nullptr)) + sizeof(R) * (1 + (a->dr != nullptr))) / 2;
-    p.depth = block_norm_depth(pieces, threads, block_norm_resident(p, kBwd));
     const size_t rows = (size_t)(per - 1) * p.threads_row * bnorm::kCh * sizeof(float);
-    const size_t smem = std::max(rows, vec ? (size_t)p.depth * pieces * 16 * threads : 0);
+    const size_t smem = std::max(rows, vec ? block_norm_ring<T>(pieces, threads) : 0);
     const auto kernel = !vec            ? bnorm::block_norm_bwd<T, R, false, 1024, 1>
                         : threads > 512 ? bnorm::block_norm_bwd<T, R, true, 1024, 1>
                         : threads > 256 ? bnorm::block_norm_bwd<T, R, true, 512, 1>

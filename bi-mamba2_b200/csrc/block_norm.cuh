@@ -32,7 +32,7 @@ constexpr int kMaxWidth = 8192;
 
 struct Params {
     long long rows, gate_rows;                                   // gate_rows: rows of x to a row of the gate, 0 where each has its own
-    int D, threads_row, w_dtype, act, blocks, depth;             // blocks: of an entry; depth: rows copied ahead
+    int D, threads_row, w_dtype, act, blocks;                    // blocks: of an entry
     float scale, eps;
     long long sx, sres, sgate, sdr, sdu;                         // row strides
     const void *x, *res, *gate, *scale_v, *w2, *w1;
@@ -49,27 +49,31 @@ template <bool VEC> __device__ __forceinline__ int channel(int t, int tr, int e)
 // A thread's eight channels of one tensor: where the next row's lie, and how they get into registers.
 template <class T, bool VEC> struct Column {
     static constexpr int kPieces = VEC ? kCh * (int)sizeof(T) / 16 : 0;   // 16-byte pieces a row
-    const T *at;                                                 // this row's first channel of the thread (VEC) or of the row
-    int slot;                                                    // first piece's place in the ring's stage
-    __device__ __forceinline__ void start(const void *p, long long row, long long stride, int t, int *slots) {
+    const T *at;                                                 // the next row's first channel of the thread (VEC) or of the row
+    long long step;
+    int slot;                                                    // first piece's place in the ring's stage, in bytes
+    __device__ __forceinline__ void start(const void *p, long long row, long long stride, long long rows, int t, int threads, int *bytes) {
         at = static_cast<const T *>(p) + row * stride + (VEC ? t * kCh : 0);
-        slot = *slots;
-        *slots += kPieces;
+        step = rows * stride;
+        slot = *bytes;
+        *bytes += kPieces * threads * 16;
     }
-    __device__ __forceinline__ void copy(uint32_t stage, int threads, bool in) const {
+    // the next row on its way (zeros where there is none, or no such channels), and on to the one after it
+    __device__ __forceinline__ void copy(uint32_t stage, int threads, bool in) {
         if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + (slot + i) * threads * 16),
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + slot + i * threads * 16),
                              "l"(reinterpret_cast<const uint4 *>(at) + i), "r"(in ? 16 : 0) : "memory");
+            at += step;
         }
     }
-    __device__ __forceinline__ void get(const uint8_t *stage, int threads, int t, int tr, int D, f2 (&v)[kPairs]) const {
+    __device__ __forceinline__ void get(const uint8_t *stage, int threads, int t, int tr, int D, bool valid, f2 (&v)[kPairs]) {
         vec::Row<T, kPairs> row;
         if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(stage + (slot + i) * threads * 16);
+                const uint4 q = *reinterpret_cast<const uint4 *>(stage + slot + i * threads * 16);
                 if constexpr (sizeof(T) == 4) {
                     row.v[2 * i] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
                     row.v[2 * i + 1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
@@ -82,9 +86,10 @@ template <class T, bool VEC> struct Column {
         } else {
             float e[kCh];
 #pragma unroll
-            for (int i = 0; i < kCh; ++i) e[i] = t + i * tr < D ? to_f<T>(at[t + i * tr]) : 0.f;
+            for (int i = 0; i < kCh; ++i) e[i] = valid && t + i * tr < D ? to_f<T>(at[t + i * tr]) : 0.f;
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) v[i] = pack(e[2 * i], e[2 * i + 1]);
+            at += step;
         }
     }
 };
@@ -141,33 +146,32 @@ template <int WARPS> __device__ __forceinline__ float row_sum(float v, float (&b
 
 // act of a gate and its slope.
 __device__ __forceinline__ void activation(int act, f2 (&a)[kPairs], f2 (&slope)[kPairs]) {
+    if (act == BISSD_GATE_NONE) {
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-        if (act == BISSD_GATE_NONE) {
-            slope[i] = pack(1.f, 1.f);
-        } else {
+        for (int i = 0; i < kPairs; ++i) slope[i] = pack(1.f, 1.f);
+    } else if (act == BISSD_GATE_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            a[i] = vec::sigmoid2(a[i]);
+            slope[i] = fma2(mul2(a[i], pack(-1.f, -1.f)), a[i], a[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
             const f2 s = vec::sigmoid2(a[i]);
-            if (act == BISSD_GATE_SIGMOID) {
-                slope[i] = fma2(mul2(s, pack(-1.f, -1.f)), s, s);
-                a[i] = s;
-            } else {
-                slope[i] = vec::silu_slope2(a[i], s);
-                a[i] = mul2(a[i], s);
-            }
+            slope[i] = vec::silu_slope2(a[i], s);
+            a[i] = mul2(a[i], s);
         }
     }
 }
 
-// The oldest of `depth` groups of copies has landed.
-__device__ __forceinline__ void wait_copies(int depth) {
-    if (depth >= 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
-}
+// Rows that a thread copies ahead: as many as leave an SM's blocks their shared memory.
+template <class T, int THREADS> struct Ahead {
+    static constexpr int rows = THREADS <= 256 ? (sizeof(T) == 4 ? 2 : 4) : (THREADS <= 512 || sizeof(T) == 2 ? 2 : 1);
+};
 
 // What both kernels walk: rows first + i of an entry (the rows that share a gate row, or all), i = blk per + grp, + step, ...  A row
-// behind the last is the last again, and nothing of it is kept.
+// behind the last is one of zeros, of which nothing is kept.
 struct Walk {
     int tr, per, grp, t, D, blk;
     long long n, first, step;
@@ -178,7 +182,6 @@ struct Walk {
         first = blockIdx.x / a.blocks * n;
         step = (long long)a.blocks * per;
     }
-    __device__ __forceinline__ long long row(long long i) const { return first + (i < n ? i : n - 1); }
 };
 
 template <class T, class R, bool VEC, int THREADS, int PER_SM>
@@ -198,33 +201,30 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) mw[i] = scw[i] = mul2(sc[i], w2[i]);
     }
+    constexpr int kAhead = Ahead<T, THREADS>::rows;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
-    int slots = 0, turn = 0, at = 0;
-    long long i = (long long)k.blk * k.per + k.grp;
+    int bytes = 0, turn = 0, at = 0;                             // of a stage of the ring; the stage in turn, in bytes
+    long long i = (long long)k.blk * k.per + k.grp, ahead = i;
+    const long long row0 = k.first + i;
     Column<T, VEC> cx, cg;
     Column<R, VEC> cr;
-    auto aim = [&](long long j) {                                // the columns at row j
-        int s = 0;
-        const long long row = k.row(j);
-        cx.start(a.x, row, a.sx, t, &s);
-        cr.start(a.res, row, a.sres, t, &s);
-        if (full) cg.start(a.gate, row, a.sgate, t, &s);
-        slots = s;
-    };
+    cx.start(a.x, row0, a.sx, k.step, t, threads, &bytes);
+    cr.start(a.res, row0, a.sres, k.step, t, threads, &bytes);
+    if (full) cg.start(a.gate, row0, a.sgate, k.step, t, threads, &bytes);
     auto copy = [&](int stage) {
-        const uint32_t to = ring + stage * slots * threads * 16;
-        cx.copy(to, threads, in);
-        cr.copy(to, threads, in);
-        if (full) cg.copy(to, threads, in);
+        const bool some = in && ahead < k.n;
+        cx.copy(ring + stage, threads, some);
+        cr.copy(ring + stage, threads, some);
+        if (full) cg.copy(ring + stage, threads, some);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += k.step;
     };
     if (a.gate && !full) {
         f2 slope[kPairs];
-        int s = 0;
-        Column<T, false> c;                                      // once a block: element by element
-        c.start(a.gate, blockIdx.x / a.blocks, a.sgate, t, &s);
+        const T *p = static_cast<const T *>(a.gate) + blockIdx.x / a.blocks * a.sgate;
         float e[kCh];
 #pragma unroll
-        for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(c.at[channel<VEC>(t, tr, j)]) : 0.f;
+        for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(p[channel<VEC>(t, tr, j)]) : 0.f;
         f2 g[kPairs];
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) g[j] = pack(e[2 * j], e[2 * j + 1]);
@@ -233,33 +233,26 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
         for (int j = 0; j < kPairs; ++j) mw[j] = mul2(g[j], scw[j]);
     }
     if (VEC)
-        for (int s = 0; s < a.depth; ++s) {
-            aim(i + s * k.step);
-            copy(s);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
+        for (int s = 0; s < kAhead; ++s) copy(s * bytes);
     const float inv = 1.f / D;
     for (long long base = (long long)k.blk * k.per; base < k.n; base += k.step, i += k.step) {
         const bool valid = i < k.n;
-        const long long row = k.row(i);
+        const long long row = k.first + i;
         f2 x[kPairs], r[kPairs];
-        const uint8_t *stage = dyn + (at * slots * threads + threadIdx.x) * 16;
-        if (VEC) wait_copies(a.depth);
-        else aim(i);
-        cx.get(stage, threads, t, tr, D, x);
-        cr.get(stage, threads, t, tr, D, r);
+        const uint8_t *stage = dyn + at + threadIdx.x * 16;
+        if (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");   // the oldest row has landed
+        cx.get(stage, threads, t, tr, D, valid, x);
+        cr.get(stage, threads, t, tr, D, valid, r);
         if (full) {
             f2 g[kPairs], slope[kPairs];
-            cg.get(stage, threads, t, tr, D, g);
+            cg.get(stage, threads, t, tr, D, valid, g);
             activation(a.act, g, slope);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) mw[j] = mul2(g[j], scw[j]);
         }
-        if (VEC) {                                               // its values are in registers: the row `depth` on takes its place
-            aim(i + a.depth * k.step);
+        if (VEC) {                                               // its values are in registers: the row kAhead on takes its place
             copy(at);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            at = at + 1 == a.depth ? 0 : at + 1;
+            at = at + bytes == kAhead * bytes ? 0 : at + bytes;
         }
         float rx = 1.f;
         if (a.w2) {
@@ -318,67 +311,58 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
         for (int j = 0; j < kPairs; ++j) act[j] = pack(e[2 * j], e[2 * j + 1]);
         activation(a.act, act, slope);
     }
+    constexpr int kAhead = Ahead<T, THREADS>::rows;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
-    int slots = 0, turn = 0, at = 0;
-    long long i = (long long)k.blk * k.per + k.grp;
+    int bytes = 0, turn = 0, at = 0;
+    long long i = (long long)k.blk * k.per + k.grp, ahead = i;
+    const long long row0 = k.first + i;
     Column<T, VEC> cx, cg, cu;
     Column<R, VEC> cr, cd;
-    auto aim = [&](long long j) {
-        int s = 0;
-        const long long row = k.row(j);
-        cx.start(a.x, row, a.sx, t, &s);
-        cr.start(a.res, row, a.sres, t, &s);
-        if (full) cg.start(a.gate, row, a.sgate, t, &s);
-        if (a.du) cu.start(a.du, row, a.sdu, t, &s);
-        if (a.dr) cd.start(a.dr, row, a.sdr, t, &s);
-        slots = s;
-    };
+    cx.start(a.x, row0, a.sx, k.step, t, threads, &bytes);
+    cr.start(a.res, row0, a.sres, k.step, t, threads, &bytes);
+    if (full) cg.start(a.gate, row0, a.sgate, k.step, t, threads, &bytes);
+    if (a.du) cu.start(a.du, row0, a.sdu, k.step, t, threads, &bytes);
+    if (a.dr) cd.start(a.dr, row0, a.sdr, k.step, t, threads, &bytes);
     auto copy = [&](int stage) {
-        const uint32_t to = ring + stage * slots * threads * 16;
-        cx.copy(to, threads, in);
-        cr.copy(to, threads, in);
-        if (full) cg.copy(to, threads, in);
-        if (a.du) cu.copy(to, threads, in);
-        if (a.dr) cd.copy(to, threads, in);
+        const bool some = in && ahead < k.n;
+        cx.copy(ring + stage, threads, some);
+        cr.copy(ring + stage, threads, some);
+        if (full) cg.copy(ring + stage, threads, some);
+        if (a.du) cu.copy(ring + stage, threads, some);
+        if (a.dr) cd.copy(ring + stage, threads, some);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += k.step;
     };
     if (VEC)
-        for (int s = 0; s < a.depth; ++s) {
-            aim(i + s * k.step);
-            copy(s);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
+        for (int s = 0; s < kAhead; ++s) copy(s * bytes);
     const float inv = 1.f / D;
     for (long long base = (long long)k.blk * k.per; base < k.n; base += k.step, i += k.step) {
         const bool valid = i < k.n;
-        const long long row = k.row(i);
-        const float rx = a.w2 ? a.rstd[row] : 1.f, rr = a.du ? a.rstd[a.rows + row] : 0.f;
-        const uint8_t *stage = dyn + (at * slots * threads + threadIdx.x) * 16;
+        const long long row = k.first + i;
+        const float rx = !a.w2 ? 1.f : valid ? a.rstd[row] : 0.f, rr = a.du && valid ? a.rstd[a.rows + row] : 0.f;
+        const uint8_t *stage = dyn + at + threadIdx.x * 16;
         f2 xh[kPairs], r[kPairs], dr[kPairs], du[kPairs];
-        if (VEC) wait_copies(a.depth);
-        else aim(i);
-        cx.get(stage, threads, t, tr, D, xh);
-        cr.get(stage, threads, t, tr, D, r);
-        if (full) cg.get(stage, threads, t, tr, D, act);
-        if (a.du) cu.get(stage, threads, t, tr, D, du);
-        if (a.dr) cd.get(stage, threads, t, tr, D, dr);
+        if (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");   // the oldest row has landed
+        cx.get(stage, threads, t, tr, D, valid, xh);
+        cr.get(stage, threads, t, tr, D, valid, r);
+        if (full) cg.get(stage, threads, t, tr, D, valid, act);
+        if (a.du) cu.get(stage, threads, t, tr, D, valid, du);
+        if (a.dr) cd.get(stage, threads, t, tr, D, valid, dr);
         if (VEC) {
-            aim(i + a.depth * k.step);
             copy(at);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            at = at + 1 == a.depth ? 0 : at + 1;
+            at = at + bytes == kAhead * bytes ? 0 : at + bytes;
         }
         if (full) activation(a.act, act, slope);
         const f2 rx2 = pack(rx, rx), rr2 = pack(rr, rr);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
             xh[j] = mul2(xh[j], rx2);
-            if (!a.dr || !valid) dr[j] = pack(0.f, 0.f);         // a row that is here for the second time adds nothing
+            if (!a.dr) dr[j] = pack(0.f, 0.f);
         }
         if (a.du) {
             f2 q = pack(0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) {
-                if (!valid) du[j] = pack(0.f, 0.f);
                 r[j] = mul2(fma2(mul2(act[j], scw[j]), xh[j], r[j]), rr2);   // rms(r)
                 d1[j] = fma2(du[j], r[j], d1[j]);
                 du[j] = mul2(du[j], w1[j]);
