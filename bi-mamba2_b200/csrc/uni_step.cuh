@@ -24,7 +24,7 @@ constexpr int kStepThreads = 256, kStepColumns = 32;
 
 // VEC columns a lane, PASSES rows a thread: kdim <= PASSES * (8 VEC).
 template <class T, int VEC, int PASSES>
-__global__ void __launch_bounds__(kStepThreads) decay_step(StepParams a) {
+__global__ void __launch_bounds__(kStepThreads, VEC == 4 && PASSES <= 4 ? 6 : 2) decay_step(StepParams a) {
     pdl_begin();
     constexpr int kLanes = kStepColumns / VEC, kRows = kStepThreads / kLanes;
     __shared__ float part[kStepThreads / 32][kStepColumns];
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kStepThreads) decay_step(StepParams a) {
         const int n = n0 + r * kRows;
         const bool in = n < a.N && c < a.P;
         if constexpr (VEC == 4) {
-            const float4 f = in ? *reinterpret_cast<const float4 *>(base + (long long)n * a.P) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 f = in ? __ldcs(reinterpret_cast<const float4 *>(base + (long long)n * a.P)) : make_float4(0.f, 0.f, 0.f, 0.f);
             s[r][0] = f.x; s[r][1] = f.y; s[r][2] = f.z; s[r][3] = f.w;
         } else {
             s[r][0] = in ? base[(long long)n * a.P] : 0.f;
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kStepThreads) decay_step(StepParams a) {
     for (int r = 0; r < PASSES; ++r) {
         const int n = n0 + r * kRows;
         if (n >= a.N || c >= a.P) continue;
-        if constexpr (VEC == 4) *reinterpret_cast<float4 *>(base + (long long)n * a.P) = make_float4(s[r][0], s[r][1], s[r][2], s[r][3]);
+        if constexpr (VEC == 4) __stcs(reinterpret_cast<float4 *>(base + (long long)n * a.P), make_float4(s[r][0], s[r][1], s[r][2], s[r][3]));
         else base[(long long)n * a.P] = s[r][0];
     }
 }
