@@ -171,6 +171,12 @@ inline int check_device() {
     static std::atomic<int> major_of[64];                        // 0 = not asked yet
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return BISSD_ERR_LAUNCH;
+    // A thread that has made no CUDA call yet has no current context, and a tensor map cannot be built without one.
+    static thread_local unsigned long long bound = 0;
+    if (dev >= 0 && dev < 64 && !(bound >> dev & 1)) {
+        if (cudaSetDevice(dev) != cudaSuccess) return BISSD_ERR_LAUNCH;
+        bound |= 1ull << dev;
+    }
     int major = (dev >= 0 && dev < 64) ? major_of[dev].load(std::memory_order_relaxed) : 0;
     if (!major) {
         if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return BISSD_ERR_LAUNCH;

@@ -124,7 +124,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     pdl_begin();
     constexpr int kSlabs = NT / 64;
     extern __shared__ uint8_t dyn[];
-    __shared__ uint64_t full[2], done[2], unused;
+    __shared__ uint64_t full[2], done[2], stored, unused;
     __shared__ uint32_t tmem_slot;
     __shared__ float w[kAhead][kQ], whole[kAhead];
     uint8_t *smK = smem_align1024(dyn), *smV = smK + 2 * kSlabs * kSlab, *smS = smV + kSlab;   // two stages of k; weighted rows; S
@@ -177,6 +177,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         mbar_init(&full[1], 1);
         mbar_init(&done[0], 1);
         mbar_init(&done[1], 1);
+        mbar_init(&stored, 1);
         fence_mbar_init();
         load(0);
     }
@@ -229,6 +230,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             }
         };
         weigh(0, smV);
+        if (a.exact && !a.tiles) weigh(1, smS);
+        if (!a.exact && i + 1 < nc) fetch(i + 1, rows);
+        if (a.tiles && i > 0) ok = ok && mbar_wait(&stored, (i - 1) & 1);
         if (a.tiles && n < NT) {                                 // what enters this chunk
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -253,27 +257,33 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         if (warp == 0 && elect_one()) {
             if (a.tiles) tma_store2(&tmTiles, smS, 0, (((c0 + place(i)) * a.h.H + h) * a.h.PB + pb) * NT);
             issue(smV, 0u);
-            if (a.tiles) tma_store_read();                       // so whoever has waited for the MMAs may write S's tile again
             umma_commit(&done[uses & 1]);
+            if (a.exact && !a.tiles) {
+                issue(smS, 1u);
+                umma_commit(&done[(uses + 1) & 1]);
+            }
+            if (a.tiles) {                                       // S's tile may be written again
+                tma_store_read();
+                mbar_arrive(&stored);
+            }
         }
-        ++uses;
-        if (a.exact) {
-            uint8_t *second = a.tiles ? smV : smS;               // with a tile under way, one buffer for the parts
+        uses += a.exact && !a.tiles ? 2 : 1;
+        if (a.exact) {                                           // the parts that are left, where the first was
 #pragma unroll
             for (int part = 1; part < 3; ++part) {
-                uint8_t *to = part == 1 ? second : smV;
-                if (ok && (part == 2 || to == smV)) ok = wait(part == 2 && to != second ? uses - 2 : uses - 1);
-                if (ok) weigh(part, to);
+                if (part == 1 && !a.tiles) continue;
+                if (ok) ok = wait(a.tiles ? uses - 1 : uses - 2);
+                if (ok) weigh(part, smV);
                 fence_async_smem();
                 ok = __syncthreads_and(ok);
                 if (ok && warp == 0 && elect_one()) {
-                    issue(to, 1u);
+                    issue(smV, 1u);
                     umma_commit(&done[uses & 1]);
                 }
                 ++uses;
             }
+            if (ok && i + 1 < nc) fetch(i + 1, rows);
         }
-        if (ok && i + 1 < nc) fetch(i + 1, rows);
         if (ok && a.exact) ok = wait(uses - 2);                  // phases are waited for one by one
         if (ok) ok = wait(uses - 1);
         if (!ok) continue;                                       // leaves at the next barrier

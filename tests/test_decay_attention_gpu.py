@@ -342,6 +342,22 @@ def test_a_row_does_not_depend_on_the_others():
         assert torch.equal(o[0], out[i]) and torch.equal(f[0], final[i])
 
 
+def test_a_thread_that_has_made_no_cuda_call():
+    """With all memory at hand, the first call of a new thread that reaches CUDA is the building of a tensor map."""
+    import threading
+    from ssd.uni.decay_attention import decay_attention
+    q, k, v, g, _ = (None if t is None else t.cuda() for t in make(torch.bfloat16, 1, 200, 2, 1, 64, 64))
+    with torch.no_grad():
+        decay_attention(q, k, v, g)
+        torch.cuda.synchronize()
+        got = []
+        thread = threading.Thread(target=lambda: got.append(decay_attention(q, k, v, g)))
+        thread.start()
+        thread.join()
+    torch.cuda.synchronize()
+    assert got and torch.equal(got[0], decay_attention(q, k, v, g))
+
+
 def test_no_second_derivative():
     from ssd.uni.decay_attention import decay_attention
     q, k, v, g, _ = (None if t is None else t.cuda().requires_grad_(True) for t in make(torch.float32, 1, 8, 1, 1, 8, 8))
