@@ -367,26 +367,30 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
               const float *start, float *end, float *states, float *decay, int *status, cudaStream_t s) {
     unitc::StatesParams p{};
     p.h = tc_heads(a, t.PB);
-    p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.exact = end != nullptr; p.v = view(cols); p.status = status;
-    const auto kernel = t.NT == 64 ? unitc::decay_states<64> : unitc::decay_states<128>;
+    p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.v = view(cols); p.status = status;
     const size_t smem = unitc::states_smem(t.NT);
     const long long grid = (long long)t.seg.most * a->nheads * t.PB;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
-    BISSD_ALLOW(kernel, smem);
+    auto launch = [&](const char *name, bool exact) -> int {
+        const auto kernel = t.NT == 64 ? (exact ? unitc::decay_states<64, true> : unitc::decay_states<64, false>)
+                                       : (exact ? unitc::decay_states<128, true> : unitc::decay_states<128, false>);
+        BISSD_ALLOW(kernel, smem);
+        BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, tiles));
+        return BISSD_OK;
+    };
     if (t.split) {
         p.fin = states; p.decay = decay;
-        BISSD_LAUNCH("decay_states_own", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, tiles));
+        BISSD_DO(launch("decay_states_own", end != nullptr));
         uni::ChainParams c{};
         c.plan = t.seg; c.H = a->nheads; c.per = a->kdim * a->vdim; c.reverse = reverse; c.nseq = a->nseq > 0 ? a->nseq : a->batch;
         c.start = start; c.states = states; c.decay = decay; c.end = end;
         BISSD_DO(launch_chain(c, s));
-        p.init = states; p.fin = p.decay = nullptr; p.exact = 0;
+        p.init = states; p.fin = p.decay = nullptr;
     } else {
         p.init = start; p.fin = end; p.by_seq = 1;
     }
     p.tiles = 1;
-    BISSD_LAUNCH("decay_states", launch_pdl(kernel, (int)grid, 256, smem, s, p, rows, tiles));
-    return BISSD_OK;
+    return launch("decay_states", !t.split && end != nullptr);
 }
 bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, const bf16 *tiles) {
     return make_map2(m, BISSD_BF16, tiles, unitc::kP, (unsigned long long)t.chunk.most * a->nheads * t.PB * t.NT, unitc::kP, t.NT);

@@ -97,15 +97,18 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
 // ---- the states that enter the chunks ------------------------------------------------------------------------------------
 // Forwards S' as above; backwards (v the outputs' gradient, k the queries) the gradient that enters each chunk from its right,
 // G' = e^{c_end} G + sum_t q_t (scale e^{c_t} do_t)^T.  A block walks the chunks of one (segment, head, 64 columns), S or G in
-// registers (a row n and 32 columns a thread).  k's rows come by TMA a chunk ahead; v's go through registers, a chunk ahead as well,
-// and are weighted on the way to shared memory; S leaves as a bf16 tile through a TMA store.  The weights need the decays alone: the
-// eight warps make those of eight chunks at a time.
-// exact: the weighted row is given to the tensor cores in three bf16 parts, each what is left of those before, so that the states
+// registers (a row n and 32 columns a thread).  k's rows come by TMA a chunk ahead; v's go through registers and are weighted on the
+// way to shared memory.  Eight warps do that, a chunk ahead too, and keep S; the ninth makes the weights, issues loads, MMAs and tile
+// stores, and the two meet at mbarriers alone.  So a step is S's way to shared memory, one product's latency and its way back,
+// with everything else in its shadow; with block-wide barriers and the weights made by one of the eight it was half as fast
+// again.  Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
+// A weight f meets bf16 rows as bf16 f1 + f2, in one rounding: v f1 + (v f2) as a multiply-add.
+// EXACT: the weighted row is given to the tensor cores in three bf16 parts, each what is left of those before, so that the states
 // that leave the library are fp32's.  The tiles that the other kernels read are bf16 in any case: they meet bf16 factors.
 struct StatesParams {
     Heads h;
     Plan seg, chunk;
-    int reverse, exact, by_seq, tiles;                           // by_seq: init and fin hold a state a sequence, not a segment
+    int reverse, by_seq, tiles;                                  // by_seq: init and fin hold a state a sequence, not a segment
     View v;                                                      // v or the outputs' gradient
     const float *init;
     float *fin, *decay;                                          // decay: (segments, H) the segment's whole decay, or NULL
@@ -116,207 +119,284 @@ __device__ __forceinline__ void tma_store_read() {
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
-constexpr int kAhead = 8;                                        // chunks whose weights are made at a time
-inline size_t states_smem(int NT) { return 1024 + 2 * (size_t)(NT / 64) * kSlab + 2 * (size_t)kSlab; }
+struct StatesShared {
+    uint64_t full[2], ready, done, weights, stored, unused;
+    uint32_t tmem;
+    int fail;
+    float decay[2];                                              // of a chunk, 2^c_end
+    alignas(16) uint32_t w[kQ];                                  // of a chunk's rows: f1 and f2, or EXACT fp32
+};
+constexpr int kStatesThreads = 288;
+inline size_t states_smem(int NT) { return 2 * (size_t)(NT / 64) * kSlab + 3 * (size_t)kSlab + sizeof(StatesShared); }
 
-template <int NT> __global__ void __launch_bounds__(256, 2)
+template <int NT, bool EXACT> __global__ void __launch_bounds__(kStatesThreads, 2)
 decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
     constexpr int kSlabs = NT / 64;
-    extern __shared__ uint8_t dyn[];
-    __shared__ uint64_t full[2], done[2], stored, unused;
-    __shared__ uint32_t tmem_slot;
-    __shared__ float w[kAhead][kQ], whole[kAhead];
-    uint8_t *smK = smem_align1024(dyn), *smV = smK + 2 * kSlabs * kSlab, *smS = smV + kSlab;   // two stages of k; weighted rows; S
+    extern __shared__ __align__(1024) uint8_t dyn[];
+    uint8_t *smK = dyn, *smV = smK + 2 * kSlabs * kSlab, *smS = smV + 2 * kSlab;   // two stages of k; two of weighted rows; S
+    StatesShared &sh = *reinterpret_cast<StatesShared *>(smS + kSlab);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pb = blockIdx.x % a.h.PB, h = blockIdx.x / a.h.PB % a.h.H, si = blockIdx.x / (a.h.PB * a.h.H), hq = h * a.h.hk / a.h.H;
     const Segment s = uni::segment(a.seg, si);
     if (s.len == 0) return;                                      // packed: fewer segments than there could be
-    const int nc = ceil_div(s.len, kQ), c0 = uni::segments(a.chunk, s.seq).x + s.idx * (a.seg.seg / kQ);
+    if (smem_u32(dyn) & 1023) {                                  // the swizzled tiles' alignment, which nothing else here sees to
+        if (tid == 0) atomicExch(a.status, kErrDecay + 4);
+        return;
+    }
+    const int nc = ceil_div(s.len, kQ);
     auto place = [&](int i) { return a.reverse ? nc - 1 - i : i; };        // chunk of the segment at step i
     auto length = [&](int i) { return min(kQ, s.len - place(i) * kQ); };
-    auto load = [&](int i) {
-        const int st = i & 1, t = s.t0 + place(i) * kQ;
-        mbar_expect_tx(&full[st], kSlabs * kSlab);
-        for (int j = 0; j < kSlabs; ++j) tma_load4(smK + (st * kSlabs + j) * kSlab, &tmK, j * 64, hq, t, s.batch, &full[st]);
-    };
-    const bool in_cols = pb * kP + (tid & 7) * 8 < a.h.P;
-    const bf16 *vp = static_cast<const bf16 *>(a.v.ptr) + (long long)s.batch * a.v.sb + (long long)h * a.v.sh + pb * kP + (tid & 7) * 8;
-    auto fetch = [&](int i, uint4 (&rows)[4]) {                  // 16 bytes of four rows of v
-        const int t = s.t0 + place(i) * kQ, len = length(i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int row = (tid >> 3) + k * 32;
-            rows[k] = row < len && in_cols ? __ldg(reinterpret_cast<const uint4 *>(vp + (long long)(t + row) * a.v.sl)) : zero8();
-        }
-    };
-    Decays decays;
-    auto ask = [&](int i) {
-        if (i < nc) decays.load(a.h, s.batch, s.t0 + place(i) * kQ, length(i), h, lane);
-    };
-    auto weights = [&](int i) {                                  // this warp's chunk of the next kAhead
-        if (i >= nc) return;
-        const int len = length(i);
-        float c[4], p[4];
-        decays.log2(a.h);
-        decays.prefix(p, lane);
-        if (a.reverse) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) c[k] = p[k] + a.h.log_scale;
-        } else {
-            decays.suffix(c, lane);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[warp][lane * 4 + k] = lane * 4 + k < len ? exp2f(c[k]) : 0.f;
-        if (lane == 31) whole[warp] = p[3];
-    };
-    ask(warp);
-    if (warp == 0) tmem_alloc(&tmem_slot, 64);
-    if (tid == 32) {
-        mbar_init(&full[0], 1);
-        mbar_init(&full[1], 1);
-        mbar_init(&done[0], 1);
-        mbar_init(&done[1], 1);
-        mbar_init(&stored, 1);
+    volatile int *fail = &sh.fail;
+    constexpr int kRounds = EXACT ? 2 : 1;                       // of an exact step that stores a tile, which has the third part's buffer
+    const bool two = EXACT && a.tiles;
+    if (warp == 0) tmem_alloc(&sh.tmem, 64);
+    if (tid == 256) {
+        mbar_init(&sh.full[0], 1);
+        mbar_init(&sh.full[1], 1);
+        mbar_init(&sh.ready, 8);
+        mbar_init(&sh.done, 1);
+        mbar_init(&sh.weights, 1);
+        mbar_init(&sh.stored, 1);
+        sh.fail = 0;
         fence_mbar_init();
-        load(0);
     }
-    uint4 rows[4];
-    fetch(0, rows);
-    const int n = (warp & 3) * 32 + lane, half = warp >> 2, col = pb * kP + half * 32;
-    const long long at = (((long long)(a.by_seq ? s.seq : si) * a.h.H + h) * a.h.N + n) * a.h.P + col;
-    float S[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) S[j] = a.init && n < a.h.N && col + j < a.h.P ? a.init[at + j] : 0.f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
-    constexpr uint32_t idesc = instr_desc(1, true, true, kP);
+    const uint32_t tmem = sh.tmem;
     bool ok = true;
-    int loads = 1, uses = 0;                                     // loads asked for, commits
-    float total = 0.f;
-    // `use` is waited for as the phase use / 2 of barrier use & 1: the parts of an exact step overlap, two at a time
-    auto wait = [&](int use) { return mbar_wait(&done[use & 1], (use >> 1) & 1); };
-    for (int i = 0; i < nc; ++i) {
-        const int st = i & 1;
-        if (i + 1 < nc) {                                        // the stage was read by the MMAs of the step before, which are done
-            if (tid == 32) load(i + 1);
-            ++loads;
-        }
-        if (i % kAhead == 0) {
-            if (i) __syncthreads();                              // the last weights have been read
-            weights(i + warp);
-            ask(i + kAhead + warp);
-            __syncthreads();
-        }
-        auto weigh = [&](int part, uint8_t *to) {                // part 0, 1 or 2 of the weighted rows
+    if (warp == 8) {
+        const int c0 = uni::segments(a.chunk, s.seq).x + s.idx * (a.seg.seg / kQ);
+        Decays d;
+        uint32_t f[4];
+        float whole = 0.f, total = 0.f;
+        auto load = [&](int i) {
+            const int st = i & 1, t = s.t0 + place(i) * kQ;
+            mbar_expect_tx(&sh.full[st], kSlabs * kSlab);
+            for (int j = 0; j < kSlabs; ++j) tma_load4(smK + (st * kSlabs + j) * kSlab, &tmK, j * 64, hq, t, s.batch, &sh.full[st]);
+        };
+        auto ask = [&](int i) {
+            if (i < nc) d.load(a.h, s.batch, s.t0 + place(i) * kQ, length(i), h, lane);
+        };
+        auto make = [&]() {                                      // the weights of what was asked for last
+            float c[4], p[4];
+            d.log2(a.h);
+            d.prefix(p, lane);
+            whole = __shfl_sync(0xffffffffu, p[3], 31);
+            if (!a.reverse) d.suffix(c, lane);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int x = tid + k * 256, row = x >> 3;
-                const float f = w[i % kAhead][row];
+                const float v = exp2f(a.reverse ? p[k] + a.h.log_scale : c[k]);
+                if constexpr (EXACT) {
+                    f[k] = __float_as_uint(v);
+                } else {
+                    const float hi = __bfloat162float(__float2bfloat16_rn(v));
+                    f[k] = pack2<bf16>(hi, v - hi);
+                }
+            }
+        };
+        auto give = [&](int i) {                                 // to the others, as chunk i's
+            *reinterpret_cast<uint4 *>(&sh.w[lane * 4]) = make_uint4(f[0], f[1], f[2], f[3]);
+            if (lane == 0) sh.decay[i & 1] = exp2f(whole);
+            total += whole;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.weights);
+        };
+        if (lane == 0) load(0);
+        ask(0);
+        make();
+        give(0);
+        ask(1);
+        if (nc > 1) make();
+        ask(2);
+        int loads = 1, round = 0;
+        constexpr uint32_t idesc = instr_desc(1, true, true, kP);
+        for (int i = 0; i < nc && ok; ++i) {
+            const int st = i & 1;
+            if (i + 1 < nc) {                                    // the stage was read by the MMAs of the step before
+                if (i > 0) ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 1);
+                if (ok && lane == 0) load(i + 1);
+                loads += ok;
+            }
+            ok = ok && ws_wait_warp(&sh.full[st], (i >> 1) & 1, fail, 2);
+            auto issue = [&](const uint8_t *v, uint32_t first) {
+#pragma unroll
+                for (int kk = 0; kk < kQ / 16; ++kk)             // where NT is 64, rows 64 ... 127 are the first 64 again: products of no use
+                    umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 0 : kSlab, 1024),
+                         smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : first);
+            };
+            for (int r = 0; r < (two ? kRounds : 1) && ok; ++r, ++round) {
+                ok = ws_wait_warp(&sh.ready, round & 1, fail, 3);
+                if (!ok) break;
+                tc_fence_after();
+                if (r == 0 && i + 1 < nc) give(i + 1);
+                if (elect_one()) {
+                    if (r == 1) {
+                        issue(smV, 1u);
+                    } else {
+                        issue(smV + (EXACT ? 0 : st * kSlab), 0u);
+                        if constexpr (EXACT) {
+                            issue(smV + kSlab, 1u);
+                            if (!a.tiles) issue(smS, 1u);
+                        }
+                    }
+                    umma_commit(&sh.done);
+                    if (r == 0 && a.tiles) {
+                        tma_store2(&tmTiles, smS, 0, (((c0 + place(i)) * a.h.H + h) * a.h.PB + pb) * NT);
+                        tma_store_read();                        // S's tile may be written again
+                        mbar_arrive(&sh.stored);
+                    }
+                }
+                __syncwarp();
+            }
+            if (ok && i + 2 < nc) {
+                make();
+                ask(i + 3);
+            }
+        }
+        if (a.decay && ok && pb == 0 && lane == 0) a.decay[(long long)si * a.h.H + h] = exp2f(total);
+        if (a.tiles && elect_one()) tma_store_wait();
+        if (!ok && elect_one()) {                                // leave nothing in flight
+            drain_mmas(&sh.unused);
+            drain_loads(sh.full, 2, loads);
+            atomicExch(a.status, kErrDecay + 0x10 + *fail);
+        }
+        __syncwarp();
+    } else {
+        // 16 bytes of rows tid / 8 + 32 k of v
+        const bool in_cols = pb * kP + (tid & 7) * 8 < a.h.P;
+        const long long vstep = 32 * a.v.sl;
+        const bf16 *vp = static_cast<const bf16 *>(a.v.ptr) + (long long)s.batch * a.v.sb + (long long)h * a.v.sh + pb * kP + (tid & 7) * 8 +
+                         (long long)(s.t0 + (tid >> 3)) * a.v.sl;
+        uint4 rows[4];
+        auto fetch = [&](int i) {
+            if (i >= nc) return;
+            const bf16 *p = vp + (long long)(place(i) * kQ) * a.v.sl;
+            const int left = in_cols ? length(i) - (tid >> 3) : 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) rows[k] = k * 32 < left ? __ldg(reinterpret_cast<const uint4 *>(p + k * vstep)) : zero8();
+        };
+        const uint32_t swz = (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);   // the thread's piece of a tile, + 4096 k
+        auto weigh = [&](uint8_t *to) {                          // bf16 rows times f1 + f2
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t f = sh.w[(tid >> 3) + k * 32];
+                const uint32_t f1 = __byte_perm(f, f, 0x1010), f2 = __byte_perm(f, f, 0x3232);
+                uint32_t e[4] = {rows[k].x, rows[k].y, rows[k].z, rows[k].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&e[q]);
+                    const __nv_bfloat162 o = __hfma2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f1),
+                                                     __hmul2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f2)));
+                    e[q] = *reinterpret_cast<const uint32_t *>(&o);
+                }
+                *reinterpret_cast<uint4 *>(to + swz + k * 4096) = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+        };
+        float ff[4];
+        auto part = [&](int which, uint8_t *to) {                // part 0, 1 or 2 of the weighted rows
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
                 float e[8], r[8];
                 unpack8<bf16>(rows[k], e);
 #pragma unroll
-                for (int m = 0; m < 8; ++m) e[m] *= f;
+                for (int m = 0; m < 8; ++m) e[m] *= ff[k];
                 uint4 out = pack8<bf16>(e);
-                for (int q = 0; q < part; ++q) {
+                for (int q = 0; q < which; ++q) {
                     unpack8<bf16>(out, r);
 #pragma unroll
                     for (int m = 0; m < 8; ++m) e[m] -= r[m];
                     out = pack8<bf16>(e);
                 }
-                *reinterpret_cast<uint4 *>(to + row * 128 + (((x & 7) ^ (row & 7)) << 4)) = out;
+                *reinterpret_cast<uint4 *>(to + swz + k * 4096) = out;
             }
         };
-        weigh(0, smV);
-        if (a.exact && !a.tiles) weigh(1, smS);
-        if (!a.exact && i + 1 < nc) fetch(i + 1, rows);
-        if (a.tiles && i > 0) ok = ok && mbar_wait(&stored, (i - 1) & 1);
-        if (a.tiles && n < NT) {                                 // what enters this chunk
+        fetch(0);
+        const int n = (warp & 3) * 32 + lane, half = warp >> 2, col = pb * kP + half * 32;
+        const long long at = (((long long)(a.by_seq ? s.seq : si) * a.h.H + h) * a.h.N + n) * a.h.P + col;
+        float S[32];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float e[8] = {S[8 * j], S[8 * j + 1], S[8 * j + 2], S[8 * j + 3], S[8 * j + 4], S[8 * j + 5], S[8 * j + 6], S[8 * j + 7]};
-                *reinterpret_cast<uint4 *>(smS + n * 128 + (((half * 4 + j) ^ (n & 7)) << 4)) = pack8<bf16>(e);
-            }
+        for (int j = 0; j < 32; ++j) S[j] = a.init && n < a.h.N && col + j < a.h.P ? a.init[at + j] : 0.f;
+        const uint32_t tl = tmem_lane_base(tmem) + half * 32;
+        auto arrive = [&]() {                                    // what this warp wrote is there, what it read of tensor memory is read
+            fence_async_smem();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.ready);
+        };
+        int round = 0;
+        if constexpr (!EXACT) {
+            ok = ws_wait_warp(&sh.weights, 0, fail, 4);
+            if (ok) weigh(smV);
+            fetch(1);
         }
-        ok = ok && mbar_wait(&full[st], (i >> 1) & 1);
-        if (ok && a.seg.packed && length(i) < kQ)
-            for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, length(i), tid, 256);
-        fence_async_smem();
-        tc_fence_before();                                       // the last step's loads from tensor memory
-        ok = __syncthreads_and(ok);
-        if (!ok) break;
-        auto issue = [&](const uint8_t *v, uint32_t first) {
+        for (int i = 0; i < nc && ok; ++i) {
+            const int st = i & 1;
+            float now;
+            if constexpr (EXACT) {
+                ok = ws_wait_warp(&sh.weights, i & 1, fail, 4);
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ff[k] = __uint_as_float(sh.w[(tid >> 3) + k * 32]);
+                part(0, smV);
+                part(1, smV + kSlab);
+                if (!a.tiles) part(2, smS);
+            }
+            now = sh.decay[st];
+            if (a.tiles) {                                       // what enters this chunk
+                if (i > 0) ok = ws_wait_warp(&sh.stored, (i - 1) & 1, fail, 5);
+                if (!ok) break;
+                if (n < NT) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float e[8] = {S[8 * j], S[8 * j + 1], S[8 * j + 2], S[8 * j + 3], S[8 * j + 4], S[8 * j + 5], S[8 * j + 6], S[8 * j + 7]};
+                        *reinterpret_cast<uint4 *>(smS + n * 128 + (((half * 4 + j) ^ (n & 7)) << 4)) = pack8<bf16>(e);
+                    }
+                }
+            }
+            if (a.seg.packed && length(i) < kQ) {
+                ok = ws_wait_warp(&sh.full[st], (i >> 1) & 1, fail, 6);
+                if (!ok) break;
+                for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, length(i), tid, 256);
+            }
+            arrive();
+            ++round;
+            if constexpr (EXACT) {
+                if (two) {                                       // the last part goes where the first was
+                    ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 7);
+                    if (!ok) break;
+                    part(2, smV);
+                    arrive();
+                    ++round;
+                }
+                fetch(i + 1);
+            } else if (i + 1 < nc) {                             // the next chunk's rows, while this one's product runs
+                ok = ws_wait_warp(&sh.weights, (i + 1) & 1, fail, 4);
+                if (!ok) break;
+                weigh(smV + (st ^ 1) * kSlab);
+                fetch(i + 2);
+            }
+            ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 8);
+            if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < kQ / 16; ++kk)                 // where NT is 64, rows 64 ... 127 are the first 64 again: products of no use
-                umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 0 : kSlab, 1024),
-                     smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : first);
-        };
-        if (warp == 0 && elect_one()) {
-            if (a.tiles) tma_store2(&tmTiles, smS, 0, (((c0 + place(i)) * a.h.H + h) * a.h.PB + pb) * NT);
-            issue(smV, 0u);
-            umma_commit(&done[uses & 1]);
-            if (a.exact && !a.tiles) {
-                issue(smS, 1u);
-                umma_commit(&done[(uses + 1) & 1]);
-            }
-            if (a.tiles) {                                       // S's tile may be written again
-                tma_store_read();
-                mbar_arrive(&stored);
+            for (int j0 = 0; j0 < 32; j0 += 16) {
+                float x[16];
+                tmem_ld16(tl + j0, x);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, x[j]);
             }
         }
-        uses += a.exact && !a.tiles ? 2 : 1;
-        if (a.exact) {                                           // the parts that are left, where the first was
-#pragma unroll
-            for (int part = 1; part < 3; ++part) {
-                if (part == 1 && !a.tiles) continue;
-                if (ok) ok = wait(a.tiles ? uses - 1 : uses - 2);
-                if (ok) weigh(part, smV);
-                fence_async_smem();
-                ok = __syncthreads_and(ok);
-                if (ok && warp == 0 && elect_one()) {
-                    issue(smV, 1u);
-                    umma_commit(&done[uses & 1]);
-                }
-                ++uses;
-            }
-            if (ok && i + 1 < nc) fetch(i + 1, rows);
-        }
-        if (ok && a.exact) ok = wait(uses - 2);                  // phases are waited for one by one
-        if (ok) ok = wait(uses - 1);
-        if (!ok) continue;                                       // leaves at the next barrier
-        tc_fence_after();
-        const float d = exp2f(whole[i % kAhead]);
-        total += whole[i % kAhead];
-        float v32[32];
-        tmem_ld32(tmem_lane_base(tmem) + half * 32, v32);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) S[j] = fmaf(S[j], d, v32[j]);
-    }
-    ok = __syncthreads_and(ok);
-    if (ok) {
-        if (a.fin && n < a.h.N) {
+        if (ok && a.fin && n < a.h.N) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
                 if (col + j < a.h.P) a.fin[at + j] = S[j];
         }
-        if (a.decay && pb == 0 && tid == 0) a.decay[(long long)si * a.h.H + h] = exp2f(total);
-    } else if (tid == 0) {
-        atomicExch(a.status, kErrDecay + 1);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
-        if (a.tiles && elect_one()) tma_store_wait();
-        if (!ok && elect_one()) {                                // leave nothing in flight
-            drain_mmas(&unused);
-            drain_loads(full, 2, loads);
-        }
-        __syncwarp();
-        tmem_dealloc(tmem, 64);
-    }
+    if (warp == 0) tmem_dealloc(tmem, 64);
 }
 
 // ---- the outputs -----------------------------------------------------------------------------------------------------
@@ -340,7 +420,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
              const __grid_constant__ CUtensorMap tmS) {
     pdl_begin();
     constexpr int kSlabs = NT / 64;
-    extern __shared__ uint8_t dyn[];
+    extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ uint64_t bar_qk, bar_v, done, unused;
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(16) float cs[2][kQ], below[2][64];      // c_t; 2^(c_63 - c_s) of the first 64 tokens
@@ -565,7 +645,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmG) {
     pdl_begin();
     constexpr int kSlabs = NT / 64, kT = 512;
-    extern __shared__ uint8_t dyn[];
+    extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ uint64_t bar_qk, bar_v, done, unused;
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(16) float c[kQ], ws[kQ], et[kQ];        // c_t; e^{c_end - c_s}; scale e^{c_t}
