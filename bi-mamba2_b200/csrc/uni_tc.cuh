@@ -98,8 +98,8 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
 // Forwards S' as above; backwards (v the outputs' gradient, k the queries) the gradient that enters each chunk from its right,
 // G' = e^{c_end} G + sum_t q_t (scale e^{c_t} do_t)^T.  A block walks the chunks of one (segment, head, 64 columns), S or G in
 // registers (a row n and 32 columns a thread).  k's rows come by TMA a chunk ahead; v's go through registers and are weighted on the
-// way to shared memory.  Eight warps do that, a chunk ahead too, and keep S; the ninth makes the weights, issues loads, MMAs and tile
-// stores, and the two meet at mbarriers alone.  So a step is S's way to shared memory, one product's latency and its way back,
+// way to shared memory.  Eight warps do that, a chunk ahead too, and keep S; the ninth issues loads and MMAs, the tenth makes the
+// weights and stores the tiles, and they meet at mbarriers alone.  So a step is S's way to shared memory, one product's latency and its way back,
 // with everything else in its shadow; with block-wide barriers and the weights made by one of the eight it was half as fast
 // again.  Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
 // A weight f meets bf16 rows as bf16 f1 + f2, in one rounding: v f1 + (v f2) as a multiply-add.
@@ -126,7 +126,7 @@ struct StatesShared {
     float decay[2];                                              // of a chunk, 2^c_end
     alignas(16) uint32_t w[kQ];                                  // of a chunk's rows: f1 and f2, or EXACT fp32
 };
-constexpr int kStatesThreads = 288;
+constexpr int kStatesThreads = 320;
 inline size_t states_smem(int NT) { return 2 * (size_t)(NT / 64) * kSlab + 3 * (size_t)kSlab + sizeof(StatesShared); }
 
 template <int NT, bool EXACT> __global__ void __launch_bounds__(kStatesThreads, 2)
@@ -148,8 +148,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     auto place = [&](int i) { return a.reverse ? nc - 1 - i : i; };        // chunk of the segment at step i
     auto length = [&](int i) { return min(kQ, s.len - place(i) * kQ); };
     volatile int *fail = &sh.fail;
-    constexpr int kRounds = EXACT ? 2 : 1;                       // of an exact step that stores a tile, which has the third part's buffer
-    const bool two = EXACT && a.tiles;
+    const bool two = EXACT && a.tiles;                           // an exact step that stores a tile, which has the third part's buffer, has two rounds
     if (warp == 0) tmem_alloc(&sh.tmem, 64);
     if (tid == 256) {
         mbar_init(&sh.full[0], 1);
@@ -167,49 +166,12 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     const uint32_t tmem = sh.tmem;
     bool ok = true;
     if (warp == 8) {
-        const int c0 = uni::segments(a.chunk, s.seq).x + s.idx * (a.seg.seg / kQ);
-        Decays d;
-        uint32_t f[4];
-        float whole = 0.f, total = 0.f;
         auto load = [&](int i) {
             const int st = i & 1, t = s.t0 + place(i) * kQ;
             mbar_expect_tx(&sh.full[st], kSlabs * kSlab);
             for (int j = 0; j < kSlabs; ++j) tma_load4(smK + (st * kSlabs + j) * kSlab, &tmK, j * 64, hq, t, s.batch, &sh.full[st]);
         };
-        auto ask = [&](int i) {
-            if (i < nc) d.load(a.h, s.batch, s.t0 + place(i) * kQ, length(i), h, lane);
-        };
-        auto make = [&]() {                                      // the weights of what was asked for last
-            float c[4], p[4];
-            d.log2(a.h);
-            d.prefix(p, lane);
-            whole = __shfl_sync(0xffffffffu, p[3], 31);
-            if (!a.reverse) d.suffix(c, lane);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float v = exp2f(a.reverse ? p[k] + a.h.log_scale : c[k]);
-                if constexpr (EXACT) {
-                    f[k] = __float_as_uint(v);
-                } else {
-                    const float hi = __bfloat162float(__float2bfloat16_rn(v));
-                    f[k] = pack2<bf16>(hi, v - hi);
-                }
-            }
-        };
-        auto give = [&](int i) {                                 // to the others, as chunk i's
-            *reinterpret_cast<uint4 *>(&sh.w[lane * 4]) = make_uint4(f[0], f[1], f[2], f[3]);
-            if (lane == 0) sh.decay[i & 1] = exp2f(whole);
-            total += whole;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.weights);
-        };
         if (lane == 0) load(0);
-        ask(0);
-        make();
-        give(0);
-        ask(1);
-        if (nc > 1) make();
-        ask(2);
         int loads = 1, round = 0;
         constexpr uint32_t idesc = instr_desc(1, true, true, kP);
         for (int i = 0; i < nc && ok; ++i) {
@@ -226,11 +188,10 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                     umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 0 : kSlab, 1024),
                          smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : first);
             };
-            for (int r = 0; r < (two ? kRounds : 1) && ok; ++r, ++round) {
+            for (int r = 0; r < (two ? 2 : 1) && ok; ++r, ++round) {
                 ok = ws_wait_warp(&sh.ready, round & 1, fail, 3);
                 if (!ok) break;
                 tc_fence_after();
-                if (r == 0 && i + 1 < nc) give(i + 1);
                 if (elect_one()) {
                     if (r == 1) {
                         issue(smV, 1u);
@@ -242,26 +203,77 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                         }
                     }
                     umma_commit(&sh.done);
-                    if (r == 0 && a.tiles) {
-                        tma_store2(&tmTiles, smS, 0, (((c0 + place(i)) * a.h.H + h) * a.h.PB + pb) * NT);
-                        tma_store_read();                        // S's tile may be written again
-                        mbar_arrive(&sh.stored);
-                    }
                 }
                 __syncwarp();
             }
-            if (ok && i + 2 < nc) {
-                make();
-                ask(i + 3);
-            }
         }
-        if (a.decay && ok && pb == 0 && lane == 0) a.decay[(long long)si * a.h.H + h] = exp2f(total);
-        if (a.tiles && elect_one()) tma_store_wait();
         if (!ok && elect_one()) {                                // leave nothing in flight
             drain_mmas(&sh.unused);
             drain_loads(sh.full, 2, loads);
             atomicExch(a.status, kErrDecay + 0x10 + *fail);
         }
+        __syncwarp();
+    } else if (warp == 9) {
+        const int c0 = uni::segments(a.chunk, s.seq).x + s.idx * (a.seg.seg / kQ);
+        Decays d;
+        uint32_t f[4];
+        float whole = 0.f, total = 0.f;
+        auto ask = [&](int i) {
+            if (i < nc) d.load(a.h, s.batch, s.t0 + place(i) * kQ, length(i), h, lane);
+        };
+        auto make = [&]() {                                      // the weights of what was asked for last
+            float c[4];
+            d.log2(a.h);
+            if (a.reverse) {
+                d.prefix(c, lane);
+                whole = __shfl_sync(0xffffffffu, c[3], 31);
+            } else {
+                d.suffix(c, lane);
+                whole = __shfl_sync(0xffffffffu, c[0] + d.v[0], 0);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float v = exp2f(a.reverse ? c[k] + a.h.log_scale : c[k]);
+                if constexpr (EXACT) {
+                    f[k] = __float_as_uint(v);
+                } else {
+                    const float hi = __bfloat162float(__float2bfloat16_rn(v));
+                    f[k] = pack2<bf16>(hi, v - hi);
+                }
+            }
+        };
+        auto give = [&](int i) {                                 // to the others, as chunk i's
+            *reinterpret_cast<uint4 *>(&sh.w[lane * 4]) = make_uint4(f[0], f[1], f[2], f[3]);
+            if (lane == 0) sh.decay[i & 1] = exp2f(whole);
+            total += whole;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.weights);
+        };
+        ask(0);
+        make();
+        give(0);
+        ask(1);
+        if (nc > 1) make();
+        ask(2);
+        for (int i = 0; i < nc; ++i) {
+            ok = ws_wait_warp(&sh.ready, (two ? 2 * i : i) & 1, fail, 9);
+            if (!ok) break;
+            if (i + 1 < nc) give(i + 1);
+            if (a.tiles && elect_one()) {
+                tma_store2(&tmTiles, smS, 0, (((c0 + place(i)) * a.h.H + h) * a.h.PB + pb) * NT);
+                tma_store_read();                                // S's tile may be written again
+                mbar_arrive(&sh.stored);
+            }
+            __syncwarp();
+            if (i + 2 < nc) {
+                make();
+                ask(i + 3);
+            }
+            if (two) ok = ws_wait_warp(&sh.ready, 1, fail, 9);   // the last part's
+            if (!ok) break;
+        }
+        if (a.decay && ok && pb == 0 && lane == 0) a.decay[(long long)si * a.h.H + h] = exp2f(total);
+        if (a.tiles && elect_one()) tma_store_wait();
         __syncwarp();
     } else {
         // 16 bytes of rows tid / 8 + 32 k of v
