@@ -71,10 +71,19 @@ struct Sizes {
     long long tokens;
 };
 
-int power_lanes(int rows) {                                      // 32 rows a thread at most
+// Lanes that share a column of `rows` rows: enough for 32 rows a thread at most, and as many as leave no thread of a block without
+// a column, down to four rows a thread (a walk is a chain of tokens: us for 253 tokens of 4 heads of 16 x 32 fp32, one lane a column
+// 126, four 56).
+int walk_lanes(int rows, int columns) {
     int l = 1;
     while (l * 32 < rows) l *= 2;
+    while (l < 32 && l * 4 < rows && uni::kWalkThreads / l > columns) l *= 2;
     return l;
+}
+int walk_rows(int rows, int lanes) {                             // rows a thread
+    int n = 4;
+    while (n * lanes < rows) n *= 2;
+    return n;
 }
 
 int decay_check(const bissd_decay_args *a, bool backward) {
@@ -97,7 +106,7 @@ Sizes sizes_of(const bissd_decay_args *a) {
     Sizes z;
     z.sequences = a->nseq > 0 ? a->nseq : a->batch;
     z.H = a->nheads; z.hk = a->nkheads; z.N = a->kdim; z.P = a->vdim;
-    z.lanes_n = power_lanes(a->kdim); z.lanes_p = power_lanes(a->vdim);
+    z.lanes_n = walk_lanes(a->kdim, a->vdim); z.lanes_p = walk_lanes(a->vdim, a->kdim);
     z.tokens = (long long)a->batch * a->seqlen;
     return z;
 }
@@ -117,32 +126,34 @@ uni::Plan plan_of(const bissd_decay_args *a, int seg, Bump &ws, uni::PlanOut *ou
     return p;
 }
 
-// Tokens to a segment on CUDA cores: long rows in as many as fill the SMs four times over, none under 256 tokens (what two more walks
-// without outputs cost then); packed sequences in segments of 256.
+// Tokens to a segment on CUDA cores: long rows in as many as fill the SMs four times over, none under 64 tokens (a token takes 0.2 us in
+// a block, and what two more launches cost is as much as 40 of them); packed sequences in segments of 256.
 int walk_segment(const bissd_decay_args *a, const Sizes &z) {
     if (a->nseq > 0) return 256;
     const long long blocks = (long long)a->batch * z.H * ceil_div(z.P * z.lanes_n, uni::kWalkThreads);
     const long long parts = std::max<long long>(1, 4 * 148 / blocks);
-    return std::max(256, ceil_div((int)((a->seqlen + parts - 1) / parts), 256) * 256);
+    const int seg = ceil_div((int)((a->seqlen + parts - 1) / parts), 64) * 64;
+    return a->seqlen <= 3 * 64 && parts > 1 ? 3 * 64 : seg;
 }
 
 int launch_walk(int dtype, const uni::WalkParams &w, cudaStream_t s) {
-    const int ipt = w.I <= 16 ? 16 : 32, cols = uni::kWalkThreads / w.lanes;
+    const int ipt = walk_rows(w.I, w.lanes), cols = uni::kWalkThreads / w.lanes;
     const size_t smem = uni::walk_smem(w.lanes, ipt);
     const long long grid = (long long)w.plan.most * w.H * ceil_div(w.J, cols);
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     return by_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const auto kernel = ipt == 16 ? uni::decay_walk<T, 16> : uni::decay_walk<T, 32>;
+        const auto kernel = ipt == 4 ? uni::decay_walk<T, 4> : ipt == 8 ? uni::decay_walk<T, 8> : ipt == 16 ? uni::decay_walk<T, 16> : uni::decay_walk<T, 32>;
         BISSD_ALLOW(kernel, smem);
         BISSD_LAUNCH(w.y ? "decay_walk" : "decay_walk_states", launch_pdl(kernel, (int)grid, uni::kWalkThreads, smem, s, w));
         return BISSD_OK;
     });
 }
 int launch_chain(const uni::ChainParams &c, cudaStream_t s) {
-    const long long grid = (long long)c.nseq * c.H * ceil_div(c.per, 256);
+    const bool quads = c.per % 4 == 0 && aligned16(c.start) && aligned16(c.states) && aligned16(c.end);
+    const long long grid = (long long)c.nseq * c.H * ceil_div(c.per, quads ? 1024 : 256);
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
-    BISSD_LAUNCH("decay_chain", launch_pdl(uni::decay_chain, (int)grid, 256, 0, s, c));
+    BISSD_LAUNCH("decay_chain", launch_pdl(quads ? uni::decay_chain<4> : uni::decay_chain<1>, (int)grid, 256, 0, s, c));
     return BISSD_OK;
 }
 int launch_plan(const bissd_decay_args *a, const uni::PlanOut &x, const uni::PlanOut *y, cudaStream_t s) {

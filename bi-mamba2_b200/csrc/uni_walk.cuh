@@ -39,7 +39,7 @@ struct WalkParams {
 inline int walk_tile(int lanes) { return lanes > 4 ? 16 : 32; }  // tokens staged at a time
 inline size_t walk_smem(int lanes, int ipt) {
     const int tile = walk_tile(lanes), cols = kWalkThreads / lanes;
-    return sizeof(float) * ((size_t)tile * 2 * lanes * (ipt + 4) + 2 * (size_t)tile * cols + tile);
+    return sizeof(float) * ((size_t)tile * 2 * lanes * (ipt + 4) + 2 * (size_t)tile * cols + 2 * tile);
 }
 
 template <class T, int IPT> __global__ void __launch_bounds__(kWalkThreads) decay_walk(WalkParams a) {
@@ -47,7 +47,7 @@ template <class T, int IPT> __global__ void __launch_bounds__(kWalkThreads) deca
     extern __shared__ float dyn[];
     if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
     const int LI = a.lanes, cols = kWalkThreads / LI, tile = LI > 4 ? 16 : 32, rowlen = LI * (IPT + 4);
-    float *as = dyn, *rs = as + tile * rowlen, *bs = rs + tile * rowlen, *ys = bs + tile * cols, *ds = ys + tile * cols;
+    float *as = dyn, *rs = as + tile * rowlen, *bs = rs + tile * rowlen, *ys = bs + tile * cols, *ds = ys + tile * cols, *es = ds + tile;
     const int jb = (a.J + cols - 1) / cols;
     const int cb = blockIdx.x % jb, h = blockIdx.x / jb % a.H, si = blockIdx.x / (jb * a.H);
     const Segment s = segment(a.plan, si);
@@ -65,51 +65,60 @@ template <class T, int IPT> __global__ void __launch_bounds__(kWalkThreads) deca
     };
     float total = 0.f;
     for (int done = 0; done < s.len; done += tile) {
-        const int n = min(tile, s.len - done);
+        const int n = min(tile, s.len - done), n4 = (n + 3) & ~3;   // four tokens at a time: those behind the last change nothing
         const int first = a.reverse ? s.t0 + s.len - done - n : s.t0 + done;   // lowest token of the tile
         __syncthreads();
-        for (int x = tid; x < n * LI * IPT; x += kWalkThreads) {
-            const int t = x / (LI * IPT), i = x % (LI * IPT), at = t * rowlen + i / IPT * (IPT + 4) + i % IPT;
-            as[at] = i < a.I ? a.a_scale * ld<T>(a.a.v.ptr, row(a.a, first + t) + i) : 0.f;
-            if (a.y) rs[at] = i < a.I ? ld<T>(a.r.v.ptr, row(a.r, first + t) + i) : 0.f;
+        // eight loads under way at a time; what lies outside is zero
+        const int across = LI * IPT;
+        for (int x0 = tid; x0 < n4 * across; x0 += 8 * kWalkThreads) {
+            float va[8], vr[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int x = x0 + k * kWalkThreads, t = x / across, i = x % across;
+                const bool in = x < n * across && i < a.I;
+                va[k] = in ? a.a_scale * ld<T>(a.a.v.ptr, row(a.a, first + t) + i) : 0.f;
+                vr[k] = in && a.y ? ld<T>(a.r.v.ptr, row(a.r, first + t) + i) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int x = x0 + k * kWalkThreads, t = x / across, i = x % across, at = t * rowlen + i / IPT * (IPT + 4) + i % IPT;
+                if (x < n4 * across) {
+                    as[at] = va[k];
+                    rs[at] = vr[k];
+                }
+            }
         }
-        for (int x = tid; x < n * cols; x += kWalkThreads) {
-            const int t = x / cols, c = cb * cols + x % cols;
-            bs[x] = c < a.J ? ld<T>(a.b.v.ptr, row(a.b, first + t) + c) : 0.f;
+        for (int x0 = tid; x0 < n4 * cols; x0 += 8 * kWalkThreads) {
+            float vb[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int x = x0 + k * kWalkThreads, t = x / cols, c = cb * cols + x % cols;
+                vb[k] = x < n * cols && c < a.J ? ld<T>(a.b.v.ptr, row(a.b, first + t) + c) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (x0 + k * kWalkThreads < n4 * cols) bs[x0 + k * kWalkThreads] = vb[k];
         }
-        if (tid < n) {
+        if (tid < n4) {
             const int t = first + tid + a.reverse;
             float g = 0.f;
-            if (!(a.reverse && s.last && t == s.t0 + s.len))
+            if (tid < n && !(a.reverse && s.last && t == s.t0 + s.len))
                 g = ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)t * a.g.sl + (long long)h * a.g.sh);
             ds[tid] = g;
+            es[tid] = expf(g);
         }
         __syncthreads();
         if (a.decay && tid == 0)
             for (int t = 0; t < n; ++t) total += ds[t];
-        for (int u = 0; u < n; ++u) {
-            const int t = a.reverse ? n - 1 - u : u;
-            const float d = expf(ds[t]), b = bs[t * cols + jc];
-            const float4 *a4 = reinterpret_cast<const float4 *>(as + t * rowlen + li * (IPT + 4));
-            const float4 *r4 = reinterpret_cast<const float4 *>(rs + t * rowlen + li * (IPT + 4));
-            if (a.y) {
-                float acc = 0.f, acc2 = 0.f;
+        for (int u = 0; u < n4; u += 4) {
+            float acc[4];
 #pragma unroll
-                for (int e = 0; e < IPT; e += 4) {
-                    const float4 x = a4[e / 4], r = r4[e / 4];
-                    st_[e] = st_[e] * d + x.x * b;
-                    st_[e + 1] = st_[e + 1] * d + x.y * b;
-                    st_[e + 2] = st_[e + 2] * d + x.z * b;
-                    st_[e + 3] = st_[e + 3] * d + x.w * b;
-                    acc += r.x * st_[e];
-                    acc2 += r.y * st_[e + 1];
-                    acc += r.z * st_[e + 2];
-                    acc2 += r.w * st_[e + 3];
-                }
-                acc += acc2;
-                for (int o = 1; o < LI; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-                if (li == 0) ys[t * cols + jc] = acc * a.y_scale;
-            } else {
+            for (int w = 0; w < 4; ++w) {
+                const int t = a.reverse ? n4 - 1 - u - w : u + w;
+                const float d = es[t], b = bs[t * cols + jc];
+                const float4 *a4 = reinterpret_cast<const float4 *>(as + t * rowlen + li * (IPT + 4));
+                const float4 *r4 = reinterpret_cast<const float4 *>(rs + t * rowlen + li * (IPT + 4));
+                float sum = 0.f, sum2 = 0.f;
 #pragma unroll
                 for (int e = 0; e < IPT; e += 4) {
                     const float4 x = a4[e / 4];
@@ -117,6 +126,24 @@ template <class T, int IPT> __global__ void __launch_bounds__(kWalkThreads) deca
                     st_[e + 1] = st_[e + 1] * d + x.y * b;
                     st_[e + 2] = st_[e + 2] * d + x.z * b;
                     st_[e + 3] = st_[e + 3] * d + x.w * b;
+                    if (a.y) {
+                        const float4 r = r4[e / 4];
+                        sum += r.x * st_[e];
+                        sum2 += r.y * st_[e + 1];
+                        sum += r.z * st_[e + 2];
+                        sum2 += r.w * st_[e + 3];
+                    }
+                }
+                acc[w] = sum + sum2;
+            }
+            if (a.y) {
+                for (int o = 1; o < LI; o <<= 1) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) acc[w] += __shfl_xor_sync(0xffffffffu, acc[w], o);
+                }
+                if (li == 0) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) ys[(a.reverse ? n4 - 1 - u - w : u + w) * cols + jc] = acc[w] * a.y_scale;
                 }
             }
         }
@@ -154,37 +181,57 @@ struct ChainParams {
     View g;
     int g_dtype;
 };
-__global__ void __launch_bounds__(256) decay_chain(ChainParams a) {
+template <int VEC> struct Quad { float v[VEC]; };
+template <int VEC> __device__ __forceinline__ Quad<VEC> quad_ld(const float *p) {
+    Quad<VEC> q;
+    if constexpr (VEC == 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(p);
+        q.v[0] = f.x; q.v[1] = f.y; q.v[2] = f.z; q.v[3] = f.w;
+    } else {
+        q.v[0] = *p;
+    }
+    return q;
+}
+template <int VEC> __device__ __forceinline__ void quad_st(float *p, const Quad<VEC> &q) {
+    if constexpr (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(q.v[0], q.v[1], q.v[2], q.v[3]);
+    else *p = q.v[0];
+}
+template <int VEC> __global__ void __launch_bounds__(256) decay_chain(ChainParams a) {
     pdl_begin();
-    const int blocks = (a.per + 255) / 256;
-    const int e = blockIdx.x % blocks * 256 + threadIdx.x, h = blockIdx.x / blocks % a.H, seq = blockIdx.x / (blocks * a.H);
+    const int blocks = (a.per + 256 * VEC - 1) / (256 * VEC);
+    const int e = (blockIdx.x % blocks * 256 + threadIdx.x) * VEC, h = blockIdx.x / blocks % a.H, seq = blockIdx.x / (blocks * a.H);
     if (e >= a.per) return;
     const long long of_seq = ((long long)seq * a.H + h) * a.per + e;
     const int2 f = segments(a.plan, seq);
-    float run = a.start ? a.start[of_seq] : 0.f;
-    for (int u0 = 0; u0 < f.y; u0 += 8) {                        // eight segments' values under way at a time
-        float own[8], d[8];
+    Quad<VEC> run = {};
+    if (a.start) run = quad_ld<VEC>(a.start + of_seq);
+    for (int u0 = 0; u0 < f.y; u0 += 4) {                        // four segments' values under way at a time
+        Quad<VEC> own[4];
+        float d[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int u = u0 + k, i = f.x + (a.reverse ? f.y - 1 - u : u);
-            own[k] = u < f.y ? a.states[((long long)i * a.H + h) * a.per + e] : 0.f;
-            d[k] = u < f.y ? a.decay[(long long)i * a.H + h] : 1.f;
+        for (int k = 0; k < 4; ++k) {
+            const int u = min(u0 + k, f.y - 1), i = f.x + (a.reverse ? f.y - 1 - u : u);
+            own[k] = quad_ld<VEC>(a.states + ((long long)i * a.H + h) * a.per + e);
+            d[k] = a.decay[(long long)i * a.H + h];
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
             const int u = u0 + k, i = f.x + (a.reverse ? f.y - 1 - u : u);
             if (u < f.y) {
-                a.states[((long long)i * a.H + h) * a.per + e] = run;
-                run = run * d[k] + own[k];
+                quad_st<VEC>(a.states + ((long long)i * a.H + h) * a.per + e, run);
+#pragma unroll
+                for (int x = 0; x < VEC; ++x) run.v[x] = run.v[x] * d[k] + own[k].v[x];
             }
         }
     }
     if (a.end) {
         if (a.first_decay && f.y > 0) {
             const Segment s = segment(a.plan, f.x);
-            run *= expf(ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)s.t0 * a.g.sl + (long long)h * a.g.sh));
+            const float d = expf(ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)s.t0 * a.g.sl + (long long)h * a.g.sh));
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) run.v[x] *= d;
         }
-        a.end[of_seq] = run;
+        quad_st<VEC>(a.end + of_seq, run);
     }
 }
 
