@@ -407,6 +407,8 @@ bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, co
     return make_map2(m, BISSD_BF16, tiles, unitc::kP, (unsigned long long)t.chunk.most * a->nheads * t.PB * t.NT, unitc::kP, t.NT);
 }
 
+constexpr double kChunkStart = 2.0;                              // a block's start and the product q.k, in tiles of v
+
 int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     const TcSpace t = tc_space(a, ws);
     int *status = reinterpret_cast<int *>(ws.base);
@@ -422,9 +424,18 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     unitc::ChunksParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
+    // blocks a (chunk, head of q): as many as fill two blocks an SM, in the fewest rounds
     const int tiles_v = a->nheads / a->nkheads * t.PB;
-    const long long all = (long long)t.chunk.most * a->nkheads * tiles_v;
-    p.vpc = (int)std::max<long long>(1, std::min<long long>(tiles_v, all / (4 * 2 * 148)));
+    const long long items = (long long)t.chunk.most * a->nkheads, slots = 2 * 148;
+    double best = 0;
+    for (int parts = 1; parts <= tiles_v; ++parts) {
+        const int vpc = ceil_div(tiles_v, parts);
+        const double time = (double)((items * ceil_div(tiles_v, vpc) + slots - 1) / slots) * (kChunkStart + vpc);
+        if (parts == 1 || time < best) {
+            best = time;
+            p.vpc = vpc;
+        }
+    }
     p.parts = ceil_div(tiles_v, p.vpc);
     const auto kernel = t.NT == 64 ? unitc::decay_chunks<64> : unitc::decay_chunks<128>;
     const size_t smem = unitc::chunks_smem(t.NT);

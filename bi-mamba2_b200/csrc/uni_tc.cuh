@@ -431,62 +431,67 @@ template <int NT> __global__ void __launch_bounds__(256, 2)
 decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
              const __grid_constant__ CUtensorMap tmS) {
     pdl_begin();
-    constexpr int kSlabs = NT / 64;
+    constexpr int kSlabs = NT / 64, kTables = 8;                 // heads whose tables are made at a time, one a warp
     extern __shared__ __align__(1024) uint8_t dyn[];
-    __shared__ uint64_t bar_qk, bar_v, done, unused;
+    __shared__ uint64_t bar_qk, bar_v, bar_s, done, done_s, unused;
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float cs[2][kQ], below[2][64];      // c_t; 2^(c_63 - c_s) of the first 64 tokens
+    __shared__ __align__(16) float cs[kTables][kQ], below[kTables][64];   // c_t; 2^(c_63 - c_s) of the first 64 tokens
     uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + 2 * kSlab, *smS = smV + kSlab;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int part = blockIdx.x % a.parts, m = blockIdx.x / a.parts % a.h.hk, ci = blockIdx.x / (a.parts * a.h.hk);
     const Segment s = uni::segment(a.chunk, ci);
     if (s.len == 0) return;
-    const int R = a.h.H / a.h.hk, v0 = part * a.vpc, nv = min(a.vpc, R * a.h.PB - v0);
+    const int R = a.h.H / a.h.hk, v0 = part * a.vpc, nv = min(a.vpc, R * a.h.PB - v0), h0 = m * R + v0 / a.h.PB;
     auto head = [&](int i) { return m * R + (v0 + i) / a.h.PB; };
+    const int heads = head(nv - 1) - h0 + 1;
     auto load_v = [&](int i) {
-        const int h = head(i), pb = (v0 + i) % a.h.PB;
-        mbar_expect_tx(&bar_v, kSlab + NT * 128);
-        tma_load4(smV, &tmV, pb * kP, h, s.t0, s.batch, &bar_v);
-        tma_load2(smS, &tmS, 0, ((ci * a.h.H + h) * a.h.PB + pb) * NT, &bar_v);
+        mbar_expect_tx(&bar_v, kSlab);
+        tma_load4(smV, &tmV, (v0 + i) % a.h.PB * kP, head(i), s.t0, s.batch, &bar_v);
     };
-    auto table = [&](int i, Decays d) {                          // one warp
+    auto load_s = [&](int i) {
+        mbar_expect_tx(&bar_s, NT * 128);
+        tma_load2(smS, &tmS, 0, ((ci * a.h.H + head(i)) * a.h.PB + (v0 + i) % a.h.PB) * NT, &bar_s);
+    };
+    Decays next;                                                 // this warp's head of the next kTables
+    auto ask = [&](int k) {
+        if (k < heads) next.load(a.h, s.batch, s.t0, s.len, h0 + k, lane);
+    };
+    auto table = [&](int k) {
+        if (k >= heads) return;
         float c[4];
-        d.log2(a.h);
-        d.prefix(c, lane);
+        next.log2(a.h);
+        next.prefix(c, lane);
         const float corner = __shfl_sync(0xffffffffu, c[3], 15);
+        *reinterpret_cast<float4 *>(&cs[warp][lane * 4]) = make_float4(c[0], c[1], c[2], c[3]);
+        if (lane < 16) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            cs[i & 1][lane * 4 + k] = c[k];
-            if (lane < 16) below[i & 1][lane * 4 + k] = exp2f(corner - c[k]);
+            for (int q = 0; q < 4; ++q) below[warp][lane * 4 + q] = exp2f(corner - c[q]);
         }
     };
+    ask(warp);
     if (warp == 0) tmem_alloc(&tmem_slot, 256);
     if (tid == 32) {
         mbar_init(&bar_qk, 1);
         mbar_init(&bar_v, 1);
+        mbar_init(&bar_s, 1);
         mbar_init(&done, 1);
+        mbar_init(&done_s, 1);
         fence_mbar_init();
         mbar_expect_tx(&bar_qk, 2 * kSlabs * kSlab);
         for (int j = 0; j < kSlabs; ++j) {
             tma_load4(smQ + j * kSlab, &tmQ, j * 64, m, s.t0, s.batch, &bar_qk);
             tma_load4(smK + j * kSlab, &tmK, j * 64, m, s.t0, s.batch, &bar_qk);
         }
+        load_s(0);
         load_v(0);
     }
-    Decays next;                                                 // warp 2: of the next head
-    auto fetch = [&](int i) {
-        if (i < nv && head(i) != head(i - 1)) next.load(a.h, s.batch, s.t0, s.len, head(i), lane);
-    };
-    if (warp == 2) {
-        next.load(a.h, s.batch, s.t0, s.len, head(0), lane);
-        table(0, next);
-        fetch(1);
-    }
+    table(warp);
+    ask(kTables + warp);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot, tl = tmem_lane_base(tmem);  // columns: 0 q.k, 128 inside the chunk, 192 from the state
-    int loads = 1, waits = 0;
+    int loads_v = 1, loads_s = 1;
     bool ok = true;
     if (warp == 0 && elect_one()) {
         ok = mbar_wait(&bar_qk, 0);
@@ -500,26 +505,31 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         }
     }
     if (ok) ok = mbar_wait(&done, 0);
-    ++waits;
+    ok = __syncthreads_and(ok);                                  // k's rows are dead: the weighted pairs take their place
+    tc_fence_after();
     const int t = (warp & 3) * 32 + lane, half = warp >> 2;      // this thread: row t, columns of `half` of each tile
     const bool diagonal = (t >> 6) == half, empty = (t >> 6) < half;
-    for (int i = 0; i < nv; ++i) {
-        if (ok) ok = mbar_wait(&bar_v, i & 1);
-        if (ok && a.chunk.packed && s.len < kQ) {
-            clear_rows(smV, s.len, tid, 256);
-            fence_async_smem();
+    for (int i = 0; i < nv && ok; ++i) {
+        const int k = head(i) - h0;
+        if (i > 0 && k % kTables == 0 && head(i) != head(i - 1)) {
+            __syncthreads();                                     // the last tables have been read
+            table(k + warp);
+            ask(k + kTables + warp);
+            __syncthreads();
         }
-        ok = __syncthreads_and(ok);
-        if (!ok) break;
-        tc_fence_after();
         if (warp == 0 && elect_one()) {                          // from the state: Q S
-            constexpr uint32_t idesc = instr_desc(1, false, true, kP);
+            ok = mbar_wait(&bar_s, i & 1);
+            if (ok) {
+                tc_fence_after();
+                constexpr uint32_t idesc = instr_desc(1, false, true, kP);
 #pragma unroll
-            for (int kk = 0; kk < NT / 16; ++kk)
-                umma(tmem + 192, smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
-                     smem_desc(smem_u32(smS) + kk * 2048, NT * 128, 1024), idesc, kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < NT / 16; ++kk)
+                    umma(tmem + 192, smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
+                         smem_desc(smem_u32(smS) + kk * 2048, NT * 128, 1024), idesc, kk > 0 ? 1u : 0u);
+                umma_commit(&done_s);
+            }
         }
-        const float *c = cs[i & 1];
+        const float *c = cs[k % kTables];
         const float ct = c[t] + a.h.log_scale;
         uint8_t *row = smK + half * kSlab + t * 128;             // 64 weighted pairs, 16-byte pieces swizzled
         if (empty) {
@@ -544,7 +554,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                         x[j + 2] = col + 2 <= td ? x[j + 2] * ex2_approx(ct - f.z) : 0.f;
                         x[j + 3] = col + 3 <= td ? x[j + 3] * ex2_approx(ct - f.w) : 0.f;
                     } else {
-                        const float4 f = *reinterpret_cast<const float4 *>(below[i & 1] + col);
+                        const float4 f = *reinterpret_cast<const float4 *>(below[k % kTables] + col);
                         x[j] *= rt * f.x;
                         x[j + 1] *= rt * f.y;
                         x[j + 2] *= rt * f.z;
@@ -558,37 +568,38 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                 }
             }
         }
+        if (a.chunk.packed && s.len < kQ) {
+            ok = ok && mbar_wait(&bar_v, i & 1);
+            if (ok) clear_rows(smV, s.len, tid, 256);
+        }
         fence_async_smem();
-        __syncthreads();
-        if (warp == 0 && elect_one()) {                          // inside the chunk: the weighted pairs times v
-            constexpr uint32_t idesc = instr_desc(1, false, true, kP);
-#pragma unroll
-            for (int kk = 0; kk < kQ / 16; ++kk)
-                umma(tmem + 128, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
-                     smem_desc(smem_u32(smV) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : 0u);
-            umma_commit(&done);
-        }
-        const bool another = i + 1 < nv && head(i + 1) != head(i);
-        if (warp == 2 && i + 1 < nv) {
-            if (another) {
-                table(i + 1, next);
-            } else {
-                for (int k = lane; k < kQ; k += 32) cs[(i + 1) & 1][k] = c[k];
-                for (int k = lane; k < 64; k += 32) below[(i + 1) & 1][k] = below[i & 1][k];
-            }
-            fetch(i + 2);
-        }
-        ok = mbar_wait(&done, waits & 1);
-        ++waits;
         ok = __syncthreads_and(ok);
         if (!ok) break;
-        tc_fence_after();
-        if (i + 1 < nv) {
-            if (tid == 32) load_v(i + 1);
-            ++loads;
+        if (warp == 0 && elect_one()) {                          // inside the chunk: the weighted pairs times v
+            ok = mbar_wait(&bar_v, i & 1);
+            if (ok) {
+                tc_fence_after();
+                constexpr uint32_t idesc = instr_desc(1, false, true, kP);
+#pragma unroll
+                for (int kk = 0; kk < kQ / 16; ++kk)
+                    umma(tmem + 128, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
+                         smem_desc(smem_u32(smV) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : 0u);
+                umma_commit(&done);
+            }
         }
+        if (i + 1 < nv) {                                        // the state's tile is long read; v's rows when all is done
+            if (tid == 32) ok = mbar_wait(&done_s, i & 1);
+            if (tid == 32 && ok) load_s(i + 1);
+            ++loads_s;
+        }
+        if (ok) ok = mbar_wait(&done, (i + 1) & 1) && mbar_wait(&done_s, i & 1);
+        if (i + 1 < nv) {
+            if (tid == 32 && ok) load_v(i + 1);
+            ++loads_v;
+        }
+        tc_fence_after();
         // o = inside + scale e^{c_t} from the state; whole rows leave through the first slab of the weighted pairs
-        {
+        if (ok) {
             const float f = exp2f(ct);
             float x[32], y[32];
             tmem_ld32(tl + 128 + half * 32, x);
@@ -597,21 +608,24 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
             for (int j = 0; j < 32; j += 8) {
                 float e[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) e[k] = fmaf(y[j + k], f, x[j + k]);
+                for (int q = 0; q < 8; ++q) e[q] = fmaf(y[j + q], f, x[j + q]);
                 *reinterpret_cast<uint4 *>(smK + t * 128 + (((half * 4 + (j >> 3)) ^ (t & 7)) << 4)) = pack8<bf16>(e);
             }
         }
         tc_fence_before();
-        __syncthreads();
-        const int h = head(i), col = (v0 + i) % a.h.PB * kP + (tid & 7) * 8;
+        ok = __syncthreads_and(ok);
+        if (!ok) break;
+        const int col = (v0 + i) % a.h.PB * kP + (tid & 7) * 8;
         if (col < a.h.P) {
-            bf16 *o = a.o + ((long long)s.batch * a.chunk.L + s.t0) * a.h.H * a.h.P + (long long)h * a.h.P + col;
+            bf16 *o = a.o + (((long long)s.batch * a.chunk.L + s.t0) * a.h.H + head(i)) * a.h.P + col;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int r = (tid >> 3) + k * 32;
+            for (int q = 0; q < 4; ++q) {
+                const int r = (tid >> 3) + q * 32;
                 if (r < s.len) *reinterpret_cast<uint4 *>(o + (long long)r * a.h.H * a.h.P) = *reinterpret_cast<const uint4 *>(smK + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
             }
         }
+        __syncthreads();                                         // the slab is the pairs' again
+        tc_fence_after();
     }
     ok = __syncthreads_and(ok);
     if (!ok && tid == 0) atomicExch(a.status, kErrDecay + 2);
@@ -621,7 +635,8 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         if (!ok && elect_one()) {                                // leave nothing in flight
             drain_mmas(&unused);
             drain_loads(&bar_qk, 1, 1);
-            drain_loads(&bar_v, 1, loads);
+            drain_loads(&bar_v, 1, loads_v);
+            drain_loads(&bar_s, 1, loads_s);
         }
         __syncwarp();
         tmem_dealloc(tmem, 256);
