@@ -11,6 +11,7 @@
 #pragma once
 #include "tc_tma.cuh"
 #include "uni_plan.cuh"
+#include "vec.cuh"
 
 namespace bissd {
 namespace unitc {
@@ -414,8 +415,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 // ---- the outputs -----------------------------------------------------------------------------------------------------
 // A block has one chunk of one head of q and k, and walks `vpc` of the tiles of v that share them: Q, K and their product stay, in
 // shared and tensor memory, and per tile come v's rows and the state.  The product, weighted by the decays and rounded to bf16 (it
-// meets v's bf16), takes K's place in shared memory.  Where a whole block of 64 x 64 lies below the diagonal, the weight is a row
-// factor times a column factor, both counted from the block's corner and at most 1; on the diagonal it is one 2^x an element.
+// meets v's bf16), takes K's place in shared memory.  Where a block of 32 x 32 lies below the diagonal, the weight is a row factor times a
+// column factor, both counted from the block's last column and at most 1; on the diagonal it is one 2^x an element.  A warp has
+// 32 rows and half of the columns up to the diagonal, in units of 16.
 // Two blocks an SM: one's loads and element-wise work run under the other's MMAs.
 struct ChunksParams {
     Heads h;
@@ -435,7 +437,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ uint64_t bar_qk, bar_v, bar_s, done, done_s, unused;
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float cs[kTables][kQ], below[kTables][64];   // c_t; 2^(c_63 - c_s) of the first 64 tokens
+    __shared__ __align__(16) float cs[kTables][kQ], below[kTables][kQ];   // c_t; 2^(c at the end of s' 32 - c_s)
     uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + 2 * kSlab, *smS = smV + kSlab;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int part = blockIdx.x % a.parts, m = blockIdx.x / a.parts % a.h.hk, ci = blockIdx.x / (a.parts * a.h.hk);
@@ -461,12 +463,9 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         float c[4];
         next.log2(a.h);
         next.prefix(c, lane);
-        const float corner = __shfl_sync(0xffffffffu, c[3], 15);
+        const float end = __shfl_sync(0xffffffffu, c[3], lane | 7);
         *reinterpret_cast<float4 *>(&cs[warp][lane * 4]) = make_float4(c[0], c[1], c[2], c[3]);
-        if (lane < 16) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) below[warp][lane * 4 + q] = exp2f(corner - c[q]);
-        }
+        *reinterpret_cast<float4 *>(&below[warp][lane * 4]) = make_float4(exp2f(end - c[0]), exp2f(end - c[1]), exp2f(end - c[2]), exp2f(end - c[3]));
     };
     ask(warp);
     if (warp == 0) tmem_alloc(&tmem_slot, 256);
@@ -507,8 +506,13 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     if (ok) ok = mbar_wait(&done, 0);
     ok = __syncthreads_and(ok);                                  // k's rows are dead: the weighted pairs take their place
     tc_fence_after();
-    const int t = (warp & 3) * 32 + lane, half = warp >> 2;      // this thread: row t, columns of `half` of each tile
-    const bool diagonal = (t >> 6) == half, empty = (t >> 6) < half;
+    const int r32 = warp & 3, t = r32 * 32 + lane, half = warp >> 2;   // this thread: row t, 32 columns of each output tile
+    const int u0 = half * (r32 + 1), u1 = u0 + r32 + 1;          // and units u0 ... u1 - 1 of 16 weighted pairs
+    auto pair_at = [&](int u) { return smK + (u >> 2) * kSlab + t * 128; };
+    auto piece = [&](int u, int j) { return (((u & 3) * 2 + j) ^ (t & 7)) << 4; };
+    if (ok && half == 1)
+        for (int u = 2 * (r32 + 1); u < 8; ++u)                  // above the diagonal
+            for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4 *>(pair_at(u) + piece(u, j)) = zero8();
     for (int i = 0; i < nv && ok; ++i) {
         const int k = head(i) - h0;
         if (i > 0 && k % kTables == 0 && head(i) != head(i - 1)) {
@@ -531,42 +535,48 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         }
         const float *c = cs[k % kTables];
         const float ct = c[t] + a.h.log_scale;
-        uint8_t *row = smK + half * kSlab + t * 128;             // 64 weighted pairs, 16-byte pieces swizzled
-        if (empty) {
-            if (i == 0) {
+        {
+            uint32_t raw[16];
+            tmem_ld16_nowait(tl + u0 * 16, raw);
+            for (int u = u0; u < u1; ++u) {
+                vec::f2 x[8];
+                tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4 *>(row + ((j ^ (t & 7)) << 4)) = zero8();
-            }
-        } else {
-            const float rt = exp2f(ct - c[63]);
+                for (int j = 0; j < 8; ++j) x[j] = vec::pack(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1]));
+                if (u + 1 < u1) tmem_ld16_nowait(tl + (u + 1) * 16, raw);
+                const int cb = u >> 1;
+                if (cb < r32) {
+                    const float rt = exp2f(ct - c[cb * 32 + 31]);
+                    const vec::f2 rt2 = vec::pack(rt, rt);
 #pragma unroll
-            for (int j0 = 0; j0 < 64; j0 += 32) {
-                float x[32];
-                tmem_ld32(tl + half * 64 + j0, x);
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 f = *reinterpret_cast<const float4 *>(below[k % kTables] + u * 16 + j * 4);
+                        x[2 * j] = vec::mul2(x[2 * j], vec::mul2(vec::pack(f.x, f.y), rt2));
+                        x[2 * j + 1] = vec::mul2(x[2 * j + 1], vec::mul2(vec::pack(f.z, f.w), rt2));
+                    }
+                } else {
+                    const int td = t - u * 16;                   // columns up to it; what is behind it may be no number
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const int col = j0 + j;
-                    if (diagonal) {
-                        const float4 f = *reinterpret_cast<const float4 *>(c + half * 64 + col);
-                        const int td = t & 63;
-                        x[j] = col <= td ? x[j] * ex2_approx(ct - f.x) : 0.f;
-                        x[j + 1] = col + 1 <= td ? x[j + 1] * ex2_approx(ct - f.y) : 0.f;
-                        x[j + 2] = col + 2 <= td ? x[j + 2] * ex2_approx(ct - f.z) : 0.f;
-                        x[j + 3] = col + 3 <= td ? x[j + 3] * ex2_approx(ct - f.w) : 0.f;
-                    } else {
-                        const float4 f = *reinterpret_cast<const float4 *>(below[k % kTables] + col);
-                        x[j] *= rt * f.x;
-                        x[j + 1] *= rt * f.y;
-                        x[j + 2] *= rt * f.z;
-                        x[j + 3] *= rt * f.w;
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 f = *reinterpret_cast<const float2 *>(c + u * 16 + j * 2);
+                        float lo, hi;
+                        vec::unpack(x[j], lo, hi);
+                        lo *= ex2_approx(ct - f.x);
+                        hi *= ex2_approx(ct - f.y);
+                        x[j] = vec::pack(2 * j <= td ? lo : 0.f, 2 * j + 1 <= td ? hi : 0.f);
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    const float e[8] = {x[j], x[j + 1], x[j + 2], x[j + 3], x[j + 4], x[j + 5], x[j + 6], x[j + 7]};
-                    *reinterpret_cast<uint4 *>(row + ((((j0 + j) >> 3) ^ (t & 7)) << 4)) = pack8<bf16>(e);
+                for (int j = 0; j < 2; ++j) {
+                    uint4 o;
+                    o.x = vec::narrow<bf16>(x[4 * j]); o.y = vec::narrow<bf16>(x[4 * j + 1]);
+                    o.z = vec::narrow<bf16>(x[4 * j + 2]); o.w = vec::narrow<bf16>(x[4 * j + 3]);
+                    *reinterpret_cast<uint4 *>(pair_at(u) + piece(u, j)) = o;
                 }
             }
+            if (r32 == 0 && half == 1)                           // the output's tile lay there
+                for (int u = 2; u < 4; ++u)
+                    for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4 *>(pair_at(u) + piece(u, j)) = zero8();
         }
         if (a.chunk.packed && s.len < kQ) {
             ok = ok && mbar_wait(&bar_v, i & 1);
