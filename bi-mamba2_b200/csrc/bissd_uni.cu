@@ -462,12 +462,21 @@ TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
         g.gstates = ws.take<float>((size_t)g.t.seg.most * a->nheads * a->kdim * a->vdim);
         g.gdecay = ws.take<float>((size_t)g.t.seg.most * a->nheads);
     }
-    // heads that share q and k are walked by one block, by several where that leaves SMs without
+    // Heads that share q and k are walked by one block, or by several: what takes the fewest rounds of one block an SM, a block's start
+    // being worth 1.5 tiles (of 5 us), and the parts of dq and dk 16 bytes a value at 5 TB/s.
     const int R = a->nheads / a->nkheads;
     const long long items = (long long)g.t.chunk.most * a->nkheads;
-    const int heads = (int)std::max<long long>(1, std::min<long long>(R, R * items / 148));
-    g.vpc = heads * g.t.PB;
-    g.parts = ceil_div(R, heads);
+    double best = 0;
+    for (int parts = 1; parts <= R; ++parts) {
+        const int heads = ceil_div(R, parts), real = ceil_div(R, heads);
+        const double rounds = (double)((items * real + 147) / 148), sums = real > 1 ? 16.0 * real * tokens * a->nkheads * a->kdim / 25e6 : 0;
+        const double time = rounds * (heads * g.t.PB + 1.5) + sums;
+        if (parts == 1 || time < best) {
+            best = time;
+            g.vpc = heads * g.t.PB;
+            g.parts = real;
+        }
+    }
     if (g.parts > 1) g.part = ws.take<float>((size_t)2 * g.parts * tokens * a->nkheads * a->kdim);
     if (a->g_per_head) g.dg_tokens = ws.take<float>((size_t)tokens * a->nheads);
     return g;

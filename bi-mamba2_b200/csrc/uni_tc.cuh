@@ -662,8 +662,10 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
 // - every pair of places before and from t on: past and future of the chunk, past and its tokens, its tokens and the future, tokens
 // among themselves; the last as sums over rows less sums over columns of the same fp32 products, so that what cancels does so
 // exactly.  Everything is laid out with s along the rows (lanes): p and d then are operands of dv and dk as they lie, and d of dq
-// read the other way.  A block has a chunk and a head of q and k, and walks (its part of) the heads of v that share them, dq and dk
-// adding up in tensor memory; twelve of its sixteen warps have weights to make, four lie above the diagonal.
+// read the other way.  p goes back to tensor memory, d to shared memory.  A block has a chunk and a head of q and k, and walks (its
+// part of) the heads of v that share them, dq and dk adding up in tensor memory; v and do come a tile ahead, the states while the pairs
+// are weighted, and dv leaves while the products of d still run.  Ten of the sixteen warps have weights to make, six lie above the
+// diagonal; one of these makes the next head's tables, one sums dg.
 struct GradsParams {
     Heads h;
     Plan chunk;
@@ -675,7 +677,26 @@ struct GradsParams {
     int dg_dtype;
     int *status;
 };
-inline size_t grads_smem(int NT) { return 1024 + 2 * (size_t)(NT / 64) * kSlab + 3 * (size_t)kSlab + 2 * (size_t)NT * 128 + 4 * (size_t)kSlab; }
+inline size_t grads_smem(int NT) { return 1024 + 2 * (size_t)(NT / 64) * kSlab + 4 * (size_t)kSlab + 3 * (size_t)kSlab + 2 * (size_t)NT * 128; }
+
+// A from tensor memory: 128 lanes, two 16-bit values of K a column.
+__device__ __forceinline__ void umma_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        :
+        : "r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        :
+        : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+          "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
 
 template <int NT> __global__ void __launch_bounds__(512, 1)
 decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -683,51 +704,72 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     pdl_begin();
     constexpr int kSlabs = NT / 64, kT = 512;
     extern __shared__ __align__(1024) uint8_t dyn[];
-    __shared__ uint64_t bar_qk, bar_v, done, unused;
+    struct Table {                                               // of a head; two take turns
+        float c[kQ], ws[kQ], et[kQ];                             // c_t; e^{c_end - c_s}; scale e^{c_t}
+        float above[kQ], beside[3][kQ];                          // weights of blocks of 32 x 32: 2^(c at the end of s' 32 - c_s), scale 2^(c_t - c at the end of the q-th 32)
+        float whole[4];                                          // c_end
+    };
+    __shared__ uint64_t bar_qk, bar_v[2], bar_s, done_1, done_a, done_b, unused;
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float c[kQ], ws[kQ], et[kQ];        // c_t; e^{c_end - c_s}; scale e^{c_t}
-    __shared__ __align__(16) float above[64], beside[64];        // weights below the diagonal blocks: e^{c_63 - c_s}, scale e^{c_t - c_63}
+    __shared__ __align__(16) Table tables[2];
     __shared__ float rowsum[4][kQ], colsum[4][kQ], past[4][kQ], future[4][kQ], cross[16];
-    uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + kSlabs * kSlab, *smD = smV + kSlab, *smE = smD + kSlab,
-            *smP = smE + kSlab, *smN = smP + 2 * kSlab, *smS = smN + 2 * kSlab, *smG = smS + NT * 128;
+    uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + kSlabs * kSlab, *smD = smV + 2 * kSlab, *smE = smD + 2 * kSlab,
+            *smN = smE + kSlab, *smS = smN + 2 * kSlab, *smG = smS + NT * 128;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int part = blockIdx.x % a.parts, m = blockIdx.x / a.parts % a.h.hk, ci = blockIdx.x / (a.parts * a.h.hk);
     const Segment sg = uni::segment(a.chunk, ci);
     if (sg.len == 0) return;
     const int len = sg.len, R = a.h.H / a.h.hk, v0 = part * a.vpc, nv = min(a.vpc, R * a.h.PB - v0);
+    const bool tail = a.chunk.packed && len < kQ;                // rows of another sequence lie behind this one's
     auto head = [&](int i) { return m * R + (v0 + i) / a.h.PB; };
+    auto first_of = [&](int i) { return (v0 + i) % a.h.PB == 0; };
     auto load_v = [&](int i) {
-        const int h = head(i), pb = (v0 + i) % a.h.PB, row = ((ci * a.h.H + h) * a.h.PB + pb) * NT;
-        mbar_expect_tx(&bar_v, 2 * kSlab + 2 * NT * 128);
-        tma_load4(smV, &tmV, pb * kP, h, sg.t0, sg.batch, &bar_v);
-        tma_load4(smD, &tmD, pb * kP, h, sg.t0, sg.batch, &bar_v);
-        tma_load2(smS, &tmS, 0, row, &bar_v);
-        tma_load2(smG, &tmG, 0, row, &bar_v);
+        const int h = head(i), pb = (v0 + i) % a.h.PB, b = i & 1;
+        mbar_expect_tx(&bar_v[b], 2 * kSlab);
+        tma_load4(smV + b * kSlab, &tmV, pb * kP, h, sg.t0, sg.batch, &bar_v[b]);
+        tma_load4(smD + b * kSlab, &tmD, pb * kP, h, sg.t0, sg.batch, &bar_v[b]);
     };
-    Decays next;                                                 // warp 0: of the head to come
-    float whole = 0.f;                                           // warp 0: c_end
-    auto table = [&]() {                                         // one warp
+    auto load_s = [&](int i) {
+        const int row = ((ci * a.h.H + head(i)) * a.h.PB + (v0 + i) % a.h.PB) * NT;
+        mbar_expect_tx(&bar_s, 2 * NT * 128);
+        tma_load2(smS, &tmS, 0, row, &bar_s);
+        tma_load2(smG, &tmG, 0, row, &bar_s);
+    };
+    Decays next;                                                 // warp 3: of the head to come
+    auto ask = [&](int i) {
+        if (i < nv) next.load(a.h, sg.batch, sg.t0, len, head(i), lane);
+    };
+    auto table = [&](Table &to) {                                // one warp
         float p[4], q[4];
         next.log2(a.h);
         next.prefix(p, lane);
         next.suffix(q, lane);
-        const float corner = __shfl_sync(0xffffffffu, p[3], 15);
-        whole = __shfl_sync(0xffffffffu, p[3], 31);
+        const float end = __shfl_sync(0xffffffffu, p[3], lane | 7);
+        float ends[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ends[k] = __shfl_sync(0xffffffffu, p[3], 8 * k + 7);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int t = lane * 4 + k;
-            c[t] = p[k];
-            et[t] = exp2f(p[k] + a.h.log_scale);
-            ws[t] = exp2f(q[k]);
-            if (lane < 16) above[t] = exp2f(corner - p[k]);
-            else beside[t - 64] = exp2f(p[k] - corner + a.h.log_scale);
+            to.c[t] = p[k];
+            to.et[t] = exp2f(p[k] + a.h.log_scale);
+            to.ws[t] = exp2f(q[k]);
+            to.above[t] = exp2f(end - p[k]);
+#pragma unroll
+            for (int b = 0; b < 3; ++b)
+                if (b < lane >> 3) to.beside[b][t] = exp2f(p[k] - ends[b] + a.h.log_scale);
         }
+        if (lane == 0) to.whole[0] = ends[3];
     };
     if (warp == 0) tmem_alloc(&tmem_slot, 512);
     if (tid == 32) {
         mbar_init(&bar_qk, 1);
-        mbar_init(&bar_v, 1);
-        mbar_init(&done, 1);
+        mbar_init(&bar_v[0], 1);
+        mbar_init(&bar_v[1], 1);
+        mbar_init(&bar_s, 1);
+        mbar_init(&done_1, 1);
+        mbar_init(&done_a, 1);
+        mbar_init(&done_b, 1);
         fence_mbar_init();
         mbar_expect_tx(&bar_qk, 2 * kSlabs * kSlab);
         for (int j = 0; j < kSlabs; ++j) {
@@ -735,178 +777,226 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             tma_load4(smK + j * kSlab, &tmK, j * 64, m, sg.t0, sg.batch, &bar_qk);
         }
         load_v(0);
+        load_s(0);
+        if (nv > 1) load_v(1);
     }
-    if (warp == 0) next.load(a.h, sg.batch, sg.t0, len, head(0), lane);
+    if (warp == 3) {
+        ask(0);
+        table(tables[0]);
+        ask(a.h.PB);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // tensor memory: 0 q.k, then p in bf16 (64 columns); 64 dv inside the chunk; 128 do.v, then dv from the future; 192 S^T q; dq; dk
     const uint32_t tmem = tmem_slot, tl = tmem_lane_base(tmem);
-    constexpr uint32_t cQ = 256, cK = 256 + NT;                  // columns of dq and dk; 0: q.k, then dv; 128: do.v, then S^T q
-    int loads = 1, waits = 0;
+    constexpr uint32_t cOwn = 64, cFar = 128, cOut = 192, cQ = 256, cK = 256 + NT;
+    int loads_v = nv > 1 ? 2 : 1, loads_s = 1;
     bool ok = mbar_wait(&bar_qk, 0);
     const int quad = warp & 3, cg = warp >> 2, s = quad * 32 + lane;   // this thread: row s; columns t of 32 cg ...; 16 of dv's 64
-    const bool diagonal = (quad >> 1) == (cg >> 1), empty = (quad >> 1) > (cg >> 1);
-    if (ok && a.chunk.packed && len < kQ)
+    if (ok && tail)
         for (int j = 0; j < kSlabs; ++j) {
             clear_rows(smQ + j * kSlab, len, tid, kT);
             clear_rows(smK + j * kSlab, len, tid, kT);
         }
     float through = 0.f;                                         // this thread's part of S.G
     for (int i = 0; i < nv; ++i) {
-        const bool first = (v0 + i) % a.h.PB == 0, last = (v0 + i) % a.h.PB == a.h.PB - 1 || i + 1 == nv;   // tiles of a head
-        if (warp == 0 && first) {
-            table();
-            if (i + a.h.PB < nv) next.load(a.h, sg.batch, sg.t0, len, head(i + a.h.PB), lane);
+        const bool first = first_of(i), last = i + 1 == nv || first_of(i + 1);   // tiles of a head
+        const Table &tb = tables[((v0 + i) / a.h.PB - v0 / a.h.PB) & 1];
+        uint8_t *sV = smV + (i & 1) * kSlab, *sD = smD + (i & 1) * kSlab;
+        if (tail) {
+            ok = ok && mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
+            if (ok) {
+                clear_rows(sV, len, tid, kT);
+                clear_rows(sD, len, tid, kT);
+            }
+            fence_async_smem();
+            ok = __syncthreads_and(ok);
+            if (!ok) break;
         }
-        ok = ok && mbar_wait(&bar_v, i & 1);
-        if (ok && a.chunk.packed && len < kQ) {
-            clear_rows(smV, len, tid, kT);
-            clear_rows(smD, len, tid, kT);
-        }
-        fence_async_smem();
-        tc_fence_before();
-        ok = __syncthreads_and(ok);
-        if (!ok) break;
         if (warp == 0 && elect_one()) {                          // q.k and do.v of all pairs, rows s
-            tc_fence_after();
-            constexpr uint32_t idesc = instr_desc(1, false, false, kQ);
+            ok = ok && mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
+            if (ok) {
+                tc_fence_after();
+                constexpr uint32_t idesc = instr_desc(1, false, false, kQ);
 #pragma unroll
-            for (int kk = 0; kk < NT / 16; ++kk)
-                umma(tmem, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
-                     smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < NT / 16; ++kk)
+                    umma(tmem, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
+                         smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-                umma(tmem + 128, smem_desc(smem_u32(smV) + kk * 32, 16, 1024), smem_desc(smem_u32(smD) + kk * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
-            umma_commit(&done);
+                for (int kk = 0; kk < 4; ++kk)
+                    umma(tmem + 128, smem_desc(smem_u32(sV) + kk * 32, 16, 1024), smem_desc(smem_u32(sD) + kk * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+                umma_commit(&done_1);
+            }
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {                            // scale e^{c_t} do_t beside do_t
-            const int x = tid + k * kT, row = x >> 3;
-            float e[8];
-            unpack8<bf16>(*reinterpret_cast<const uint4 *>(smD + x * 16), e);
-            const float f = et[row];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] *= f;
-            *reinterpret_cast<uint4 *>(smE + x * 16) = pack8<bf16>(e);
-        }
-        if (first) through = 0.f;
-        for (int x = tid; x < NT * 8; x += kT) {
-            float e[8], f[8];
-            unpack8<bf16>(*reinterpret_cast<const uint4 *>(smS + x * 16), e);
-            unpack8<bf16>(*reinterpret_cast<const uint4 *>(smG + x * 16), f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) through = fmaf(e[j], f[j], through);
-        }
-        ok = mbar_wait(&done, waits & 1);
-        ++waits;
-        tc_fence_after();
+        if (ok) ok = mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
         if (ok) {
-            // rows of 64 t, 16-byte pieces swizzled
-            uint8_t *prow = smP + (cg >> 1) * kSlab + s * 128, *drow = smN + (cg >> 1) * kSlab + s * 128;
-            float x[32], y[32], of_row = 0.f, of_column = 0.f;   // for dg: d (q.k) over this row, over column 32 cg + lane
-            if (!empty) {
-                tmem_ld32(tl + cg * 32, x);
-                tmem_ld32(tl + 128 + cg * 32, y);
-                const float cs = c[s] - a.h.log_scale, fs = above[s & 63];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {                        // scale e^{c_t} do_t beside do_t
+                const int x = tid + k * kT, row = x >> 3;
+                float e[8];
+                unpack8<bf16>(*reinterpret_cast<const uint4 *>(sD + x * 16), e);
+                const float f = tb.et[row];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] *= f;
+                *reinterpret_cast<uint4 *>(smE + x * 16) = pack8<bf16>(e);
+            }
+            ok = mbar_wait(&done_1, i & 1);
+        }
+        tc_fence_after();
+        const bool some = cg >= quad;                            // a block on the diagonal or below it
+        float x[32], y[32];
+        if (ok && some) {
+            tmem_ld32(tl + cg * 32, x);
+            tmem_ld32(tl + 128 + cg * 32, y);
+        }
+        tc_fence_before();
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory");   // p goes where these 32 rows' q.k was
+        tc_fence_after();
+        if (ok && i > 0) ok = mbar_wait(&done_b, (i - 1) & 1);   // d of the tile before has been read
+        if (ok) {
+            uint8_t *drow = smN + (cg >> 1) * kSlab + s * 128;   // rows of 64 t, 16-byte pieces swizzled
+            uint32_t p[16];
+            float of_row = 0.f, of_column = 0.f;                 // for dg: d (q.k) over this row, over column 32 cg + lane
+            if (some) {
+                const float cs = tb.c[s] - a.h.log_scale, fs = tb.above[s];
+                const float4 *f4 = reinterpret_cast<const float4 *>(cg == quad ? tb.c + cg * 32 : tb.beside[quad] + cg * 32);
+                vec::f2 sum = vec::pack(0.f, 0.f);
 #pragma unroll
                 for (int j0 = 0; j0 < 32; j0 += 8) {
-                    float p[8], d[8];
+                    uint32_t d[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int t = cg * 32 + j0 + j;
-                        const float w = diagonal ? (t >= s ? ex2_approx(c[t] - cs) : 0.f) : fs * beside[t & 63];
-                        p[j] = w * x[j0 + j];
-                        d[j] = w * y[j0 + j];
-                        x[j0 + j] = t > s ? d[j] * x[j0 + j] : 0.f;   // a token's own pair flows nowhere
-                        of_row += x[j0 + j];
+                    for (int j = j0; j < j0 + 8; j += 4) {
+                        const float4 f = f4[j / 4];
+                        vec::f2 w0, w1;
+                        if (cg == quad) {
+                            w0 = vec::pack(j >= lane ? ex2_approx(f.x - cs) : 0.f, j + 1 >= lane ? ex2_approx(f.y - cs) : 0.f);
+                            w1 = vec::pack(j + 2 >= lane ? ex2_approx(f.z - cs) : 0.f, j + 3 >= lane ? ex2_approx(f.w - cs) : 0.f);
+                        } else {
+                            const vec::f2 fs2 = vec::pack(fs, fs);
+                            w0 = vec::mul2(vec::pack(f.x, f.y), fs2);
+                            w1 = vec::mul2(vec::pack(f.z, f.w), fs2);
+                        }
+                        const vec::f2 x0 = vec::pack(x[j], x[j + 1]), x1 = vec::pack(x[j + 2], x[j + 3]);
+                        const vec::f2 y0 = vec::mul2(vec::pack(y[j], y[j + 1]), w0), y1 = vec::mul2(vec::pack(y[j + 2], y[j + 3]), w1);
+                        p[j / 2] = vec::narrow<bf16>(vec::mul2(x0, w0));
+                        p[j / 2 + 1] = vec::narrow<bf16>(vec::mul2(x1, w1));
+                        d[(j - j0) / 2] = vec::narrow<bf16>(y0);
+                        d[(j - j0) / 2 + 1] = vec::narrow<bf16>(y1);
+                        const vec::f2 z0 = vec::mul2(x0, y0), z1 = vec::mul2(x1, y1);   // a token's own pair is in its row's and its column's sum
+                        sum = vec::add2(sum, vec::add2(z0, z1));
+                        vec::unpack(z0, x[j], x[j + 1]);
+                        vec::unpack(z1, x[j + 2], x[j + 3]);
                     }
-                    const int piece = ((cg & 1) * 4 + j0 / 8) ^ (s & 7);
-                    *reinterpret_cast<uint4 *>(prow + (piece << 4)) = pack8<bf16>(p);
-                    *reinterpret_cast<uint4 *>(drow + (piece << 4)) = pack8<bf16>(d);
+                    *reinterpret_cast<uint4 *>(drow + ((((cg & 1) * 4 + j0 / 8) ^ (s & 7)) << 4)) = make_uint4(d[0], d[1], d[2], d[3]);
                 }
+                float lo, hi;
+                vec::unpack(sum, lo, hi);
+                of_row = lo + hi;
                 auto value = [&](auto k) { return x[decltype(k)::value]; };
                 of_column = warp_sums<32>(value, lane);
-            } else if (i == 0) {
+            } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int piece = ((cg & 1) * 4 + j) ^ (s & 7);
-                    *reinterpret_cast<uint4 *>(prow + (piece << 4)) = zero8();
-                    *reinterpret_cast<uint4 *>(drow + (piece << 4)) = zero8();
+                for (int j = 0; j < 16; ++j) p[j] = 0u;
+                if (i == 0) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4 *>(drow + ((((cg & 1) * 4 + j) ^ (s & 7)) << 4)) = zero8();
                 }
             }
+            tmem_st16(tl + cg * 16, p);
             rowsum[cg][s] = of_row + (first ? 0.f : rowsum[cg][s]);
             colsum[quad][cg * 32 + lane] = of_column + (first ? 0.f : colsum[quad][cg * 32 + lane]);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {                        // e^{c_end - c_s} v_s in v_s' place
                 const int q = tid + k * kT;
-                uint4 *v = reinterpret_cast<uint4 *>(smV + q * 16);
+                uint4 *v = reinterpret_cast<uint4 *>(sV + q * 16);
                 float e[8];
                 unpack8<bf16>(*v, e);
-                const float f = ws[q >> 3];
+                const float f = tb.ws[q >> 3];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) e[j] *= f;
                 *v = pack8<bf16>(e);
             }
+            if (warp == 3 && i + 1 < nv && first_of(i + 1)) {    // a warp above the diagonal: the next head's table
+                table(tables[((v0 + i + 1) / a.h.PB - v0 / a.h.PB) & 1]);
+                ask(i + 1 + a.h.PB);
+            }
             fence_async_smem();
+            tmem_st_wait();
         }
         tc_fence_before();
         ok = __syncthreads_and(ok);
         if (!ok) break;
-        if (warp == 0 && elect_one()) {
-            tc_fence_after();
-            constexpr uint32_t narrow = instr_desc(1, false, true, kP), wide = instr_desc(1, false, false, NT);
-            const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), p0 = smem_u32(smP), n0 = smem_u32(smN);
-            const uint32_t v_ = smem_u32(smV), d_ = smem_u32(smD), e_ = smem_u32(smE), s_ = smem_u32(smS), g_ = smem_u32(smG);
-#pragma unroll
-            for (int kk = 0; kk < kQ / 16; ++kk)                 // dv from the chunk, from the future; S^T q
-                umma(tmem, smem_desc(p0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(d_ + kk * 2048, kSlab, 1024), narrow, kk > 0 ? 1u : 0u);
-#pragma unroll
-            for (int kk = 0; kk < NT / 16; ++kk)
-                umma(tmem + 64, smem_desc(k0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(g_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
-#pragma unroll
-            for (int kk = 0; kk < NT / 16; ++kk)
-                umma(tmem + 128, smem_desc(q0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(s_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
-#pragma unroll
-            for (int kk = 0; kk < kQ / 16; ++kk) {               // dq and dk from the chunk
-                umma(tmem + cQ, smem_desc(n0 + kk * 2048, kSlab, 1024), smem_desc(k0 + kk * 2048, kSlab, 1024), instr_desc(1, true, true, NT),
-                     i > 0 || kk > 0 ? 1u : 0u);
-                umma(tmem + cK, smem_desc(n0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(q0 + kk * 2048, kSlab, 1024),
-                     instr_desc(1, false, true, NT), i > 0 || kk > 0 ? 1u : 0u);
-            }
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {                     // dq from the past, dk from the future
-                umma(tmem + cQ, smem_desc(e_ + kk * 32, 16, 1024), smem_desc(s_ + kk * 32, 16, 1024), wide, 1u);
-                umma(tmem + cK, smem_desc(v_ + kk * 32, 16, 1024), smem_desc(g_ + kk * 32, 16, 1024), wide, 1u);
-            }
-            umma_commit(&done);
+        if (i > 0 && i + 1 < nv) {                               // the tile before has left its buffers
+            if (tid == 32) load_v(i + 1);
+            ++loads_v;
         }
+        if (warp == 0 && elect_one()) {
+            ok = mbar_wait(&bar_s, i & 1);
+            if (ok) {
+                tc_fence_after();
+                constexpr uint32_t narrow = instr_desc(1, false, true, kP), wide = instr_desc(1, false, false, NT);
+                const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), n0 = smem_u32(smN);
+                const uint32_t v_ = smem_u32(sV), d_ = smem_u32(sD), e_ = smem_u32(smE), s_ = smem_u32(smS), g_ = smem_u32(smG);
+#pragma unroll
+                for (int kk = 0; kk < kQ / 16; ++kk)             // dv from the chunk, from the future; S^T q
+                    umma_tmem(tmem + cOwn, tmem + kk * 8, smem_desc(d_ + kk * 2048, kSlab, 1024), narrow, kk > 0 ? 1u : 0u);
+#pragma unroll
+                for (int kk = 0; kk < NT / 16; ++kk)
+                    umma(tmem + cFar, smem_desc(k0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(g_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
+#pragma unroll
+                for (int kk = 0; kk < NT / 16; ++kk)
+                    umma(tmem + cOut, smem_desc(q0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(s_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {                 // dq from the past, dk from the future
+                    umma(tmem + cQ, smem_desc(e_ + kk * 32, 16, 1024), smem_desc(s_ + kk * 32, 16, 1024), wide, i > 0 || kk > 0 ? 1u : 0u);
+                    umma(tmem + cK, smem_desc(v_ + kk * 32, 16, 1024), smem_desc(g_ + kk * 32, 16, 1024), wide, i > 0 || kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&done_a);
+#pragma unroll
+                for (int kk = 0; kk < kQ / 16; ++kk) {           // dq and dk from the chunk, while dv leaves
+                    umma(tmem + cQ, smem_desc(n0 + kk * 2048, kSlab, 1024), smem_desc(k0 + kk * 2048, kSlab, 1024), instr_desc(1, true, true, NT), 1u);
+                    umma(tmem + cK, smem_desc(n0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(q0 + kk * 2048, kSlab, 1024), instr_desc(1, false, true, NT), 1u);
+                }
+                umma_commit(&done_b);
+            }
+        }
+        if (ok) ok = mbar_wait(&bar_s, i & 1);
+        if (first) through = 0.f;
+        if (ok)
+            for (int q = tid; q < NT * 8; q += kT) {
+                float e[8], f[8];
+                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smS + q * 16), e);
+                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smG + q * 16), f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) through = fmaf(e[j], f[j], through);
+            }
         if (last) {
             float v = through;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             if (lane == 0) cross[warp] = v;
         }
-        ok = mbar_wait(&done, waits & 1);
-        ++waits;
+        if (ok) ok = mbar_wait(&done_a, i & 1);
         tc_fence_after();
         if (ok) {                                                // row s (or t), columns 16 cg ... of v's 64
             float own[16], far[16], o[16], e[8], f = 0.f, p = 0.f;
-            tmem_ld16(tl + cg * 16, own);
-            tmem_ld16(tl + 64 + cg * 16, far);
-            tmem_ld16(tl + 128 + cg * 16, o);
-            const float w = ws[s];
+            tmem_ld16(tl + cOwn + cg * 16, own);
+            tmem_ld16(tl + cFar + cg * 16, far);
+            tmem_ld16(tl + cOut + cg * 16, o);
+            const float w = tb.ws[s];
 #pragma unroll
             for (int j = 0; j < 16; j += 8) {
-                const int piece = ((cg * 2 + j / 8) ^ (s & 7)) << 4;
-                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smV + s * 128 + piece), e);
+                const int at = s * 128 + (((cg * 2 + j / 8) ^ (s & 7)) << 4);
+                unpack8<bf16>(*reinterpret_cast<const uint4 *>(sV + at), e);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) f = fmaf(e[k], far[j + k], f);
-                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smE + s * 128 + piece), e);
+                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smE + at), e);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) p = fmaf(e[k], o[j + k], p);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) e[k] = fmaf(w, far[j + k], own[j + k]);
-                *reinterpret_cast<uint4 *>(smP + kSlab + s * 128 + piece) = pack8<bf16>(e);   // every row there is written anew
+                *reinterpret_cast<uint4 *>(sV + at) = pack8<bf16>(e);   // dv, where this thread alone has read v
             }
             future[cg][s] = f + (first ? 0.f : future[cg][s]);
             past[cg][s] = p + (first ? 0.f : past[cg][s]);
@@ -915,8 +1005,8 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         ok = __syncthreads_and(ok);
         if (!ok) break;
         if (i + 1 < nv) {
-            if (tid == 32) load_v(i + 1);
-            ++loads;
+            if (tid == 32) load_s(i + 1);
+            ++loads_s;
         }
         const int h = head(i), col = (v0 + i) % a.h.PB * kP + (tid & 7) * 8;
         const long long token = (long long)sg.batch * a.chunk.L + sg.t0;
@@ -926,14 +1016,14 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 const int r = (tid >> 3) + k * 64;
                 if (r < len)
                     *reinterpret_cast<uint4 *>(a.dv + ((token + r) * a.h.H + h) * a.h.P + col) =
-                        *reinterpret_cast<const uint4 *>(smP + kSlab + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
+                        *reinterpret_cast<const uint4 *>(sV + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
             }
         }
-        if (last && warp == 0 && a.dg) {
+        if (last && warp == 7 && a.dg) {
             float all = lane < 16 ? cross[lane] : 0.f, x[4], b[4];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-            all *= exp2f(whole);
+            all *= exp2f(tb.whole[0]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int t = lane * 4 + k;
@@ -963,6 +1053,8 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             }
         }
     }
+    if (ok) ok = mbar_wait(&done_b, (nv - 1) & 1);
+    tc_fence_after();
     ok = __syncthreads_and(ok);
     if (ok) {                                                    // dq and dk: rows s (or t), NT / 4 columns a thread
         constexpr int kCols = NT / 4;
@@ -970,7 +1062,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
 #pragma unroll
         for (int what = 0; what < 2; ++what) {
             const uint32_t at = tl + (what ? cK : cQ) + cg * kCols;
-            uint8_t *to = what ? smN : smP;
+            uint8_t *to = what ? smN : smV;
 #pragma unroll
             for (int j0 = 0; j0 < kCols; j0 += 16) {
                 float x[16];
@@ -997,7 +1089,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 const int what = x / (kQ * (NT / 8)), r = x / (NT / 8) % kQ, j = x % (NT / 8);
                 if (r < len && j < pieces)
                     *reinterpret_cast<uint4 *>((what ? a.dk : a.dq) + ((token + r) * a.h.hk + m) * a.h.N + j * 8) =
-                        *reinterpret_cast<const uint4 *>((what ? smN : smP) + j / 8 * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4));
+                        *reinterpret_cast<const uint4 *>((what ? smN : smV) + j / 8 * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4));
             }
         }
     } else if (tid == 0) {
@@ -1009,7 +1101,8 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         if (!ok && elect_one()) {                                // leave nothing in flight
             drain_mmas(&unused);
             drain_loads(&bar_qk, 1, 1);
-            drain_loads(&bar_v, 1, loads);
+            drain_loads(bar_v, 2, loads_v);
+            drain_loads(&bar_s, 1, loads_s);
         }
         __syncwarp();
         tmem_dealloc(tmem, 512);
