@@ -664,7 +664,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
 // exactly.  Everything is laid out with s along the rows (lanes): p and d then are operands of dv and dk as they lie, and d of dq
 // read the other way.  p goes back to tensor memory, d to shared memory.  A block has a chunk and a head of q and k, and walks (its
 // part of) the heads of v that share them, dq and dk adding up in tensor memory; v and do come a tile ahead, the states while the pairs
-// are weighted, and dv leaves while the products of d still run.  Ten of the sixteen warps have weights to make, six lie above the
+// are weighted, and the products of d run under the next tile's first ones, when nobody waits for them.  Ten of the sixteen warps have weights to make, six lie above the
 // diagonal; one of these makes the next head's tables, one sums dg.
 struct GradsParams {
     Heads h;
@@ -703,6 +703,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmG) {
     pdl_begin();
     constexpr int kSlabs = NT / 64, kT = 512;
+    constexpr int kTables = 3, kIssue = 7, kSums = 11;           // warps above the diagonal
     extern __shared__ __align__(1024) uint8_t dyn[];
     struct Table {                                               // of a head; two take turns
         float c[kQ], ws[kQ], et[kQ];                             // c_t; e^{c_end - c_s}; scale e^{c_t}
@@ -712,7 +713,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     __shared__ uint64_t bar_qk, bar_v[2], bar_s, done_1, done_a, done_b, unused;
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(16) Table tables[2];
-    __shared__ float rowsum[4][kQ], colsum[4][kQ], past[4][kQ], future[4][kQ], cross[16];
+    __shared__ __align__(16) float rowsum[4][kQ], colsum[4][kQ], past[4][kQ], future[4][kQ], cross[16];
     uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + kSlabs * kSlab, *smD = smV + 2 * kSlab, *smE = smD + 2 * kSlab,
             *smN = smE + kSlab, *smS = smN + 2 * kSlab, *smG = smS + NT * 128;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -735,11 +736,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         tma_load2(smS, &tmS, 0, row, &bar_s);
         tma_load2(smG, &tmG, 0, row, &bar_s);
     };
-    Decays next;                                                 // warp 3: of the head to come
-    auto ask = [&](int i) {
-        if (i < nv) next.load(a.h, sg.batch, sg.t0, len, head(i), lane);
-    };
-    auto table = [&](Table &to) {                                // one warp
+    auto table = [&](Table &to, Decays &next) {                  // one warp
         float p[4], q[4];
         next.log2(a.h);
         next.prefix(p, lane);
@@ -748,17 +745,16 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         float ends[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) ends[k] = __shfl_sync(0xffffffffu, p[3], 8 * k + 7);
+        auto four = [&](float *o, float x0, float x1, float x2, float x3) { *reinterpret_cast<float4 *>(o + lane * 4) = make_float4(x0, x1, x2, x3); };
+        four(to.c, p[0], p[1], p[2], p[3]);
+        four(to.above, ex2_approx(end - p[0]), ex2_approx(end - p[1]), ex2_approx(end - p[2]), ex2_approx(end - p[3]));
+        four(to.ws, ex2_approx(q[0]), ex2_approx(q[1]), ex2_approx(q[2]), ex2_approx(q[3]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int t = lane * 4 + k;
-            to.c[t] = p[k];
-            to.et[t] = exp2f(p[k] + a.h.log_scale);
-            to.ws[t] = exp2f(q[k]);
-            to.above[t] = exp2f(end - p[k]);
+        for (int k = 0; k < 4; ++k) p[k] += a.h.log_scale;
+        four(to.et, ex2_approx(p[0]), ex2_approx(p[1]), ex2_approx(p[2]), ex2_approx(p[3]));
 #pragma unroll
-            for (int b = 0; b < 3; ++b)
-                if (b < lane >> 3) to.beside[b][t] = exp2f(p[k] - ends[b] + a.h.log_scale);
-        }
+        for (int b = 0; b < 3; ++b)                              // of use in the blocks behind the b-th
+            four(to.beside[b], ex2_approx(p[0] - ends[b]), ex2_approx(p[1] - ends[b]), ex2_approx(p[2] - ends[b]), ex2_approx(p[3] - ends[b]));
         if (lane == 0) to.whole[0] = ends[3];
     };
     if (warp == 0) tmem_alloc(&tmem_slot, 512);
@@ -780,10 +776,10 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         load_s(0);
         if (nv > 1) load_v(1);
     }
-    if (warp == 3) {
-        ask(0);
-        table(tables[0]);
-        ask(a.h.PB);
+    if (warp == kTables) {
+        Decays d;
+        d.load(a.h, sg.batch, sg.t0, len, head(0), lane);
+        table(tables[0], d);
     }
     tc_fence_before();
     __syncthreads();
@@ -800,6 +796,16 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             clear_rows(smK + j * kSlab, len, tid, kT);
         }
     float through = 0.f;                                         // this thread's part of S.G
+    auto from_chunk = [&]() {                                    // dq and dk of the chunk's own pairs; one thread
+        constexpr uint32_t iq = instr_desc(1, true, true, NT), ik = instr_desc(1, false, true, NT);
+        const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), n0 = smem_u32(smN);
+#pragma unroll
+        for (int kk = 0; kk < kQ / 16; ++kk) {
+            umma(tmem + cQ, smem_desc(n0 + kk * 2048, kSlab, 1024), smem_desc(k0 + kk * 2048, kSlab, 1024), iq, 1u);
+            umma(tmem + cK, smem_desc(n0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(q0 + kk * 2048, kSlab, 1024), ik, 1u);
+        }
+        umma_commit(&done_b);
+    };
     for (int i = 0; i < nv; ++i) {
         const bool first = first_of(i), last = i + 1 == nv || first_of(i + 1);   // tiles of a head
         const Table &tb = tables[((v0 + i) / a.h.PB - v0 / a.h.PB) & 1];
@@ -814,7 +820,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             ok = __syncthreads_and(ok);
             if (!ok) break;
         }
-        if (warp == 0 && elect_one()) {                          // q.k and do.v of all pairs, rows s
+        if (warp == kIssue && elect_one()) {                     // q.k and do.v of all pairs, rows s
             ok = ok && mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
             if (ok) {
                 tc_fence_after();
@@ -827,7 +833,13 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 for (int kk = 0; kk < 4; ++kk)
                     umma(tmem + 128, smem_desc(smem_u32(sV) + kk * 32, 16, 1024), smem_desc(smem_u32(sD) + kk * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
                 umma_commit(&done_1);
+                if (i > 0) from_chunk();                         // of the tile before: here nothing waits for them
             }
+        }
+        if (warp == kTables && i + 1 < nv && first_of(i + 1)) {  // the next head's; the turn before the last one has been read
+            Decays d;
+            d.load(a.h, sg.batch, sg.t0, len, head(i + 1), lane);
+            table(tables[((v0 + i + 1) / a.h.PB - v0 / a.h.PB) & 1], d);
         }
         if (ok) ok = mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
         if (ok) {
@@ -917,10 +929,6 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 for (int j = 0; j < 8; ++j) e[j] *= f;
                 *v = pack8<bf16>(e);
             }
-            if (warp == 3 && i + 1 < nv && first_of(i + 1)) {    // a warp above the diagonal: the next head's table
-                table(tables[((v0 + i + 1) / a.h.PB - v0 / a.h.PB) & 1]);
-                ask(i + 1 + a.h.PB);
-            }
             fence_async_smem();
             tmem_st_wait();
         }
@@ -931,12 +939,12 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             if (tid == 32) load_v(i + 1);
             ++loads_v;
         }
-        if (warp == 0 && elect_one()) {
+        if (warp == kIssue && elect_one()) {
             ok = mbar_wait(&bar_s, i & 1);
             if (ok) {
                 tc_fence_after();
                 constexpr uint32_t narrow = instr_desc(1, false, true, kP), wide = instr_desc(1, false, false, NT);
-                const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), n0 = smem_u32(smN);
+                const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK);
                 const uint32_t v_ = smem_u32(sV), d_ = smem_u32(sD), e_ = smem_u32(smE), s_ = smem_u32(smS), g_ = smem_u32(smG);
 #pragma unroll
                 for (int kk = 0; kk < kQ / 16; ++kk)             // dv from the chunk, from the future; S^T q
@@ -953,12 +961,6 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                     umma(tmem + cK, smem_desc(v_ + kk * 32, 16, 1024), smem_desc(g_ + kk * 32, 16, 1024), wide, i > 0 || kk > 0 ? 1u : 0u);
                 }
                 umma_commit(&done_a);
-#pragma unroll
-                for (int kk = 0; kk < kQ / 16; ++kk) {           // dq and dk from the chunk, while dv leaves
-                    umma(tmem + cQ, smem_desc(n0 + kk * 2048, kSlab, 1024), smem_desc(k0 + kk * 2048, kSlab, 1024), instr_desc(1, true, true, NT), 1u);
-                    umma(tmem + cK, smem_desc(n0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(q0 + kk * 2048, kSlab, 1024), instr_desc(1, false, true, NT), 1u);
-                }
-                umma_commit(&done_b);
             }
         }
         if (ok) ok = mbar_wait(&bar_s, i & 1);
@@ -971,6 +973,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
 #pragma unroll
                 for (int j = 0; j < 8; ++j) through = fmaf(e[j], f[j], through);
             }
+        const float whole = tb.whole[0];                         // read here: behind the next barrier its table may be another head's
         if (last) {
             float v = through;
 #pragma unroll
@@ -1019,20 +1022,17 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                         *reinterpret_cast<const uint4 *>(sV + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
             }
         }
-        if (last && warp == 7 && a.dg) {
-            float all = lane < 16 ? cross[lane] : 0.f, x[4], b[4];
+        if (last && warp == kSums && a.dg) {
+            float all = lane < 16 ? cross[lane] : 0.f, x[4] = {}, b[4] = {};
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-            all *= exp2f(tb.whole[0]);
+            all *= ex2_approx(whole);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int t = lane * 4 + k;
-                x[k] = b[k] = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[k] += past[j][t] + (colsum[j][t] - rowsum[j][t]);
-                    b[k] += future[j][t];
-                }
+            for (int j = 0; j < 4; ++j) {
+                const float4 u = *reinterpret_cast<const float4 *>(&past[j][lane * 4]), v = *reinterpret_cast<const float4 *>(&colsum[j][lane * 4]);
+                const float4 w = *reinterpret_cast<const float4 *>(&rowsum[j][lane * 4]), z = *reinterpret_cast<const float4 *>(&future[j][lane * 4]);
+                x[0] += u.x + (v.x - w.x); x[1] += u.y + (v.y - w.y); x[2] += u.z + (v.z - w.z); x[3] += u.w + (v.w - w.w);
+                b[0] += z.x; b[1] += z.y; b[2] += z.z; b[3] += z.w;
             }
             // sums of x from each token on, of b before each
             float xs = x[0] + x[1] + x[2] + x[3], bs = b[0] + b[1] + b[2] + b[3];
@@ -1053,6 +1053,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             }
         }
     }
+    if (ok && warp == kIssue && elect_one()) from_chunk();
     if (ok) ok = mbar_wait(&done_b, (nv - 1) & 1);
     tc_fence_after();
     ok = __syncthreads_and(ok);
@@ -1095,18 +1096,16 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     } else if (tid == 0) {
         atomicExch(a.status, kErrDecay + 3);
     }
+    if (!ok && warp == kIssue && elect_one()) {                  // leave nothing in flight
+        drain_mmas(&unused);
+        drain_loads(&bar_qk, 1, 1);
+        drain_loads(bar_v, 2, loads_v);
+        drain_loads(&bar_s, 1, loads_s);
+    }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
-        if (!ok && elect_one()) {                                // leave nothing in flight
-            drain_mmas(&unused);
-            drain_loads(&bar_qk, 1, 1);
-            drain_loads(bar_v, 2, loads_v);
-            drain_loads(&bar_s, 1, loads_s);
-        }
-        __syncwarp();
-        tmem_dealloc(tmem, 512);
-    }
+    if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
 // dq and dk of chunks whose heads were walked by several blocks: their parts added up in order.
