@@ -444,15 +444,15 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     const Segment s = uni::segment(a.chunk, ci);
     if (s.len == 0) return;
     const int R = a.h.H / a.h.hk, v0 = part * a.vpc, nv = min(a.vpc, R * a.h.PB - v0), h0 = m * R + v0 / a.h.PB;
-    auto head = [&](int i) { return m * R + (v0 + i) / a.h.PB; };
-    const int heads = head(nv - 1) - h0 + 1;
-    auto load_v = [&](int i) {
+    int h = h0, pb = v0 - v0 / a.h.PB * a.h.PB;                  // of the present tile
+    const int heads = (pb + nv + a.h.PB - 1) / a.h.PB;
+    auto load_v = [&](int h, int pb) {
         mbar_expect_tx(&bar_v, kSlab);
-        tma_load4(smV, &tmV, (v0 + i) % a.h.PB * kP, head(i), s.t0, s.batch, &bar_v);
+        tma_load4(smV, &tmV, pb * kP, h, s.t0, s.batch, &bar_v);
     };
-    auto load_s = [&](int i) {
+    auto load_s = [&](int h, int pb) {
         mbar_expect_tx(&bar_s, NT * 128);
-        tma_load2(smS, &tmS, 0, ((ci * a.h.H + head(i)) * a.h.PB + (v0 + i) % a.h.PB) * NT, &bar_s);
+        tma_load2(smS, &tmS, 0, ((ci * a.h.H + h) * a.h.PB + pb) * NT, &bar_s);
     };
     Decays next;                                                 // this warp's head of the next kTables
     auto ask = [&](int k) {
@@ -481,8 +481,8 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
             tma_load4(smQ + j * kSlab, &tmQ, j * 64, m, s.t0, s.batch, &bar_qk);
             tma_load4(smK + j * kSlab, &tmK, j * 64, m, s.t0, s.batch, &bar_qk);
         }
-        load_s(0);
-        load_v(0);
+        load_s(h, pb);
+        load_v(h, pb);
     }
     table(warp);
     ask(kTables + warp);
@@ -513,9 +513,11 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     if (ok && half == 1)
         for (int u = 2 * (r32 + 1); u < 8; ++u)                  // above the diagonal
             for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4 *>(pair_at(u) + piece(u, j)) = zero8();
+    bf16 *out = a.o + ((long long)s.batch * a.chunk.L + s.t0 + (tid >> 3)) * a.h.H * a.h.P;   // the first of the rows this thread writes
+    const long long row32 = 32LL * a.h.H * a.h.P;
     for (int i = 0; i < nv && ok; ++i) {
-        const int k = head(i) - h0;
-        if (i > 0 && k % kTables == 0 && head(i) != head(i - 1)) {
+        const int k = h - h0, h1 = h + (pb + 1 == a.h.PB), pb1 = pb + 1 == a.h.PB ? 0 : pb + 1;   // and the next tile's
+        if (i > 0 && k % kTables == 0 && pb == 0) {
             __syncthreads();                                     // the last tables have been read
             table(k + warp);
             ask(k + kTables + warp);
@@ -599,12 +601,12 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         }
         if (i + 1 < nv) {                                        // the state's tile is long read; v's rows when all is done
             if (tid == 32) ok = mbar_wait(&done_s, i & 1);
-            if (tid == 32 && ok) load_s(i + 1);
+            if (tid == 32 && ok) load_s(h1, pb1);
             ++loads_s;
         }
         if (ok) ok = mbar_wait(&done, (i + 1) & 1) && mbar_wait(&done_s, i & 1);
         if (i + 1 < nv) {
-            if (tid == 32 && ok) load_v(i + 1);
+            if (tid == 32 && ok) load_v(h1, pb1);
             ++loads_v;
         }
         tc_fence_after();
@@ -625,17 +627,19 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         tc_fence_before();
         ok = __syncthreads_and(ok);
         if (!ok) break;
-        const int col = (v0 + i) % a.h.PB * kP + (tid & 7) * 8;
+        const int col = pb * kP + (tid & 7) * 8;
         if (col < a.h.P) {
-            bf16 *o = a.o + (((long long)s.batch * a.chunk.L + s.t0) * a.h.H + head(i)) * a.h.P + col;
+            bf16 *o = out + h * a.h.P + col;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int r = (tid >> 3) + q * 32;
-                if (r < s.len) *reinterpret_cast<uint4 *>(o + (long long)r * a.h.H * a.h.P) = *reinterpret_cast<const uint4 *>(smK + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
+                if (r < s.len) *reinterpret_cast<uint4 *>(o + q * row32) = *reinterpret_cast<const uint4 *>(smK + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
             }
         }
         __syncthreads();                                         // the slab is the pairs' again
         tc_fence_after();
+        h = h1;
+        pb = pb1;
     }
     ok = __syncthreads_and(ok);
     if (!ok && tid == 0) atomicExch(a.status, kErrDecay + 2);
@@ -722,16 +726,15 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     if (sg.len == 0) return;
     const int len = sg.len, R = a.h.H / a.h.hk, v0 = part * a.vpc, nv = min(a.vpc, R * a.h.PB - v0);
     const bool tail = a.chunk.packed && len < kQ;                // rows of another sequence lie behind this one's
-    auto head = [&](int i) { return m * R + (v0 + i) / a.h.PB; };
-    auto first_of = [&](int i) { return (v0 + i) % a.h.PB == 0; };
-    auto load_v = [&](int i) {
-        const int h = head(i), pb = (v0 + i) % a.h.PB, b = i & 1;
+    const int h0 = m * R + v0 / a.h.PB;                          // the block's first head; it starts with the head's first tile
+    auto load_v = [&](int i, int h, int pb) {
+        const int b = i & 1;
         mbar_expect_tx(&bar_v[b], 2 * kSlab);
         tma_load4(smV + b * kSlab, &tmV, pb * kP, h, sg.t0, sg.batch, &bar_v[b]);
         tma_load4(smD + b * kSlab, &tmD, pb * kP, h, sg.t0, sg.batch, &bar_v[b]);
     };
-    auto load_s = [&](int i) {
-        const int row = ((ci * a.h.H + head(i)) * a.h.PB + (v0 + i) % a.h.PB) * NT;
+    auto load_s = [&](int h, int pb) {
+        const int row = ((ci * a.h.H + h) * a.h.PB + pb) * NT;
         mbar_expect_tx(&bar_s, 2 * NT * 128);
         tma_load2(smS, &tmS, 0, row, &bar_s);
         tma_load2(smG, &tmG, 0, row, &bar_s);
@@ -772,13 +775,13 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             tma_load4(smQ + j * kSlab, &tmQ, j * 64, m, sg.t0, sg.batch, &bar_qk);
             tma_load4(smK + j * kSlab, &tmK, j * 64, m, sg.t0, sg.batch, &bar_qk);
         }
-        load_v(0);
-        load_s(0);
-        if (nv > 1) load_v(1);
+        load_v(0, h0, 0);
+        load_s(h0, 0);
+        if (nv > 1) load_v(1, h0 + (a.h.PB == 1), a.h.PB == 1 ? 0 : 1);
     }
     if (warp == kTables) {
         Decays d;
-        d.load(a.h, sg.batch, sg.t0, len, head(0), lane);
+        d.load(a.h, sg.batch, sg.t0, len, h0, lane);
         table(tables[0], d);
     }
     tc_fence_before();
@@ -796,6 +799,8 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             clear_rows(smK + j * kSlab, len, tid, kT);
         }
     float through = 0.f;                                         // this thread's part of S.G
+    const long long token = (long long)sg.batch * a.chunk.L + sg.t0;
+    bf16 *dv = a.dv + (token + (tid >> 3)) * a.h.H * a.h.P;      // the first of the two rows this thread writes of each tile
     auto from_chunk = [&]() {                                    // dq and dk of the chunk's own pairs; one thread
         constexpr uint32_t iq = instr_desc(1, true, true, NT), ik = instr_desc(1, false, true, NT);
         const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), n0 = smem_u32(smN);
@@ -806,9 +811,11 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         }
         umma_commit(&done_b);
     };
+    int h = h0, pb = 0;                                          // of tile i
     for (int i = 0; i < nv; ++i) {
-        const bool first = first_of(i), last = i + 1 == nv || first_of(i + 1);   // tiles of a head
-        const Table &tb = tables[((v0 + i) / a.h.PB - v0 / a.h.PB) & 1];
+        const bool first = pb == 0, last = pb + 1 == a.h.PB;     // tiles of a head
+        const int h1 = h + last, pb1 = last ? 0 : pb + 1;        // of the next one
+        const Table &tb = tables[(h - h0) & 1];
         uint8_t *sV = smV + (i & 1) * kSlab, *sD = smD + (i & 1) * kSlab;
         if (tail) {
             ok = ok && mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
@@ -836,10 +843,10 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 if (i > 0) from_chunk();                         // of the tile before: here nothing waits for them
             }
         }
-        if (warp == kTables && i + 1 < nv && first_of(i + 1)) {  // the next head's; the turn before the last one has been read
+        if (warp == kTables && i + 1 < nv && last) {             // the next head's; the turn before the last one has been read
             Decays d;
-            d.load(a.h, sg.batch, sg.t0, len, head(i + 1), lane);
-            table(tables[((v0 + i + 1) / a.h.PB - v0 / a.h.PB) & 1], d);
+            d.load(a.h, sg.batch, sg.t0, len, h1, lane);
+            table(tables[(h1 - h0) & 1], d);
         }
         if (ok) ok = mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
         if (ok) {
@@ -936,7 +943,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         ok = __syncthreads_and(ok);
         if (!ok) break;
         if (i > 0 && i + 1 < nv) {                               // the tile before has left its buffers
-            if (tid == 32) load_v(i + 1);
+            if (tid == 32) load_v(i + 1, h1, pb1);
             ++loads_v;
         }
         if (warp == kIssue && elect_one()) {
@@ -1008,17 +1015,17 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         ok = __syncthreads_and(ok);
         if (!ok) break;
         if (i + 1 < nv) {
-            if (tid == 32) load_s(i + 1);
+            if (tid == 32) load_s(h1, pb1);
             ++loads_s;
         }
-        const int h = head(i), col = (v0 + i) % a.h.PB * kP + (tid & 7) * 8;
-        const long long token = (long long)sg.batch * a.chunk.L + sg.t0;
+        const int col = pb * kP + (tid & 7) * 8;
         if (col < a.h.P) {
+            bf16 *o = dv + h * a.h.P + col;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int r = (tid >> 3) + k * 64;
                 if (r < len)
-                    *reinterpret_cast<uint4 *>(a.dv + ((token + r) * a.h.H + h) * a.h.P + col) =
+                    *reinterpret_cast<uint4 *>(o + k * 64 * (long long)a.h.H * a.h.P) =
                         *reinterpret_cast<const uint4 *>(sV + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
             }
         }
@@ -1052,6 +1059,8 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 bs += b[k];
             }
         }
+        h = h1;
+        pb = pb1;
     }
     if (ok && warp == kIssue && elect_one()) from_chunk();
     if (ok) ok = mbar_wait(&done_b, (nv - 1) & 1);
@@ -1059,7 +1068,6 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     ok = __syncthreads_and(ok);
     if (ok) {                                                    // dq and dk: rows s (or t), NT / 4 columns a thread
         constexpr int kCols = NT / 4;
-        const long long token = (long long)sg.batch * a.chunk.L + sg.t0;
 #pragma unroll
         for (int what = 0; what < 2; ++what) {
             const uint32_t at = tl + (what ? cK : cQ) + cg * kCols;
