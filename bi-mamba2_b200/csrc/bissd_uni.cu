@@ -374,7 +374,7 @@ bool tc_map(CUtensorMap *m, const bissd_decay_args *a, const bissd_tensor &t, in
 }
 
 // The states that enter the chunks (or the gradients, backwards), as bf16 tiles; those that enter and leave the sequences in fp32.
-int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const bissd_tensor &cols, const CUtensorMap &tiles, bool reverse,
+int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &vmap, const bissd_tensor &cols, const CUtensorMap &tiles, bool reverse,
               const float *start, float *end, float *states, float *decay, int *status, cudaStream_t s) {
     unitc::StatesParams p{};
     p.h = tc_heads(a, t.PB);
@@ -386,7 +386,7 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
         const auto kernel = t.NT == 64 ? (exact ? unitc::decay_states<64, true> : unitc::decay_states<64, false>)
                                        : (exact ? unitc::decay_states<128, true> : unitc::decay_states<128, false>);
         BISSD_ALLOW(kernel, smem);
-        BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, tiles));
+        BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, vmap, tiles));
         return BISSD_OK;
     };
     if (t.split) {
@@ -420,7 +420,7 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
     BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
     BISSD_DO(launch_gaps(a, a->dtype, a->o, a->nheads * a->vdim, t.chunk_table.bounds, s));
-    BISSD_DO(tc_states(a, t, k, a->v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, s));
+    BISSD_DO(tc_states(a, t, k, v, a->v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, s));
     unitc::ChunksParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
@@ -507,8 +507,8 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     if (g.part)
         for (int i = 0; i < 2 * g.parts; ++i)
             BISSD_DO(launch_gaps(a, BISSD_F32, g.part + (size_t)i * a->seqlen * a->nkheads * a->kdim, a->nkheads * a->kdim, bounds, s));
-    BISSD_DO(tc_states(a, t, k, a->v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
-    BISSD_DO(tc_states(a, t, q, a->dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, s));
+    BISSD_DO(tc_states(a, t, k, v, a->v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
+    BISSD_DO(tc_states(a, t, q, dout, a->dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, s));
     unitc::GradsParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.vpc = g.vpc; p.parts = g.parts;

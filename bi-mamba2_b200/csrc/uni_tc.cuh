@@ -98,11 +98,10 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
 // ---- the states that enter the chunks ------------------------------------------------------------------------------------
 // Forwards S' as above; backwards (v the outputs' gradient, k the queries) the gradient that enters each chunk from its right,
 // G' = e^{c_end} G + sum_t q_t (scale e^{c_t} do_t)^T.  A block walks the chunks of one (segment, head, 64 columns), S or G in
-// registers (a row n and 32 columns a thread).  k's rows come by TMA a chunk ahead; v's go through registers and are weighted on the
-// way to shared memory.  Eight warps do that, a chunk ahead too, and keep S; the ninth issues loads and MMAs, the tenth makes the
-// weights and stores the tiles, and they meet at mbarriers alone.  So a step is S's way to shared memory, one product's latency and its way back,
-// with everything else in its shadow; with block-wide barriers and the weights made by one of the eight it was half as fast
-// again.  Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
+// registers (a row n and 32 columns a thread).  k's and v's rows come by TMA a chunk ahead.  Eight warps weight v's in place and keep S;
+// the ninth issues loads and MMAs, the tenth makes the weights and stores the tiles, and they meet at mbarriers alone: a step is S's
+// way to shared memory, one product's latency, its way back and the weighting.  (The weighting in the product's shadow, from rows
+// loaded to registers, made it longer: the loads from tensor memory then waited for those rows.)  Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
 // A weight f meets bf16 rows as bf16 f1 + f2, in one rounding: v f1 + (v f2) as a multiply-add.
 // EXACT: the weighted row is given to the tensor cores in three bf16 parts, each what is left of those before, so that the states
 // that leave the library are fp32's.  The tiles that the other kernels read are bf16 in any case: they meet bf16 factors.
@@ -131,7 +130,7 @@ constexpr int kStatesThreads = 320;
 inline size_t states_smem(int NT) { return 2 * (size_t)(NT / 64) * kSlab + 3 * (size_t)kSlab + sizeof(StatesShared); }
 
 template <int NT, bool EXACT> __global__ void __launch_bounds__(kStatesThreads, 2)
-decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmTiles) {
+decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
     constexpr int kSlabs = NT / 64;
     extern __shared__ __align__(1024) uint8_t dyn[];
@@ -169,8 +168,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     if (warp == 8) {
         auto load = [&](int i) {
             const int st = i & 1, t = s.t0 + place(i) * kQ;
-            mbar_expect_tx(&sh.full[st], kSlabs * kSlab);
+            mbar_expect_tx(&sh.full[st], (kSlabs + !EXACT) * kSlab);
             for (int j = 0; j < kSlabs; ++j) tma_load4(smK + (st * kSlabs + j) * kSlab, &tmK, j * 64, hq, t, s.batch, &sh.full[st]);
+            if (!EXACT) tma_load4(smV + st * kSlab, &tmV, pb * kP, h, t, s.batch, &sh.full[st]);
         };
         if (lane == 0) load(0);
         int loads = 1, round = 0;
@@ -291,12 +291,13 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             for (int k = 0; k < 4; ++k) rows[k] = k * 32 < left ? __ldg(reinterpret_cast<const uint4 *>(p + k * vstep)) : zero8();
         };
         const uint32_t swz = (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);   // the thread's piece of a tile, + 4096 k
-        auto weigh = [&](uint8_t *to) {                          // bf16 rows times f1 + f2
+        auto weigh = [&](uint8_t *v, int len) {                  // bf16 rows times f1 + f2, in their place
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t f = sh.w[(tid >> 3) + k * 32];
                 const uint32_t f1 = __byte_perm(f, f, 0x1010), f2 = __byte_perm(f, f, 0x3232);
-                uint32_t e[4] = {rows[k].x, rows[k].y, rows[k].z, rows[k].w};
+                const uint4 row = *reinterpret_cast<const uint4 *>(v + swz + k * 4096);
+                uint32_t e[4] = {row.x, row.y, row.z, row.w};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&e[q]);
@@ -304,7 +305,8 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                                                      __hmul2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f2)));
                     e[q] = *reinterpret_cast<const uint32_t *>(&o);
                 }
-                *reinterpret_cast<uint4 *>(to + swz + k * 4096) = make_uint4(e[0], e[1], e[2], e[3]);
+                // rows behind the sequence's end may be of another, and no numbers
+                *reinterpret_cast<uint4 *>(v + swz + k * 4096) = (tid >> 3) + k * 32 < len ? make_uint4(e[0], e[1], e[2], e[3]) : zero8();
             }
         };
         float ff[4];
@@ -325,7 +327,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 *reinterpret_cast<uint4 *>(to + swz + k * 4096) = out;
             }
         };
-        fetch(0);
+        if constexpr (EXACT) fetch(0);
         const int n = (warp & 3) * 32 + lane, half = warp >> 2, col = pb * kP + half * 32;
         const long long at = (((long long)(a.by_seq ? s.seq : si) * a.h.H + h) * a.h.N + n) * a.h.P + col;
         float S[32];
@@ -339,11 +341,15 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             if (lane == 0) mbar_arrive(&sh.ready);
         };
         int round = 0;
-        if constexpr (!EXACT) {
-            ok = ws_wait_warp(&sh.weights, 0, fail, 4);
-            if (ok) weigh(smV);
-            fetch(1);
-        }
+        auto prepare = [&](int i) {                              // chunk i's rows
+            const int st = i & 1;
+            if (!ws_wait_warp(&sh.weights, i & 1, fail, 4) || !ws_wait_warp(&sh.full[st], (i >> 1) & 1, fail, 6)) return false;
+            weigh(smV + st * kSlab, length(i));
+            if (a.seg.packed && length(i) < kQ)
+                for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, length(i), tid, 256);
+            return true;
+        };
+        if constexpr (!EXACT) ok = prepare(0);
         for (int i = 0; i < nc && ok; ++i) {
             const int st = i & 1;
             float now;
@@ -368,7 +374,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                     }
                 }
             }
-            if (a.seg.packed && length(i) < kQ) {
+            if (EXACT && a.seg.packed && length(i) < kQ) {
                 ok = ws_wait_warp(&sh.full[st], (i >> 1) & 1, fail, 6);
                 if (!ok) break;
                 for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, length(i), tid, 256);
@@ -384,11 +390,6 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                     ++round;
                 }
                 fetch(i + 1);
-            } else if (i + 1 < nc) {                             // the next chunk's rows, while this one's product runs
-                ok = ws_wait_warp(&sh.weights, (i + 1) & 1, fail, 4);
-                if (!ok) break;
-                weigh(smV + (st ^ 1) * kSlab);
-                fetch(i + 2);
             }
             ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 8);
             if (!ok) break;
@@ -400,6 +401,8 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
                 for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, x[j]);
             }
+            if constexpr (!EXACT)
+                if (i + 1 < nc) ok = prepare(i + 1);
         }
         if (ok && a.fin && n < a.h.N) {
 #pragma unroll
