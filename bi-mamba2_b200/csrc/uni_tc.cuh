@@ -120,7 +120,7 @@ __device__ __forceinline__ void tma_store_read() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 struct StatesShared {
-    uint64_t full[2], ready, done, weights, stored, unused;
+    uint64_t full[2], full_v, ready, staged, done, weights, stored, unused;   // staged: ready for the first time in a step
     uint32_t tmem;
     int fail;
     float decay[2];                                              // of a chunk, 2^c_end
@@ -148,12 +148,14 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     auto place = [&](int i) { return a.reverse ? nc - 1 - i : i; };        // chunk of the segment at step i
     auto length = [&](int i) { return min(kQ, s.len - place(i) * kQ); };
     volatile int *fail = &sh.fail;
-    const bool two = EXACT && a.tiles;                           // an exact step that stores a tile, which has the third part's buffer, has two rounds
+    const bool direct = EXACT && a.tiles;                        // v's rows straight to registers: a tile of S has their buffer
     if (warp == 0) tmem_alloc(&sh.tmem, 64);
     if (tid == 256) {
         mbar_init(&sh.full[0], 1);
         mbar_init(&sh.full[1], 1);
+        mbar_init(&sh.full_v, 1);
         mbar_init(&sh.ready, 8);
+        mbar_init(&sh.staged, 8);
         mbar_init(&sh.done, 1);
         mbar_init(&sh.weights, 1);
         mbar_init(&sh.stored, 1);
@@ -172,8 +174,13 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             for (int j = 0; j < kSlabs; ++j) tma_load4(smK + (st * kSlabs + j) * kSlab, &tmK, j * 64, hq, t, s.batch, &sh.full[st]);
             if (!EXACT) tma_load4(smV + st * kSlab, &tmV, pb * kP, h, t, s.batch, &sh.full[st]);
         };
+        auto load_v = [&](int i) {                               // EXACT
+            mbar_expect_tx(&sh.full_v, kSlab);
+            tma_load4(smS, &tmV, pb * kP, h, s.t0 + place(i) * kQ, s.batch, &sh.full_v);
+        };
         if (lane == 0) load(0);
-        int loads = 1, round = 0;
+        if (EXACT && !direct && lane == 0) load_v(0);
+        int loads = 1, loads_v = EXACT && !direct, round = 0;
         constexpr uint32_t idesc = instr_desc(1, true, true, kP);
         for (int i = 0; i < nc && ok; ++i) {
             const int st = i & 1;
@@ -189,19 +196,20 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                     umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 0 : kSlab, 1024),
                          smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : first);
             };
-            for (int r = 0; r < (two ? 2 : 1) && ok; ++r, ++round) {
+            for (int r = 0; r < (EXACT ? 2 : 1) && ok; ++r, ++round) {   // the third part goes where the first was: two rounds a step
                 ok = ws_wait_warp(&sh.ready, round & 1, fail, 3);
                 if (!ok) break;
                 tc_fence_after();
+                if (EXACT && !direct && r == 0 && i + 1 < nc) {  // this chunk's rows are in registers
+                    if (lane == 0) load_v(i + 1);
+                    ++loads_v;
+                }
                 if (elect_one()) {
                     if (r == 1) {
                         issue(smV, 1u);
                     } else {
                         issue(smV + (EXACT ? 0 : st * kSlab), 0u);
-                        if constexpr (EXACT) {
-                            issue(smV + kSlab, 1u);
-                            if (!a.tiles) issue(smS, 1u);
-                        }
+                        if constexpr (EXACT) issue(smV + kSlab, 1u);
                     }
                     umma_commit(&sh.done);
                 }
@@ -211,6 +219,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         if (!ok && elect_one()) {                                // leave nothing in flight
             drain_mmas(&sh.unused);
             drain_loads(sh.full, 2, loads);
+            drain_loads(&sh.full_v, 1, loads_v);
             atomicExch(a.status, kErrDecay + 0x10 + *fail);
         }
         __syncwarp();
@@ -257,7 +266,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         if (nc > 1) make();
         ask(2);
         for (int i = 0; i < nc; ++i) {
-            ok = ws_wait_warp(&sh.ready, (two ? 2 * i : i) & 1, fail, 9);
+            ok = ws_wait_warp(&sh.staged, i & 1, fail, 9);       // the next one cannot come before this warp's weights: none is missed
             if (!ok) break;
             if (i + 1 < nc) give(i + 1);
             if (a.tiles && elect_one()) {
@@ -270,8 +279,6 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 make();
                 ask(i + 3);
             }
-            if (two) ok = ws_wait_warp(&sh.ready, 1, fail, 9);   // the last part's
-            if (!ok) break;
         }
         if (a.decay && ok && pb == 0 && lane == 0) a.decay[(long long)si * a.h.H + h] = exp2f(total);
         if (a.tiles && elect_one()) tma_store_wait();
@@ -309,36 +316,43 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 *reinterpret_cast<uint4 *>(v + swz + k * 4096) = (tid >> 3) + k * 32 < len ? make_uint4(e[0], e[1], e[2], e[3]) : zero8();
             }
         };
-        float ff[4];
-        auto part = [&](int which, uint8_t *to) {                // part 0, 1 or 2 of the weighted rows
+        auto parts = [&]() {                                     // the first two parts of the weighted rows to their buffers, the third kept
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                float e[8], r[8];
-                unpack8<bf16>(rows[k], e);
+                const float f = __uint_as_float(sh.w[(tid >> 3) + k * 32]);
+                uint32_t e[4] = {rows[k].x, rows[k].y, rows[k].z, rows[k].w}, o1[4], o2[4];
 #pragma unroll
-                for (int m = 0; m < 8; ++m) e[m] *= ff[k];
-                uint4 out = pack8<bf16>(e);
-                for (int q = 0; q < which; ++q) {
-                    unpack8<bf16>(out, r);
-#pragma unroll
-                    for (int m = 0; m < 8; ++m) e[m] -= r[m];
-                    out = pack8<bf16>(e);
+                for (int q = 0; q < 4; ++q) {
+                    float x, y, hx, hy;
+                    unpack2<bf16>(e[q], x, y);
+                    x *= f;
+                    y *= f;
+                    o1[q] = pack2<bf16>(x, y);
+                    unpack2<bf16>(o1[q], hx, hy);
+                    x -= hx;
+                    y -= hy;
+                    o2[q] = pack2<bf16>(x, y);
+                    unpack2<bf16>(o2[q], hx, hy);
+                    e[q] = pack2<bf16>(x - hx, y - hy);
                 }
-                *reinterpret_cast<uint4 *>(to + swz + k * 4096) = out;
+                *reinterpret_cast<uint4 *>(smV + swz + k * 4096) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+                *reinterpret_cast<uint4 *>(smV + kSlab + swz + k * 4096) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+                rows[k] = make_uint4(e[0], e[1], e[2], e[3]);
             }
         };
-        if constexpr (EXACT) fetch(0);
+        if (direct) fetch(0);
         const int n = (warp & 3) * 32 + lane, half = warp >> 2, col = pb * kP + half * 32;
         const long long at = (((long long)(a.by_seq ? s.seq : si) * a.h.H + h) * a.h.N + n) * a.h.P + col;
         float S[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) S[j] = a.init && n < a.h.N && col + j < a.h.P ? a.init[at + j] : 0.f;
         const uint32_t tl = tmem_lane_base(tmem) + half * 32;
-        auto arrive = [&]() {                                    // what this warp wrote is there, what it read of tensor memory is read
+        auto arrive = [&](bool first) {                          // what this warp wrote is there, what it read of tensor memory is read
             fence_async_smem();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.ready);
+            if (lane == 0 && first) mbar_arrive(&sh.staged);
         };
         int round = 0;
         auto prepare = [&](int i) {                              // chunk i's rows
@@ -354,13 +368,14 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             const int st = i & 1;
             float now;
             if constexpr (EXACT) {
-                ok = ws_wait_warp(&sh.weights, i & 1, fail, 4);
+                ok = ws_wait_warp(&sh.weights, i & 1, fail, 4) && (direct || ws_wait_warp(&sh.full_v, i & 1, fail, 10));
                 if (!ok) break;
+                if (!direct) {
+                    const int len = length(i) - (tid >> 3);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) ff[k] = __uint_as_float(sh.w[(tid >> 3) + k * 32]);
-                part(0, smV);
-                part(1, smV + kSlab);
-                if (!a.tiles) part(2, smS);
+                    for (int k = 0; k < 4; ++k) rows[k] = k * 32 < len ? *reinterpret_cast<const uint4 *>(smS + swz + k * 4096) : zero8();
+                }
+                parts();
             }
             now = sh.decay[st];
             if (a.tiles) {                                       // what enters this chunk
@@ -379,17 +394,15 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 if (!ok) break;
                 for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, length(i), tid, 256);
             }
-            arrive();
+            arrive(true);
             ++round;
             if constexpr (EXACT) {
-                if (two) {                                       // the last part goes where the first was
-                    ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 7);
-                    if (!ok) break;
-                    part(2, smV);
-                    arrive();
-                    ++round;
-                }
-                fetch(i + 1);
+                ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 7);
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4 *>(smV + swz + k * 4096) = rows[k];
+                arrive(false);
+                ++round;
             }
             ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 8);
             if (!ok) break;
@@ -401,8 +414,11 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
                 for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, x[j]);
             }
-            if constexpr (!EXACT)
+            if constexpr (!EXACT) {
                 if (i + 1 < nc) ok = prepare(i + 1);
+            } else if (direct) {
+                fetch(i + 1);
+            }
         }
         if (ok && a.fin && n < a.h.N) {
 #pragma unroll

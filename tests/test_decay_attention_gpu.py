@@ -139,6 +139,19 @@ def test_forward_and_backward_match_the_definition(dtype, size):
     check(dtype, tensors, dout, torch.randn(b, h, n, p, generator=gen) if initial else None)
 
 
+@pytest.mark.parametrize("size", [(1, 3001, 2, 1, 64, 64), (1, 2100, 1, 1, 128, 80)], ids=str)
+def test_long_rows_in_several_segments(size):
+    """Few heads and many chunks: the states of a row are walked in segments of several chunks each."""
+    b, L, h, hk, n, p = size
+    gen = torch.Generator().manual_seed(3)
+    q, k, v, g, init = make(torch.bfloat16, b, L, h, hk, n, p, initial=True, seed=L)
+    g = (g.float() / 50).to(g.dtype)                  # a state outlives its segment
+    check(torch.bfloat16, (q, k, v, g, init), torch.randn(b, L, h, p, generator=gen).to(torch.bfloat16), torch.randn(b, h, n, p, generator=gen))
+    bounds = [5, 1300, 1301, 2000, L]
+    init = torch.randn(4, h, n, p, generator=gen)
+    check(torch.bfloat16, (q, k, v, g, init), torch.randn(b, L, h, p, generator=gen).to(torch.bfloat16), torch.randn(4, h, n, p, generator=gen), bounds)
+
+
 PACKED = [[0, 5, 6, 6, 134, 390, 400], [3, 131, 131, 259, 300], [0, 0, 0], [0, 1, 2, 3, 4], [10, 700]]
 
 
