@@ -345,15 +345,16 @@ int tc_segment(const bissd_decay_args *a, int PB) {
     const long long parts = std::max<long long>(1, std::min<long long>(2 * 148 / blocks, chunks / 4));
     return (int)((chunks + parts - 1) / parts) * unitc::kQ;
 }
-TcSpace tc_space(const bissd_decay_args *a, Bump &ws) {
+size_t tc_tile_values(const bissd_decay_args *a, const TcSpace &t) { return (size_t)t.chunk.most * a->nheads * t.PB * t.NT * unitc::kP; }
+TcSpace tc_space(const bissd_decay_args *a, Bump &ws, bool backward) {
     TcSpace t{};
     t.NT = a->kdim <= 64 ? 64 : 128;
     t.PB = ceil_div(a->vdim, unitc::kP);
     t.chunk = plan_of(a, unitc::kQ, ws, &t.chunk_table);
     t.seg = plan_of(a, tc_segment(a, t.PB), ws, &t.seg_table);
     t.split = t.seg.packed || t.seg.per_seq > 1;
-    t.tiles = ws.take<bf16>((size_t)t.chunk.most * a->nheads * t.PB * t.NT * unitc::kP);
-    if (t.split) {
+    t.tiles = a->saved ? static_cast<bf16 *>(a->saved) : ws.take<bf16>(tc_tile_values(a, t));
+    if (t.split && !(a->saved && backward)) {
         t.states = ws.take<float>((size_t)t.seg.most * a->nheads * a->kdim * a->vdim);
         t.decay = ws.take<float>((size_t)t.seg.most * a->nheads);
     }
@@ -410,7 +411,7 @@ bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, co
 constexpr double kChunkStart = 2.0;                              // a block's start and the product q.k, in tiles of v
 
 int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
-    const TcSpace t = tc_space(a, ws);
+    const TcSpace t = tc_space(a, ws, false);
     int *status = reinterpret_cast<int *>(ws.base);
     if ((long long)t.chunk.most * a->nheads * t.PB * t.NT > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     CUtensorMap q, k, v, tiles;
@@ -455,9 +456,9 @@ struct TcGradSpace {
 };
 TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
     TcGradSpace g{};
-    g.t = tc_space(a, ws);
+    g.t = tc_space(a, ws, true);
     const long long tokens = (long long)a->batch * a->seqlen;
-    g.grads = ws.take<bf16>((size_t)g.t.chunk.most * a->nheads * g.t.PB * g.t.NT * unitc::kP);
+    g.grads = ws.take<bf16>(tc_tile_values(a, g.t));
     if (g.t.split) {
         g.gstates = ws.take<float>((size_t)g.t.seg.most * a->nheads * a->kdim * a->vdim);
         g.gdecay = ws.take<float>((size_t)g.t.seg.most * a->nheads);
@@ -507,7 +508,7 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     if (g.part)
         for (int i = 0; i < 2 * g.parts; ++i)
             BISSD_DO(launch_gaps(a, BISSD_F32, g.part + (size_t)i * a->seqlen * a->nkheads * a->kdim, a->nkheads * a->kdim, bounds, s));
-    BISSD_DO(tc_states(a, t, k, v, a->v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
+    if (!a->saved) BISSD_DO(tc_states(a, t, k, v, a->v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
     BISSD_DO(tc_states(a, t, q, dout, a->dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, s));
     unitc::GradsParams p{};
     p.h = tc_heads(a, t.PB);
@@ -538,13 +539,25 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
 
 extern "C" {
 
+int bissd_decay_saved_bytes(const bissd_decay_args *a, size_t *bytes) {
+    const int rc = decay_check(a, false);
+    if (rc != BISSD_OK) return rc;
+    if (!bytes) return BISSD_ERR_NULL;
+    *bytes = 0;
+    if (tc_sizes(a)) {                                           // the states that enter the chunks
+        Bump b{nullptr};
+        *bytes = align256(tc_tile_values(a, tc_space(a, b, false)) * sizeof(bf16));
+    }
+    return BISSD_OK;
+}
+
 int bissd_decay_workspace_bytes(const bissd_decay_args *a, size_t *fwd_bytes, size_t *bwd_bytes) {
     const int rc = decay_check(a, false);
     if (rc != BISSD_OK) return rc;
     if (fwd_bytes) {
         Bump b{nullptr}, c{nullptr};                              // which of the two runs is known at the call
         walk_space(a, b, false);
-        if (tc_sizes(a)) tc_space(a, c);
+        if (tc_sizes(a)) tc_space(a, c, false);
         *fwd_bytes = std::max(b.used, c.used);
     }
     if (bwd_bytes) {
@@ -561,7 +574,7 @@ int bissd_decay_forward(const bissd_decay_args *a, void *workspace, size_t works
     BISSD_DO(bissd_decay_workspace_bytes(a, &need, nullptr));
     BISSD_DO(decay_pointers(a, false));
     if (!workspace || workspace_bytes < need) return BISSD_ERR_WORKSPACE;
-    if (reinterpret_cast<uintptr_t>(workspace) % 256) return BISSD_ERR_ALIGN;
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 || reinterpret_cast<uintptr_t>(a->saved) % 256) return BISSD_ERR_ALIGN;
     BISSD_DO(check_device());
     Bump b{static_cast<char *>(workspace)};
     const auto s = static_cast<cudaStream_t>(stream);
@@ -573,7 +586,7 @@ int bissd_decay_backward(const bissd_decay_args *a, void *workspace, size_t work
     BISSD_DO(bissd_decay_workspace_bytes(a, nullptr, &need));
     BISSD_DO(decay_pointers(a, true));
     if (!workspace || workspace_bytes < need) return BISSD_ERR_WORKSPACE;
-    if (reinterpret_cast<uintptr_t>(workspace) % 256) return BISSD_ERR_ALIGN;
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 || reinterpret_cast<uintptr_t>(a->saved) % 256) return BISSD_ERR_ALIGN;
     BISSD_DO(check_device());
     Bump b{static_cast<char *>(workspace)};
     const auto s = static_cast<cudaStream_t>(stream);

@@ -113,10 +113,10 @@ at::DimVector state_shape(const Tensor &q, const Tensor &v, const Config &cfg) {
 }
 
 struct Attention {
-    Tensor out, final_;
+    Tensor out, final_, saved;
 };
 Attention attention_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g_, const Tensor &initial_, const Tensor &cu,
-                            const Config &cfg, bool finals) {
+                            const Config &cfg, bool finals, bool keep) {
     const Tensor q = in_place(q_), k = in_place(k_), v = in_place(v_), initial = contiguous(initial_);
     const Tensor g = g_.dim() == 1 ? g_.contiguous() : g_;
     Attention r;
@@ -131,6 +131,11 @@ Attention attention_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_
     a.o = ptr(r.out);
     a.final_state = static_cast<float *>(ptr(r.final_));
     size_t bytes = 0;
+    if (keep) {
+        bissd_check(bissd_decay_saved_bytes(&a, &bytes));
+        if (bytes) r.saved = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+        a.saved = ptr(r.saved);
+    }
     bissd_check(bissd_decay_workspace_bytes(&a, &bytes, nullptr));
     const Scratch ws(bytes);
     const auto stream = c10::cuda::getCurrentCUDAStream(q.device().index());
@@ -144,8 +149,8 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
                                  const OptTensor &initial, const OptTensor &cu, double scale, int64_t nseq, bool finals, bool check_status) {
         at::AutoDispatchBelowADInplaceOrView below;
         const Config cfg{scale, nseq, check_status};
-        Attention r = attention_forward(q, k, v, g, value(initial), value(cu), cfg, finals);
-        ctx->save_for_backward({q, k, v, g, value(initial), value(cu)});
+        Attention r = attention_forward(q, k, v, g, value(initial), value(cu), cfg, finals, true);
+        ctx->save_for_backward({q, k, v, g, value(initial), value(cu), r.saved});
         auto &s = ctx->saved_data;
         s["scale"] = scale; s["nseq"] = nseq; s["check_status"] = check_status;
         ctx->set_materialize_grads(false);
@@ -174,6 +179,7 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
             return {dq, dk, dv, dg, dinitial, none, none, none, none, none};
         }
         bissd_decay_args a = decay_args(q, k, v, g, initial, cu, cfg);
+        a.saved = ptr(saved[6]);
         a.dout = tensor4(dout);
         a.dq = ptr(dq); a.dk = ptr(dk); a.dv = ptr(dv); a.dg = ptr(dg);
         a.dfinal_state = static_cast<const float *>(ptr(dfinal));
@@ -241,7 +247,7 @@ py::object decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, co
             r = AttentionFn::apply(q, k, v, g, initial, cu.defined() ? OptTensor(cu) : OptTensor(), cfg.scale, nseq, finals, check_status);
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
-            Attention o = attention_forward(q, k, v, g, init, cu, cfg, finals);
+            Attention o = attention_forward(q, k, v, g, init, cu, cfg, finals, false);
             r = finals ? variable_list{o.out, o.final_} : variable_list{o.out};
         }
     }

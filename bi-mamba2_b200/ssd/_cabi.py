@@ -69,7 +69,7 @@ class DecayArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("batch", "seqlen", "nheads", "nkheads", "kdim", "vdim", "nseq", "dtype", "g_dtype",
                                          "g_per_head")] + \
                [("scale", C.c_float), ("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", C.c_void_p), ("g", Tensor),
-                ("cu_seqlens", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p),
+                ("cu_seqlens", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p), ("saved", C.c_void_p),
                 ("dout", Tensor), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dg", C.c_void_p),
                 ("dfinal_state", C.c_void_p), ("dinitial_state", C.c_void_p)]
 
@@ -93,7 +93,7 @@ EXPORTS = ("bissd_abi_version", "bissd_strerror", "bissd_last_cuda_error", "biss
            "bissd_forward_static_scratch", "bissd_chain_boundaries", "bissd_rmsnorm_gated_workspace_bytes", "bissd_rmsnorm_gated_forward",
            "bissd_rmsnorm_gated_backward", "bissd_dwconv_silu_workspace_bytes", "bissd_dwconv_silu_forward",
            "bissd_dwconv_silu_backward", "bissd_backward_into", "bissd_layer_params_in", "bissd_layer_params_out",
-           "bissd_decay_workspace_bytes", "bissd_decay_forward", "bissd_decay_backward", "bissd_decay_step",
+           "bissd_decay_saved_bytes", "bissd_decay_workspace_bytes", "bissd_decay_forward", "bissd_decay_backward", "bissd_decay_step",
            "bissd_block_norm_workspace_bytes", "bissd_block_norm_forward", "bissd_block_norm_backward")
 
 STATIC_SCRATCH_BYTES = 16 << 20      # BISSD_STATIC_SCRATCH_BYTES
@@ -149,7 +149,8 @@ def load():
     lib.bissd_dwconv_silu_forward.argtypes = [C.POINTER(ConvArgs), C.c_void_p]
     lib.bissd_dwconv_silu_backward.restype = C.c_int
     lib.bissd_dwconv_silu_backward.argtypes = [C.POINTER(ConvArgs), C.c_void_p, C.c_size_t, C.c_void_p]
-    for name, args in (("bissd_decay_workspace_bytes", [C.POINTER(DecayArgs), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+    for name, args in (("bissd_decay_saved_bytes", [C.POINTER(DecayArgs), C.POINTER(C.c_size_t)]),
+                       ("bissd_decay_workspace_bytes", [C.POINTER(DecayArgs), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
                        ("bissd_decay_forward", [C.POINTER(DecayArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
                        ("bissd_decay_backward", [C.POINTER(DecayArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
                        ("bissd_decay_step", [C.POINTER(DecayStepArgs), C.c_void_p]),

@@ -291,6 +291,8 @@ typedef struct bissd_decay_args {
     const int32_t *cu_seqlens;           /* (nseq + 1) */
     const float *initial_state;          /* (sequences, nheads, kdim, vdim) contiguous, or NULL: zeros */
     float *final_state;                  /* the same shape; may be NULL */
+    void *saved;                         /* bissd_decay_saved_bytes(), written by the forward pass and read by the backward pass of the same
+                                            arguments, 256-byte aligned; NULL: the backward pass works it out again */
     /* backward: */
     bissd_tensor dout;
     void *dq, *dk, *dv;                  /* contiguous, like q, k, v */
@@ -299,7 +301,8 @@ typedef struct bissd_decay_args {
     float *dinitial_state;               /* may be NULL */
 } bissd_decay_args;
 
-/* Scratch of either pass, a multiple of 256; workspace must be 256-byte aligned. */
+/* Scratch of either pass, a multiple of 256; workspace must be 256-byte aligned.  Less where `saved` is not NULL. */
+int bissd_decay_saved_bytes(const bissd_decay_args *args, size_t *bytes);   /* 0: nothing is worth keeping */
 int bissd_decay_workspace_bytes(const bissd_decay_args *args, size_t *fwd_bytes, size_t *bwd_bytes);
 int bissd_decay_forward(const bissd_decay_args *args, void *workspace, size_t workspace_bytes, void *stream);
 int bissd_decay_backward(const bissd_decay_args *args, void *workspace, size_t workspace_bytes, void *stream);
