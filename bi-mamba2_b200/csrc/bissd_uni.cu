@@ -337,13 +337,26 @@ struct TcSpace {
     float *states, *decay;
 };
 
-// Tokens to a segment: the walk over the chunks has a block for each (row, head, 64 columns), two blocks an SM; where that leaves
-// SMs without, rows are cut, into pieces of four chunks at least (a piece is walked twice, the first time without results).
+// Tokens to a segment of the walk over the chunks, a block for each (segment, head, 64 columns), two blocks an SM.  A walk in pieces
+// needs each piece's own sum first and a chain over them, so it pays where rows are long and heads few; packed sequences are taken
+// to be up to three times as long as their mean.  us, measured: a step of the walk 2.1, of one for exact states 3.3, a block's start 6, a
+// chain 6 (3 rows of 8 chunks, 32 blocks each: 62 in two pieces, 22 in one).
 int tc_segment(const bissd_decay_args *a, int PB) {
     const int chunks = ceil_div(a->seqlen, unitc::kQ);
-    const long long blocks = (long long)a->batch * a->nheads * PB;
-    const long long parts = std::max<long long>(1, std::min<long long>(2 * 148 / blocks, chunks / 4));
-    return (int)((chunks + parts - 1) / parts) * unitc::kQ;
+    const double heads = (double)a->nheads * PB, work = (double)a->batch * chunks * heads / (2 * 148);
+    const int longest = a->nseq > 0 ? std::min(chunks, ceil_div(3 * chunks, a->nseq)) : chunks;
+    int best = chunks;
+    double least = std::max<double>(longest, work) * 2.1 + 6;
+    for (int parts = 2; parts <= std::min(longest / 4, 128); ++parts) {
+        const int steps = ceil_div(longest, parts);
+        const double segments = ((double)a->batch * ceil_div(chunks, steps) + a->nseq) * heads, rounds = std::ceil(segments / (2 * 148));
+        const double time = rounds * (steps * (2.1 + 3.3) + 2 * 6) + 6 + segments * a->kdim * unitc::kP * 12 / 5e6;   // a chain moves 12 bytes a value
+        if (time < least) {
+            least = time;
+            best = steps;
+        }
+    }
+    return best * unitc::kQ;
 }
 size_t tc_tile_values(const bissd_decay_args *a, const TcSpace &t) { return (size_t)t.chunk.most * a->nheads * t.PB * t.NT * unitc::kP; }
 TcSpace tc_space(const bissd_decay_args *a, Bump &ws, bool backward) {
@@ -352,7 +365,7 @@ TcSpace tc_space(const bissd_decay_args *a, Bump &ws, bool backward) {
     t.PB = ceil_div(a->vdim, unitc::kP);
     t.chunk = plan_of(a, unitc::kQ, ws, &t.chunk_table);
     t.seg = plan_of(a, tc_segment(a, t.PB), ws, &t.seg_table);
-    t.split = t.seg.packed || t.seg.per_seq > 1;
+    t.split = t.seg.per_seq > 1;
     t.tiles = a->saved ? static_cast<bf16 *>(a->saved) : ws.take<bf16>(tc_tile_values(a, t));
     if (t.split && !(a->saved && backward)) {
         t.states = ws.take<float>((size_t)t.seg.most * a->nheads * a->kdim * a->vdim);
@@ -400,6 +413,9 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
         p.init = states; p.fin = p.decay = nullptr;
     } else {
         p.init = start; p.fin = end; p.by_seq = 1;
+        if (end && a->nseq > 0)
+            BISSD_LAUNCH("decay_empty", launch_pdl(uni::decay_empty, std::min((int)a->nseq, 148), 256, 0, s, start, end, (long long)a->nheads * a->kdim * a->vdim,
+                                                   (const int *)t.seg_table.bounds, (int)a->nseq));
     }
     p.tiles = 1;
     return launch("decay_states", !t.split && end != nullptr);

@@ -116,5 +116,13 @@ template <class T> __global__ void __launch_bounds__(256) decay_gaps(T *out, lon
     }
 }
 
+// States of sequences without a token: as they were (start NULL: zeros).
+__global__ void __launch_bounds__(256) decay_empty(const float *start, float *end, long long per, const int *bounds, int nseq) {
+    pdl_begin();
+    for (int s = blockIdx.x; s < nseq; s += gridDim.x)
+        if (bounds[s] == bounds[s + 1])
+            for (long long e = threadIdx.x; e < per; e += 256) end[s * per + e] = start ? start[s * per + e] : 0.f;
+}
+
 }  // namespace uni
 }  // namespace bissd
