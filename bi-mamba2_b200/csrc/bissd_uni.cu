@@ -161,15 +161,22 @@ int launch_plan(const bissd_decay_args *a, const uni::PlanOut &x, const uni::Pla
     BISSD_LAUNCH("decay_plan", launch_pdl(uni::decay_plan, y ? 2 : 1, 1024, 0, s, a->cu_seqlens, (int)a->nseq, (int)a->seqlen, x, y ? *y : x));
     return BISSD_OK;
 }
-int launch_gaps(const bissd_decay_args *a, int dtype, void *out, int row, const int *bounds, cudaStream_t s) {
-    if (a->nseq == 0 || !out) return BISSD_OK;
-    return by_dtype(dtype, [&](auto t) -> int {
-        using T = decltype(t);
-        BISSD_LAUNCH("decay_gaps", launch_pdl(uni::decay_gaps<T>, 32, 256, 0, s, static_cast<T *>(out), (long long)row, row, (int)a->seqlen,
-                                              bounds, (int)a->nseq));
+// What packed sequences leave over: rows of outputs that belong to none of them, and the states of those without a token.
+struct Rest {
+    uni::RestParams p{};
+    void rows(void *out, int dtype, long long elems) {
+        if (!out) return;
+        p.out[p.outs] = static_cast<char *>(out);
+        p.bytes[p.outs++] = elems * (long long)dtype_size(dtype);
+    }
+    int launch(const bissd_decay_args *a, const int *bounds, cudaStream_t s) {
+        if (a->nseq == 0) return BISSD_OK;
+        p.L = a->seqlen; p.nseq = a->nseq; p.bounds = bounds;
+        p.per = (long long)a->nheads * a->kdim * a->vdim;
+        BISSD_LAUNCH("decay_rest", launch_pdl(uni::decay_rest, 148, 256, 0, s, p));
         return BISSD_OK;
-    });
-}
+    }
+};
 
 struct Walks {                                                   // what the launches on CUDA cores share
     const bissd_decay_args *a;
@@ -240,7 +247,9 @@ int walk_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     const Walks w = walks_of(a, sp.plan);
     int *status = reinterpret_cast<int *>(ws.base);
     BISSD_DO(launch_plan(a, sp.table, nullptr, s));
-    BISSD_DO(launch_gaps(a, a->dtype, a->o, w.z.H * w.z.P, sp.table.bounds, s));
+    Rest rest;
+    rest.rows(a->o, a->dtype, w.z.H * w.z.P);
+    BISSD_DO(rest.launch(a, sp.table.bounds, s));
     uni::WalkParams p = walk_params(w, w.k, w.v, w.q, false);
     p.status = status;
     if (sp.states) {                                             // each segment's own sum, then what enters each
@@ -261,11 +270,13 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     const Walks w = walks_of(a, sp.plan);
     const Sizes &z = w.z;
     BISSD_DO(launch_plan(a, sp.table, nullptr, s));
-    BISSD_DO(launch_gaps(a, a->dtype, a->dv, z.H * z.P, sp.table.bounds, s));
-    if (a->dg && !a->g_per_head) BISSD_DO(launch_gaps(a, a->g_dtype, a->dg, z.H, sp.table.bounds, s));
-    BISSD_DO(launch_gaps(a, BISSD_F32, sp.dg_tokens, z.H, sp.table.bounds, s));
-    BISSD_DO(launch_gaps(a, BISSD_F32, sp.dqh, z.H * z.N, sp.table.bounds, s));
-    BISSD_DO(launch_gaps(a, BISSD_F32, sp.dkh, z.H * z.N, sp.table.bounds, s));
+    Rest rest;
+    rest.rows(a->dv, a->dtype, z.H * z.P);
+    if (!a->g_per_head) rest.rows(a->dg, a->g_dtype, z.H);
+    rest.rows(sp.dg_tokens, BISSD_F32, z.H);
+    rest.rows(sp.dqh, BISSD_F32, (long long)z.H * z.N);
+    rest.rows(sp.dkh, BISSD_F32, (long long)z.H * z.N);
+    BISSD_DO(rest.launch(a, sp.table.bounds, s));
     // states that enter the segments from the left, gradients that enter them from the right
     uni::WalkParams p = walk_params(w, w.k, w.v, w.q, false);
     p.status = reinterpret_cast<int *>(ws.base);
@@ -388,11 +399,11 @@ bool tc_map(CUtensorMap *m, const bissd_decay_args *a, const bissd_tensor &t, in
 }
 
 // The states that enter the chunks (or the gradients, backwards), as bf16 tiles; those that enter and leave the sequences in fp32.
-int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &vmap, const bissd_tensor &cols, const CUtensorMap &tiles, bool reverse,
+int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &cols, const CUtensorMap &tiles, bool reverse,
               const float *start, float *end, float *states, float *decay, int *status, cudaStream_t s) {
     unitc::StatesParams p{};
     p.h = tc_heads(a, t.PB);
-    p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.v = view(cols); p.status = status;
+    p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.status = status;
     const size_t smem = unitc::states_smem(t.NT);
     const long long grid = (long long)t.seg.most * a->nheads * t.PB;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
@@ -400,7 +411,7 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
         const auto kernel = t.NT == 64 ? (exact ? unitc::decay_states<64, true> : unitc::decay_states<64, false>)
                                        : (exact ? unitc::decay_states<128, true> : unitc::decay_states<128, false>);
         BISSD_ALLOW(kernel, smem);
-        BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, vmap, tiles));
+        BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, cols, tiles));
         return BISSD_OK;
     };
     if (t.split) {
@@ -413,9 +424,6 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
         p.init = states; p.fin = p.decay = nullptr;
     } else {
         p.init = start; p.fin = end; p.by_seq = 1;
-        if (end && a->nseq > 0)
-            BISSD_LAUNCH("decay_empty", launch_pdl(uni::decay_empty, std::min((int)a->nseq, 148), 256, 0, s, start, end, (long long)a->nheads * a->kdim * a->vdim,
-                                                   (const int *)t.seg_table.bounds, (int)a->nseq));
     }
     p.tiles = 1;
     return launch("decay_states", !t.split && end != nullptr);
@@ -436,8 +444,12 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
         return note_cuda(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
     BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
     BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
-    BISSD_DO(launch_gaps(a, a->dtype, a->o, a->nheads * a->vdim, t.chunk_table.bounds, s));
-    BISSD_DO(tc_states(a, t, k, v, a->v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, s));
+    Rest rest;
+    rest.rows(a->o, a->dtype, a->nheads * a->vdim);
+    rest.p.start = a->initial_state;
+    rest.p.end = t.split ? nullptr : a->final_state;             // the chain sees to them otherwise
+    BISSD_DO(rest.launch(a, t.chunk_table.bounds, s));
+    BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, s));
     unitc::ChunksParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
@@ -515,17 +527,18 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
         return note_cuda(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
     BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
     BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
-    const int *bounds = t.chunk_table.bounds;
-    BISSD_DO(launch_gaps(a, a->dtype, a->dv, a->nheads * a->vdim, bounds, s));
-    BISSD_DO(launch_gaps(a, a->dtype, a->dq, a->nkheads * a->kdim, bounds, s));
-    BISSD_DO(launch_gaps(a, a->dtype, a->dk, a->nkheads * a->kdim, bounds, s));
-    if (!a->g_per_head) BISSD_DO(launch_gaps(a, a->g_dtype, a->dg, a->nheads, bounds, s));
-    BISSD_DO(launch_gaps(a, BISSD_F32, g.dg_tokens, a->nheads, bounds, s));
-    if (g.part)
-        for (int i = 0; i < 2 * g.parts; ++i)
-            BISSD_DO(launch_gaps(a, BISSD_F32, g.part + (size_t)i * a->seqlen * a->nkheads * a->kdim, a->nkheads * a->kdim, bounds, s));
-    if (!a->saved) BISSD_DO(tc_states(a, t, k, v, a->v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
-    BISSD_DO(tc_states(a, t, q, dout, a->dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, s));
+    Rest rest;
+    rest.rows(a->dv, a->dtype, a->nheads * a->vdim);
+    rest.rows(a->dq, a->dtype, a->nkheads * a->kdim);
+    rest.rows(a->dk, a->dtype, a->nkheads * a->kdim);
+    if (!a->g_per_head) rest.rows(a->dg, a->g_dtype, a->nheads);
+    rest.rows(g.dg_tokens, BISSD_F32, a->nheads);
+    rest.p.start = a->dfinal_state;
+    rest.p.end = t.split ? nullptr : a->dinitial_state;
+    rest.p.parts = g.part; rest.p.n_parts = g.part ? 2 * g.parts : 0; rest.p.part_row = (long long)a->nkheads * a->kdim;
+    BISSD_DO(rest.launch(a, t.chunk_table.bounds, s));
+    if (!a->saved) BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
+    BISSD_DO(tc_states(a, t, q, dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, s));
     unitc::GradsParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.vpc = g.vpc; p.parts = g.parts;

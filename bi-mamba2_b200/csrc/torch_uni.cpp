@@ -310,24 +310,39 @@ struct NormConfig {
     double scale, eps;
     int64_t act, gate_rows;
 };
-// Rows of `width` channels a fixed stride apart, 16-byte aligned where they can be; else a copy.
-Tensor rows_of(const Tensor &t, int64_t width) {
-    if (!t.defined()) return t;
-    Tensor r = t.reshape({-1, width});
-    const bool repeats = r.size(0) > 1 && r.stride(0) < width;
-    return (width > 1 && r.stride(1) != 1) || repeats ? r.contiguous() : r;
+// Rows of `width` channels a fixed stride apart; a copy where they are not.
+struct Rows {
+    Tensor t;
+    void *p = nullptr;
+    int64_t n = 0, stride = 0;
+};
+Rows rows_of(const Tensor &t, int64_t width) {
+    Rows r;
+    if (!t.defined()) return r;
+    r.t = t;
+    r.n = t.numel() / width;
+    if (t.is_contiguous()) {
+        r.stride = width;
+    } else {
+        r.t = t.reshape({-1, width});
+        const bool repeats = r.n > 1 && r.t.stride(0) < width;
+        if ((width > 1 && r.t.stride(1) != 1) || repeats) r.t = r.t.contiguous();
+        r.stride = r.t.stride(0);
+    }
+    r.p = ptr(r.t);
+    return r;
 }
-bissd_block_norm_args norm_args(const Tensor &x, const Tensor &res, const Tensor &gate, const Tensor &scale, const Tensor &post, const Tensor &pre,
-                                const NormConfig &c) {
+bissd_block_norm_args norm_args(const Rows &x, const Rows &res, const Rows &gate, int64_t width, const Tensor &scale, const Tensor &post,
+                                const Tensor &pre, const NormConfig &c) {
     bissd_block_norm_args a{};
-    a.rows = x.size(0); a.width = (int)x.size(1); a.gate_rows = gate.defined() ? c.gate_rows : 0;
-    a.dtype = dtype_code(x.scalar_type()); a.r_dtype = dtype_code(res.scalar_type());
+    a.rows = x.n; a.width = (int)width; a.gate_rows = gate.p ? c.gate_rows : 0;
+    a.dtype = dtype_code(x.t.scalar_type()); a.r_dtype = dtype_code(res.t.scalar_type());
     a.w_dtype = a.dtype;
     for (const Tensor *w : {&scale, &post, &pre})
         if (w->defined()) a.w_dtype = dtype_code(w->scalar_type());
     a.gate_act = (int)c.act; a.scale = (float)c.scale; a.eps = (float)c.eps;
-    a.x = ptr(x); a.residual = ptr(res); a.gate = ptr(gate); a.scale_vector = ptr(scale); a.post_weight = ptr(post); a.pre_weight = ptr(pre);
-    a.stride_x = x.stride(0); a.stride_residual = res.stride(0); a.stride_gate = gate.defined() ? gate.stride(0) : 0;
+    a.x = x.p; a.residual = res.p; a.gate = gate.p; a.scale_vector = ptr(scale); a.post_weight = ptr(post); a.pre_weight = ptr(pre);
+    a.stride_x = x.stride; a.stride_residual = res.stride; a.stride_gate = gate.stride;
     return a;
 }
 struct Normed {
@@ -340,12 +355,12 @@ Normed norm_forward(const Tensor &x_, const Tensor &res_, const Tensor &gate_, c
     if (pre_.defined()) o.u = at::empty(x_.sizes(), x_.options());
     if (x_.numel() == 0) return o;
     const int64_t d = x_.size(-1);
-    const Tensor x = rows_of(x_, d), res = rows_of(res_, d), gate = rows_of(gate_, d);
+    const Rows x = rows_of(x_, d), res = rows_of(res_, d), gate = rows_of(gate_, d);
     const Tensor scale = contiguous(scale_), post = contiguous(post_), pre = contiguous(pre_);
-    bissd_block_norm_args a = norm_args(x, res, gate, scale, post, pre, c);
-    if (keep) o.rstd = at::empty({2, x.size(0)}, x.options().dtype(at::kFloat));
+    bissd_block_norm_args a = norm_args(x, res, gate, d, scale, post, pre, c);
+    if (keep) o.rstd = at::empty({2, x.n}, x_.options().dtype(at::kFloat));
     a.r = ptr(o.r); a.normed = ptr(o.u); a.rstd = static_cast<float *>(ptr(o.rstd));
-    bissd_check(bissd_block_norm_forward(&a, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()));
+    bissd_check(bissd_block_norm_forward(&a, c10::cuda::getCurrentCUDAStream(x_.device().index()).stream()));
     return o;
 }
 
@@ -380,19 +395,19 @@ struct NormFn : public torch::autograd::Function<NormFn> {
         } else {
             const int64_t d = v[0].size(-1);
             auto typed = [&](const Tensor &t, const Tensor &like) { return !t.defined() || t.scalar_type() == like.scalar_type() ? t : t.to(like.scalar_type()); };
-            const Tensor x = rows_of(v[0], d), res = rows_of(v[1], d), gate = rows_of(v[2], d);
+            const Rows x = rows_of(v[0], d), res = rows_of(v[1], d), gate = rows_of(v[2], d);
             const Tensor scale = contiguous(v[3]), post = contiguous(v[4]), pre = contiguous(v[5]);
-            const Tensor dr = rows_of(typed(go[0], v[1]), d), du = go.size() > 1 ? rows_of(typed(go[1], v[0]), d) : none;
-            if (dpre.defined() && !du.defined()) dpre.zero_();
-            bissd_block_norm_args a = norm_args(x, res, gate, scale, post, pre, c);
+            const Rows dr = rows_of(typed(go[0], v[1]), d), du = go.size() > 1 ? rows_of(typed(go[1], v[0]), d) : Rows();
+            if (dpre.defined() && !du.p) dpre.zero_();
+            bissd_block_norm_args a = norm_args(x, res, gate, d, scale, post, pre, c);
             a.rstd = static_cast<float *>(ptr(v[6]));
-            a.dr = ptr(dr); a.dnormed = ptr(du);
-            a.stride_dr = dr.defined() ? dr.stride(0) : 0; a.stride_dnormed = du.defined() ? du.stride(0) : 0;
+            a.dr = dr.p; a.dnormed = du.p;
+            a.stride_dr = dr.stride; a.stride_dnormed = du.stride;
             a.dx = ptr(dx); a.dresidual = ptr(dres); a.dgate = ptr(dgate); a.dscale = ptr(dscale); a.dpost = ptr(dpost); a.dpre = ptr(dpre);
             size_t bytes = 0;
             bissd_check(bissd_block_norm_workspace_bytes(&a, &bytes));
             const Scratch ws(bytes);
-            bissd_check(bissd_block_norm_backward(&a, ws.p.get(), bytes, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()));
+            bissd_check(bissd_block_norm_backward(&a, ws.p.get(), bytes, c10::cuda::getCurrentCUDAStream(v[0].device().index()).stream()));
         }
         return {dx, dres, dgate, dscale, dpost, dpre, none, none, none, none};
     }

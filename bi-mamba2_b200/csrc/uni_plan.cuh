@@ -106,22 +106,36 @@ __global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int 
     }
 }
 
-// Zeros in the rows of a packed output that belong to no sequence: those before the first one and behind the last.
-template <class T> __global__ void __launch_bounds__(256) decay_gaps(T *out, long long row_stride, int row_elems, int L, const int *bounds, int nseq) {
+// What packed sequences leave over.  Zeros in the rows of outputs that belong to no sequence, those before the first one and behind
+// the last; and the states of sequences without a token, which stay as they were (start NULL: zeros).
+struct RestParams {
+    int L, nseq, outs;
+    const int *bounds;
+    char *out[6];                                                // outputs and their rows' bytes, even
+    long long bytes[6];
+    float *parts;                                                // n_parts arrays of (L, part_row), or NULL
+    int n_parts;
+    long long part_row;
+    const float *start;
+    float *end;                                                  // (nseq, per), or NULL
+    long long per;
+};
+__global__ void __launch_bounds__(256) decay_rest(RestParams a) {
     pdl_begin();
-    const int head = bounds[0], tail = bounds[nseq], rows = head + L - tail;
+    const int head = a.bounds[0], tail = a.bounds[a.nseq], rows = head + a.L - tail;
     for (int i = blockIdx.x; i < rows; i += gridDim.x) {
-        T *row = out + (long long)(i < head ? i : tail + i - head) * row_stride;
-        for (int e = threadIdx.x; e < row_elems; e += 256) row[e] = from_f<T>(0.f);
+        const long long row = i < head ? i : tail + i - head;
+        for (int o = 0; o < a.outs; ++o) {
+            uint16_t *p = reinterpret_cast<uint16_t *>(a.out[o] + row * a.bytes[o]);
+            for (long long e = threadIdx.x; e < a.bytes[o] / 2; e += 256) p[e] = 0;
+        }
+        for (int k = 0; k < a.n_parts; ++k)
+            for (long long e = threadIdx.x; e < a.part_row; e += 256) a.parts[((long long)k * a.L + row) * a.part_row + e] = 0.f;
     }
-}
-
-// States of sequences without a token: as they were (start NULL: zeros).
-__global__ void __launch_bounds__(256) decay_empty(const float *start, float *end, long long per, const int *bounds, int nseq) {
-    pdl_begin();
-    for (int s = blockIdx.x; s < nseq; s += gridDim.x)
-        if (bounds[s] == bounds[s + 1])
-            for (long long e = threadIdx.x; e < per; e += 256) end[s * per + e] = start ? start[s * per + e] : 0.f;
+    if (a.end)
+        for (int s = blockIdx.x; s < a.nseq; s += gridDim.x)
+            if (a.bounds[s] == a.bounds[s + 1])
+                for (long long e = threadIdx.x; e < a.per; e += 256) a.end[s * a.per + e] = a.start ? a.start[s * a.per + e] : 0.f;
 }
 
 }  // namespace uni

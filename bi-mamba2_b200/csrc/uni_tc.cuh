@@ -109,7 +109,6 @@ struct StatesParams {
     Heads h;
     Plan seg, chunk;
     int reverse, by_seq, tiles;                                  // by_seq: init and fin hold a state a sequence, not a segment
-    View v;                                                      // v or the outputs' gradient
     const float *init;
     float *fin, *decay;                                          // decay: (segments, H) the segment's whole decay, or NULL
     int *status;
@@ -148,7 +147,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     auto place = [&](int i) { return a.reverse ? nc - 1 - i : i; };        // chunk of the segment at step i
     auto length = [&](int i) { return min(kQ, s.len - place(i) * kQ); };
     volatile int *fail = &sh.fail;
-    const bool direct = EXACT && a.tiles;                        // v's rows straight to registers: a tile of S has their buffer
+    uint8_t *raw = a.tiles ? smV + kSlab : smS;                  // EXACT: where v's rows arrive, the third buffer or the second part's
     if (warp == 0) tmem_alloc(&sh.tmem, 64);
     if (tid == 256) {
         mbar_init(&sh.full[0], 1);
@@ -176,11 +175,11 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         };
         auto load_v = [&](int i) {                               // EXACT
             mbar_expect_tx(&sh.full_v, kSlab);
-            tma_load4(smS, &tmV, pb * kP, h, s.t0 + place(i) * kQ, s.batch, &sh.full_v);
+            tma_load4(raw, &tmV, pb * kP, h, s.t0 + place(i) * kQ, s.batch, &sh.full_v);
         };
         if (lane == 0) load(0);
-        if (EXACT && !direct && lane == 0) load_v(0);
-        int loads = 1, loads_v = EXACT && !direct, round = 0;
+        if (EXACT && lane == 0) load_v(0);
+        int loads = 1, loads_v = EXACT, round = 0;
         constexpr uint32_t idesc = instr_desc(1, true, true, kP);
         for (int i = 0; i < nc && ok; ++i) {
             const int st = i & 1;
@@ -200,7 +199,8 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 ok = ws_wait_warp(&sh.ready, round & 1, fail, 3);
                 if (!ok) break;
                 tc_fence_after();
-                if (EXACT && !direct && r == 0 && i + 1 < nc) {  // this chunk's rows are in registers
+                const bool more = EXACT && r == 0 && i + 1 < nc;
+                if (more && !a.tiles) {                          // this chunk's rows are in registers
                     if (lane == 0) load_v(i + 1);
                     ++loads_v;
                 }
@@ -214,6 +214,12 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                     umma_commit(&sh.done);
                 }
                 __syncwarp();
+                if (more && a.tiles) {                           // the second part has been read
+                    ok = ws_wait_warp(&sh.done, round & 1, fail, 11);
+                    if (!ok) break;
+                    if (lane == 0) load_v(i + 1);
+                    ++loads_v;
+                }
             }
         }
         if (!ok && elect_one()) {                                // leave nothing in flight
@@ -284,19 +290,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         if (a.tiles && elect_one()) tma_store_wait();
         __syncwarp();
     } else {
-        // 16 bytes of rows tid / 8 + 32 k of v
-        const bool in_cols = pb * kP + (tid & 7) * 8 < a.h.P;
-        const long long vstep = 32 * a.v.sl;
-        const bf16 *vp = static_cast<const bf16 *>(a.v.ptr) + (long long)s.batch * a.v.sb + (long long)h * a.v.sh + pb * kP + (tid & 7) * 8 +
-                         (long long)(s.t0 + (tid >> 3)) * a.v.sl;
-        uint4 rows[4];
-        auto fetch = [&](int i) {
-            if (i >= nc) return;
-            const bf16 *p = vp + (long long)(place(i) * kQ) * a.v.sl;
-            const int left = in_cols ? length(i) - (tid >> 3) : 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) rows[k] = k * 32 < left ? __ldg(reinterpret_cast<const uint4 *>(p + k * vstep)) : zero8();
-        };
+        uint4 rows[4];                                           // EXACT: 16 bytes of rows tid / 8 + 32 k of v
         const uint32_t swz = (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);   // the thread's piece of a tile, + 4096 k
         auto weigh = [&](uint8_t *v, int len) {                  // bf16 rows times f1 + f2, in their place
 #pragma unroll
@@ -340,7 +334,6 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 rows[k] = make_uint4(e[0], e[1], e[2], e[3]);
             }
         };
-        if (direct) fetch(0);
         const int n = (warp & 3) * 32 + lane, half = warp >> 2, col = pb * kP + half * 32;
         const long long at = (((long long)(a.by_seq ? s.seq : si) * a.h.H + h) * a.h.N + n) * a.h.P + col;
         float S[32];
@@ -368,13 +361,11 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             const int st = i & 1;
             float now;
             if constexpr (EXACT) {
-                ok = ws_wait_warp(&sh.weights, i & 1, fail, 4) && (direct || ws_wait_warp(&sh.full_v, i & 1, fail, 10));
+                ok = ws_wait_warp(&sh.weights, i & 1, fail, 4) && ws_wait_warp(&sh.full_v, i & 1, fail, 10);
                 if (!ok) break;
-                if (!direct) {
-                    const int len = length(i) - (tid >> 3);
+                const int len = length(i) - (tid >> 3);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) rows[k] = k * 32 < len ? *reinterpret_cast<const uint4 *>(smS + swz + k * 4096) : zero8();
-                }
+                for (int k = 0; k < 4; ++k) rows[k] = k * 32 < len ? *reinterpret_cast<const uint4 *>(raw + swz + k * 4096) : zero8();
                 parts();
             }
             now = sh.decay[st];
@@ -414,11 +405,8 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
                 for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, x[j]);
             }
-            if constexpr (!EXACT) {
+            if constexpr (!EXACT)
                 if (i + 1 < nc) ok = prepare(i + 1);
-            } else if (direct) {
-                fetch(i + 1);
-            }
         }
         if (ok && a.fin && n < a.h.N) {
 #pragma unroll
