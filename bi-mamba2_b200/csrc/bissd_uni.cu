@@ -547,7 +547,8 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     p.dg = a->dg ? (a->g_per_head ? g.dg_tokens : a->dg) : nullptr;
     p.dg_dtype = a->g_per_head ? BISSD_F32 : a->g_dtype;
     p.status = status;
-    const auto kernel = t.NT == 64 ? unitc::decay_grads<64> : unitc::decay_grads<128>;
+    const auto kernel = t.NT == 64 ? (p.dg ? unitc::decay_grads<64, true> : unitc::decay_grads<64, false>)
+                                   : (p.dg ? unitc::decay_grads<128, true> : unitc::decay_grads<128, false>);
     const size_t smem = unitc::grads_smem(t.NT);
     const long long grid = (long long)t.chunk.most * a->nkheads * p.parts;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;

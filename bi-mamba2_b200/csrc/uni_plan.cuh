@@ -63,15 +63,15 @@ template <class F> __device__ __forceinline__ int block_scan(int v, int *warps, 
 // caller's array holds.
 __global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int L, PlanOut a, PlanOut b) {
     pdl_begin();
-    __shared__ int warps[32], carry[2];
+    __shared__ int warps[32], carry[2], near_first[1025], near_bounds[1025];   // of up to 1024 sequences: the search below is a chain of reads
     const PlanOut o = blockIdx.x ? b : a;
     const int tid = threadIdx.x;
     auto most = [](int x, int y) { return max(x, y); };
     auto sum = [](int x, int y) { return x + y; };
     auto inside = [&](int i) { return max(0, min(cu[i], L)); };
     if (tid == 0) {
-        o.first[0] = carry[1] = 0;
-        o.bounds[0] = carry[0] = inside(0);
+        o.first[0] = carry[1] = near_first[0] = 0;
+        o.bounds[0] = carry[0] = near_bounds[0] = inside(0);
     }
     __syncthreads();
     for (int s0 = 0; s0 < nseq; s0 += 1024) {
@@ -82,6 +82,10 @@ __global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int 
         if (s < nseq) {
             o.first[s + 1] = upto;
             o.bounds[s + 1] = end;
+            if (s < 1024) {
+                near_first[s + 1] = upto;
+                near_bounds[s + 1] = end;
+            }
         }
         __syncthreads();
         if (tid == 1023) {
@@ -90,6 +94,7 @@ __global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int 
         }
         __syncthreads();
     }
+    const int *first = nseq <= 1024 ? near_first : o.first, *bounds = nseq <= 1024 ? near_bounds : o.bounds;
     for (int i = tid; i < o.most; i += 1024) {
         int lo = 0, hi = nseq;                                   // the sequence that segment i belongs to: first[lo] <= i < first[lo + 1]
         if (i >= carry[1]) {
@@ -98,11 +103,11 @@ __global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int 
         }
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (o.first[mid] <= i) lo = mid;
+            if (first[mid] <= i) lo = mid;
             else hi = mid;
         }
-        const int idx = i - o.first[lo], t0 = o.bounds[lo] + idx * o.seg;
-        o.table[i] = make_int4(t0, min(o.seg, o.bounds[lo + 1] - t0), lo, 2 * idx + (t0 + o.seg >= o.bounds[lo + 1]));
+        const int idx = i - first[lo], t0 = bounds[lo] + idx * o.seg;
+        o.table[i] = make_int4(t0, min(o.seg, bounds[lo + 1] - t0), lo, 2 * idx + (t0 + o.seg >= bounds[lo + 1]));
     }
 }
 

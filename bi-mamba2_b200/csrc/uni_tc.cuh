@@ -684,7 +684,7 @@ struct GradsParams {
     bf16 *dq, *dk, *dv;                                          // contiguous
     float *part;                                                 // parts > 1: (2, parts, tokens, hk, N), dq and dk
     long long tokens;
-    void *dg;                                                    // (tokens, H), or NULL
+    void *dg;                                                    // DG: (tokens, H)
     int dg_dtype;
     int *status;
 };
@@ -709,7 +709,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         : "memory");
 }
 
-template <int NT> __global__ void __launch_bounds__(512, 1)
+template <int NT, bool DG> __global__ void __launch_bounds__(512, 1)
 decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmG) {
     pdl_begin();
@@ -909,18 +909,22 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                         p[j / 2 + 1] = vec::narrow<bf16>(vec::mul2(x1, w1));
                         d[(j - j0) / 2] = vec::narrow<bf16>(y0);
                         d[(j - j0) / 2 + 1] = vec::narrow<bf16>(y1);
-                        const vec::f2 z0 = vec::mul2(x0, y0), z1 = vec::mul2(x1, y1);   // a token's own pair is in its row's and its column's sum
-                        sum = vec::add2(sum, vec::add2(z0, z1));
-                        vec::unpack(z0, x[j], x[j + 1]);
-                        vec::unpack(z1, x[j + 2], x[j + 3]);
+                        if constexpr (DG) {                      // a token's own pair is in its row's and its column's sum
+                            const vec::f2 z0 = vec::mul2(x0, y0), z1 = vec::mul2(x1, y1);
+                            sum = vec::add2(sum, vec::add2(z0, z1));
+                            vec::unpack(z0, x[j], x[j + 1]);
+                            vec::unpack(z1, x[j + 2], x[j + 3]);
+                        }
                     }
                     *reinterpret_cast<uint4 *>(drow + ((((cg & 1) * 4 + j0 / 8) ^ (s & 7)) << 4)) = make_uint4(d[0], d[1], d[2], d[3]);
                 }
-                float lo, hi;
-                vec::unpack(sum, lo, hi);
-                of_row = lo + hi;
-                auto value = [&](auto k) { return x[decltype(k)::value]; };
-                of_column = warp_sums<32>(value, lane);
+                if constexpr (DG) {
+                    float lo, hi;
+                    vec::unpack(sum, lo, hi);
+                    of_row = lo + hi;
+                    auto value = [&](auto k) { return x[decltype(k)::value]; };
+                    of_column = warp_sums<32>(value, lane);
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) p[j] = 0u;
@@ -930,8 +934,10 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 }
             }
             tmem_st16(tl + cg * 16, p);
-            rowsum[cg][s] = of_row + (first ? 0.f : rowsum[cg][s]);
-            colsum[quad][cg * 32 + lane] = of_column + (first ? 0.f : colsum[quad][cg * 32 + lane]);
+            if constexpr (DG) {
+                rowsum[cg][s] = of_row + (first ? 0.f : rowsum[cg][s]);
+                colsum[quad][cg * 32 + lane] = of_column + (first ? 0.f : colsum[quad][cg * 32 + lane]);
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {                        // e^{c_end - c_s} v_s in v_s' place
                 const int q = tid + k * kT;
@@ -967,7 +973,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 for (int kk = 0; kk < NT / 16; ++kk)
                     umma(tmem + cFar, smem_desc(k0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(g_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
 #pragma unroll
-                for (int kk = 0; kk < NT / 16; ++kk)
+                for (int kk = 0; kk < (DG ? NT / 16 : 0); ++kk)
                     umma(tmem + cOut, smem_desc(q0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(s_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {                 // dq from the past, dk from the future
@@ -977,22 +983,25 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 umma_commit(&done_a);
             }
         }
-        if (ok) ok = mbar_wait(&bar_s, i & 1);
-        if (first) through = 0.f;
-        if (ok)
-            for (int q = tid; q < NT * 8; q += kT) {
-                float e[8], f[8];
-                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smS + q * 16), e);
-                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smG + q * 16), f);
+        float whole = 0.f;
+        if constexpr (DG) {
+            if (ok) ok = mbar_wait(&bar_s, i & 1);
+            if (first) through = 0.f;
+            if (ok)
+                for (int q = tid; q < NT * 8; q += kT) {
+                    float e[8], f[8];
+                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(smS + q * 16), e);
+                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(smG + q * 16), f);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) through = fmaf(e[j], f[j], through);
+                    for (int j = 0; j < 8; ++j) through = fmaf(e[j], f[j], through);
+                }
+            whole = tb.whole[0];                         // read here: behind the next barrier its table may be another head's
+            if (last) {
+                float v = through;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                if (lane == 0) cross[warp] = v;
             }
-        const float whole = tb.whole[0];                         // read here: behind the next barrier its table may be another head's
-        if (last) {
-            float v = through;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) cross[warp] = v;
         }
         if (ok) ok = mbar_wait(&done_a, i & 1);
         tc_fence_after();
@@ -1000,23 +1009,27 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             float own[16], far[16], o[16], e[8], f = 0.f, p = 0.f;
             tmem_ld16(tl + cOwn + cg * 16, own);
             tmem_ld16(tl + cFar + cg * 16, far);
-            tmem_ld16(tl + cOut + cg * 16, o);
+            if constexpr (DG) tmem_ld16(tl + cOut + cg * 16, o);
             const float w = tb.ws[s];
 #pragma unroll
             for (int j = 0; j < 16; j += 8) {
                 const int at = s * 128 + (((cg * 2 + j / 8) ^ (s & 7)) << 4);
-                unpack8<bf16>(*reinterpret_cast<const uint4 *>(sV + at), e);
+                if constexpr (DG) {
+                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(sV + at), e);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) f = fmaf(e[k], far[j + k], f);
-                unpack8<bf16>(*reinterpret_cast<const uint4 *>(smE + at), e);
+                    for (int k = 0; k < 8; ++k) f = fmaf(e[k], far[j + k], f);
+                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(smE + at), e);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) p = fmaf(e[k], o[j + k], p);
+                    for (int k = 0; k < 8; ++k) p = fmaf(e[k], o[j + k], p);
+                }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) e[k] = fmaf(w, far[j + k], own[j + k]);
                 *reinterpret_cast<uint4 *>(sV + at) = pack8<bf16>(e);   // dv, where this thread alone has read v
             }
-            future[cg][s] = f + (first ? 0.f : future[cg][s]);
-            past[cg][s] = p + (first ? 0.f : past[cg][s]);
+            if constexpr (DG) {
+                future[cg][s] = f + (first ? 0.f : future[cg][s]);
+                past[cg][s] = p + (first ? 0.f : past[cg][s]);
+            }
         }
         tc_fence_before();
         ok = __syncthreads_and(ok);
@@ -1036,7 +1049,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                         *reinterpret_cast<const uint4 *>(sV + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
             }
         }
-        if (last && warp == kSums && a.dg) {
+        if (DG && last && warp == kSums) {
             float all = lane < 16 ? cross[lane] : 0.f, x[4] = {}, b[4] = {};
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
