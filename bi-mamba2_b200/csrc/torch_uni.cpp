@@ -2,9 +2,11 @@
 // library calls and the autograd nodes.  One call from Python each; whatever is wrong with the arguments is raised from here.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -61,6 +63,20 @@ bool wants_grad(std::initializer_list<const Tensor *> ts) {
     for (const Tensor *t : ts)
         if (t->defined() && t->requires_grad()) return true;
     return false;
+}
+// A leaf whose gradient an eager graph still alive also leads to keeps that graph's stream: PyTorch's engine then waits across streams in
+// the middle of a captured backward pass, which spoils the capture and can end the process.  Refused before anything is recorded.
+void refuse_mixed_capture(const char *who, std::initializer_list<const Tensor *> ts) {
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    for (const Tensor *t : ts) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node) continue;
+        const auto stream = node->stream();
+        if (stream && *stream != c10::cuda::getCurrentCUDAStream(t->device().index()).unwrap())
+            throw std::runtime_error(std::string(who) + ": captured with gradients while an eager graph of the same leaves is alive on another "
+                                     "stream; release that graph first");
+    }
 }
 // As the kernels read it in place: unit inner stride and, for 16-bit tensors, 16-byte aligned rows that do not repeat; else a copy.
 Tensor in_place(const Tensor &t) {
@@ -239,6 +255,7 @@ py::object decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, co
     const Tensor init = value(initial);
     Tensor cu = value(cu_);
     const bool grad = wants_grad({&q, &k, &v, &g, &init});
+    if (grad) refuse_mixed_capture(kAttention, {&q, &k, &v, &g, &init});
     variable_list r;
     {
         py::gil_scoped_release nogil;
@@ -451,6 +468,7 @@ py::object block_norm(const Tensor &x, const Tensor &residual, const OptTensor &
         if (opt[i]->defined()) on_device(kNorm, names[i], *opt[i], dev);
     const c10::cuda::CUDAGuard guard(dev);
     const bool grad = wants_grad({&x, &residual, &gate, &scale, &post, &pre});
+    if (grad) refuse_mixed_capture(kNorm, {&x, &residual, &gate, &scale, &post, &pre});
     variable_list r;
     {
         py::gil_scoped_release nogil;

@@ -7,6 +7,10 @@ Same constructor arguments, parameter names (state_dict keys) and forward semant
 plain library GEMMs (cuBLAS through nn.Linear).  `use_mem_eff_path=True` runs everything after in_proj as one autograd
 node that saves only the projection's output and the scan's output and recomputes the rest in the backward pass
 (ssd/bi/split_conv1d_scan.py).
+
+Beside it stands what a decoder needs: `DecayAttention`, the causal mixer (whole sequences, packed ones, and single tokens from a pool of
+states), `Block`, a residual block around either mixer with the norms before and after it, its gate and its scale in one kernel,
+and `DecayDecoder`, a stack of blocks with prompts and single tokens.
 """
 import math
 
@@ -18,6 +22,8 @@ from ssd.bi.conv_silu import dwconv1d_silu
 from ssd.bi.layernorm_gated import RMSNorm as RMSNormGated
 from ssd.bi.split_conv1d_scan import bimamba_split_conv1d_scan_combined, native_layer
 from ssd.bi.ssd_combined import bimamba_chunk_scan_combined
+from ssd.block_norm import block_norm
+from ssd.uni.decay_attention import decay_attention, decay_attention_step
 
 
 class Mamba2:
@@ -116,3 +122,110 @@ class BiMamba2(nn.Module):
         y = y.reshape(b, l, self.d_inner)
         y = self.norm(y, z)
         return self.out_proj(y)
+
+
+class DecayAttention(nn.Module):
+    """Causal mixer: in_proj -> (q | k | v | dt) -> log decays -exp(A_log) softplus(dt + dt_bias) -> decay_attention -> out_proj.
+
+    d_state and headdim are the sizes of a head's key and value, ngroups the heads of q and k, as BiMamba2 names them.
+    """
+
+    def __init__(self, d_model, d_state=64, headdim=64, ngroups=1, expand=1, dt_min=0.001, dt_max=0.1, dt_init_floor=1e-4, bias=False,
+                 device=None, dtype=None):
+        factory_kwargs = {"device": device, "dtype": dtype}
+        super().__init__()
+        self.d_model, self.d_state, self.headdim, self.ngroups = d_model, d_state, headdim, ngroups
+        self.d_inner = expand * d_model
+        assert self.d_inner % headdim == 0
+        self.nheads = self.d_inner // headdim
+        assert self.nheads % ngroups == 0
+        # order of the projection's output channels: [q, k, v, dt]
+        self.in_proj = nn.Linear(d_model, 2 * ngroups * d_state + self.d_inner + self.nheads, bias=bias, **factory_kwargs)
+        dt = torch.exp(torch.rand(self.nheads, device=device) * (math.log(dt_max) - math.log(dt_min)) + math.log(dt_min))
+        dt = torch.clamp(dt, min=dt_init_floor)
+        self.dt_bias = nn.Parameter(dt + torch.log(-torch.expm1(-dt)))
+        self.dt_bias._no_weight_decay = True
+        self.A_log = nn.Parameter(torch.zeros(self.nheads, device=device))
+        self.A_log._no_weight_decay = True
+        self.out_proj = nn.Linear(self.d_inner, d_model, bias=bias, **factory_kwargs)
+
+    def _project(self, u):
+        qk = self.ngroups * self.d_state
+        q, k, v, dt = torch.split(self.in_proj(u), [qk, qk, self.d_inner, self.nheads], dim=-1)
+        g = -torch.exp(self.A_log.float()) * F.softplus(dt.float() + self.dt_bias.float())
+        heads = lambda t, n: t.unflatten(-1, (n, -1))
+        return heads(q, self.ngroups), heads(k, self.ngroups), heads(v, self.nheads), g.to(v.dtype)
+
+    def init_states(self, slots):
+        """Empty states for `slots` requests."""
+        return torch.zeros(slots, self.nheads, self.d_state, self.headdim, dtype=torch.float32, device=self.A_log.device)
+
+    def forward(self, u, initial_state=None, return_final_state=False, cu_seqlens=None):
+        """u: (batch, seqlen, d_model) -> same shape, and with return_final_state the states after the sequences."""
+        out = decay_attention(*self._project(u), initial_state=initial_state, return_final_state=return_final_state, cu_seqlens=cu_seqlens)
+        y, state = out if return_final_state else (out, None)
+        y = self.out_proj(y.flatten(-2))
+        return (y, state) if return_final_state else y
+
+    def step(self, u, states, slots=None):
+        """One token of every request, u: (batch, d_model); `states` is updated in place (see decay_attention_step)."""
+        return self.out_proj(decay_attention_step(states, *self._project(u), slots=slots).flatten(-2))
+
+
+class Block(nn.Module):
+    """A residual block: out = residual + scale * act(gate) * rms(mixer(u)) * post_weight, and rms(out) * next_weight, the next block's u.
+
+    mixer: any module from (batch, seqlen, d_model) to the same shape, BiMamba2 and DecayAttention among them.  gate_activation: None
+    (no gate), "sigmoid" or "silu" of a projection of u.
+    """
+
+    def __init__(self, d_model, mixer, gate_activation="sigmoid", scale_init=1.0, eps=1e-5, device=None, dtype=None):
+        factory_kwargs = {"device": device, "dtype": dtype}
+        super().__init__()
+        self.mixer, self.gate_activation, self.eps = mixer, gate_activation, eps
+        self.gate_proj = nn.Linear(d_model, d_model, bias=False, **factory_kwargs) if gate_activation is not None else None
+        self.post_weight = nn.Parameter(torch.ones(d_model, device=device))
+        self.scale = nn.Parameter(torch.full((d_model,), float(scale_init), device=device))
+        self.next_weight = nn.Parameter(torch.ones(d_model, device=device))
+
+    def join(self, y, u, residual):
+        """What the mixer gave for u, joined to the residual stream: (stream, next u)."""
+        gate = None if self.gate_proj is None else self.gate_proj(u)
+        return block_norm(y, residual, gate=gate, scale=self.scale, post_weight=self.post_weight, pre_weight=self.next_weight,
+                          gate_activation=self.gate_activation, eps=self.eps)
+
+    def forward(self, u, residual, **kwargs):
+        return self.join(self.mixer(u, **kwargs), u, residual)
+
+
+class DecayDecoder(nn.Module):
+    """Blocks of DecayAttention over embedded tokens: training, prompts (also packed) and single tokens from pools of states.
+
+    d_model: a multiple of 256, at most 4096 (the first norm's range).  The residual stream is float32 whatever the blocks compute in.
+    """
+
+    def __init__(self, d_model, n_layers, gate_activation="sigmoid", eps=1e-5, device=None, dtype=None, **mixer_kwargs):
+        super().__init__()
+        self.norm = RMSNormGated(d_model, eps=eps, device=device, dtype=torch.float32)
+        self.blocks = nn.ModuleList(
+            Block(d_model, DecayAttention(d_model, device=device, dtype=dtype, **mixer_kwargs), gate_activation, eps=eps, device=device,
+                  dtype=dtype) for _ in range(n_layers))
+
+    def init_states(self, slots):
+        return [block.mixer.init_states(slots) for block in self.blocks]
+
+    def forward(self, x, initial_states=None, return_final_states=False, cu_seqlens=None):
+        """x: (batch, seqlen, d_model) -> the normed stream behind the last block, and with return_final_states a list of states."""
+        u, residual, finals = self.norm(x), x.float(), []
+        for i, block in enumerate(self.blocks):
+            y, state = block.mixer(u, None if initial_states is None else initial_states[i], True, cu_seqlens)
+            u, residual = reversed(block.join(y, u, residual))
+            finals.append(state)
+        return (u, finals) if return_final_states else u
+
+    def step(self, x, states, slots=None):
+        """One token of every request, x: (batch, d_model); the states are updated in place.  Under torch.no_grad()."""
+        u, residual = self.norm(x), x.float()
+        for block, state in zip(self.blocks, states):
+            u, residual = reversed(block.join(block.mixer.step(u, state, slots), u, residual))
+        return u
