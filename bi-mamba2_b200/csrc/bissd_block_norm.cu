@@ -59,7 +59,10 @@ static int block_norm_blocks(const bnorm::Params &p, int resident) {
     return (int)std::min<long long>(want, (p.rows / entries + per - 1) / per);
 }
 constexpr int kFwd = 3, kBwd = 2;                                // blocks of 256 threads an SM: what the registers allow
-static int block_norm_resident(const bnorm::Params &p, int of_256) { return std::max(1, 256 * of_256 / block_norm_threads(p)); }
+static int block_norm_resident(const bnorm::Params &p, int of_256) {
+    const int threads = block_norm_threads(p);
+    return threads > 256 && threads <= 512 && of_256 == kFwd ? 2 : std::max(1, 256 * of_256 / threads);
+}
 
 // Bytes of the rows that a block copies ahead.
 template <class T> static size_t block_norm_ring(int pieces, int threads) {
@@ -75,10 +78,9 @@ template <class T, class R> static int block_norm_forward_impl(const bissd_block
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     const int pieces = (int)(sizeof(T) * (a->gate && p.gate_rows == 0 ? 2 : 1) + sizeof(R)) / 2;
     const size_t smem = vec ? block_norm_ring<T>(pieces, threads) : 0;
-    const auto kernel = !vec            ? bnorm::block_norm_fwd<T, R, false, 1024, 1>
-                        : threads > 512 ? bnorm::block_norm_fwd<T, R, true, 1024, 1>
-                        : threads > 256 ? bnorm::block_norm_fwd<T, R, true, 512, 1>
-                                        : bnorm::block_norm_fwd<T, R, true, 256, kFwd>;
+    const auto kernel = threads > 512   ? (vec ? bnorm::block_norm_fwd<T, R, true, 1024, 1> : bnorm::block_norm_fwd<T, R, false, 1024, 1>)
+                        : threads > 256 ? (vec ? bnorm::block_norm_fwd<T, R, true, 512, 2> : bnorm::block_norm_fwd<T, R, false, 512, 2>)
+                                        : (vec ? bnorm::block_norm_fwd<T, R, true, 256, kFwd> : bnorm::block_norm_fwd<T, R, false, 256, kFwd>);
     BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
     BISSD_LAUNCH("block_norm_fwd", launch_pdl(kernel, (int)grid, threads, smem, s, p));
     return BISSD_OK;
@@ -94,10 +96,9 @@ template <class T, class R> static int block_norm_backward_impl(const bissd_bloc
     const int pieces = (int)(sizeof(T) * (1 + (a->gate && p.gate_rows == 0) + (a->dnormed != nullptr)) + sizeof(R) * (1 + (a->dr != nullptr))) / 2;
     const size_t rows = (size_t)(per - 1) * p.threads_row * bnorm::kCh * sizeof(float);
     const size_t smem = std::max(rows, vec ? block_norm_ring<T>(pieces, threads) : 0);
-    const auto kernel = !vec            ? bnorm::block_norm_bwd<T, R, false, 1024, 1>
-                        : threads > 512 ? bnorm::block_norm_bwd<T, R, true, 1024, 1>
-                        : threads > 256 ? bnorm::block_norm_bwd<T, R, true, 512, 1>
-                                        : bnorm::block_norm_bwd<T, R, true, 256, kBwd>;
+    const auto kernel = threads > 512   ? (vec ? bnorm::block_norm_bwd<T, R, true, 1024, 1> : bnorm::block_norm_bwd<T, R, false, 1024, 1>)
+                        : threads > 256 ? (vec ? bnorm::block_norm_bwd<T, R, true, 512, 1> : bnorm::block_norm_bwd<T, R, false, 512, 1>)
+                                        : (vec ? bnorm::block_norm_bwd<T, R, true, 256, kBwd> : bnorm::block_norm_bwd<T, R, false, 256, kBwd>);
     BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
     BISSD_LAUNCH("block_norm_bwd", launch_pdl(kernel, (int)(entries * p.blocks), threads, smem, s, p));
     bnorm::SumParams q{};

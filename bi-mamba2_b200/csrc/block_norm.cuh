@@ -140,7 +140,13 @@ template <int WARPS> __device__ __forceinline__ float row_sum(float v, float (&b
     if ((threadIdx.x & 31) == 0) buf[warp] = v;
     __syncthreads();
     float s = 0.f;
-    for (int i = 0; i < per; ++i) s += buf[first + i];
+    if (per <= 8) {
+        for (int i = 0; i < per; ++i) s += buf[first + i];
+        return s;
+    }
+    const int lane = threadIdx.x & 31;                           // a lane for each warp of the row
+    if (lane < per) s = buf[first + lane];
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
 }
 
