@@ -12,6 +12,8 @@ static bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 1
 
 static int block_norm_sizes(const bissd_block_norm_args *a) {
     if (!a) return BISSD_ERR_NULL;
+    for (const int64_t n : {a->rows, a->stride_x, a->stride_residual, a->stride_gate, a->stride_dr, a->stride_dnormed})
+        if (n < 0 || n > 0x3fffffff) return BISSD_ERR_SHAPE;     // rows and strides are 32-bit in the kernels, offsets 64
     if (a->rows <= 0 || a->width <= 0 || a->width > bnorm::kMaxWidth || a->gate_rows < 0 || (a->gate_rows > 0 && a->rows % a->gate_rows))
         return BISSD_ERR_SHAPE;
     if (!dtype_ok(a->dtype) || (a->r_dtype != a->dtype && a->r_dtype != BISSD_F32) || (a->w_dtype != a->dtype && a->w_dtype != BISSD_F32))
@@ -40,13 +42,13 @@ static bool block_norm_vec(const bissd_block_norm_args *a) {
 static long long block_norm_entries(const bnorm::Params &p) { return p.gate && p.gate_rows > 0 ? p.rows / p.gate_rows : 1; }
 static bnorm::Params block_norm_params(const bissd_block_norm_args *a) {
     bnorm::Params p{};
-    p.rows = a->rows;
-    p.gate_rows = a->gate_rows == 1 ? 0 : a->gate_rows;          // a gate row for each row
+    p.rows = (int)a->rows;
+    p.gate_rows = a->gate_rows == 1 ? 0 : (int)a->gate_rows;          // a gate row for each row
     p.D = a->width;
     p.threads_row = ceil_div(ceil_div(a->width, bnorm::kCh), 32) * 32;
     p.w_dtype = a->w_dtype; p.act = a->gate_act;
     p.scale = a->scale; p.eps = a->eps;
-    p.sx = a->stride_x; p.sres = a->stride_residual; p.sgate = a->stride_gate; p.sdr = a->stride_dr; p.sdu = a->stride_dnormed;
+    p.sx = (int)a->stride_x; p.sres = (int)a->stride_residual; p.sgate = (int)a->stride_gate; p.sdr = (int)a->stride_dr; p.sdu = (int)a->stride_dnormed;
     p.x = a->x; p.res = a->residual; p.gate = a->gate; p.scale_v = a->scale_vector; p.w2 = a->post_weight; p.w1 = a->pre_weight;
     p.r = a->r; p.u = a->pre_weight ? a->normed : nullptr; p.rstd = a->rstd;
     p.dr = a->dr; p.du = a->dnormed; p.dx = a->dx; p.dres = a->dresidual; p.dgate = a->gate ? a->dgate : nullptr;

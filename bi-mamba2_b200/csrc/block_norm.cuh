@@ -31,10 +31,10 @@ constexpr int kCh = 8, kPairs = kCh / 2;                         // channels a t
 constexpr int kMaxWidth = 8192;
 
 struct Params {
-    long long rows, gate_rows;                                   // gate_rows: rows of x to a row of the gate, 0 where each has its own
+    int rows, gate_rows;                                         // gate_rows: rows of x to a row of the gate, 0 where each has its own
     int D, threads_row, w_dtype, act, blocks;                    // blocks: of an entry
     float scale, eps;
-    long long sx, sres, sgate, sdr, sdu;                         // row strides
+    int sx, sres, sgate, sdr, sdu;                               // row strides
     const void *x, *res, *gate, *scale_v, *w2, *w1;
     void *r, *u;
     float *rstd;                                                 // [2][rows]: of x, of r
@@ -46,29 +46,27 @@ struct Params {
 // Channel e of thread t of a row.
 template <bool VEC> __device__ __forceinline__ int channel(int t, int tr, int e) { return VEC ? t * kCh + e : t + e * tr; }
 
-// A thread's eight channels of one tensor: where the next row's lie, and how they get into registers.
+// A thread's eight channels of one tensor, and how a row's get into registers.
 template <class T, bool VEC> struct Column {
     static constexpr int kPieces = VEC ? kCh * (int)sizeof(T) / 16 : 0;   // 16-byte pieces a row
-    const T *at;                                                 // the next row's first channel of the thread (VEC) or of the row
-    long long step;
     int slot;                                                    // first piece's place in the ring's stage, in bytes
-    __device__ __forceinline__ void start(const void *p, long long row, long long stride, long long rows, int t, int threads, int *bytes) {
-        at = static_cast<const T *>(p) + row * stride + (VEC ? t * kCh : 0);
-        step = rows * stride;
+    __device__ __forceinline__ void start(int threads, int *bytes) {
         slot = *bytes;
         *bytes += kPieces * threads * 16;
     }
-    // the next row on its way (zeros where there is none, or no such channels), and on to the one after it
-    __device__ __forceinline__ void copy(uint32_t stage, int threads, bool in) {
+    // A row on its way: zeros where there is none, or no such channels.  Addresses are made anew from the parameters, a multiply-add each:
+    // kept and advanced they cost registers that the backward kernel does not have (269 us so, 285 kept, 65536 rows of 1024).
+    __device__ __forceinline__ void copy(const void *p, int row, int stride, int t, uint32_t stage, int threads, bool in) const {
         if constexpr (VEC) {
+            const T *at = static_cast<const T *>(p) + ((long long)row * stride + t * kCh);
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + slot + i * threads * 16),
                              "l"(reinterpret_cast<const uint4 *>(at) + i), "r"(in ? 16 : 0) : "memory");
-            at += step;
         }
     }
-    __device__ __forceinline__ void get(const uint8_t *stage, int threads, int t, int tr, int D, bool valid, f2 (&v)[kPairs]) {
+    __device__ __forceinline__ void get(const void *p, int at_row, int stride, const uint8_t *stage, int threads, int t, int tr, int D,
+                                        bool valid, f2 (&v)[kPairs]) const {
         vec::Row<T, kPairs> row;
         if constexpr (VEC) {
 #pragma unroll
@@ -84,12 +82,12 @@ template <class T, bool VEC> struct Column {
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) v[i] = vec::widen<T>(row.v[i]);
         } else {
+            const T *at = static_cast<const T *>(p) + (long long)at_row * stride;
             float e[kCh];
 #pragma unroll
             for (int i = 0; i < kCh; ++i) e[i] = valid && t + i * tr < D ? to_f<T>(at[t + i * tr]) : 0.f;
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) v[i] = pack(e[2 * i], e[2 * i + 1]);
-            at += step;
         }
     }
 };
@@ -179,14 +177,13 @@ template <class T, int THREADS> struct Ahead {
 // What both kernels walk: rows first + i of an entry (the rows that share a gate row, or all), i = blk per + grp, + step, ...  A row
 // behind the last is one of zeros, of which nothing is kept.
 struct Walk {
-    int tr, per, grp, t, D, blk;
-    long long n, first, step;
+    int tr, per, grp, t, D, blk, n, first, step;
     __device__ __forceinline__ Walk(const Params &a) {
         tr = a.threads_row; per = blockDim.x / tr; grp = threadIdx.x / tr; t = threadIdx.x % tr; D = a.D;
         blk = blockIdx.x % a.blocks;
         n = a.gate && a.gate_rows > 0 ? a.gate_rows : a.rows;
         first = blockIdx.x / a.blocks * n;
-        step = (long long)a.blocks * per;
+        step = a.blocks * per;
     }
 };
 
@@ -210,24 +207,24 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     constexpr int kAhead = Ahead<T, THREADS>::rows;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
     int bytes = 0, turn = 0, at = 0;                             // of a stage of the ring; the stage in turn, in bytes
-    long long i = (long long)k.blk * k.per + k.grp, ahead = i;
-    const long long row0 = k.first + i;
+    int i = k.blk * k.per + k.grp, ahead = i;
     Column<T, VEC> cx, cg;
     Column<R, VEC> cr;
-    cx.start(a.x, row0, a.sx, k.step, t, threads, &bytes);
-    cr.start(a.res, row0, a.sres, k.step, t, threads, &bytes);
-    if (full) cg.start(a.gate, row0, a.sgate, k.step, t, threads, &bytes);
+    cx.start(threads, &bytes);
+    cr.start(threads, &bytes);
+    if (full) cg.start(threads, &bytes);
     auto copy = [&](int stage) {
         const bool some = in && ahead < k.n;
-        cx.copy(ring + stage, threads, some);
-        cr.copy(ring + stage, threads, some);
-        if (full) cg.copy(ring + stage, threads, some);
+        const int to = k.first + ahead;
+        cx.copy(a.x, to, a.sx, t, ring + stage, threads, some);
+        cr.copy(a.res, to, a.sres, t, ring + stage, threads, some);
+        if (full) cg.copy(a.gate, to, a.sgate, t, ring + stage, threads, some);
         asm volatile("cp.async.commit_group;" ::: "memory");
         ahead += k.step;
     };
     if (a.gate && !full) {
         f2 slope[kPairs];
-        const T *p = static_cast<const T *>(a.gate) + blockIdx.x / a.blocks * a.sgate;
+        const T *p = static_cast<const T *>(a.gate) + (long long)(blockIdx.x / a.blocks) * a.sgate;
         float e[kCh];
 #pragma unroll
         for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(p[channel<VEC>(t, tr, j)]) : 0.f;
@@ -241,17 +238,17 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     if (VEC)
         for (int s = 0; s < kAhead; ++s) copy(s * bytes);
     const float inv = 1.f / D;
-    for (long long base = (long long)k.blk * k.per; base < k.n; base += k.step, i += k.step) {
+    for (int base = k.blk * k.per; base < k.n; base += k.step, i += k.step) {
         const bool valid = i < k.n;
-        const long long row = k.first + i;
+        const int row = k.first + i;
         f2 x[kPairs], r[kPairs];
         const uint8_t *stage = dyn + at + threadIdx.x * 16;
         if (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");   // the oldest row has landed
-        cx.get(stage, threads, t, tr, D, valid, x);
-        cr.get(stage, threads, t, tr, D, valid, r);
+        cx.get(a.x, row, a.sx, stage, threads, t, tr, D, valid, x);
+        cr.get(a.res, row, a.sres, stage, threads, t, tr, D, valid, r);
         if (full) {
             f2 g[kPairs], slope[kPairs];
-            cg.get(stage, threads, t, tr, D, valid, g);
+            cg.get(a.gate, row, a.sgate, stage, threads, t, tr, D, valid, g);
             activation(a.act, g, slope);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) mw[j] = mul2(g[j], scw[j]);
@@ -309,7 +306,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
         }
     }
     if (a.gate && !full) {
-        const T *p = static_cast<const T *>(a.gate) + blockIdx.x / a.blocks * a.sgate;
+        const T *p = static_cast<const T *>(a.gate) + (long long)(blockIdx.x / a.blocks) * a.sgate;
         float e[kCh];
 #pragma unroll
         for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(p[channel<VEC>(t, tr, j)]) : 0.f;
@@ -320,40 +317,40 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
     constexpr int kAhead = Ahead<T, THREADS>::rows;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
     int bytes = 0, turn = 0, at = 0;
-    long long i = (long long)k.blk * k.per + k.grp, ahead = i;
-    const long long row0 = k.first + i;
+    int i = k.blk * k.per + k.grp, ahead = i;
     Column<T, VEC> cx, cg, cu;
     Column<R, VEC> cr, cd;
-    cx.start(a.x, row0, a.sx, k.step, t, threads, &bytes);
-    cr.start(a.res, row0, a.sres, k.step, t, threads, &bytes);
-    if (full) cg.start(a.gate, row0, a.sgate, k.step, t, threads, &bytes);
-    if (a.du) cu.start(a.du, row0, a.sdu, k.step, t, threads, &bytes);
-    if (a.dr) cd.start(a.dr, row0, a.sdr, k.step, t, threads, &bytes);
+    cx.start(threads, &bytes);
+    cr.start(threads, &bytes);
+    if (full) cg.start(threads, &bytes);
+    if (a.du) cu.start(threads, &bytes);
+    if (a.dr) cd.start(threads, &bytes);
     auto copy = [&](int stage) {
         const bool some = in && ahead < k.n;
-        cx.copy(ring + stage, threads, some);
-        cr.copy(ring + stage, threads, some);
-        if (full) cg.copy(ring + stage, threads, some);
-        if (a.du) cu.copy(ring + stage, threads, some);
-        if (a.dr) cd.copy(ring + stage, threads, some);
+        const int to = k.first + ahead;
+        cx.copy(a.x, to, a.sx, t, ring + stage, threads, some);
+        cr.copy(a.res, to, a.sres, t, ring + stage, threads, some);
+        if (full) cg.copy(a.gate, to, a.sgate, t, ring + stage, threads, some);
+        if (a.du) cu.copy(a.du, to, a.sdu, t, ring + stage, threads, some);
+        if (a.dr) cd.copy(a.dr, to, a.sdr, t, ring + stage, threads, some);
         asm volatile("cp.async.commit_group;" ::: "memory");
         ahead += k.step;
     };
     if (VEC)
         for (int s = 0; s < kAhead; ++s) copy(s * bytes);
     const float inv = 1.f / D;
-    for (long long base = (long long)k.blk * k.per; base < k.n; base += k.step, i += k.step) {
+    for (int base = k.blk * k.per; base < k.n; base += k.step, i += k.step) {
         const bool valid = i < k.n;
-        const long long row = k.first + i;
+        const int row = k.first + i;
         const float rx = !a.w2 ? 1.f : valid ? a.rstd[row] : 0.f, rr = a.du && valid ? a.rstd[a.rows + row] : 0.f;
         const uint8_t *stage = dyn + at + threadIdx.x * 16;
         f2 xh[kPairs], r[kPairs], dr[kPairs], du[kPairs];
         if (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");   // the oldest row has landed
-        cx.get(stage, threads, t, tr, D, valid, xh);
-        cr.get(stage, threads, t, tr, D, valid, r);
-        if (full) cg.get(stage, threads, t, tr, D, valid, act);
-        if (a.du) cu.get(stage, threads, t, tr, D, valid, du);
-        if (a.dr) cd.get(stage, threads, t, tr, D, valid, dr);
+        cx.get(a.x, row, a.sx, stage, threads, t, tr, D, valid, xh);
+        cr.get(a.res, row, a.sres, stage, threads, t, tr, D, valid, r);
+        if (full) cg.get(a.gate, row, a.sgate, stage, threads, t, tr, D, valid, act);
+        if (a.du) cu.get(a.du, row, a.sdu, stage, threads, t, tr, D, valid, du);
+        if (a.dr) cd.get(a.dr, row, a.sdr, stage, threads, t, tr, D, valid, dr);
         if (VEC) {
             copy(at);
             at = at + bytes == kAhead * bytes ? 0 : at + bytes;

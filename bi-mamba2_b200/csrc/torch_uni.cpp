@@ -343,8 +343,9 @@ Rows rows_of(const Tensor &t, int64_t width) {
     } else {
         r.t = t.reshape({-1, width});
         const bool repeats = r.n > 1 && r.t.stride(0) < width;
-        if ((width > 1 && r.t.stride(1) != 1) || repeats) r.t = r.t.contiguous();
-        r.stride = r.t.stride(0);
+        const bool far = r.t.stride(0) > 0x3fffffff;             // the kernels' strides have 32 bits
+        if ((width > 1 && r.t.stride(1) != 1) || repeats || (far && r.n > 1)) r.t = r.t.contiguous();
+        r.stride = r.n > 1 ? r.t.stride(0) : width;
     }
     r.p = ptr(r.t);
     return r;

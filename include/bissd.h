@@ -331,9 +331,10 @@ int bissd_decay_step(const bissd_decay_step_args *args, void *stream);
  *     normed = rms(r) pre_weight                                      rms(t) = t / sqrt(mean(t^2) + eps)
  * x: the block's output, r: the residual stream after the block, normed: the next block's input.  `rows` rows of `width`
  * contiguous channels, 1 ... 8192.  gate: NULL, one row for each row of x, or (gate_rows > 0) one for every gate_rows
- * rows of x, gate_rows dividing rows.  The inputs' rows lie stride_* elements apart, the outputs are contiguous.  scale: the number, or (width) values where scale_vector is not NULL.  Weights
- * and scale_vector are w_dtype: fp32 or dtype.  residual, r and their gradients are r_dtype: dtype or fp32, and rms(r) is
- * taken of r before it is rounded.  The backward pass reads what the forward pass wrote to rstd (2 * rows fp32). */
+ * rows of x, gate_rows dividing rows.  The inputs' rows lie stride_* elements apart, the outputs are contiguous; rows and
+ * strides are at most 2^30 - 1.  scale: the number, or (width) values where scale_vector is not NULL.  Weights and
+ * scale_vector are w_dtype: fp32 or dtype.  residual, r and their gradients are r_dtype: dtype or fp32, and rms(r) is taken
+ * of r before it is rounded.  The backward pass reads what the forward pass wrote to rstd (2 * rows fp32). */
 enum { BISSD_GATE_NONE = 0, BISSD_GATE_SIGMOID = 1, BISSD_GATE_SILU = 2 };
 typedef struct bissd_block_norm_args {
     int64_t rows, gate_rows;
