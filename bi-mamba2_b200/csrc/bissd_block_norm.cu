@@ -28,8 +28,11 @@ static int block_norm_check(const bissd_block_norm_args *a, bool backward) {
     if (backward && a->dnormed && !a->pre_weight) return BISSD_ERR_NULL;
     return block_norm_sizes(a);
 }
-// Rows side by side in a block: up to 256 threads.
-static int block_norm_threads(const bnorm::Params &p) { return p.threads_row * std::max(1, 256 / p.threads_row); }
+// Rows side by side in a block: up to 256 threads.  A row of more than 512 is two blocks' in the backward pass.
+static int block_norm_pair(const bnorm::Params &p, bool backward) { return backward && p.threads_row > 512 ? 2 : 1; }
+static int block_norm_threads(const bnorm::Params &p, bool backward) {
+    return p.threads_row * std::max(1, 256 / p.threads_row) / block_norm_pair(p, backward);
+}
 // 16-byte pieces: every row starts at a multiple of 16 bytes
 static bool block_norm_vec(const bissd_block_norm_args *a) {
     bool ok = a->width % 8 == 0;
@@ -45,7 +48,8 @@ static bnorm::Params block_norm_params(const bissd_block_norm_args *a) {
     p.rows = (int)a->rows;
     p.gate_rows = a->gate_rows == 1 ? 0 : (int)a->gate_rows;          // a gate row for each row
     p.D = a->width;
-    p.threads_row = ceil_div(ceil_div(a->width, bnorm::kCh), 32) * 32;
+    const int threads = ceil_div(a->width, bnorm::kCh), whole = threads > 512 ? 64 : 32;   // of a row: whole warps, also in two blocks
+    p.threads_row = ceil_div(threads, whole) * whole;
     p.w_dtype = a->w_dtype; p.act = a->gate_act;
     p.scale = a->scale; p.eps = a->eps;
     p.sx = (int)a->stride_x; p.sres = (int)a->stride_residual; p.sgate = (int)a->stride_gate; p.sdr = (int)a->stride_dr; p.sdu = (int)a->stride_dnormed;
@@ -54,55 +58,63 @@ static bnorm::Params block_norm_params(const bissd_block_norm_args *a) {
     p.dr = a->dr; p.du = a->dnormed; p.dx = a->dx; p.dres = a->dresidual; p.dgate = a->gate ? a->dgate : nullptr;
     return p;
 }
-// Blocks to an entry: `resident` of them an SM, shared by the entries, and no more than there are rows.
-static int block_norm_blocks(const bnorm::Params &p, int resident) {
-    const long long entries = block_norm_entries(p), per = block_norm_threads(p) / p.threads_row;
-    const long long want = std::max<long long>(1, 148LL * resident / entries);
-    return (int)std::min<long long>(want, (p.rows / entries + per - 1) / per);
-}
 constexpr int kFwd = 3, kBwd = 2;                                // blocks of 256 threads an SM: what the registers allow
-static int block_norm_resident(const bnorm::Params &p, int of_256) {
-    const int threads = block_norm_threads(p);
-    return threads > 256 && threads <= 512 && of_256 == kFwd ? 2 : std::max(1, 256 * of_256 / threads);
+constexpr int kFwdWide = 2, kBwdWide = 1;                        // of up to 512 (and one of 1024)
+// Blocks (or pairs) to an entry: those that are resident, shared by the entries, and no more than there are rows.
+static int block_norm_blocks(const bnorm::Params &p, bool backward) {
+    const int threads = block_norm_threads(p, backward);
+    const int resident = threads <= 256 ? (backward ? kBwd : kFwd) : backward ? kBwdWide : threads <= 512 ? kFwdWide : 1;
+    const long long entries = block_norm_entries(p), per = std::max(1, threads / p.threads_row);
+    const long long want = std::max<long long>(1, 148LL * resident / block_norm_pair(p, backward) / entries);
+    return (int)std::min<long long>(want, (p.rows / entries + per - 1) / per);
 }
 
 // Bytes of the rows that a block copies ahead.
-template <class T> static size_t block_norm_ring(int pieces, int threads) {
-    const int rows = threads > 512 ? bnorm::Ahead<T, 1024>::rows : threads > 256 ? bnorm::Ahead<T, 512>::rows : bnorm::Ahead<T, 256>::rows;
+template <class T> static size_t block_norm_ring(int pieces, int threads, bool backward) {
+    const int rows = threads <= 256   ? bnorm::Ahead<T, 256, 1>::rows
+                     : backward       ? bnorm::Ahead<T, 512, kBwdWide>::rows
+                     : threads <= 512 ? bnorm::Ahead<T, 512, kFwdWide>::rows
+                                      : bnorm::Ahead<T, 1024, 1>::rows;
     return (size_t)rows * pieces * 16 * threads;
+}
+typedef void (*BlockNormKernel)(bnorm::Params);
+template <class T, class R, bool VEC> static BlockNormKernel block_norm_kernel(int threads, int pair, bool backward) {
+    if (backward)
+        return pair > 1        ? bnorm::block_norm_bwd<T, R, VEC, true, 512, kBwdWide>
+               : threads > 256 ? bnorm::block_norm_bwd<T, R, VEC, false, 512, kBwdWide>
+                               : bnorm::block_norm_bwd<T, R, VEC, false, 256, kBwd>;
+    return threads > 512   ? bnorm::block_norm_fwd<T, R, VEC, false, 1024, 1>
+           : threads > 256 ? bnorm::block_norm_fwd<T, R, VEC, false, 512, kFwdWide>
+                           : bnorm::block_norm_fwd<T, R, VEC, false, 256, kFwd>;
 }
 template <class T, class R> static int block_norm_forward_impl(const bissd_block_norm_args *a, cudaStream_t s) {
     bnorm::Params p = block_norm_params(a);
-    const int threads = block_norm_threads(p);
+    const int threads = block_norm_threads(p, false);
     const bool vec = block_norm_vec(a);
-    p.blocks = block_norm_blocks(p, block_norm_resident(p, kFwd));
+    p.blocks = block_norm_blocks(p, false);
     const long long grid = block_norm_entries(p) * p.blocks;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     const int pieces = (int)(sizeof(T) * (a->gate && p.gate_rows == 0 ? 2 : 1) + sizeof(R)) / 2;
-    const size_t smem = vec ? block_norm_ring<T>(pieces, threads) : 0;
-    const auto kernel = threads > 512   ? (vec ? bnorm::block_norm_fwd<T, R, true, 1024, 1> : bnorm::block_norm_fwd<T, R, false, 1024, 1>)
-                        : threads > 256 ? (vec ? bnorm::block_norm_fwd<T, R, true, 512, 2> : bnorm::block_norm_fwd<T, R, false, 512, 2>)
-                                        : (vec ? bnorm::block_norm_fwd<T, R, true, 256, kFwd> : bnorm::block_norm_fwd<T, R, false, 256, kFwd>);
+    const size_t smem = vec ? block_norm_ring<T>(pieces, threads, false) : 0;
+    const auto kernel = vec ? block_norm_kernel<T, R, true>(threads, 1, false) : block_norm_kernel<T, R, false>(threads, 1, false);
     BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
     BISSD_LAUNCH("block_norm_fwd", launch_pdl(kernel, (int)grid, threads, smem, s, p));
     return BISSD_OK;
 }
 template <class T, class R> static int block_norm_backward_impl(const bissd_block_norm_args *a, float *part, cudaStream_t s) {
     bnorm::Params p = block_norm_params(a);
-    const int threads = block_norm_threads(p), per = threads / p.threads_row;
+    const int threads = block_norm_threads(p, true), pair = block_norm_pair(p, true), per = std::max(1, threads / p.threads_row);
     const bool vec = block_norm_vec(a);
     const long long entries = block_norm_entries(p);
-    p.blocks = block_norm_blocks(p, block_norm_resident(p, kBwd));
-    if (entries * p.blocks > 0x7fffffffLL || (entries + 3) * ceil_div(p.D, 32) > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    p.blocks = block_norm_blocks(p, true);
+    if (entries * p.blocks > 0x3fffffffLL || (entries + 3) * ceil_div(p.D, 32) > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     p.part = part;
     const int pieces = (int)(sizeof(T) * (1 + (a->gate && p.gate_rows == 0) + (a->dnormed != nullptr)) + sizeof(R) * (1 + (a->dr != nullptr))) / 2;
     const size_t rows = (size_t)(per - 1) * p.threads_row * bnorm::kCh * sizeof(float);
-    const size_t smem = std::max(rows, vec ? block_norm_ring<T>(pieces, threads) : 0);
-    const auto kernel = threads > 512   ? (vec ? bnorm::block_norm_bwd<T, R, true, 1024, 1> : bnorm::block_norm_bwd<T, R, false, 1024, 1>)
-                        : threads > 256 ? (vec ? bnorm::block_norm_bwd<T, R, true, 512, 1> : bnorm::block_norm_bwd<T, R, false, 512, 1>)
-                                        : (vec ? bnorm::block_norm_bwd<T, R, true, 256, kBwd> : bnorm::block_norm_bwd<T, R, false, 256, kBwd>);
+    const size_t smem = std::max(rows, vec ? block_norm_ring<T>(pieces, threads, true) : 0);
+    const auto kernel = vec ? block_norm_kernel<T, R, true>(threads, pair, true) : block_norm_kernel<T, R, false>(threads, pair, true);
     BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
-    BISSD_LAUNCH("block_norm_bwd", launch_pdl(kernel, (int)(entries * p.blocks), threads, smem, s, p));
+    BISSD_LAUNCH("block_norm_bwd", launch_cluster(kernel, (int)(entries * p.blocks) * pair, threads, smem, s, pair, p));
     bnorm::SumParams q{};
     q.part = part; q.D = p.D; q.blocks = p.blocks; q.entries = (int)entries; q.w_dtype = p.w_dtype; q.g_dtype = a->dtype;
     q.dpre = a->dnormed ? a->dpre : nullptr; q.dpost = a->post_weight ? a->dpost : nullptr;
@@ -124,7 +136,7 @@ int bissd_block_norm_workspace_bytes(const bissd_block_norm_args *a, size_t *bwd
     const int rc = block_norm_sizes(a);
     if (rc != BISSD_OK) return rc;
     const bnorm::Params p = block_norm_params(a);
-    if (bwd_bytes) *bwd_bytes = align256((size_t)block_norm_entries(p) * block_norm_blocks(p, block_norm_resident(p, kBwd)) * 4 * p.D * sizeof(float));
+    if (bwd_bytes) *bwd_bytes = align256((size_t)block_norm_entries(p) * block_norm_blocks(p, true) * 4 * p.D * sizeof(float));
     return BISSD_OK;
 }
 

@@ -7,7 +7,9 @@
 // width / 8 threads with eight channels each - neighbouring ones (16-byte accesses), or where width or addresses do not allow that,
 // ones a stride apart - and a block walks rows with the weights in registers.  With 16-byte accesses a thread's pieces of the
 // next rows come by asynchronous copies into shared memory of its own, several rows ahead: held in registers, one row ahead, they
-// left two blocks an SM waiting.  Arithmetic is on pairs of channels (two multiply-adds an instruction).  r is formed
+// left two blocks an SM waiting.  Above 4096 channels a row of the backward pass is two blocks' of a cluster: one block of 1024
+// threads left a thread 64 registers, too few (1445 us for 950, 16004 gated rows of 8192; the forward pass, which fits, loses by the
+// meetings of a pair, 472 us for 365).  Arithmetic is on pairs of channels (two multiply-adds an instruction).  r is formed
 // again in the backward pass, from what the forward pass read, so that no rounding of it enters.  Sums over rows: in registers over a
 // block's rows - act, w2 and scale are factors of them that wait until the end, so that dw2, dscale and the gradient of a shared gate row
 // come from one sum of dr' x^ (act) - then over the blocks in a second kernel, always in one order.
@@ -131,29 +133,47 @@ __device__ __forceinline__ float both(f2 v) {
 // others in the call between.  A row of at most eight warps has eight places, zeros behind its warps' sums, so that two wide reads
 // fetch them all: read one by one, their
 // place found by a division, they cost 339 us instead of 310 (65536 rows of 1024, gated, forward and backward).
-struct RowSums {
+// A row of two blocks: both write all sums, and meet.
+template <bool PAIR> struct RowSums {
     float at[2][32];
+    __device__ __forceinline__ static void meet() {              // the cluster's blocks; whole warps call
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     __device__ __forceinline__ void start() {
         if (threadIdx.x < 64) at[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
-        __syncthreads();
+        if (PAIR)
+            meet();                                              // the other block has begun
+        else
+            __syncthreads();
     }
     __device__ __forceinline__ float operator()(float v, int &turn, int tr, int row) {   // row: of the block's
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (tr == 32) return v;
+        if (!PAIR && tr == 32) return v;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = tr >> 5;
         float *buf = at[turn];
         turn ^= 1;
-        if (per <= 8) {
+        if (!PAIR && per <= 8) {
             if (lane == 0) buf[row * 8 + warp - row * per] = v;
             __syncthreads();
             const float4 *w = reinterpret_cast<const float4 *>(buf + row * 8);
             const float4 a = w[0], b = w[1];
             return ((((((a.x + a.y) + a.z) + a.w) + b.x) + b.y) + b.z) + b.w;
         }
-        if (lane == 0) buf[warp] = v;                            // one row a block: a lane for each warp
-        __syncthreads();
-        float s = lane < per ? buf[lane] : 0.f;
+        if (PAIR) {                                              // lanes 0 and 1: to either block
+            if (lane < 2) {
+                uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(buf + (blockIdx.x & 1) * (per >> 1) + warp));
+                asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(to) : "r"(lane));
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+            }
+            meet();
+        } else {                                                 // one row a block
+            if (lane == 0) buf[warp] = v;
+            __syncthreads();
+        }
+        float s = lane < per ? buf[lane] : 0.f;                  // a lane for each warp
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         return s;
@@ -182,30 +202,32 @@ __device__ __forceinline__ void activation(int act, f2 (&a)[kPairs], f2 (&slope)
 }
 
 // Rows that a thread copies ahead: as many as leave an SM's blocks their shared memory.
-template <class T, int THREADS> struct Ahead {
-    static constexpr int rows = THREADS <= 256 ? (sizeof(T) == 4 ? 2 : 4) : (THREADS <= 512 || sizeof(T) == 2 ? 2 : 1);
+template <class T, int THREADS, int PER_SM> struct Ahead {
+    static constexpr int rows = THREADS <= 256 ? (sizeof(T) == 4 ? 2 : 4) : THREADS <= 512 ? (PER_SM == 1 && sizeof(T) == 2 ? 3 : 2) : sizeof(T) == 2 ? 2 : 1;
 };
 
 // What both kernels walk: rows first + i of an entry (the rows that share a gate row, or all), i = blk per + grp, + step, ...  A row
-// behind the last is one of zeros, of which nothing is kept.
+// behind the last is one of zeros, of which nothing is kept.  PAIR: a row is a cluster's of two blocks.
 struct Walk {
-    int tr, per, grp, t, D, blk, n, first, step;
-    __device__ __forceinline__ Walk(const Params &a) {
-        tr = a.threads_row; per = blockDim.x / tr; grp = threadIdx.x / tr; t = threadIdx.x % tr; D = a.D;
-        blk = blockIdx.x % a.blocks;
+    int tr, per, grp, t, D, blk, entry, n, first, step;
+    __device__ __forceinline__ Walk(const Params &a, bool pair) {
+        const int x = pair ? blockIdx.x >> 1 : blockIdx.x;
+        tr = a.threads_row; per = pair ? 1 : blockDim.x / tr; grp = pair ? 0 : threadIdx.x / tr;
+        t = pair ? (blockIdx.x & 1) * blockDim.x + threadIdx.x : threadIdx.x % tr; D = a.D;
+        blk = x % a.blocks; entry = x / a.blocks;
         n = a.gate && a.gate_rows > 0 ? a.gate_rows : a.rows;
-        first = blockIdx.x / a.blocks * n;
+        first = entry * n;
         step = a.blocks * per;
     }
 };
 
-template <class T, class R, bool VEC, int THREADS, int PER_SM>
+template <class T, class R, bool VEC, bool PAIR, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     pdl_begin();
     extern __shared__ __align__(16) uint8_t dyn[];
-    __shared__ __align__(16) RowSums row_sum;
+    __shared__ __align__(16) RowSums<PAIR> row_sum;
     row_sum.start();
-    const Walk k(a);
+    const Walk k(a, PAIR);
     const int t = k.t, tr = k.tr, D = k.D, threads = blockDim.x;
     const bool full = a.gate && a.gate_rows == 0, in = t * kCh < D;
     f2 mw[kPairs], w1[kPairs], scw[kPairs];                      // scale act w2; scale w2
@@ -217,7 +239,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) mw[i] = scw[i] = mul2(sc[i], w2[i]);
     }
-    constexpr int kAhead = Ahead<T, THREADS>::rows;
+    constexpr int kAhead = Ahead<T, THREADS, PER_SM>::rows;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
     int bytes = 0, turn = 0, at = 0;                             // of a stage of the ring; the stage in turn, in bytes
     int i = k.blk * k.per + k.grp, ahead = i;
@@ -237,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     };
     if (a.gate && !full) {
         f2 slope[kPairs];
-        const T *p = static_cast<const T *>(a.gate) + (long long)(blockIdx.x / a.blocks) * a.sgate;
+        const T *p = static_cast<const T *>(a.gate) + (long long)k.entry * a.sgate;
         float e[kCh];
 #pragma unroll
         for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(p[channel<VEC>(t, tr, j)]) : 0.f;
@@ -297,13 +319,13 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <class T, class R, bool VEC, int THREADS, int PER_SM>
+template <class T, class R, bool VEC, bool PAIR, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
     pdl_begin();
     extern __shared__ __align__(16) uint8_t dyn[];
-    __shared__ __align__(16) RowSums row_sum;
+    __shared__ __align__(16) RowSums<PAIR> row_sum;
     row_sum.start();
-    const Walk k(a);
+    const Walk k(a, PAIR);
     const int t = k.t, tr = k.tr, D = k.D, threads = blockDim.x;
     const bool full = a.gate && a.gate_rows == 0, in = t * kCh < D;
     f2 w1[kPairs], scw[kPairs], act[kPairs], slope[kPairs], d1[kPairs], d2[kPairs];   // scw: scale w2; d2: sums of dr' x^ (act)
@@ -320,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
         }
     }
     if (a.gate && !full) {
-        const T *p = static_cast<const T *>(a.gate) + (long long)(blockIdx.x / a.blocks) * a.sgate;
+        const T *p = static_cast<const T *>(a.gate) + (long long)k.entry * a.sgate;
         float e[kCh];
 #pragma unroll
         for (int j = 0; j < kCh; ++j) e[j] = channel<VEC>(t, tr, j) < D ? to_f<T>(p[channel<VEC>(t, tr, j)]) : 0.f;
@@ -328,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
         for (int j = 0; j < kPairs; ++j) act[j] = pack(e[2 * j], e[2 * j + 1]);
         activation(a.act, act, slope);
     }
-    constexpr int kAhead = Ahead<T, THREADS>::rows;
+    constexpr int kAhead = Ahead<T, THREADS, PER_SM>::rows;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(dyn)) + threadIdx.x * 16;
     int bytes = 0, turn = 0, at = 0;
     int i = k.blk * k.per + k.grp, ahead = i;
@@ -422,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
     if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
     // rows side by side in this block added up, then one partial row a block
     float *sums = reinterpret_cast<float *>(dyn);
-    const long long part = (long long)blockIdx.x * 4 * D;
+    const long long part = (long long)(PAIR ? blockIdx.x >> 1 : blockIdx.x) * 4 * D;
 #pragma unroll
     for (int what = 0; what < 2; ++what) {
         f2(&v)[kPairs] = what ? d2 : d1;
