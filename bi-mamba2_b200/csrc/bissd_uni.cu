@@ -404,12 +404,12 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
     unitc::StatesParams p{};
     p.h = tc_heads(a, t.PB);
     p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.status = status;
-    const size_t smem = unitc::states_smem(t.NT);
     const long long grid = (long long)t.seg.most * a->nheads * t.PB;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     auto launch = [&](const char *name, bool exact) -> int {
         const auto kernel = t.NT == 64 ? (exact ? unitc::decay_states<64, true> : unitc::decay_states<64, false>)
                                        : (exact ? unitc::decay_states<128, true> : unitc::decay_states<128, false>);
+        const size_t smem = unitc::states_smem(t.NT, exact);
         BISSD_ALLOW(kernel, smem);
         BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, cols, tiles));
         return BISSD_OK;

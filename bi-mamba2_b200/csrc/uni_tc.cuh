@@ -104,7 +104,10 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
 // loaded to registers, made it longer: the loads from tensor memory then waited for those rows.)  Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
 // A weight f meets bf16 rows as bf16 f1 + f2, in one rounding: v f1 + (v f2) as a multiply-add.
 // EXACT: the weighted row is given to the tensor cores in three bf16 parts, each what is left of those before, so that the states
-// that leave the library are fp32's.  The tiles that the other kernels read are bf16 in any case: they meet bf16 factors.
+// that leave the library are fp32's.  The tiles that the other kernels read are bf16 in any case: they meet bf16 factors.  The parts
+// lie side by side and take one product of 192 columns, which reads k once, and meet again as three sums: shared memory bounds this
+// (as three products of 64 columns, in two rounds, 190 us for 142: 512 chunks of 32 heads, 128 x 64 states).  The third part goes
+// where v's rows came, in front of the others or behind them in turn, and k has one buffer: its next rows come while v's are weighted.
 struct StatesParams {
     Heads h;
     Plan seg, chunk;
@@ -119,21 +122,22 @@ __device__ __forceinline__ void tma_store_read() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 struct StatesShared {
-    uint64_t full[2], full_v, ready, staged, done, weights, stored, unused;   // staged: ready for the first time in a step
+    uint64_t full[2], full_v[2], ready, done, weights, stored, unused;
     uint32_t tmem;
     int fail;
     float decay[2];                                              // of a chunk, 2^c_end
     alignas(16) uint32_t w[kQ];                                  // of a chunk's rows: f1 and f2, or EXACT fp32
 };
 constexpr int kStatesThreads = 320;
-inline size_t states_smem(int NT) { return 2 * (size_t)(NT / 64) * kSlab + 3 * (size_t)kSlab + sizeof(StatesShared); }
+inline size_t states_smem(int NT, bool exact) { return (exact ? NT / 64 + 5 : 2 * (NT / 64) + 3) * (size_t)kSlab + sizeof(StatesShared); }
 
 template <int NT, bool EXACT> __global__ void __launch_bounds__(kStatesThreads, 2)
 decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
     constexpr int kSlabs = NT / 64;
     extern __shared__ __align__(1024) uint8_t dyn[];
-    uint8_t *smK = dyn, *smV = smK + 2 * kSlabs * kSlab, *smS = smV + 2 * kSlab;   // two stages of k; two of weighted rows; S
+    // two stages of k, two of weighted rows, S.  EXACT: one of k, v's rows, two parts, v's rows, S
+    uint8_t *smK = dyn, *smV = smK + (EXACT ? 1 : 2) * kSlabs * kSlab, *smS = smV + (EXACT ? 4 : 2) * kSlab;
     StatesShared &sh = *reinterpret_cast<StatesShared *>(smS + kSlab);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pb = blockIdx.x % a.h.PB, h = blockIdx.x / a.h.PB % a.h.H, si = blockIdx.x / (a.h.PB * a.h.H), hq = h * a.h.hk / a.h.H;
@@ -147,14 +151,13 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     auto place = [&](int i) { return a.reverse ? nc - 1 - i : i; };        // chunk of the segment at step i
     auto length = [&](int i) { return min(kQ, s.len - place(i) * kQ); };
     volatile int *fail = &sh.fail;
-    uint8_t *raw = a.tiles ? smV + kSlab : smS;                  // EXACT: where v's rows arrive, the third buffer or the second part's
-    if (warp == 0) tmem_alloc(&sh.tmem, 64);
+    if (warp == 0) tmem_alloc(&sh.tmem, EXACT ? 256 : 64);
     if (tid == 256) {
         mbar_init(&sh.full[0], 1);
         mbar_init(&sh.full[1], 1);
-        mbar_init(&sh.full_v, 1);
+        mbar_init(&sh.full_v[0], 1);
+        mbar_init(&sh.full_v[1], 1);
         mbar_init(&sh.ready, 8);
-        mbar_init(&sh.staged, 8);
         mbar_init(&sh.done, 1);
         mbar_init(&sh.weights, 1);
         mbar_init(&sh.stored, 1);
@@ -168,64 +171,59 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     bool ok = true;
     if (warp == 8) {
         auto load = [&](int i) {
-            const int st = i & 1, t = s.t0 + place(i) * kQ;
+            const int st = EXACT ? 0 : i & 1, t = s.t0 + place(i) * kQ;
             mbar_expect_tx(&sh.full[st], (kSlabs + !EXACT) * kSlab);
             for (int j = 0; j < kSlabs; ++j) tma_load4(smK + (st * kSlabs + j) * kSlab, &tmK, j * 64, hq, t, s.batch, &sh.full[st]);
             if (!EXACT) tma_load4(smV + st * kSlab, &tmV, pb * kP, h, t, s.batch, &sh.full[st]);
+            if (EXACT && i + 1 < nc)                             // the next one's as far as L2: their load waits for the buffer
+                for (int j = 0; j < kSlabs; ++j)
+                    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(&tmK), "r"(j * 64), "r"(hq),
+                                 "r"(s.t0 + place(i + 1) * kQ), "r"(s.batch) : "memory");
         };
         auto load_v = [&](int i) {                               // EXACT
-            mbar_expect_tx(&sh.full_v, kSlab);
-            tma_load4(raw, &tmV, pb * kP, h, s.t0 + place(i) * kQ, s.batch, &sh.full_v);
+            mbar_expect_tx(&sh.full_v[i & 1], kSlab);
+            tma_load4(smV + (i & 1) * 3 * kSlab, &tmV, pb * kP, h, s.t0 + place(i) * kQ, s.batch, &sh.full_v[i & 1]);
         };
-        if (lane == 0) load(0);
-        if (EXACT && lane == 0) load_v(0);
-        int loads = 1, loads_v = EXACT, round = 0;
-        constexpr uint32_t idesc = instr_desc(1, true, true, kP);
+        int loads = 1, loads_v = EXACT ? min(nc, 2) : 0;
+        if (lane == 0) {
+            load(0);
+            for (int i = 0; i < loads_v; ++i) load_v(i);
+        }
+        constexpr uint32_t idesc = instr_desc(1, true, true, EXACT ? 3 * kP : kP);
         for (int i = 0; i < nc && ok; ++i) {
-            const int st = i & 1;
-            if (i + 1 < nc) {                                    // the stage was read by the MMAs of the step before
-                if (i > 0) ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 1);
+            const int st = EXACT ? 0 : i & 1;
+            if (!EXACT && i + 1 < nc) {                          // the stage was read by the MMAs of the step before
+                if (i > 0) ok = ws_wait_warp(&sh.done, (i - 1) & 1, fail, 1);
                 if (ok && lane == 0) load(i + 1);
                 loads += ok;
             }
-            ok = ok && ws_wait_warp(&sh.full[st], (i >> 1) & 1, fail, 2);
-            auto issue = [&](const uint8_t *v, uint32_t first) {
+            ok = ok && ws_wait_warp(&sh.full[st], (EXACT ? i : i >> 1) & 1, fail, 2) && ws_wait_warp(&sh.ready, i & 1, fail, 3);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint8_t *v = smV + (i & 1) * kSlab;
 #pragma unroll
                 for (int kk = 0; kk < kQ / 16; ++kk)             // where NT is 64, rows 64 ... 127 are the first 64 again: products of no use
                     umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 0 : kSlab, 1024),
-                         smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : first);
-            };
-            for (int r = 0; r < (EXACT ? 2 : 1) && ok; ++r, ++round) {   // the third part goes where the first was: two rounds a step
-                ok = ws_wait_warp(&sh.ready, round & 1, fail, 3);
+                         smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0);
+                umma_commit(&sh.done);
+            }
+            __syncwarp();
+            if (EXACT && i + 1 < nc) {
+                ok = ws_wait_warp(&sh.done, i & 1, fail, 1);
                 if (!ok) break;
-                tc_fence_after();
-                const bool more = EXACT && r == 0 && i + 1 < nc;
-                if (more && !a.tiles) {                          // this chunk's rows are in registers
-                    if (lane == 0) load_v(i + 1);
-                    ++loads_v;
-                }
-                if (elect_one()) {
-                    if (r == 1) {
-                        issue(smV, 1u);
-                    } else {
-                        issue(smV + (EXACT ? 0 : st * kSlab), 0u);
-                        if constexpr (EXACT) issue(smV + kSlab, 1u);
-                    }
-                    umma_commit(&sh.done);
-                }
-                __syncwarp();
-                if (more && a.tiles) {                           // the second part has been read
-                    ok = ws_wait_warp(&sh.done, round & 1, fail, 11);
-                    if (!ok) break;
-                    if (lane == 0) load_v(i + 1);
+                if (lane == 0) load(i + 1);
+                ++loads;
+                if (i + 2 < nc) {
+                    if (lane == 0) load_v(i + 2);
                     ++loads_v;
                 }
             }
         }
         if (!ok && elect_one()) {                                // leave nothing in flight
             drain_mmas(&sh.unused);
-            drain_loads(sh.full, 2, loads);
-            drain_loads(&sh.full_v, 1, loads_v);
+            drain_loads(sh.full, EXACT ? 1 : 2, loads);
+            drain_loads(sh.full_v, 2, loads_v);
             atomicExch(a.status, kErrDecay + 0x10 + *fail);
         }
         __syncwarp();
@@ -272,7 +270,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         if (nc > 1) make();
         ask(2);
         for (int i = 0; i < nc; ++i) {
-            ok = ws_wait_warp(&sh.staged, i & 1, fail, 9);       // the next one cannot come before this warp's weights: none is missed
+            ok = ws_wait_warp(&sh.ready, i & 1, fail, 9);       // the next one cannot come before this warp's weights: none is missed
             if (!ok) break;
             if (i + 1 < nc) give(i + 1);
             if (a.tiles && elect_one()) {
@@ -290,7 +288,6 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         if (a.tiles && elect_one()) tma_store_wait();
         __syncwarp();
     } else {
-        uint4 rows[4];                                           // EXACT: 16 bytes of rows tid / 8 + 32 k of v
         const uint32_t swz = (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);   // the thread's piece of a tile, + 4096 k
         auto weigh = [&](uint8_t *v, int len) {                  // bf16 rows times f1 + f2, in their place
 #pragma unroll
@@ -310,11 +307,13 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 *reinterpret_cast<uint4 *>(v + swz + k * 4096) = (tid >> 3) + k * 32 < len ? make_uint4(e[0], e[1], e[2], e[3]) : zero8();
             }
         };
-        auto parts = [&]() {                                     // the first two parts of the weighted rows to their buffers, the third kept
+        auto parts = [&](int i, int len) {                       // chunk i's weighted rows: the third part in their place
+            uint8_t *third = smV + (i & 1) * 3 * kSlab + swz, *first = smV + kSlab + swz;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float f = __uint_as_float(sh.w[(tid >> 3) + k * 32]);
-                uint32_t e[4] = {rows[k].x, rows[k].y, rows[k].z, rows[k].w}, o1[4], o2[4];
+                const uint4 row = (tid >> 3) + k * 32 < len ? *reinterpret_cast<const uint4 *>(third + k * 4096) : zero8();
+                uint32_t e[4] = {row.x, row.y, row.z, row.w}, o1[4], o2[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     float x, y, hx, hy;
@@ -329,9 +328,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                     unpack2<bf16>(o2[q], hx, hy);
                     e[q] = pack2<bf16>(x - hx, y - hy);
                 }
-                *reinterpret_cast<uint4 *>(smV + swz + k * 4096) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-                *reinterpret_cast<uint4 *>(smV + kSlab + swz + k * 4096) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
-                rows[k] = make_uint4(e[0], e[1], e[2], e[3]);
+                *reinterpret_cast<uint4 *>(first + k * 4096) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+                *reinterpret_cast<uint4 *>(first + kSlab + k * 4096) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+                *reinterpret_cast<uint4 *>(third + k * 4096) = make_uint4(e[0], e[1], e[2], e[3]);
             }
         };
         const int n = (warp & 3) * 32 + lane, half = warp >> 2, col = pb * kP + half * 32;
@@ -340,14 +339,12 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
         for (int j = 0; j < 32; ++j) S[j] = a.init && n < a.h.N && col + j < a.h.P ? a.init[at + j] : 0.f;
         const uint32_t tl = tmem_lane_base(tmem) + half * 32;
-        auto arrive = [&](bool first) {                          // what this warp wrote is there, what it read of tensor memory is read
+        auto arrive = [&] {                                      // what this warp wrote is there, what it read of tensor memory is read
             fence_async_smem();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.ready);
-            if (lane == 0 && first) mbar_arrive(&sh.staged);
         };
-        int round = 0;
         auto prepare = [&](int i) {                              // chunk i's rows
             const int st = i & 1;
             if (!ws_wait_warp(&sh.weights, i & 1, fail, 4) || !ws_wait_warp(&sh.full[st], (i >> 1) & 1, fail, 6)) return false;
@@ -361,12 +358,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             const int st = i & 1;
             float now;
             if constexpr (EXACT) {
-                ok = ws_wait_warp(&sh.weights, i & 1, fail, 4) && ws_wait_warp(&sh.full_v, i & 1, fail, 10);
+                ok = ws_wait_warp(&sh.weights, i & 1, fail, 4) && ws_wait_warp(&sh.full_v[st], (i >> 1) & 1, fail, 10);
                 if (!ok) break;
-                const int len = length(i) - (tid >> 3);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) rows[k] = k * 32 < len ? *reinterpret_cast<const uint4 *>(raw + swz + k * 4096) : zero8();
-                parts();
+                parts(i, length(i));
             }
             now = sh.decay[st];
             if (a.tiles) {                                       // what enters this chunk
@@ -381,21 +375,12 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 }
             }
             if (EXACT && a.seg.packed && length(i) < kQ) {
-                ok = ws_wait_warp(&sh.full[st], (i >> 1) & 1, fail, 6);
+                ok = ws_wait_warp(&sh.full[0], i & 1, fail, 6);
                 if (!ok) break;
-                for (int j = 0; j < kSlabs; ++j) clear_rows(smK + (st * kSlabs + j) * kSlab, length(i), tid, 256);
+                for (int j = 0; j < kSlabs; ++j) clear_rows(smK + j * kSlab, length(i), tid, 256);
             }
-            arrive(true);
-            ++round;
-            if constexpr (EXACT) {
-                ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 7);
-                if (!ok) break;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4 *>(smV + swz + k * 4096) = rows[k];
-                arrive(false);
-                ++round;
-            }
-            ok = ws_wait_warp(&sh.done, (round - 1) & 1, fail, 8);
+            arrive();
+            ok = ws_wait_warp(&sh.done, i & 1, fail, 8);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -404,6 +389,14 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 tmem_ld16(tl + j0, x);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, x[j]);
+                if constexpr (EXACT) {
+                    tmem_ld16(tl + kP + j0, x);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) S[j0 + j] += x[j];
+                    tmem_ld16(tl + 2 * kP + j0, x);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) S[j0 + j] += x[j];
+                }
             }
             if constexpr (!EXACT)
                 if (i + 1 < nc) ok = prepare(i + 1);
@@ -416,7 +409,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, 64);
+    if (warp == 0) tmem_dealloc(tmem, EXACT ? 256 : 64);
 }
 
 // ---- the outputs -----------------------------------------------------------------------------------------------------
