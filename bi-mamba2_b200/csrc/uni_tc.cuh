@@ -95,6 +95,24 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
     for (int i = from * 8 + tid; i < kQ * 8; i += threads) *reinterpret_cast<uint4 *>(slab + i * 16) = zero8();
 }
 
+// A weight f as bf16 f1 + f2, and eight bf16 values times it in one rounding: v f1 + (v f2) as a multiply-add.
+__device__ __forceinline__ uint32_t halves(float f) {
+    const float hi = __bfloat162float(__float2bfloat16_rn(f));
+    return pack2<bf16>(hi, f - hi);
+}
+__device__ __forceinline__ uint4 weighted(const uint4 &row, uint32_t f) {
+    const uint32_t f1 = __byte_perm(f, f, 0x1010), f2 = __byte_perm(f, f, 0x3232);
+    uint32_t e[4] = {row.x, row.y, row.z, row.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&e[q]);
+        const __nv_bfloat162 o = __hfma2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f1),
+                                         __hmul2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f2)));
+        e[q] = *reinterpret_cast<const uint32_t *>(&o);
+    }
+    return make_uint4(e[0], e[1], e[2], e[3]);
+}
+
 // ---- the states that enter the chunks ------------------------------------------------------------------------------------
 // Forwards S' as above; backwards (v the outputs' gradient, k the queries) the gradient that enters each chunk from its right,
 // G' = e^{c_end} G + sum_t q_t (scale e^{c_t} do_t)^T.  A block walks the chunks of one (segment, head, 64 columns), S or G in
@@ -102,7 +120,6 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
 // the ninth issues loads and MMAs, the tenth makes the weights and stores the tiles, and they meet at mbarriers alone: a step is S's
 // way to shared memory, one product's latency, its way back and the weighting.  (The weighting in the product's shadow, from rows
 // loaded to registers, made it longer: the loads from tensor memory then waited for those rows.)  Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
-// A weight f meets bf16 rows as bf16 f1 + f2, in one rounding: v f1 + (v f2) as a multiply-add.
 // EXACT: the weighted row is given to the tensor cores in three bf16 parts, each what is left of those before, so that the states
 // that leave the library are fp32's.  The tiles that the other kernels read are bf16 in any case: they meet bf16 factors.  The parts
 // lie side by side and take one product of 192 columns, which reads k once, and meet again as three sums: shared memory bounds this
@@ -202,7 +219,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             tc_fence_after();
             if (elect_one()) {
                 const uint8_t *v = smV + (i & 1) * kSlab;
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < kQ / 16; ++kk)             // where NT is 64, rows 64 ... 127 are the first 64 again: products of no use
                     umma(tmem, smem_desc(smem_u32(smK + st * kSlabs * kSlab) + kk * 2048, NT == 64 ? 0 : kSlab, 1024),
                          smem_desc(smem_u32(v) + kk * 2048, kSlab, 1024), idesc, kk > 0);
@@ -248,12 +265,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float v = exp2f(a.reverse ? c[k] + a.h.log_scale : c[k]);
-                if constexpr (EXACT) {
-                    f[k] = __float_as_uint(v);
-                } else {
-                    const float hi = __bfloat162float(__float2bfloat16_rn(v));
-                    f[k] = pack2<bf16>(hi, v - hi);
-                }
+                f[k] = EXACT ? __float_as_uint(v) : halves(v);
             }
         };
         auto give = [&](int i) {                                 // to the others, as chunk i's
@@ -292,19 +304,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         auto weigh = [&](uint8_t *v, int len) {                  // bf16 rows times f1 + f2, in their place
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t f = sh.w[(tid >> 3) + k * 32];
-                const uint32_t f1 = __byte_perm(f, f, 0x1010), f2 = __byte_perm(f, f, 0x3232);
-                const uint4 row = *reinterpret_cast<const uint4 *>(v + swz + k * 4096);
-                uint32_t e[4] = {row.x, row.y, row.z, row.w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&e[q]);
-                    const __nv_bfloat162 o = __hfma2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f1),
-                                                     __hmul2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f2)));
-                    e[q] = *reinterpret_cast<const uint32_t *>(&o);
-                }
+                const uint4 row = weighted(*reinterpret_cast<const uint4 *>(v + swz + k * 4096), sh.w[(tid >> 3) + k * 32]);
                 // rows behind the sequence's end may be of another, and no numbers
-                *reinterpret_cast<uint4 *>(v + swz + k * 4096) = (tid >> 3) + k * 32 < len ? make_uint4(e[0], e[1], e[2], e[3]) : zero8();
+                *reinterpret_cast<uint4 *>(v + swz + k * 4096) = (tid >> 3) + k * 32 < len ? row : zero8();
             }
         };
         auto parts = [&](int i, int len) {                       // chunk i's weighted rows: the third part in their place
@@ -496,7 +498,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         ok = mbar_wait(&bar_qk, 0);
         if (ok) {
             constexpr uint32_t idesc = instr_desc(1, false, false, kQ);
-#pragma unroll
+#pragma unroll 1
             for (int kk = 0; kk < NT / 16; ++kk)
                 umma(tmem, smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
                      smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
@@ -528,7 +530,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
             if (ok) {
                 tc_fence_after();
                 constexpr uint32_t idesc = instr_desc(1, false, true, kP);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < NT / 16; ++kk)
                     umma(tmem + 192, smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
                          smem_desc(smem_u32(smS) + kk * 2048, NT * 128, 1024), idesc, kk > 0 ? 1u : 0u);
@@ -592,7 +594,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
             if (ok) {
                 tc_fence_after();
                 constexpr uint32_t idesc = instr_desc(1, false, true, kP);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < kQ / 16; ++kk)
                     umma(tmem + 128, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
                          smem_desc(smem_u32(smV) + kk * 2048, kSlab, 1024), idesc, kk > 0 ? 1u : 0u);
@@ -707,10 +709,11 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmG) {
     pdl_begin();
     constexpr int kSlabs = NT / 64, kT = 512;
-    constexpr int kTables = 3, kIssue = 7, kSums = 11;           // warps above the diagonal
+    constexpr int kTables = 2, kHelp = 3, kIssue = 7, kSums = 11;   // warps above the diagonal
     extern __shared__ __align__(1024) uint8_t dyn[];
     struct Table {                                               // of a head; two take turns
-        float c[kQ], ws[kQ], et[kQ];                             // c_t; e^{c_end - c_s}; scale e^{c_t}
+        float c[kQ], ws[kQ];                                     // c_t; e^{c_end - c_s}
+        uint32_t wv[kQ], wd[kQ];                                 // that and scale e^{c_t} in halves, for v and do
         float above[kQ], beside[3][kQ];                          // weights of blocks of 32 x 32: 2^(c at the end of s' 32 - c_s), scale 2^(c_t - c at the end of the q-th 32)
         float whole[4];                                          // c_end
     };
@@ -751,10 +754,14 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         auto four = [&](float *o, float x0, float x1, float x2, float x3) { *reinterpret_cast<float4 *>(o + lane * 4) = make_float4(x0, x1, x2, x3); };
         four(to.c, p[0], p[1], p[2], p[3]);
         four(to.above, ex2_approx(end - p[0]), ex2_approx(end - p[1]), ex2_approx(end - p[2]), ex2_approx(end - p[3]));
-        four(to.ws, ex2_approx(q[0]), ex2_approx(q[1]), ex2_approx(q[2]), ex2_approx(q[3]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = ex2_approx(q[k]);
+        four(to.ws, q[0], q[1], q[2], q[3]);
+        *reinterpret_cast<uint4 *>(to.wv + lane * 4) = make_uint4(halves(q[0]), halves(q[1]), halves(q[2]), halves(q[3]));
 #pragma unroll
         for (int k = 0; k < 4; ++k) p[k] += a.h.log_scale;
-        four(to.et, ex2_approx(p[0]), ex2_approx(p[1]), ex2_approx(p[2]), ex2_approx(p[3]));
+        *reinterpret_cast<uint4 *>(to.wd + lane * 4) =
+            make_uint4(halves(ex2_approx(p[0])), halves(ex2_approx(p[1])), halves(ex2_approx(p[2])), halves(ex2_approx(p[3])));
 #pragma unroll
         for (int b = 0; b < 3; ++b)                              // of use in the blocks behind the b-th
             four(to.beside[b], ex2_approx(p[0] - ends[b]), ex2_approx(p[1] - ends[b]), ex2_approx(p[2] - ends[b]), ex2_approx(p[3] - ends[b]));
@@ -800,11 +807,29 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         }
     float through = 0.f;                                         // this thread's part of S.G
     const long long token = (long long)sg.batch * a.chunk.L + sg.t0;
-    bf16 *dv = a.dv + (token + (tid >> 3)) * a.h.H * a.h.P;      // the first of the two rows this thread writes of each tile
+    // 16-byte pieces of a tile of 128 x 64, two a thread; the issuing warp's are another's
+    const int reps = warp == kIssue ? 0 : warp == kHelp ? 2 : 1;
+    auto pieces = [&](auto f) {
+        for (int r = 0; r < reps; ++r) {
+            f(tid + r * (kIssue - kHelp) * 32);
+            f(tid + r * (kIssue - kHelp) * 32 + kT);
+        }
+    };
+    auto put_dv = [&](int i, int h, int pb) {                    // tile i's from v's place
+        const uint8_t *from = smV + (i & 1) * kSlab;
+        bf16 *dv = a.dv + (token * a.h.H + h) * a.h.P + pb * kP;
+        const int row_values = a.h.H * a.h.P;
+        pieces([&](int x) {
+            const int r = x >> 3, col = (x & 7) * 8;
+            if (r < len && pb * kP + col < a.h.P)
+                *reinterpret_cast<uint4 *>(dv + (long long)r * row_values + col) =
+                    *reinterpret_cast<const uint4 *>(from + r * 128 + (((x & 7) ^ (r & 7)) << 4));
+        });
+    };
     auto from_chunk = [&]() {                                    // dq and dk of the chunk's own pairs; one thread
         constexpr uint32_t iq = instr_desc(1, true, true, NT), ik = instr_desc(1, false, true, NT);
         const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), n0 = smem_u32(smN);
-#pragma unroll
+#pragma unroll 1
         for (int kk = 0; kk < kQ / 16; ++kk) {
             umma(tmem + cQ, smem_desc(n0 + kk * 2048, kSlab, 1024), smem_desc(k0 + kk * 2048, kSlab, 1024), iq, 1u);
             umma(tmem + cK, smem_desc(n0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(q0 + kk * 2048, kSlab, 1024), ik, 1u);
@@ -832,11 +857,11 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             if (ok) {
                 tc_fence_after();
                 constexpr uint32_t idesc = instr_desc(1, false, false, kQ);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < NT / 16; ++kk)
                     umma(tmem, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
                          smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < 4; ++kk)
                     umma(tmem + 128, smem_desc(smem_u32(sV) + kk * 32, 16, 1024), smem_desc(smem_u32(sD) + kk * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
                 umma_commit(&done_1);
@@ -848,18 +873,12 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             d.load(a.h, sg.batch, sg.t0, len, h1, lane);
             table(tables[(h1 - h0) & 1], d);
         }
+        if (ok && i > 0) put_dv(i - 1, h0 + (i - 1) / a.h.PB, pb == 0 ? a.h.PB - 1 : pb - 1);
         if (ok) ok = mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
         if (ok) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {                        // scale e^{c_t} do_t beside do_t
-                const int x = tid + k * kT, row = x >> 3;
-                float e[8];
-                unpack8<bf16>(*reinterpret_cast<const uint4 *>(sD + x * 16), e);
-                const float f = tb.et[row];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] *= f;
-                *reinterpret_cast<uint4 *>(smE + x * 16) = pack8<bf16>(e);
-            }
+            pieces([&](int x) {                                  // scale e^{c_t} do_t beside do_t
+                *reinterpret_cast<uint4 *>(smE + x * 16) = weighted(*reinterpret_cast<const uint4 *>(sD + x * 16), tb.wd[x >> 3]);
+            });
             ok = mbar_wait(&done_1, i & 1);
         }
         tc_fence_after();
@@ -919,6 +938,11 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                     of_column = warp_sums<32>(value, lane);
                 }
             } else {
+                const int light = (quad == 3 ? 3 : quad - 1) + cg;   // of six warps
+                for (int x = light * 32 + lane; x < kQ * 8; x += 6 * 32) {   // e^{c_end - c_s} v_s in v_s' place
+                    uint4 *v = reinterpret_cast<uint4 *>(sV + x * 16);
+                    *v = weighted(*v, tb.wv[x >> 3]);
+                }
 #pragma unroll
                 for (int j = 0; j < 16; ++j) p[j] = 0u;
                 if (i == 0) {
@@ -930,17 +954,6 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             if constexpr (DG) {
                 rowsum[cg][s] = of_row + (first ? 0.f : rowsum[cg][s]);
                 colsum[quad][cg * 32 + lane] = of_column + (first ? 0.f : colsum[quad][cg * 32 + lane]);
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {                        // e^{c_end - c_s} v_s in v_s' place
-                const int q = tid + k * kT;
-                uint4 *v = reinterpret_cast<uint4 *>(sV + q * 16);
-                float e[8];
-                unpack8<bf16>(*v, e);
-                const float f = tb.ws[q >> 3];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] *= f;
-                *v = pack8<bf16>(e);
             }
             fence_async_smem();
             tmem_st_wait();
@@ -959,16 +972,16 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 constexpr uint32_t narrow = instr_desc(1, false, true, kP), wide = instr_desc(1, false, false, NT);
                 const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK);
                 const uint32_t v_ = smem_u32(sV), d_ = smem_u32(sD), e_ = smem_u32(smE), s_ = smem_u32(smS), g_ = smem_u32(smG);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < kQ / 16; ++kk)             // dv from the chunk, from the future; S^T q
                     umma_tmem(tmem + cOwn, tmem + kk * 8, smem_desc(d_ + kk * 2048, kSlab, 1024), narrow, kk > 0 ? 1u : 0u);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < NT / 16; ++kk)
                     umma(tmem + cFar, smem_desc(k0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(g_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < (DG ? NT / 16 : 0); ++kk)
                     umma(tmem + cOut, smem_desc(q0 + kk / 4 * kSlab + kk % 4 * 32, 16, 1024), smem_desc(s_ + kk * 2048, NT * 128, 1024), narrow, kk > 0 ? 1u : 0u);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < 4; ++kk) {                 // dq from the past, dk from the future
                     umma(tmem + cQ, smem_desc(e_ + kk * 32, 16, 1024), smem_desc(s_ + kk * 32, 16, 1024), wide, i > 0 || kk > 0 ? 1u : 0u);
                     umma(tmem + cK, smem_desc(v_ + kk * 32, 16, 1024), smem_desc(g_ + kk * 32, 16, 1024), wide, i > 0 || kk > 0 ? 1u : 0u);
@@ -1031,17 +1044,6 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             if (tid == 32) load_s(h1, pb1);
             ++loads_s;
         }
-        const int col = pb * kP + (tid & 7) * 8;
-        if (col < a.h.P) {
-            bf16 *o = dv + h * a.h.P + col;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int r = (tid >> 3) + k * 64;
-                if (r < len)
-                    *reinterpret_cast<uint4 *>(o + k * 64 * (long long)a.h.H * a.h.P) =
-                        *reinterpret_cast<const uint4 *>(sV + r * 128 + (((tid & 7) ^ (r & 7)) << 4));
-            }
-        }
         if (DG && last && warp == kSums) {
             float all = lane < 16 ? cross[lane] : 0.f, x[4] = {}, b[4] = {};
 #pragma unroll
@@ -1076,6 +1078,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         pb = pb1;
     }
     if (ok && warp == kIssue && elect_one()) from_chunk();
+    if (ok) put_dv(nv - 1, h0 + (nv - 1) / a.h.PB, (nv - 1) % a.h.PB);
     if (ok) ok = mbar_wait(&done_b, (nv - 1) & 1);
     tc_fence_after();
     ok = __syncthreads_and(ok);
