@@ -113,6 +113,12 @@ __device__ __forceinline__ uint4 weighted(const uint4 &row, uint32_t f) {
     return make_uint4(e[0], e[1], e[2], e[3]);
 }
 
+__device__ __forceinline__ float both(vec::f2 v) {
+    float a, b;
+    vec::unpack(v, a, b);
+    return a + b;
+}
+
 // ---- the states that enter the chunks ------------------------------------------------------------------------------------
 // Forwards S' as above; backwards (v the outputs' gradient, k the queries) the gradient that enters each chunk from its right,
 // G' = e^{c_end} G + sum_t q_t (scale e^{c_t} do_t)^T.  A block walks the chunks of one (segment, head, 64 columns), S or G in
@@ -931,9 +937,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                     *reinterpret_cast<uint4 *>(drow + ((((cg & 1) * 4 + j0 / 8) ^ (s & 7)) << 4)) = make_uint4(d[0], d[1], d[2], d[3]);
                 }
                 if constexpr (DG) {
-                    float lo, hi;
-                    vec::unpack(sum, lo, hi);
-                    of_row = lo + hi;
+                    of_row = both(sum);
                     auto value = [&](auto k) { return x[decltype(k)::value]; };
                     of_column = warp_sums<32>(value, lane);
                 }
@@ -995,11 +999,11 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             if (first) through = 0.f;
             if (ok)
                 for (int q = tid; q < NT * 8; q += kT) {
-                    float e[8], f[8];
-                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(smS + q * 16), e);
-                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(smG + q * 16), f);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) through = fmaf(e[j], f[j], through);
+                    const uint4 e = *reinterpret_cast<const uint4 *>(smS + q * 16), f = *reinterpret_cast<const uint4 *>(smG + q * 16);
+                    vec::f2 v = vec::mul2(vec::widen<bf16>(e.x), vec::widen<bf16>(f.x));
+                    v = vec::fma2(vec::widen<bf16>(e.y), vec::widen<bf16>(f.y), v);
+                    v = vec::fma2(vec::widen<bf16>(e.z), vec::widen<bf16>(f.z), v);
+                    through += both(vec::fma2(vec::widen<bf16>(e.w), vec::widen<bf16>(f.w), v));
                 }
             whole = tb.whole[0];                         // read here: behind the next barrier its table may be another head's
             if (last) {
@@ -1012,29 +1016,32 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         if (ok) ok = mbar_wait(&done_a, i & 1);
         tc_fence_after();
         if (ok) {                                                // row s (or t), columns 16 cg ... of v's 64
-            float own[16], far[16], o[16], e[8], f = 0.f, p = 0.f;
+            float own[16], far[16], o[16];
+            vec::f2 f = vec::pack(0.f, 0.f), p = f;
             tmem_ld16(tl + cOwn + cg * 16, own);
             tmem_ld16(tl + cFar + cg * 16, far);
             if constexpr (DG) tmem_ld16(tl + cOut + cg * 16, o);
-            const float w = tb.ws[s];
+            const vec::f2 w = vec::pack(tb.ws[s], tb.ws[s]);
 #pragma unroll
             for (int j = 0; j < 16; j += 8) {
                 const int at = s * 128 + (((cg * 2 + j / 8) ^ (s & 7)) << 4);
-                if constexpr (DG) {
-                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(sV + at), e);
+                const uint4 v = *reinterpret_cast<const uint4 *>(sV + at), d = *reinterpret_cast<const uint4 *>(smE + at);
+                const uint32_t vs[4] = {v.x, v.y, v.z, v.w}, ds[4] = {d.x, d.y, d.z, d.w};
+                uint32_t to[4];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) f = fmaf(e[k], far[j + k], f);
-                    unpack8<bf16>(*reinterpret_cast<const uint4 *>(smE + at), e);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) p = fmaf(e[k], o[j + k], p);
+                for (int k = 0; k < 4; ++k) {
+                    const vec::f2 far2 = vec::pack(far[j + 2 * k], far[j + 2 * k + 1]);
+                    if constexpr (DG) {
+                        f = vec::fma2(vec::widen<bf16>(vs[k]), far2, f);
+                        p = vec::fma2(vec::widen<bf16>(ds[k]), vec::pack(o[j + 2 * k], o[j + 2 * k + 1]), p);
+                    }
+                    to[k] = vec::narrow<bf16>(vec::fma2(w, far2, vec::pack(own[j + 2 * k], own[j + 2 * k + 1])));
                 }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) e[k] = fmaf(w, far[j + k], own[j + k]);
-                *reinterpret_cast<uint4 *>(sV + at) = pack8<bf16>(e);   // dv, where this thread alone has read v
+                *reinterpret_cast<uint4 *>(sV + at) = make_uint4(to[0], to[1], to[2], to[3]);   // dv, where this thread alone has read v
             }
             if constexpr (DG) {
-                future[cg][s] = f + (first ? 0.f : future[cg][s]);
-                past[cg][s] = p + (first ? 0.f : past[cg][s]);
+                future[cg][s] = both(f) + (first ? 0.f : future[cg][s]);
+                past[cg][s] = both(p) + (first ? 0.f : past[cg][s]);
             }
         }
         tc_fence_before();
