@@ -156,11 +156,6 @@ int launch_chain(const uni::ChainParams &c, cudaStream_t s) {
     BISSD_LAUNCH("decay_chain", launch_pdl(quads ? uni::decay_chain<4> : uni::decay_chain<1>, (int)grid, 256, 0, s, c));
     return BISSD_OK;
 }
-int launch_plan(const bissd_decay_args *a, const uni::PlanOut &x, const uni::PlanOut *y, cudaStream_t s) {
-    if (a->nseq == 0) return BISSD_OK;
-    BISSD_LAUNCH("decay_plan", launch_pdl(uni::decay_plan, y ? 2 : 1, 1024, 0, s, a->cu_seqlens, (int)a->nseq, (int)a->seqlen, x, y ? *y : x));
-    return BISSD_OK;
-}
 // What packed sequences leave over: rows of outputs that belong to none of them, and the states of those without a token.
 struct Rest {
     uni::RestParams p{};
@@ -169,11 +164,15 @@ struct Rest {
         p.out[p.outs] = static_cast<char *>(out);
         p.bytes[p.outs++] = elems * (long long)dtype_size(dtype);
     }
-    int launch(const bissd_decay_args *a, const int *bounds, cudaStream_t s) {
+    // The tables of segments, and what they leave over.
+    int launch(const bissd_decay_args *a, const uni::PlanOut &x, const uni::PlanOut *y, cudaStream_t s) {
         if (a->nseq == 0) return BISSD_OK;
-        p.L = a->seqlen; p.nseq = a->nseq; p.bounds = bounds;
+        p.L = a->seqlen; p.nseq = a->nseq;
         p.per = (long long)a->nheads * a->kdim * a->vdim;
-        BISSD_LAUNCH("decay_rest", launch_pdl(uni::decay_rest, 148, 256, 0, s, p));
+        const int tables = y ? 2 : 1, others = a->nseq <= uni::kNear ? 148 : 0;
+        BISSD_LAUNCH("decay_plan", launch_pdl(uni::decay_plan, tables + others, 1024, 0, s, a->cu_seqlens, (int)a->nseq, (int)a->seqlen, x, y ? *y : x,
+                                              tables, p));
+        if (!others) BISSD_LAUNCH("decay_rest", launch_pdl(uni::decay_rest, 148, 1024, 0, s, p, (const int *)x.bounds));
         return BISSD_OK;
     }
 };
@@ -246,10 +245,9 @@ int walk_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     const WalkSpace sp = walk_space(a, ws, false);
     const Walks w = walks_of(a, sp.plan);
     int *status = reinterpret_cast<int *>(ws.base);
-    BISSD_DO(launch_plan(a, sp.table, nullptr, s));
     Rest rest;
     rest.rows(a->o, a->dtype, w.z.H * w.z.P);
-    BISSD_DO(rest.launch(a, sp.table.bounds, s));
+    BISSD_DO(rest.launch(a, sp.table, nullptr, s));
     uni::WalkParams p = walk_params(w, w.k, w.v, w.q, false);
     p.status = status;
     if (sp.states) {                                             // each segment's own sum, then what enters each
@@ -269,14 +267,13 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     const WalkSpace sp = walk_space(a, ws, true);
     const Walks w = walks_of(a, sp.plan);
     const Sizes &z = w.z;
-    BISSD_DO(launch_plan(a, sp.table, nullptr, s));
     Rest rest;
     rest.rows(a->dv, a->dtype, z.H * z.P);
     if (!a->g_per_head) rest.rows(a->dg, a->g_dtype, z.H);
     rest.rows(sp.dg_tokens, BISSD_F32, z.H);
     rest.rows(sp.dqh, BISSD_F32, (long long)z.H * z.N);
     rest.rows(sp.dkh, BISSD_F32, (long long)z.H * z.N);
-    BISSD_DO(rest.launch(a, sp.table.bounds, s));
+    BISSD_DO(rest.launch(a, sp.table, nullptr, s));
     // states that enter the segments from the left, gradients that enter them from the right
     uni::WalkParams p = walk_params(w, w.k, w.v, w.q, false);
     p.status = reinterpret_cast<int *>(ws.base);
@@ -400,10 +397,11 @@ bool tc_map(CUtensorMap *m, const bissd_decay_args *a, const bissd_tensor &t, in
 
 // The states that enter the chunks (or the gradients, backwards), as bf16 tiles; those that enter and leave the sequences in fp32.
 int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &cols, const CUtensorMap &tiles, bool reverse,
-              const float *start, float *end, float *states, float *decay, int *status, cudaStream_t s) {
+              const float *start, float *end, float *states, float *decay, int *status, bool clear, cudaStream_t s) {
     unitc::StatesParams p{};
     p.h = tc_heads(a, t.PB);
     p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.status = status;
+    p.clear = clear;
     const long long grid = (long long)t.seg.most * a->nheads * t.PB;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     auto launch = [&](const char *name, bool exact) -> int {
@@ -412,6 +410,7 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
         const size_t smem = unitc::states_smem(t.NT, exact);
         BISSD_ALLOW(kernel, smem);
         BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, cols, tiles));
+        p.clear = 0;
         return BISSD_OK;
     };
     if (t.split) {
@@ -442,14 +441,13 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     if (!tc_map(&q, a, a->q, a->kdim, a->nkheads) || !tc_map(&k, a, a->k, a->kdim, a->nkheads) || !tc_map(&v, a, a->v, a->vdim, a->nheads) ||
         !tc_tile_map(&tiles, a, t, t.tiles))
         return note_cuda(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
-    BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
-    BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
     Rest rest;
+    rest.p.status = status;
     rest.rows(a->o, a->dtype, a->nheads * a->vdim);
     rest.p.start = a->initial_state;
     rest.p.end = t.split ? nullptr : a->final_state;             // the chain sees to them otherwise
-    BISSD_DO(rest.launch(a, t.chunk_table.bounds, s));
-    BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, s));
+    BISSD_DO(rest.launch(a, t.chunk_table, &t.seg_table, s));
+    BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, a->nseq == 0, s));
     unitc::ChunksParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
@@ -525,9 +523,8 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     if (!tc_map(&q, a, a->q, a->kdim, a->nkheads) || !tc_map(&k, a, a->k, a->kdim, a->nkheads) || !tc_map(&v, a, a->v, a->vdim, a->nheads) ||
         !tc_map(&dout, a, a->dout, a->vdim, a->nheads) || !tc_tile_map(&tiles, a, t, t.tiles) || !tc_tile_map(&grads, a, t, g.grads))
         return note_cuda(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
-    BISSD_DO(note_cuda(cudaMemsetAsync(status, 0, sizeof(int), s), "cudaMemsetAsync"));
-    BISSD_DO(launch_plan(a, t.chunk_table, &t.seg_table, s));
     Rest rest;
+    rest.p.status = status;
     rest.rows(a->dv, a->dtype, a->nheads * a->vdim);
     rest.rows(a->dq, a->dtype, a->nkheads * a->kdim);
     rest.rows(a->dk, a->dtype, a->nkheads * a->kdim);
@@ -536,9 +533,9 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     rest.p.start = a->dfinal_state;
     rest.p.end = t.split ? nullptr : a->dinitial_state;
     rest.p.parts = g.part; rest.p.n_parts = g.part ? 2 * g.parts : 0; rest.p.part_row = (long long)a->nkheads * a->kdim;
-    BISSD_DO(rest.launch(a, t.chunk_table.bounds, s));
-    if (!a->saved) BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, s));
-    BISSD_DO(tc_states(a, t, q, dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, s));
+    BISSD_DO(rest.launch(a, t.chunk_table, &t.seg_table, s));
+    if (!a->saved) BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, a->nseq == 0, s));
+    BISSD_DO(tc_states(a, t, q, dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, a->saved && a->nseq == 0, s));
     unitc::GradsParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.vpc = g.vpc; p.parts = g.parts;

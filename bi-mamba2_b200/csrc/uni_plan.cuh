@@ -54,35 +54,83 @@ template <class F> __device__ __forceinline__ int block_scan(int v, int *warps, 
     __syncthreads();
     if (lane == 31) warps[warp] = v;
     __syncthreads();
-    int before = none;
-    for (int w = 0; w < warp; ++w) before = op(before, warps[w]);
+    int before = lane < warp ? warps[lane] : none;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before = op(before, __shfl_xor_sync(0xffffffffu, before, o));
     return op(before, v);
 }
 
-// A block for each table.  Boundaries are taken to 0 ... L and never back, so every segment lies inside the tensors whatever the
-// caller's array holds.
-__global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int L, PlanOut a, PlanOut b) {
+// What packed sequences leave over.  Zeros in the rows of outputs that belong to no sequence, those before the first one and behind
+// the last; and the states of sequences without a token, which stay as they were (start NULL: zeros).
+struct RestParams {
+    int L, nseq, outs;
+    char *out[6];                                                // outputs and their rows' bytes, even
+    long long bytes[6];
+    float *parts;                                                // n_parts arrays of (L, part_row), or NULL
+    int n_parts;
+    long long part_row;
+    const float *start;
+    float *end;                                                  // (nseq, per), or NULL
+    long long per;
+    int *status;                                                 // cleared, or NULL
+};
+// One of `blocks` blocks' share; bounds: nseq + 1.
+__device__ __forceinline__ void rest_of(const RestParams &a, const int *bounds, int block, int blocks) {
+    const int head = bounds[0], tail = bounds[a.nseq], rows = head + a.L - tail;
+    for (int i = block; i < rows; i += blocks) {
+        const long long row = i < head ? i : tail + i - head;
+        for (int o = 0; o < a.outs; ++o) {
+            uint16_t *p = reinterpret_cast<uint16_t *>(a.out[o] + row * a.bytes[o]);
+            for (long long e = threadIdx.x; e < a.bytes[o] / 2; e += blockDim.x) p[e] = 0;
+        }
+        for (int k = 0; k < a.n_parts; ++k)
+            for (long long e = threadIdx.x; e < a.part_row; e += blockDim.x) a.parts[((long long)k * a.L + row) * a.part_row + e] = 0.f;
+    }
+    if (a.end)
+        for (int s = block; s < a.nseq; s += blocks)
+            if (bounds[s] == bounds[s + 1])
+                for (long long e = threadIdx.x; e < a.per; e += blockDim.x) a.end[s * a.per + e] = a.start ? a.start[s * a.per + e] : 0.f;
+}
+__global__ void __launch_bounds__(1024) decay_rest(RestParams a, const int *bounds) {
     pdl_begin();
-    __shared__ int warps[32], carry[2], near_first[1025], near_bounds[1025];   // of up to 1024 sequences: the search below is a chain of reads
+    rest_of(a, bounds, blockIdx.x, gridDim.x);
+}
+
+constexpr int kNear = 1024;                                      // sequences that one pass of a block's scan covers
+// A block for each of `tables` tables, and up to kNear sequences blocks behind them for what these leave over: every block finds all
+// boundaries, and a launch is saved.  Boundaries are taken to 0 ... L and never back, so every segment lies inside the tensors whatever
+// the caller's array holds.
+__global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int L, PlanOut a, PlanOut b, int tables, RestParams rest) {
+    pdl_begin();
+    __shared__ int warps[32], carry[2], near_first[kNear + 1], near_bounds[kNear + 1];   // the search below is a chain of reads
+    const bool plans = blockIdx.x < tables;
     const PlanOut o = blockIdx.x ? b : a;
     const int tid = threadIdx.x;
     auto most = [](int x, int y) { return max(x, y); };
     auto sum = [](int x, int y) { return x + y; };
     auto inside = [&](int i) { return max(0, min(cu[i], L)); };
+    if (rest.status && blockIdx.x == 0 && tid == 0) *rest.status = 0;
     if (tid == 0) {
-        o.first[0] = carry[1] = near_first[0] = 0;
-        o.bounds[0] = carry[0] = near_bounds[0] = inside(0);
+        carry[1] = near_first[0] = 0;
+        carry[0] = near_bounds[0] = inside(0);
+        if (plans) {
+            o.first[0] = 0;
+            o.bounds[0] = carry[0];
+        }
     }
     __syncthreads();
     for (int s0 = 0; s0 < nseq; s0 += 1024) {
         const int s = s0 + tid;
-        const int end = max(carry[0], block_scan(s < nseq ? inside(s + 1) : 0, warps, most, 0));
-        const int start = max(carry[0], block_scan(s < nseq ? inside(s) : 0, warps, most, 0));
+        const int to = s < nseq ? inside(s + 1) : 0, from = s < nseq ? inside(s) : 0;
+        const int end = max(carry[0], block_scan(to, warps, most, 0));
+        const int start = max(carry[0], block_scan(from, warps, most, 0));
         const int upto = carry[1] + block_scan(s < nseq ? (end - start + o.seg - 1) / o.seg : 0, warps, sum, 0);
         if (s < nseq) {
-            o.first[s + 1] = upto;
-            o.bounds[s + 1] = end;
-            if (s < 1024) {
+            if (plans) {
+                o.first[s + 1] = upto;
+                o.bounds[s + 1] = end;
+            }
+            if (s < kNear) {
                 near_first[s + 1] = upto;
                 near_bounds[s + 1] = end;
             }
@@ -94,7 +142,11 @@ __global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int 
         }
         __syncthreads();
     }
-    const int *first = nseq <= 1024 ? near_first : o.first, *bounds = nseq <= 1024 ? near_bounds : o.bounds;
+    if (!plans) {
+        rest_of(rest, near_bounds, blockIdx.x - tables, gridDim.x - tables);
+        return;
+    }
+    const int *first = nseq <= kNear ? near_first : o.first, *bounds = nseq <= kNear ? near_bounds : o.bounds;
     for (int i = tid; i < o.most; i += 1024) {
         int lo = 0, hi = nseq;                                   // the sequence that segment i belongs to: first[lo] <= i < first[lo + 1]
         if (i >= carry[1]) {
@@ -109,38 +161,6 @@ __global__ void __launch_bounds__(1024) decay_plan(const int *cu, int nseq, int 
         const int idx = i - first[lo], t0 = bounds[lo] + idx * o.seg;
         o.table[i] = make_int4(t0, min(o.seg, bounds[lo + 1] - t0), lo, 2 * idx + (t0 + o.seg >= bounds[lo + 1]));
     }
-}
-
-// What packed sequences leave over.  Zeros in the rows of outputs that belong to no sequence, those before the first one and behind
-// the last; and the states of sequences without a token, which stay as they were (start NULL: zeros).
-struct RestParams {
-    int L, nseq, outs;
-    const int *bounds;
-    char *out[6];                                                // outputs and their rows' bytes, even
-    long long bytes[6];
-    float *parts;                                                // n_parts arrays of (L, part_row), or NULL
-    int n_parts;
-    long long part_row;
-    const float *start;
-    float *end;                                                  // (nseq, per), or NULL
-    long long per;
-};
-__global__ void __launch_bounds__(256) decay_rest(RestParams a) {
-    pdl_begin();
-    const int head = a.bounds[0], tail = a.bounds[a.nseq], rows = head + a.L - tail;
-    for (int i = blockIdx.x; i < rows; i += gridDim.x) {
-        const long long row = i < head ? i : tail + i - head;
-        for (int o = 0; o < a.outs; ++o) {
-            uint16_t *p = reinterpret_cast<uint16_t *>(a.out[o] + row * a.bytes[o]);
-            for (long long e = threadIdx.x; e < a.bytes[o] / 2; e += 256) p[e] = 0;
-        }
-        for (int k = 0; k < a.n_parts; ++k)
-            for (long long e = threadIdx.x; e < a.part_row; e += 256) a.parts[((long long)k * a.L + row) * a.part_row + e] = 0.f;
-    }
-    if (a.end)
-        for (int s = blockIdx.x; s < a.nseq; s += gridDim.x)
-            if (a.bounds[s] == a.bounds[s + 1])
-                for (long long e = threadIdx.x; e < a.per; e += 256) a.end[s * a.per + e] = a.start ? a.start[s * a.per + e] : 0.f;
 }
 
 }  // namespace uni

@@ -138,6 +138,7 @@ struct StatesParams {
     const float *init;
     float *fin, *decay;                                          // decay: (segments, H) the segment's whole decay, or NULL
     int *status;
+    int clear;                                                   // the status, by the first block: any wait of another takes far longer to run out
 };
 // The thread's tile stores so far have read their shared memory.
 __device__ __forceinline__ void tma_store_read() {
@@ -157,6 +158,7 @@ inline size_t states_smem(int NT, bool exact) { return (exact ? NT / 64 + 5 : 2 
 template <int NT, bool EXACT> __global__ void __launch_bounds__(kStatesThreads, 2)
 decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
+    if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
     constexpr int kSlabs = NT / 64;
     extern __shared__ __align__(1024) uint8_t dyn[];
     // two stages of k, two of weighted rows, S.  EXACT: one of k, v's rows, two parts, v's rows, S
