@@ -66,6 +66,8 @@ struct Bump {                                                    // the workspac
     }
 };
 
+constexpr int kSms = 148;                                        // of the GPU this is written for
+
 struct Sizes {
     int sequences, H, hk, N, P, lanes_n, lanes_p;                // lanes that share a column when S's rows are kdim, vdim
     long long tokens;
@@ -86,14 +88,13 @@ int walk_rows(int rows, int lanes) {                             // rows a threa
     return n;
 }
 
-int decay_check(const bissd_decay_args *a, bool backward) {
+int decay_check(const bissd_decay_args *a) {
     if (!a) return BISSD_ERR_NULL;
     if (a->batch <= 0 || a->seqlen <= 0 || a->nheads <= 0 || a->nkheads <= 0 || a->nheads % a->nkheads || a->kdim <= 0 || a->kdim > 256 ||
         a->vdim <= 0 || a->vdim > 256 || a->nseq < 0 || (a->nseq > 0 && a->batch != 1))
         return BISSD_ERR_SHAPE;
     if (!dtype_ok(a->dtype) || !dtype_ok(a->g_dtype)) return BISSD_ERR_DTYPE;
     if ((long long)a->batch * a->seqlen > 0x7fffffffLL / 256) return BISSD_ERR_SHAPE;
-    (void)backward;
     return BISSD_OK;
 }
 int decay_pointers(const bissd_decay_args *a, bool backward) {
@@ -131,7 +132,7 @@ uni::Plan plan_of(const bissd_decay_args *a, int seg, Bump &ws, uni::PlanOut *ou
 int walk_segment(const bissd_decay_args *a, const Sizes &z) {
     if (a->nseq > 0) return 256;
     const long long blocks = (long long)a->batch * z.H * ceil_div(z.P * z.lanes_n, uni::kWalkThreads);
-    const long long parts = std::max<long long>(1, 4 * 148 / blocks);
+    const long long parts = std::max<long long>(1, 4 * kSms / blocks);
     const int seg = ceil_div((int)((a->seqlen + parts - 1) / parts), 64) * 64;
     return a->seqlen <= 3 * 64 && parts > 1 ? 3 * 64 : seg;
 }
@@ -169,10 +170,10 @@ struct Rest {
         if (a->nseq == 0) return BISSD_OK;
         p.L = a->seqlen; p.nseq = a->nseq;
         p.per = (long long)a->nheads * a->kdim * a->vdim;
-        const int tables = y ? 2 : 1, others = a->nseq <= uni::kNear ? 148 : 0;
+        const int tables = y ? 2 : 1, others = a->nseq <= uni::kNear ? kSms : 0;
         BISSD_LAUNCH("decay_plan", launch_pdl(uni::decay_plan, tables + others, 1024, 0, s, a->cu_seqlens, (int)a->nseq, (int)a->seqlen, x, y ? *y : x,
                                               tables, p));
-        if (!others) BISSD_LAUNCH("decay_rest", launch_pdl(uni::decay_rest, 148, 1024, 0, s, p, (const int *)x.bounds));
+        if (!others) BISSD_LAUNCH("decay_rest", launch_pdl(uni::decay_rest, kSms, 1024, 0, s, p, (const int *)x.bounds));
         return BISSD_OK;
     }
 };
@@ -347,18 +348,19 @@ struct TcSpace {
 
 // Tokens to a segment of the walk over the chunks, a block for each (segment, head, 64 columns), two blocks an SM.  A walk in pieces
 // needs each piece's own sum first and a chain over them, so it pays where rows are long and heads few; packed sequences are taken
-// to be up to three times as long as their mean.  us, measured: a step of the walk 2.1, of one for exact states 3.3, a block's start 6, a
-// chain 6 (3 rows of 8 chunks, 32 blocks each: 62 in two pieces, 22 in one).
+// to be up to three times as long as their mean.  us, measured: a step of the walk 2.2, of one for exact states 2.6, a block's start 6, a
+// chain 6 (3 rows of 8 chunks, 32 blocks each: 62 in two pieces, 22 in one; 512 chunks of 32 heads: 277 in 9 pieces, 1130 in one by
+// these figures).
 int tc_segment(const bissd_decay_args *a, int PB) {
     const int chunks = ceil_div(a->seqlen, unitc::kQ);
-    const double heads = (double)a->nheads * PB, work = (double)a->batch * chunks * heads / (2 * 148);
+    const double heads = (double)a->nheads * PB, work = (double)a->batch * chunks * heads / (2 * kSms);
     const int longest = a->nseq > 0 ? std::min(chunks, ceil_div(3 * chunks, a->nseq)) : chunks;
     int best = chunks;
-    double least = std::max<double>(longest, work) * 2.1 + 6;
+    double least = std::max<double>(longest, work) * 2.2 + 6;
     for (int parts = 2; parts <= std::min(longest / 4, 128); ++parts) {
         const int steps = ceil_div(longest, parts);
-        const double segments = ((double)a->batch * ceil_div(chunks, steps) + a->nseq) * heads, rounds = std::ceil(segments / (2 * 148));
-        const double time = rounds * (steps * (2.1 + 3.3) + 2 * 6) + 6 + segments * a->kdim * unitc::kP * 12 / 5e6;   // a chain moves 12 bytes a value
+        const double segments = ((double)a->batch * ceil_div(chunks, steps) + a->nseq) * heads, rounds = std::ceil(segments / (2 * kSms));
+        const double time = rounds * (steps * (2.2 + 2.6) + 2 * 6) + 6 + segments * a->kdim * unitc::kP * 12 / 5e6;   // a chain moves 12 bytes a value
         if (time < least) {
             least = time;
             best = steps;
@@ -453,7 +455,7 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
     // blocks a (chunk, head of q): as many as fill two blocks an SM, in the fewest rounds
     const int tiles_v = a->nheads / a->nkheads * t.PB;
-    const long long items = (long long)t.chunk.most * a->nkheads, slots = 2 * 148;
+    const long long items = (long long)t.chunk.most * a->nkheads, slots = 2 * kSms;
     double best = 0;
     for (int parts = 1; parts <= tiles_v; ++parts) {
         const int vpc = ceil_div(tiles_v, parts);
@@ -490,13 +492,13 @@ TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
         g.gdecay = ws.take<float>((size_t)g.t.seg.most * a->nheads);
     }
     // Heads that share q and k are walked by one block, or by several: what takes the fewest rounds of one block an SM, a block's start
-    // being worth 1.5 tiles (of 5 us), and the parts of dq and dk 16 bytes a value at 5 TB/s.
+    // being worth 1.5 tiles (of 6 us), and the parts of dq and dk 16 bytes a value at 5 TB/s.
     const int R = a->nheads / a->nkheads;
     const long long items = (long long)g.t.chunk.most * a->nkheads;
     double best = 0;
     for (int parts = 1; parts <= R; ++parts) {
         const int heads = ceil_div(R, parts), real = ceil_div(R, heads);
-        const double rounds = (double)((items * real + 147) / 148), sums = real > 1 ? 16.0 * real * tokens * a->nkheads * a->kdim / 25e6 : 0;
+        const double rounds = (double)((items * real + kSms - 1) / kSms), sums = real > 1 ? 16.0 * real * tokens * a->nkheads * a->kdim / 30e6 : 0;
         const double time = rounds * (heads * g.t.PB + 1.5) + sums;
         if (parts == 1 || time < best) {
             best = time;
@@ -567,7 +569,7 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
 extern "C" {
 
 int bissd_decay_saved_bytes(const bissd_decay_args *a, size_t *bytes) {
-    const int rc = decay_check(a, false);
+    const int rc = decay_check(a);
     if (rc != BISSD_OK) return rc;
     if (!bytes) return BISSD_ERR_NULL;
     *bytes = 0;
@@ -579,7 +581,7 @@ int bissd_decay_saved_bytes(const bissd_decay_args *a, size_t *bytes) {
 }
 
 int bissd_decay_workspace_bytes(const bissd_decay_args *a, size_t *fwd_bytes, size_t *bwd_bytes) {
-    const int rc = decay_check(a, false);
+    const int rc = decay_check(a);
     if (rc != BISSD_OK) return rc;
     if (fwd_bytes) {
         Bump b{nullptr}, c{nullptr};                              // which of the two runs is known at the call
