@@ -320,13 +320,12 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
 
 using tc::make_map2;
 using tc::make_map4;
-using unitc::bf16;
 
 // ---- on the tensor cores ----------------------------------------------------------------------------------------------
 
-// bf16 with head sizes and rows that 16-byte loads fit, a positive scale (it is added to the decays' logarithms).
+// 16-bit types with head sizes and rows that 16-byte loads fit, a positive scale (it is added to the decays' logarithms).
 bool tc_sizes(const bissd_decay_args *a) {
-    return a->dtype == BISSD_BF16 && a->kdim % 8 == 0 && a->kdim <= 128 && a->vdim % 8 == 0 && a->scale > 0.f && std::isfinite(a->scale);
+    return a->dtype != BISSD_F32 && a->kdim % 8 == 0 && a->kdim <= 128 && a->vdim % 8 == 0 && a->scale > 0.f && std::isfinite(a->scale);
 }
 bool tc_tensor(const bissd_tensor &t, long long batch, long long seq, long long heads) {
     auto fits = [](long long stride, long long n) { return n == 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38)); };
@@ -342,7 +341,7 @@ struct TcSpace {
     uni::Plan seg, chunk;
     uni::PlanOut seg_table{}, chunk_table{};
     bool split;                                                  // sequences in several segments, or packed
-    bf16 *tiles;
+    uint16_t *tiles;                                              // states as 16-bit tiles
     float *states, *decay;
 };
 
@@ -376,7 +375,7 @@ TcSpace tc_space(const bissd_decay_args *a, Bump &ws, bool backward) {
     t.chunk = plan_of(a, unitc::kQ, ws, &t.chunk_table);
     t.seg = plan_of(a, tc_segment(a, t.PB), ws, &t.seg_table);
     t.split = t.seg.per_seq > 1;
-    t.tiles = a->saved ? static_cast<bf16 *>(a->saved) : ws.take<bf16>(tc_tile_values(a, t));
+    t.tiles = a->saved ? static_cast<uint16_t *>(a->saved) : ws.take<uint16_t>(tc_tile_values(a, t));
     if (t.split && !(a->saved && backward)) {
         t.states = ws.take<float>((size_t)t.seg.most * a->nheads * a->kdim * a->vdim);
         t.decay = ws.take<float>((size_t)t.seg.most * a->nheads);
@@ -393,11 +392,20 @@ unitc::Heads tc_heads(const bissd_decay_args *a, int PB) {
 }
 bool tc_map(CUtensorMap *m, const bissd_decay_args *a, const bissd_tensor &t, int inner, int heads) {
     auto bytes = [](long long stride, int n) { return n == 1 ? 16ULL : (unsigned long long)stride * 2; };
-    return make_map4(m, BISSD_BF16, t.ptr, {(unsigned long long)inner, (unsigned long long)heads, (unsigned long long)a->seqlen, (unsigned long long)a->batch},
+    return make_map4(m, a->dtype, t.ptr, {(unsigned long long)inner, (unsigned long long)heads, (unsigned long long)a->seqlen, (unsigned long long)a->batch},
                      {bytes(t.stride_head, heads), bytes(t.stride_seq, a->seqlen), bytes(t.stride_batch, a->batch)}, {64, 1, unitc::kQ, 1});
 }
 
-// The states that enter the chunks (or the gradients, backwards), as bf16 tiles; those that enter and leave the sequences in fp32.
+template <class T> auto states_kernel(int NT, bool exact) {
+    return NT == 64 ? (exact ? unitc::decay_states<T, 64, true> : unitc::decay_states<T, 64, false>)
+                    : (exact ? unitc::decay_states<T, 128, true> : unitc::decay_states<T, 128, false>);
+}
+template <class T> auto chunks_kernel(int NT) { return NT == 64 ? unitc::decay_chunks<T, 64> : unitc::decay_chunks<T, 128>; }
+template <class T> auto grads_kernel(int NT, bool dg) {
+    return NT == 64 ? (dg ? unitc::decay_grads<T, 64, true> : unitc::decay_grads<T, 64, false>)
+                    : (dg ? unitc::decay_grads<T, 128, true> : unitc::decay_grads<T, 128, false>);
+}
+// The states that enter the chunks (or the gradients, backwards), as 16-bit tiles; those that enter and leave the sequences in fp32.
 int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &cols, const CUtensorMap &tiles, bool reverse,
               const float *start, float *end, float *states, float *decay, int *status, bool clear, cudaStream_t s) {
     unitc::StatesParams p{};
@@ -407,8 +415,7 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
     const long long grid = (long long)t.seg.most * a->nheads * t.PB;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     auto launch = [&](const char *name, bool exact) -> int {
-        const auto kernel = t.NT == 64 ? (exact ? unitc::decay_states<64, true> : unitc::decay_states<64, false>)
-                                       : (exact ? unitc::decay_states<128, true> : unitc::decay_states<128, false>);
+        const auto kernel = a->dtype == BISSD_BF16 ? states_kernel<__nv_bfloat16>(t.NT, exact) : states_kernel<__half>(t.NT, exact);
         const size_t smem = unitc::states_smem(t.NT, exact);
         BISSD_ALLOW(kernel, smem);
         BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, cols, tiles));
@@ -429,8 +436,8 @@ int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &ro
     p.tiles = 1;
     return launch("decay_states", !t.split && end != nullptr);
 }
-bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, const bf16 *tiles) {
-    return make_map2(m, BISSD_BF16, tiles, unitc::kP, (unsigned long long)t.chunk.most * a->nheads * t.PB * t.NT, unitc::kP, t.NT);
+bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, const uint16_t *tiles) {
+    return make_map2(m, a->dtype, tiles, unitc::kP, (unsigned long long)t.chunk.most * a->nheads * t.PB * t.NT, unitc::kP, t.NT);
 }
 
 constexpr double kChunkStart = 2.0;                              // a block's start and the product q.k, in tiles of v
@@ -452,7 +459,7 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, a->nseq == 0, s));
     unitc::ChunksParams p{};
     p.h = tc_heads(a, t.PB);
-    p.chunk = t.chunk; p.o = static_cast<bf16 *>(a->o); p.status = status;
+    p.chunk = t.chunk; p.o = a->o; p.status = status;
     // blocks a (chunk, head of q): as many as fill two blocks an SM, in the fewest rounds
     const int tiles_v = a->nheads / a->nkheads * t.PB;
     const long long items = (long long)t.chunk.most * a->nkheads, slots = 2 * kSms;
@@ -466,7 +473,7 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
         }
     }
     p.parts = ceil_div(tiles_v, p.vpc);
-    const auto kernel = t.NT == 64 ? unitc::decay_chunks<64> : unitc::decay_chunks<128>;
+    const auto kernel = a->dtype == BISSD_BF16 ? chunks_kernel<__nv_bfloat16>(t.NT) : chunks_kernel<__half>(t.NT);
     const size_t smem = unitc::chunks_smem(t.NT);
     const long long grid = (long long)t.chunk.most * a->nkheads * p.parts;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
@@ -477,7 +484,7 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
 
 struct TcGradSpace {
     TcSpace t;
-    bf16 *grads;                                                 // tiles of the states' gradients
+    uint16_t *grads;                                                 // tiles of the states' gradients
     float *gstates, *gdecay;
     int vpc, parts;
     float *part, *dg_tokens;
@@ -486,7 +493,7 @@ TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
     TcGradSpace g{};
     g.t = tc_space(a, ws, true);
     const long long tokens = (long long)a->batch * a->seqlen;
-    g.grads = ws.take<bf16>(tc_tile_values(a, g.t));
+    g.grads = ws.take<uint16_t>(tc_tile_values(a, g.t));
     if (g.t.split) {
         g.gstates = ws.take<float>((size_t)g.t.seg.most * a->nheads * a->kdim * a->vdim);
         g.gdecay = ws.take<float>((size_t)g.t.seg.most * a->nheads);
@@ -541,13 +548,13 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     unitc::GradsParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.vpc = g.vpc; p.parts = g.parts;
-    p.dq = static_cast<bf16 *>(a->dq); p.dk = static_cast<bf16 *>(a->dk); p.dv = static_cast<bf16 *>(a->dv);
+    p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
     p.part = g.part; p.tokens = (long long)a->batch * a->seqlen;
     p.dg = a->dg ? (a->g_per_head ? g.dg_tokens : a->dg) : nullptr;
     p.dg_dtype = a->g_per_head ? BISSD_F32 : a->g_dtype;
     p.status = status;
-    const auto kernel = t.NT == 64 ? (p.dg ? unitc::decay_grads<64, true> : unitc::decay_grads<64, false>)
-                                   : (p.dg ? unitc::decay_grads<128, true> : unitc::decay_grads<128, false>);
+    const bool dg = p.dg != nullptr;
+    const auto kernel = a->dtype == BISSD_BF16 ? grads_kernel<__nv_bfloat16>(t.NT, dg) : grads_kernel<__half>(t.NT, dg);
     const size_t smem = unitc::grads_smem(t.NT);
     const long long grid = (long long)t.chunk.most * a->nkheads * p.parts;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
@@ -555,8 +562,15 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     BISSD_LAUNCH("decay_grads", launch_pdl(kernel, (int)grid, 512, smem, s, p, q, k, v, dout, tiles, grads));
     if (g.parts > 1) {
         const long long each = p.tokens * a->nkheads * a->kdim;
-        BISSD_LAUNCH("decay_sum_parts", launch_pdl(unitc::decay_sum_parts, (int)((2 * each / 4 + 255) / 256), 256, 0, s, (const float *)g.part, g.parts, each,
-                                                   p.dq, p.dk));
+        const int blocks = (int)((2 * each / 4 + 255) / 256);
+        const int rc = by_dtype(a->dtype, [&](auto x) -> int {
+            using T = decltype(x);
+            if constexpr (sizeof(T) == 2)
+                BISSD_LAUNCH("decay_sum_parts", launch_pdl(unitc::decay_sum_parts<T>, blocks, 256, 0, s, (const float *)g.part, g.parts, each,
+                                                           static_cast<T *>(a->dq), static_cast<T *>(a->dk)));
+            return BISSD_OK;
+        });
+        if (rc != BISSD_OK) return rc;
     }
     if (a->dg && a->g_per_head)
         BISSD_LAUNCH("decay_dg_heads", launch_pdl(uni::decay_dg_heads, (int)a->nheads, 1024, 0, s, (const float *)g.dg_tokens, p.tokens, (int)a->nheads, a->dg,
@@ -575,7 +589,7 @@ int bissd_decay_saved_bytes(const bissd_decay_args *a, size_t *bytes) {
     *bytes = 0;
     if (tc_sizes(a)) {                                           // the states that enter the chunks
         Bump b{nullptr};
-        *bytes = align256(tc_tile_values(a, tc_space(a, b, false)) * sizeof(bf16));
+        *bytes = align256(tc_tile_values(a, tc_space(a, b, false)) * sizeof(uint16_t));
     }
     return BISSD_OK;
 }

@@ -1,4 +1,4 @@
-// The causal decay attention on the tensor cores (bf16), in chunks of 128 tokens.  With c_t the sum of the chunk's log decays up to
+// The causal decay attention on the tensor cores (bf16 or fp16: T), in chunks of 128 tokens.  With c_t the sum of the chunk's log decays up to
 // and with token t, and S the state that enters the chunk,
 //     o_t = scale [ e^{c_t} S^T q_t + sum_{s <= t} e^{c_t - c_s} (q_t.k_s) v_s ],    S' = e^{c_end} S + sum_s k_s (e^{c_end - c_s} v_s)^T
 // so a chunk is four products of 128 rows; only S' waits for the chunk before it.
@@ -19,7 +19,6 @@ namespace unitc {
 using namespace tc;
 using uni::Plan;
 using uni::Segment;
-typedef __nv_bfloat16 bf16;
 
 constexpr int kQ = 128;                                          // tokens a chunk
 constexpr int kP = 64;                                           // columns of v a tile
@@ -50,9 +49,13 @@ struct Decays {
             }
         }
     }
-    __device__ __forceinline__ void log2(const Heads &a) {       // bf16 or fp32
+    __device__ __forceinline__ void log2(const Heads &a) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = fmaxf(__uint_as_float(a.g_dtype == BISSD_F32 ? raw[i] : raw[i] << 16) * 1.44269504f, -200.f);
+        for (int i = 0; i < 4; ++i) {
+            const float g = a.g_dtype == BISSD_F16 ? __half2float(__ushort_as_half((unsigned short)raw[i]))
+                                                   : __uint_as_float(a.g_dtype == BISSD_F32 ? raw[i] : raw[i] << 16);
+            v[i] = fmaxf(g * 1.44269504f, -200.f);
+        }
     }
     // Sums up to and with each token.
     __device__ __forceinline__ void prefix(float (&c)[4], int lane) const {
@@ -95,24 +98,26 @@ __device__ __forceinline__ void clear_rows(uint8_t *slab, int from, int tid, int
     for (int i = from * 8 + tid; i < kQ * 8; i += threads) *reinterpret_cast<uint4 *>(slab + i * 16) = zero8();
 }
 
-// A weight f as bf16 f1 + f2, and eight bf16 values times it in one rounding: v f1 + (v f2) as a multiply-add.
-__device__ __forceinline__ uint32_t halves(float f) {
-    const float hi = __bfloat162float(__float2bfloat16_rn(f));
-    return pack2<bf16>(hi, f - hi);
+// A weight f as f1 + f2 of type T, and eight values of T times it in one rounding: v f1 + (v f2) as a multiply-add.
+template <class T> struct PairOf;
+template <> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct PairOf<__half> { using type = __half2; };
+template <class T> __device__ __forceinline__ uint32_t halves(float f) {
+    const float hi = to_f<T>(from_f<T>(f));
+    return pack2<T>(hi, f - hi);
 }
-__device__ __forceinline__ uint4 weighted(const uint4 &row, uint32_t f) {
+template <class T> __device__ __forceinline__ uint4 weighted(const uint4 &row, uint32_t f) {
+    using T2 = typename PairOf<T>::type;
     const uint32_t f1 = __byte_perm(f, f, 0x1010), f2 = __byte_perm(f, f, 0x3232);
     uint32_t e[4] = {row.x, row.y, row.z, row.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&e[q]);
-        const __nv_bfloat162 o = __hfma2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f1),
-                                         __hmul2(v, *reinterpret_cast<const __nv_bfloat162 *>(&f2)));
+        const T2 v = *reinterpret_cast<const T2 *>(&e[q]);
+        const T2 o = __hfma2(v, *reinterpret_cast<const T2 *>(&f1), __hmul2(v, *reinterpret_cast<const T2 *>(&f2)));
         e[q] = *reinterpret_cast<const uint32_t *>(&o);
     }
     return make_uint4(e[0], e[1], e[2], e[3]);
 }
-
 __device__ __forceinline__ float both(vec::f2 v) {
     float a, b;
     vec::unpack(v, a, b);
@@ -125,11 +130,13 @@ __device__ __forceinline__ float both(vec::f2 v) {
 // registers (a row n and 32 columns a thread).  k's and v's rows come by TMA a chunk ahead.  Eight warps weight v's in place and keep S;
 // the ninth issues loads and MMAs, the tenth makes the weights and stores the tiles, and they meet at mbarriers alone: a step is S's
 // way to shared memory, one product's latency, its way back and the weighting.  (The weighting in the product's shadow, from rows
-// loaded to registers, made it longer: the loads from tensor memory then waited for those rows.)  Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
-// EXACT: the weighted row is given to the tensor cores in three bf16 parts, each what is left of those before, so that the states
-// that leave the library are fp32's.  The tiles that the other kernels read are bf16 in any case: they meet bf16 factors.  The parts
+// loaded to registers, made it longer: the loads from tensor memory then waited for those rows.)
+// Two blocks an SM, to the byte: the barriers lie behind the tiles, and there is no other shared memory.
+// EXACT: the weighted row is given to the tensor cores in three 16-bit parts, each what is left of those before, so that the states
+// that leave the library are fp32's.  The tiles that the other kernels read are 16-bit in any case: they meet 16-bit factors.  The parts
 // lie side by side and take one product of 192 columns, which reads k once, and meet again as three sums: shared memory bounds this
-// (as three products of 64 columns, in two rounds, 190 us for 142: 512 chunks of 32 heads, 128 x 64 states).  The third part goes
+// (as three products of 64 columns, in two rounds, 190 us for 142: 512 chunks of 32 heads, 128 x 64 states, sums alone; the walk
+// proper, not EXACT, takes 124 for 0.54 GB).  The third part goes
 // where v's rows came, in front of the others or behind them in turn, and k has one buffer: its next rows come while v's are weighted.
 struct StatesParams {
     Heads h;
@@ -155,7 +162,7 @@ struct StatesShared {
 constexpr int kStatesThreads = 320;
 inline size_t states_smem(int NT, bool exact) { return (exact ? NT / 64 + 5 : 2 * (NT / 64) + 3) * (size_t)kSlab + sizeof(StatesShared); }
 
-template <int NT, bool EXACT> __global__ void __launch_bounds__(kStatesThreads, 2)
+template <class T, int NT, bool EXACT> __global__ void __launch_bounds__(kStatesThreads, 2)
 decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
     if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
@@ -214,7 +221,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             load(0);
             for (int i = 0; i < loads_v; ++i) load_v(i);
         }
-        constexpr uint32_t idesc = instr_desc(1, true, true, EXACT ? 3 * kP : kP);
+        constexpr uint32_t idesc = instr_desc(AbFmt<T>::v, true, true, EXACT ? 3 * kP : kP);
         for (int i = 0; i < nc && ok; ++i) {
             const int st = EXACT ? 0 : i & 1;
             if (!EXACT && i + 1 < nc) {                          // the stage was read by the MMAs of the step before
@@ -273,7 +280,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float v = exp2f(a.reverse ? c[k] + a.h.log_scale : c[k]);
-                f[k] = EXACT ? __float_as_uint(v) : halves(v);
+                f[k] = EXACT ? __float_as_uint(v) : halves<T>(v);
             }
         };
         auto give = [&](int i) {                                 // to the others, as chunk i's
@@ -309,14 +316,15 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         __syncwarp();
     } else {
         const uint32_t swz = (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);   // the thread's piece of a tile, + 4096 k
-        auto weigh = [&](uint8_t *v, int len) {                  // bf16 rows times f1 + f2, in their place
+        auto weigh = [&](uint8_t *v, int len) {                  // rows times f1 + f2, in their place
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint4 row = weighted(*reinterpret_cast<const uint4 *>(v + swz + k * 4096), sh.w[(tid >> 3) + k * 32]);
+                const uint4 row = weighted<T>(*reinterpret_cast<const uint4 *>(v + swz + k * 4096), sh.w[(tid >> 3) + k * 32]);
                 // rows behind the sequence's end may be of another, and no numbers
                 *reinterpret_cast<uint4 *>(v + swz + k * 4096) = (tid >> 3) + k * 32 < len ? row : zero8();
             }
         };
+        constexpr float kUp = std::is_same<T, __half>::value ? 2048.f : 1.f;   // fp16: keeps the second and third part out of its small numbers
         auto parts = [&](int i, int len) {                       // chunk i's weighted rows: the third part in their place
             uint8_t *third = smV + (i & 1) * 3 * kSlab + swz, *first = smV + kSlab + swz;
 #pragma unroll
@@ -327,16 +335,16 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     float x, y, hx, hy;
-                    unpack2<bf16>(e[q], x, y);
+                    unpack2<T>(e[q], x, y);
                     x *= f;
                     y *= f;
-                    o1[q] = pack2<bf16>(x, y);
-                    unpack2<bf16>(o1[q], hx, hy);
-                    x -= hx;
-                    y -= hy;
-                    o2[q] = pack2<bf16>(x, y);
-                    unpack2<bf16>(o2[q], hx, hy);
-                    e[q] = pack2<bf16>(x - hx, y - hy);
+                    o1[q] = pack2<T>(x, y);
+                    unpack2<T>(o1[q], hx, hy);
+                    x = (x - hx) * kUp;
+                    y = (y - hy) * kUp;
+                    o2[q] = pack2<T>(x, y);
+                    unpack2<T>(o2[q], hx, hy);
+                    e[q] = pack2<T>((x - hx) * kUp, (y - hy) * kUp);
                 }
                 *reinterpret_cast<uint4 *>(first + k * 4096) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
                 *reinterpret_cast<uint4 *>(first + kSlab + k * 4096) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
@@ -380,7 +388,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float e[8] = {S[8 * j], S[8 * j + 1], S[8 * j + 2], S[8 * j + 3], S[8 * j + 4], S[8 * j + 5], S[8 * j + 6], S[8 * j + 7]};
-                        *reinterpret_cast<uint4 *>(smS + n * 128 + (((half * 4 + j) ^ (n & 7)) << 4)) = pack8<bf16>(e);
+                        *reinterpret_cast<uint4 *>(smS + n * 128 + (((half * 4 + j) ^ (n & 7)) << 4)) = pack8<T>(e);
                     }
                 }
             }
@@ -397,15 +405,16 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
             for (int j0 = 0; j0 < 32; j0 += 16) {
                 float x[16];
                 tmem_ld16(tl + j0, x);
+                if constexpr (EXACT) {                           // the buffer that comes first or last has the third part
+                    float y[16], z[16];
+                    tmem_ld16(tl + kP + j0, y);
+                    tmem_ld16(tl + 2 * kP + j0, z);
+                    const float fx = st ? 1.f : 1.f / (kUp * kUp), fy = st ? 1.f / kUp : 1.f, fz = st ? 1.f / (kUp * kUp) : 1.f / kUp;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, x[j]);
-                if constexpr (EXACT) {
-                    tmem_ld16(tl + kP + j0, x);
+                    for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, kUp == 1.f ? x[j] + (y[j] + z[j]) : fmaf(x[j], fx, fmaf(y[j], fy, z[j] * fz)));
+                } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) S[j0 + j] += x[j];
-                    tmem_ld16(tl + 2 * kP + j0, x);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) S[j0 + j] += x[j];
+                    for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(S[j0 + j], now, x[j]);
                 }
             }
             if constexpr (!EXACT)
@@ -424,22 +433,24 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 
 // ---- the outputs -----------------------------------------------------------------------------------------------------
 // A block has one chunk of one head of q and k, and walks `vpc` of the tiles of v that share them: Q, K and their product stay, in
-// shared and tensor memory, and per tile come v's rows and the state.  The product, weighted by the decays and rounded to bf16 (it
-// meets v's bf16), takes K's place in shared memory.  Where a block of 32 x 32 lies below the diagonal, the weight is a row factor times a
+// shared and tensor memory, and per tile come v's rows and the state.  The product, weighted by the decays and rounded to T (it
+// meets v's T), takes K's place in shared memory.  Where a block of 32 x 32 lies below the diagonal, the weight is a row factor times a
 // column factor, both counted from the block's last column and at most 1; on the diagonal it is one 2^x an element.  A warp has
 // 32 rows and half of the columns up to the diagonal, in units of 16.
-// Two blocks an SM: one's loads and element-wise work run under the other's MMAs.
+// Two blocks an SM: one's loads and element-wise work run under the other's MMAs.  Bound by memory where rows are long: 512 chunks of
+// 32 heads, 128 x 64 states, 1.05 GB in 210 us (4.8 TB/s).  Stores from registers, without the way through shared memory, took 244
+// us, 512 threads a block 264.
 struct ChunksParams {
     Heads h;
     Plan chunk;
     int vpc, parts;                                              // tiles of v a block, blocks a (chunk, head of q)
     int tiles_rows;                                              // NT
-    bf16 *o;                                                     // (tokens, H, P) contiguous
+    void *o;                                                     // (tokens, H, P) contiguous
     int *status;
 };
 inline size_t chunks_smem(int NT) { return 1024 + (size_t)(NT / 64) * kSlab + 2 * (size_t)kSlab + (size_t)kSlab + (size_t)NT * 128; }
 
-template <int NT> __global__ void __launch_bounds__(256, 2)
+template <class T, int NT> __global__ void __launch_bounds__(256, 2)
 decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
              const __grid_constant__ CUtensorMap tmS) {
     pdl_begin();
@@ -505,7 +516,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     if (warp == 0 && elect_one()) {
         ok = mbar_wait(&bar_qk, 0);
         if (ok) {
-            constexpr uint32_t idesc = instr_desc(1, false, false, kQ);
+            constexpr uint32_t idesc = instr_desc(AbFmt<T>::v, false, false, kQ);
 #pragma unroll 1
             for (int kk = 0; kk < NT / 16; ++kk)
                 umma(tmem, smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
@@ -523,7 +534,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     if (ok && half == 1)
         for (int u = 2 * (r32 + 1); u < 8; ++u)                  // above the diagonal
             for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4 *>(pair_at(u) + piece(u, j)) = zero8();
-    bf16 *out = a.o + ((long long)s.batch * a.chunk.L + s.t0 + (tid >> 3)) * a.h.H * a.h.P;   // the first of the rows this thread writes
+    T *out = static_cast<T *>(a.o) + ((long long)s.batch * a.chunk.L + s.t0 + (tid >> 3)) * a.h.H * a.h.P;   // the first of the rows this thread writes
     const long long row32 = 32LL * a.h.H * a.h.P;
     for (int i = 0; i < nv && ok; ++i) {
         const int k = h - h0, h1 = h + (pb + 1 == a.h.PB), pb1 = pb + 1 == a.h.PB ? 0 : pb + 1;   // and the next tile's
@@ -537,7 +548,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
             ok = mbar_wait(&bar_s, i & 1);
             if (ok) {
                 tc_fence_after();
-                constexpr uint32_t idesc = instr_desc(1, false, true, kP);
+                constexpr uint32_t idesc = instr_desc(AbFmt<T>::v, false, true, kP);
 #pragma unroll 1
                 for (int kk = 0; kk < NT / 16; ++kk)
                     umma(tmem + 192, smem_desc(smem_u32(smQ + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
@@ -581,8 +592,8 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     uint4 o;
-                    o.x = vec::narrow<bf16>(x[4 * j]); o.y = vec::narrow<bf16>(x[4 * j + 1]);
-                    o.z = vec::narrow<bf16>(x[4 * j + 2]); o.w = vec::narrow<bf16>(x[4 * j + 3]);
+                    o.x = vec::narrow<T>(x[4 * j]); o.y = vec::narrow<T>(x[4 * j + 1]);
+                    o.z = vec::narrow<T>(x[4 * j + 2]); o.w = vec::narrow<T>(x[4 * j + 3]);
                     *reinterpret_cast<uint4 *>(pair_at(u) + piece(u, j)) = o;
                 }
             }
@@ -601,7 +612,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
             ok = mbar_wait(&bar_v, i & 1);
             if (ok) {
                 tc_fence_after();
-                constexpr uint32_t idesc = instr_desc(1, false, true, kP);
+                constexpr uint32_t idesc = instr_desc(AbFmt<T>::v, false, true, kP);
 #pragma unroll 1
                 for (int kk = 0; kk < kQ / 16; ++kk)
                     umma(tmem + 128, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
@@ -631,7 +642,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                 float e[8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) e[q] = fmaf(y[j + q], f, x[j + q]);
-                *reinterpret_cast<uint4 *>(smK + t * 128 + (((half * 4 + (j >> 3)) ^ (t & 7)) << 4)) = pack8<bf16>(e);
+                *reinterpret_cast<uint4 *>(smK + t * 128 + (((half * 4 + (j >> 3)) ^ (t & 7)) << 4)) = pack8<T>(e);
             }
         }
         tc_fence_before();
@@ -639,7 +650,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         if (!ok) break;
         const int col = pb * kP + (tid & 7) * 8;
         if (col < a.h.P) {
-            bf16 *o = out + h * a.h.P + col;
+            T *o = out + h * a.h.P + col;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int r = (tid >> 3) + q * 32;
@@ -679,12 +690,14 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
 // read the other way.  p goes back to tensor memory, d to shared memory.  A block has a chunk and a head of q and k, and walks (its
 // part of) the heads of v that share them, dq and dk adding up in tensor memory; v and do come a tile ahead, the states while the pairs
 // are weighted, and the products of d run under the next tile's first ones, when nobody waits for them.  Ten of the sixteen warps have weights to make, six lie above the
-// diagonal; one of these makes the next head's tables, one sums dg.
+// diagonal: one of these makes the next head's tables, one sums dg, one issues the products, and together they weight v.  A tile's
+// products (3300 cycles, most from shared memory) and its arithmetic (7000) take turns: 128 chunks of 24 heads, 128 x 64 states, 161 us on 128
+// SMs.  The loops of products are not unrolled: a shorter body ran 180 -> 170 us.
 struct GradsParams {
     Heads h;
     Plan chunk;
     int vpc, parts;                                              // tiles of v a block (whole heads), blocks a (chunk, head of q)
-    bf16 *dq, *dk, *dv;                                          // contiguous
+    void *dq, *dk, *dv;                                          // contiguous
     float *part;                                                 // parts > 1: (2, parts, tokens, hk, N), dq and dk
     long long tokens;
     void *dg;                                                    // DG: (tokens, H)
@@ -712,7 +725,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         : "memory");
 }
 
-template <int NT, bool DG> __global__ void __launch_bounds__(512, 1)
+template <class T, int NT, bool DG> __global__ void __launch_bounds__(512, 1)
 decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmG) {
     pdl_begin();
@@ -765,11 +778,11 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
 #pragma unroll
         for (int k = 0; k < 4; ++k) q[k] = ex2_approx(q[k]);
         four(to.ws, q[0], q[1], q[2], q[3]);
-        *reinterpret_cast<uint4 *>(to.wv + lane * 4) = make_uint4(halves(q[0]), halves(q[1]), halves(q[2]), halves(q[3]));
+        *reinterpret_cast<uint4 *>(to.wv + lane * 4) = make_uint4(halves<T>(q[0]), halves<T>(q[1]), halves<T>(q[2]), halves<T>(q[3]));
 #pragma unroll
         for (int k = 0; k < 4; ++k) p[k] += a.h.log_scale;
         *reinterpret_cast<uint4 *>(to.wd + lane * 4) =
-            make_uint4(halves(ex2_approx(p[0])), halves(ex2_approx(p[1])), halves(ex2_approx(p[2])), halves(ex2_approx(p[3])));
+            make_uint4(halves<T>(ex2_approx(p[0])), halves<T>(ex2_approx(p[1])), halves<T>(ex2_approx(p[2])), halves<T>(ex2_approx(p[3])));
 #pragma unroll
         for (int b = 0; b < 3; ++b)                              // of use in the blocks behind the b-th
             four(to.beside[b], ex2_approx(p[0] - ends[b]), ex2_approx(p[1] - ends[b]), ex2_approx(p[2] - ends[b]), ex2_approx(p[3] - ends[b]));
@@ -802,7 +815,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    // tensor memory: 0 q.k, then p in bf16 (64 columns); 64 dv inside the chunk; 128 do.v, then dv from the future; 192 S^T q; dq; dk
+    // tensor memory: 0 q.k, then p as T (64 columns); 64 dv inside the chunk; 128 do.v, then dv from the future; 192 S^T q; dq; dk
     const uint32_t tmem = tmem_slot, tl = tmem_lane_base(tmem);
     constexpr uint32_t cOwn = 64, cFar = 128, cOut = 192, cQ = 256, cK = 256 + NT;
     int loads_v = nv > 1 ? 2 : 1, loads_s = 1;
@@ -825,7 +838,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     };
     auto put_dv = [&](int i, int h, int pb) {                    // tile i's from v's place
         const uint8_t *from = smV + (i & 1) * kSlab;
-        bf16 *dv = a.dv + (token * a.h.H + h) * a.h.P + pb * kP;
+        T *dv = static_cast<T *>(a.dv) + (token * a.h.H + h) * a.h.P + pb * kP;
         const int row_values = a.h.H * a.h.P;
         pieces([&](int x) {
             const int r = x >> 3, col = (x & 7) * 8;
@@ -835,7 +848,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         });
     };
     auto from_chunk = [&]() {                                    // dq and dk of the chunk's own pairs; one thread
-        constexpr uint32_t iq = instr_desc(1, true, true, NT), ik = instr_desc(1, false, true, NT);
+        constexpr uint32_t iq = instr_desc(AbFmt<T>::v, true, true, NT), ik = instr_desc(AbFmt<T>::v, false, true, NT);
         const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK), n0 = smem_u32(smN);
 #pragma unroll 1
         for (int kk = 0; kk < kQ / 16; ++kk) {
@@ -864,7 +877,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             ok = ok && mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
             if (ok) {
                 tc_fence_after();
-                constexpr uint32_t idesc = instr_desc(1, false, false, kQ);
+                constexpr uint32_t idesc = instr_desc(AbFmt<T>::v, false, false, kQ);
 #pragma unroll 1
                 for (int kk = 0; kk < NT / 16; ++kk)
                     umma(tmem, smem_desc(smem_u32(smK + kk / 4 * kSlab) + kk % 4 * 32, 16, 1024),
@@ -885,7 +898,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         if (ok) ok = mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
         if (ok) {
             pieces([&](int x) {                                  // scale e^{c_t} do_t beside do_t
-                *reinterpret_cast<uint4 *>(smE + x * 16) = weighted(*reinterpret_cast<const uint4 *>(sD + x * 16), tb.wd[x >> 3]);
+                *reinterpret_cast<uint4 *>(smE + x * 16) = weighted<T>(*reinterpret_cast<const uint4 *>(sD + x * 16), tb.wd[x >> 3]);
             });
             ok = mbar_wait(&done_1, i & 1);
         }
@@ -925,10 +938,10 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                         }
                         const vec::f2 x0 = vec::pack(x[j], x[j + 1]), x1 = vec::pack(x[j + 2], x[j + 3]);
                         const vec::f2 y0 = vec::mul2(vec::pack(y[j], y[j + 1]), w0), y1 = vec::mul2(vec::pack(y[j + 2], y[j + 3]), w1);
-                        p[j / 2] = vec::narrow<bf16>(vec::mul2(x0, w0));
-                        p[j / 2 + 1] = vec::narrow<bf16>(vec::mul2(x1, w1));
-                        d[(j - j0) / 2] = vec::narrow<bf16>(y0);
-                        d[(j - j0) / 2 + 1] = vec::narrow<bf16>(y1);
+                        p[j / 2] = vec::narrow<T>(vec::mul2(x0, w0));
+                        p[j / 2 + 1] = vec::narrow<T>(vec::mul2(x1, w1));
+                        d[(j - j0) / 2] = vec::narrow<T>(y0);
+                        d[(j - j0) / 2 + 1] = vec::narrow<T>(y1);
                         if constexpr (DG) {                      // a token's own pair is in its row's and its column's sum
                             const vec::f2 z0 = vec::mul2(x0, y0), z1 = vec::mul2(x1, y1);
                             sum = vec::add2(sum, vec::add2(z0, z1));
@@ -947,7 +960,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 const int light = (quad == 3 ? 3 : quad - 1) + cg;   // of six warps
                 for (int x = light * 32 + lane; x < kQ * 8; x += 6 * 32) {   // e^{c_end - c_s} v_s in v_s' place
                     uint4 *v = reinterpret_cast<uint4 *>(sV + x * 16);
-                    *v = weighted(*v, tb.wv[x >> 3]);
+                    *v = weighted<T>(*v, tb.wv[x >> 3]);
                 }
 #pragma unroll
                 for (int j = 0; j < 16; ++j) p[j] = 0u;
@@ -975,7 +988,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             ok = mbar_wait(&bar_s, i & 1);
             if (ok) {
                 tc_fence_after();
-                constexpr uint32_t narrow = instr_desc(1, false, true, kP), wide = instr_desc(1, false, false, NT);
+                constexpr uint32_t narrow = instr_desc(AbFmt<T>::v, false, true, kP), wide = instr_desc(AbFmt<T>::v, false, false, NT);
                 const uint32_t q0 = smem_u32(smQ), k0 = smem_u32(smK);
                 const uint32_t v_ = smem_u32(sV), d_ = smem_u32(sD), e_ = smem_u32(smE), s_ = smem_u32(smS), g_ = smem_u32(smG);
 #pragma unroll 1
@@ -1002,10 +1015,10 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             if (ok)
                 for (int q = tid; q < NT * 8; q += kT) {
                     const uint4 e = *reinterpret_cast<const uint4 *>(smS + q * 16), f = *reinterpret_cast<const uint4 *>(smG + q * 16);
-                    vec::f2 v = vec::mul2(vec::widen<bf16>(e.x), vec::widen<bf16>(f.x));
-                    v = vec::fma2(vec::widen<bf16>(e.y), vec::widen<bf16>(f.y), v);
-                    v = vec::fma2(vec::widen<bf16>(e.z), vec::widen<bf16>(f.z), v);
-                    through += both(vec::fma2(vec::widen<bf16>(e.w), vec::widen<bf16>(f.w), v));
+                    vec::f2 v = vec::mul2(vec::widen<T>(e.x), vec::widen<T>(f.x));
+                    v = vec::fma2(vec::widen<T>(e.y), vec::widen<T>(f.y), v);
+                    v = vec::fma2(vec::widen<T>(e.z), vec::widen<T>(f.z), v);
+                    through += both(vec::fma2(vec::widen<T>(e.w), vec::widen<T>(f.w), v));
                 }
             whole = tb.whole[0];                         // read here: behind the next barrier its table may be another head's
             if (last) {
@@ -1034,10 +1047,10 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 for (int k = 0; k < 4; ++k) {
                     const vec::f2 far2 = vec::pack(far[j + 2 * k], far[j + 2 * k + 1]);
                     if constexpr (DG) {
-                        f = vec::fma2(vec::widen<bf16>(vs[k]), far2, f);
-                        p = vec::fma2(vec::widen<bf16>(ds[k]), vec::pack(o[j + 2 * k], o[j + 2 * k + 1]), p);
+                        f = vec::fma2(vec::widen<T>(vs[k]), far2, f);
+                        p = vec::fma2(vec::widen<T>(ds[k]), vec::pack(o[j + 2 * k], o[j + 2 * k + 1]), p);
                     }
-                    to[k] = vec::narrow<bf16>(vec::fma2(w, far2, vec::pack(own[j + 2 * k], own[j + 2 * k + 1])));
+                    to[k] = vec::narrow<T>(vec::fma2(w, far2, vec::pack(own[j + 2 * k], own[j + 2 * k + 1])));
                 }
                 *reinterpret_cast<uint4 *>(sV + at) = make_uint4(to[0], to[1], to[2], to[3]);   // dv, where this thread alone has read v
             }
@@ -1111,7 +1124,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
 #pragma unroll
                     for (int j = 0; j < 16; j += 8) {
                         const float e[8] = {x[j], x[j + 1], x[j + 2], x[j + 3], x[j + 4], x[j + 5], x[j + 6], x[j + 7]};
-                        *reinterpret_cast<uint4 *>(to + (n + j) / 64 * kSlab + s * 128 + ((((n + j) % 64 / 8) ^ (s & 7)) << 4)) = pack8<bf16>(e);
+                        *reinterpret_cast<uint4 *>(to + (n + j) / 64 * kSlab + s * 128 + ((((n + j) % 64 / 8) ^ (s & 7)) << 4)) = pack8<T>(e);
                     }
                 }
             }
@@ -1122,7 +1135,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             for (int x = tid; x < 2 * kQ * (NT / 8); x += kT) {
                 const int what = x / (kQ * (NT / 8)), r = x / (NT / 8) % kQ, j = x % (NT / 8);
                 if (r < len && j < pieces)
-                    *reinterpret_cast<uint4 *>((what ? a.dk : a.dq) + ((token + r) * a.h.hk + m) * a.h.N + j * 8) =
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(what ? a.dk : a.dq) + ((token + r) * a.h.hk + m) * a.h.N + j * 8) =
                         *reinterpret_cast<const uint4 *>((what ? smN : smV) + j / 8 * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4));
             }
         }
@@ -1142,7 +1155,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
 }
 
 // dq and dk of chunks whose heads were walked by several blocks: their parts added up in order.
-__global__ void __launch_bounds__(256) decay_sum_parts(const float *part, int parts, long long each, bf16 *dq, bf16 *dk) {
+template <class T> __global__ void __launch_bounds__(256) decay_sum_parts(const float *part, int parts, long long each, T *dq, T *dk) {
     pdl_begin();
     const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= 2 * each) return;
@@ -1154,8 +1167,8 @@ __global__ void __launch_bounds__(256) decay_sum_parts(const float *part, int pa
         v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
     }
     uint2 o;
-    o.x = pack2<bf16>(v.x, v.y);
-    o.y = pack2<bf16>(v.z, v.w);
+    o.x = pack2<T>(v.x, v.y);
+    o.y = pack2<T>(v.z, v.w);
     *reinterpret_cast<uint2 *>((what ? dk : dq) + (i - what * each)) = o;
 }
 

@@ -38,8 +38,13 @@ def decay_attention(q, k, v, g, scale=None, initial_state=None, return_final_sta
         up to cu_seqlens[i + 1], and there are n states.  Sequences may be empty.  Boundaries are taken to 0 ... seqlen and never back;
         tokens of no sequence have zeros for outputs and gradients.
 
-    On the tensor cores (bfloat16, kdim up to 128, head sizes that are multiples of 8, scale > 0) a value of v, or of a gradient, that is
-    not finite reaches all 128 tokens of its chunk of the sequence, also those before it; other sequences never.
+    On the tensor cores (16-bit types, kdim up to 128, head sizes that are multiples of 8, scale > 0) a value of v, or of a gradient, that
+    is not finite reaches all 128 tokens of its chunk of the sequence, also those before it; other sequences never.  The state that
+    enters a chunk of 128 tokens, the products scale * q.k of its pairs and their gradients' like are rounded to the tensors' type on the way: in
+    float16 they must stay below 65504, and gradients lose bits where it has few (below 2^-14).  The states handed in and out are
+    float32 throughout.  How a call is split over the GPU follows its sizes: the last bits of a row may depend on the number of rows.
+
+    A call has at most 2^23 - 1 tokens.
 
     Differentiable once with respect to q, k, v, g and initial_state.  Returns the output (like v), or (output, final states).
     Gradients of one q, k or g that several heads or tokens share are summed in float32 in a fixed order, as everything is.
