@@ -33,14 +33,19 @@ static int block_norm_pair(const bnorm::Params &p, bool backward) { return backw
 static int block_norm_threads(const bnorm::Params &p, bool backward) {
     return p.threads_row * std::max(1, 256 / p.threads_row) / block_norm_pair(p, backward);
 }
-// 16-byte pieces: every row starts at a multiple of 16 bytes
-static bool block_norm_vec(const bissd_block_norm_args *a) {
-    bool ok = a->width % 8 == 0;
-    for (const void *p : {a->x, a->residual, a->gate, (const void *)a->r, (const void *)a->normed, a->dr, a->dnormed, (const void *)a->dx,
-                          (const void *)a->dresidual, (const void *)a->dgate})
-        ok = ok && aligned16(p);
-    for (const int64_t s : {a->stride_x, a->stride_residual, a->stride_gate, a->stride_dr, a->stride_dnormed}) ok = ok && s % 8 == 0;
-    return ok;
+// Channels that lie aligned together in every row: 8 (16 bytes of the narrower type), 2, or 0 where not even pairs do.
+static int block_norm_vec(const bissd_block_norm_args *a) {
+    const size_t es = a->dtype == BISSD_F32 ? 4 : 2, rs = a->r_dtype == BISSD_F32 ? 4 : 2;
+    auto fits = [&](int n) {
+        bool ok = a->width % n == 0;
+        for (const void *p : {a->x, a->gate, (const void *)a->normed, a->dnormed, (const void *)a->dx, (const void *)a->dgate})
+            ok = ok && reinterpret_cast<uintptr_t>(p) % (n == 8 ? 16 : 2 * es) == 0;
+        for (const void *p : {a->residual, (const void *)a->r, a->dr, (const void *)a->dresidual})
+            ok = ok && reinterpret_cast<uintptr_t>(p) % (n == 8 ? 16 : 2 * rs) == 0;
+        for (const int64_t s : {a->stride_x, a->stride_residual, a->stride_gate, a->stride_dr, a->stride_dnormed}) ok = ok && s % n == 0;
+        return ok;
+    };
+    return fits(8) ? 8 : fits(2) ? 2 : 0;
 }
 static long long block_norm_entries(const bnorm::Params &p) { return p.gate && p.gate_rows > 0 ? p.rows / p.gate_rows : 1; }
 static bnorm::Params block_norm_params(const bissd_block_norm_args *a) {
@@ -78,7 +83,7 @@ template <class T> static size_t block_norm_ring(int pieces, int threads, bool b
     return (size_t)rows * pieces * 16 * threads;
 }
 typedef void (*BlockNormKernel)(bnorm::Params);
-template <class T, class R, bool VEC> static BlockNormKernel block_norm_kernel(int threads, int pair, bool backward) {
+template <class T, class R, int VEC> static BlockNormKernel block_norm_kernel(int threads, int pair, bool backward) {
     if (backward)
         return pair > 1        ? bnorm::block_norm_bwd<T, R, VEC, true, 512, kBwdWide>
                : threads > 256 ? bnorm::block_norm_bwd<T, R, VEC, false, 512, kBwdWide>
@@ -87,16 +92,21 @@ template <class T, class R, bool VEC> static BlockNormKernel block_norm_kernel(i
            : threads > 256 ? bnorm::block_norm_fwd<T, R, VEC, false, 512, kFwdWide>
                            : bnorm::block_norm_fwd<T, R, VEC, false, 256, kFwd>;
 }
+template <class T, class R> static BlockNormKernel block_norm_pick(int vec, int threads, int pair, bool backward) {
+    return vec == 8   ? block_norm_kernel<T, R, 8>(threads, pair, backward)
+           : vec == 2 ? block_norm_kernel<T, R, 2>(threads, pair, backward)
+                      : block_norm_kernel<T, R, 0>(threads, pair, backward);
+}
 template <class T, class R> static int block_norm_forward_impl(const bissd_block_norm_args *a, cudaStream_t s) {
     bnorm::Params p = block_norm_params(a);
     const int threads = block_norm_threads(p, false);
-    const bool vec = block_norm_vec(a);
+    const int vec = block_norm_vec(a);
     p.blocks = block_norm_blocks(p, false);
     const long long grid = block_norm_entries(p) * p.blocks;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     const int pieces = (int)(sizeof(T) * (a->gate && p.gate_rows == 0 ? 2 : 1) + sizeof(R)) / 2;
     const size_t smem = vec ? block_norm_ring<T>(pieces, threads, false) : 0;
-    const auto kernel = vec ? block_norm_kernel<T, R, true>(threads, 1, false) : block_norm_kernel<T, R, false>(threads, 1, false);
+    const auto kernel = block_norm_pick<T, R>(vec, threads, 1, false);
     BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
     BISSD_LAUNCH("block_norm_fwd", launch_pdl(kernel, (int)grid, threads, smem, s, p));
     return BISSD_OK;
@@ -104,7 +114,7 @@ template <class T, class R> static int block_norm_forward_impl(const bissd_block
 template <class T, class R> static int block_norm_backward_impl(const bissd_block_norm_args *a, float *part, cudaStream_t s) {
     bnorm::Params p = block_norm_params(a);
     const int threads = block_norm_threads(p, true), pair = block_norm_pair(p, true), per = std::max(1, threads / p.threads_row);
-    const bool vec = block_norm_vec(a);
+    const int vec = block_norm_vec(a);
     const long long entries = block_norm_entries(p);
     p.blocks = block_norm_blocks(p, true);
     if (entries * p.blocks > 0x3fffffffLL || (entries + 3) * ceil_div(p.D, 32) > 0x7fffffffLL) return BISSD_ERR_SHAPE;
@@ -112,7 +122,7 @@ template <class T, class R> static int block_norm_backward_impl(const bissd_bloc
     const int pieces = (int)(sizeof(T) * (1 + (a->gate && p.gate_rows == 0) + (a->dnormed != nullptr)) + sizeof(R) * (1 + (a->dr != nullptr))) / 2;
     const size_t rows = (size_t)(per - 1) * p.threads_row * bnorm::kCh * sizeof(float);
     const size_t smem = std::max(rows, vec ? block_norm_ring<T>(pieces, threads, true) : 0);
-    const auto kernel = vec ? block_norm_kernel<T, R, true>(threads, pair, true) : block_norm_kernel<T, R, false>(threads, pair, true);
+    const auto kernel = block_norm_pick<T, R>(vec, threads, pair, true);
     BISSD_ALLOW(kernel, smem + 512);                             // the limit is on static memory too
     BISSD_LAUNCH("block_norm_bwd", launch_cluster(kernel, (int)(entries * p.blocks) * pair, threads, smem, s, pair, p));
     bnorm::SumParams q{};

@@ -4,8 +4,8 @@
 //     dr' = dr + rstd(r) (t - r^ mean(t r^)),   dresidual = dr',   dn = dr' m,   dw1 = sum_rows du r^,   dw2 = sum_rows dn x^,
 //     dx = rstd(x) (dn w2 - x^ mean(dn w2 x^)),   dscale = sum_rows dr' act(gate) n,   dgate = dr' scale n act'(gate)
 // Bound by the rows' bytes: each tensor is read or written once, everything between stays in registers.  A row has
-// width / 8 threads with eight channels each - neighbouring ones (16-byte accesses), or where width or addresses do not allow that,
-// ones a stride apart - and a block walks rows with the weights in registers.  With 16-byte accesses a thread's pieces of the
+// width / 8 threads with eight channels each - neighbouring ones (16-byte accesses, or by pairs where the width is even and no more), or
+// where width or addresses do not allow that, ones a stride apart - and a block walks rows with the weights in registers.  Where neighbours are a thread's, its pieces of the
 // next rows come by asynchronous copies into shared memory of its own, several rows ahead: held in registers, one row ahead, they
 // left two blocks an SM waiting.  Above 4096 channels a row of the backward pass is two blocks' of a cluster: one block of 1024
 // threads left a thread 64 registers, too few (1445 us for 950, 16004 gated rows of 8192; the forward pass, which fits, loses by the
@@ -46,34 +46,42 @@ struct Params {
     float *part;                                                 // [blocks][4][D]: dw1, dw2, dscale, dgate of a shared row
 };
 
-// Channel e of thread t of a row.
-template <bool VEC> __device__ __forceinline__ int channel(int t, int tr, int e) { return VEC ? t * kCh + e : t + e * tr; }
+// Channel e of thread t of a row.  VEC: 8 where a thread's eight channels are neighbours that 16-byte accesses fit, 2 where pairs of them
+// are what lies aligned, 0 where they lie a stride apart, single (2790 rows of 4236, forward: 45 us by pairs, 89 single).
+template <int VEC> __device__ __forceinline__ int channel(int t, int tr, int e) { return VEC ? t * kCh + e : t + e * tr; }
 
 // A thread's eight channels of one tensor, and how a row's get into registers.
-template <class T, bool VEC> struct Column {
-    static constexpr int kPieces = VEC ? kCh * (int)sizeof(T) / 16 : 0;   // 16-byte pieces a row
+template <class T, int VEC> struct Column {
+    static constexpr int kCells = VEC ? kCh * (int)sizeof(T) / 16 : 0;   // of 16 bytes, that a row takes in shared memory
+    static constexpr int kPiece = VEC == 8 ? 16 : 2 * (int)sizeof(T), kPieces = kCells * 16 / kPiece;   // how it comes there
     int slot;                                                    // first piece's place in the ring's stage, in bytes
     __device__ __forceinline__ void start(int threads, int *bytes) {
         slot = *bytes;
-        *bytes += kPieces * threads * 16;
+        *bytes += kCells * threads * 16;
     }
     // A row on its way: zeros where there is none, or no such channels.  Addresses are made anew from the parameters, a multiply-add each:
     // kept and advanced they cost registers that the backward kernel does not have (16 us of 285, 65536 rows of 1024).
-    __device__ __forceinline__ void copy(const void *p, int row, int stride, int t, uint32_t stage, int threads, bool in) const {
-        if constexpr (VEC) {
+    __device__ __forceinline__ void copy(const void *p, int row, int stride, int t, int D, uint32_t stage, int threads, bool in) const {
+        if constexpr (VEC == 8) {
             const T *at = static_cast<const T *>(p) + ((long long)row * stride + t * kCh);
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + slot + i * threads * 16),
                              "l"(reinterpret_cast<const uint4 *>(at) + i), "r"(in ? 16 : 0) : "memory");
+        } else if constexpr (VEC == 2) {
+            const T *at = static_cast<const T *>(p) + ((long long)row * stride + t * kCh);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)                    // a pair of channels
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(stage + slot + i * kPiece / 16 * threads * 16 + i * kPiece % 16),
+                             "l"(at + 2 * i), "n"(kPiece), "r"(in && t * kCh + 2 * i < D ? kPiece : 0) : "memory");
         }
     }
     __device__ __forceinline__ void get(const void *p, int at_row, int stride, const uint8_t *stage, int threads, int t, int tr, int D,
                                         bool valid, f2 (&v)[kPairs]) const {
         vec::Row<T, kPairs> row;
-        if constexpr (VEC) {
+        if constexpr (VEC > 0) {
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
+            for (int i = 0; i < kCells; ++i) {
                 const uint4 q = *reinterpret_cast<const uint4 *>(stage + slot + i * threads * 16);
                 if constexpr (sizeof(T) == 4) {
                     row.v[2 * i] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
@@ -94,10 +102,14 @@ template <class T, bool VEC> struct Column {
         }
     }
 };
-template <class T, bool VEC>
+template <class T, int VEC>
 __device__ __forceinline__ void put(void *p, long long row, int t, int tr, int D, const f2 (&v)[kPairs]) {
     T *base = static_cast<T *>(p) + row * D;
-    if constexpr (VEC) {
+    if constexpr (VEC == 2) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+            if (t * kCh + 2 * i < D) *reinterpret_cast<typename vec::Pair<T>::raw *>(base + t * kCh + 2 * i) = vec::narrow<T>(v[i]);
+    } else if constexpr (VEC == 8) {
         if (t * kCh >= D) return;
         vec::Row<T, kPairs> o;
 #pragma unroll
@@ -113,7 +125,7 @@ __device__ __forceinline__ void put(void *p, long long row, int t, int tr, int D
         }
     }
 }
-template <bool VEC> __device__ __forceinline__ void weights(const void *p, int dtype, float none, int t, int tr, int D, f2 (&w)[kPairs]) {
+template <int VEC> __device__ __forceinline__ void weights(const void *p, int dtype, float none, int t, int tr, int D, f2 (&w)[kPairs]) {
     float e[kCh];
 #pragma unroll
     for (int i = 0; i < kCh; ++i) {
@@ -221,7 +233,7 @@ struct Walk {
     }
 };
 
-template <class T, class R, bool VEC, bool PAIR, int THREADS, int PER_SM>
+template <class T, class R, int VEC, bool PAIR, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     pdl_begin();
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -251,9 +263,9 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     auto copy = [&](int stage) {
         const bool some = in && ahead < k.n;
         const int to = k.first + ahead;
-        cx.copy(a.x, to, a.sx, t, ring + stage, threads, some);
-        cr.copy(a.res, to, a.sres, t, ring + stage, threads, some);
-        if (full) cg.copy(a.gate, to, a.sgate, t, ring + stage, threads, some);
+        cx.copy(a.x, to, a.sx, t, D, ring + stage, threads, some);
+        cr.copy(a.res, to, a.sres, t, D, ring + stage, threads, some);
+        if (full) cg.copy(a.gate, to, a.sgate, t, D, ring + stage, threads, some);
         asm volatile("cp.async.commit_group;" ::: "memory");
         ahead += k.step;
     };
@@ -319,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_fwd(Params a) {
     if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <class T, class R, bool VEC, bool PAIR, int THREADS, int PER_SM>
+template <class T, class R, int VEC, bool PAIR, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
     pdl_begin();
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -364,11 +376,11 @@ __global__ void __launch_bounds__(THREADS, PER_SM) block_norm_bwd(Params a) {
     auto copy = [&](int stage) {
         const bool some = in && ahead < k.n;
         const int to = k.first + ahead;
-        cx.copy(a.x, to, a.sx, t, ring + stage, threads, some);
-        cr.copy(a.res, to, a.sres, t, ring + stage, threads, some);
-        if (full) cg.copy(a.gate, to, a.sgate, t, ring + stage, threads, some);
-        if (a.du) cu.copy(a.du, to, a.sdu, t, ring + stage, threads, some);
-        if (a.dr) cd.copy(a.dr, to, a.sdr, t, ring + stage, threads, some);
+        cx.copy(a.x, to, a.sx, t, D, ring + stage, threads, some);
+        cr.copy(a.res, to, a.sres, t, D, ring + stage, threads, some);
+        if (full) cg.copy(a.gate, to, a.sgate, t, D, ring + stage, threads, some);
+        if (a.du) cu.copy(a.du, to, a.sdu, t, D, ring + stage, threads, some);
+        if (a.dr) cd.copy(a.dr, to, a.sdr, t, D, ring + stage, threads, some);
         asm volatile("cp.async.commit_group;" ::: "memory");
         ahead += k.step;
     };

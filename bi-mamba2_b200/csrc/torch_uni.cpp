@@ -259,7 +259,7 @@ py::object decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, co
     variable_list r;
     {
         py::gil_scoped_release nogil;
-        if (cu.defined()) cu = cu.to(at::kInt).contiguous();
+        if (cu.defined()) cu = (cu.scalar_type() == at::kLong ? cu.clamp(0, q.size(1)).to(at::kInt) : cu).contiguous();   // what lies outside would wrap
         if (grad) {
             r = AttentionFn::apply(q, k, v, g, initial, cu.defined() ? OptTensor(cu) : OptTensor(), cfg.scale, nseq, finals, check_status);
         } else {
@@ -439,6 +439,7 @@ py::object block_norm(const Tensor &x, const Tensor &residual, const OptTensor &
     if (d < 1 || d > 8192) bad(kNorm, ": width must be 1 to 8192, not ", d);
     const auto st = x.scalar_type();
     if (dtype_code(st) < 0) bad(kNorm, ": x must be float32, bfloat16 or float16");
+    if (x.numel() / d > 0x3fffffff) bad(kNorm, ": more than ", int64_t(0x3fffffff), " rows");
     if (residual.scalar_type() != st && residual.scalar_type() != at::kFloat) bad(kNorm, ": residual must be float32 or of x's type");
     at::ScalarType wt = at::kFloat;
     bool first = true;

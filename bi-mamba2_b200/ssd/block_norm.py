@@ -18,7 +18,7 @@ _ops = None
 def block_norm(x, residual, gate=None, scale=1.0, post_weight=None, pre_weight=None, gate_activation=None, eps=1e-5):
     """Returns (out, normed), or out alone without pre_weight.
 
-    x: (..., width), width 1 to 8192, float32, bfloat16 or float16; residual: x's shape, x's type or float32.
+    x: (..., width), width 1 to 8192 and fewer than 2^30 rows, float32, bfloat16 or float16; residual: x's shape, x's type or float32.
     gate: of x's type, x's shape or one row for each entry of the first dimension - (batch, 1, width) beside (batch, seqlen, width),
         or one row for all.  gate_activation: None, "sigmoid" or "silu".
     scale: a number or (width) values; post_weight, pre_weight: (width).  Those given are of one type, float32 or x's.
