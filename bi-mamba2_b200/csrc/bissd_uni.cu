@@ -137,6 +137,9 @@ int walk_segment(const bissd_decay_args *a, const Sizes &z) {
     return a->seqlen <= 3 * 64 && parts > 1 ? 3 * 64 : seg;
 }
 
+template <class T, bool Y> auto walk_kernel(int ipt) {
+    return ipt == 4 ? uni::decay_walk<T, 4, Y> : ipt == 8 ? uni::decay_walk<T, 8, Y> : ipt == 16 ? uni::decay_walk<T, 16, Y> : uni::decay_walk<T, 32, Y>;
+}
 int launch_walk(int dtype, const uni::WalkParams &w, cudaStream_t s) {
     const int ipt = walk_rows(w.I, w.lanes), cols = uni::kWalkThreads / w.lanes;
     const size_t smem = uni::walk_smem(w.lanes, ipt);
@@ -144,7 +147,7 @@ int launch_walk(int dtype, const uni::WalkParams &w, cudaStream_t s) {
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     return by_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const auto kernel = ipt == 4 ? uni::decay_walk<T, 4> : ipt == 8 ? uni::decay_walk<T, 8> : ipt == 16 ? uni::decay_walk<T, 16> : uni::decay_walk<T, 32>;
+        const auto kernel = w.y ? walk_kernel<T, true>(ipt) : walk_kernel<T, false>(ipt);
         BISSD_ALLOW(kernel, smem);
         BISSD_LAUNCH(w.y ? "decay_walk" : "decay_walk_states", launch_pdl(kernel, (int)grid, uni::kWalkThreads, smem, s, w));
         return BISSD_OK;
