@@ -303,7 +303,7 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     uni::FinishParams f{};
     f.L = a->seqlen; f.H = z.H; f.hk = z.hk; f.N = z.N; f.tokens = z.tokens; f.q = w.q.v; f.k = w.k.v;
     f.dqh = sp.dqh; f.dkh = sp.dkh; f.dq = a->dq; f.dk = a->dk; f.flow = sp.flow;
-    const long long grid = (z.tokens * z.hk + 7) / 8;
+    const long long grid = (z.tokens * (z.hk + (a->dg ? z.H : 0)) + 7) / 8;
     if (grid > 0x7fffffffLL || (long long)sp.plan.most * z.H > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     BISSD_DO(by_dtype(a->dtype, [&](auto t) -> int {
         BISSD_LAUNCH("decay_finish", launch_pdl(uni::decay_finish<decltype(t)>, (int)grid, 256, 0, s, f));
