@@ -127,14 +127,16 @@ uni::Plan plan_of(const bissd_decay_args *a, int seg, Bump &ws, uni::PlanOut *ou
     return p;
 }
 
-// Tokens to a segment on CUDA cores: long rows in as many as fill the SMs four times over, none under 64 tokens (a token takes 0.2 us in
-// a block, and what two more launches cost is as much as 40 of them); packed sequences in segments of 256.
+// Tokens to a segment on CUDA cores: rows in as many as fill the SMs four times over, but a token takes 0.2 us in a block, twice, and a
+// segment 0.25 in the chain: none under the root of 0.6 tokens, or under 32, and rows of up to 96 in one (two launches fewer).  With 64
+// at least and one up to 192, us: 4 heads of 16 x 32 fp32, 192 tokens 26.5 for 11.7, 253 17.5 for 12.1; 24 of 112 x 128, 128
+// tokens 46 for 51, 400 148 for 103.  Packed sequences in segments of 256.
 int walk_segment(const bissd_decay_args *a, const Sizes &z) {
     if (a->nseq > 0) return 256;
     const long long blocks = (long long)a->batch * z.H * ceil_div(z.P * z.lanes_n, uni::kWalkThreads);
     const long long parts = std::max<long long>(1, 4 * kSms / blocks);
-    const int seg = ceil_div((int)((a->seqlen + parts - 1) / parts), 64) * 64;
-    return a->seqlen <= 3 * 64 && parts > 1 ? 3 * 64 : seg;
+    const int least = std::max(32, (int)std::sqrt(0.6 * a->seqlen)), seg = std::max(least, (int)((a->seqlen + parts - 1) / parts));
+    return a->seqlen <= 96 || parts == 1 ? a->seqlen : ceil_div(seg, 16) * 16;
 }
 
 template <class T, bool Y> auto walk_kernel(int ipt) {
