@@ -130,9 +130,9 @@ uni::Plan plan_of(const bissd_decay_args *a, int seg, Bump &ws, uni::PlanOut *ou
 // Tokens to a segment on CUDA cores: rows in as many as fill the SMs four times over, but a token takes 0.2 us in a block, twice, and a
 // segment 0.25 in the chain: none under the root of 0.6 tokens, or under 32, and rows of up to 96 in one (two launches fewer).  With 64
 // at least and one up to 192, us: 4 heads of 16 x 32 fp32, 192 tokens 26.5 for 11.7, 253 17.5 for 12.1; 24 of 112 x 128, 128
-// tokens 46 for 51, 400 148 for 103.  Packed sequences in segments of 256.
+// tokens 46 for 51, 400 148 for 103.  The same for packed sequences: 2048 tokens of 8, 8 heads of 64 x 64, in segments of 256 171, in
+// these 113.
 int walk_segment(const bissd_decay_args *a, const Sizes &z) {
-    if (a->nseq > 0) return 256;
     const long long blocks = (long long)a->batch * z.H * ceil_div(z.P * z.lanes_n, uni::kWalkThreads);
     const long long parts = std::max<long long>(1, 4 * kSms / blocks);
     const int least = std::max(32, (int)std::sqrt(0.6 * a->seqlen)), seg = std::max(least, (int)((a->seqlen + parts - 1) / parts));
