@@ -1008,8 +1008,15 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 umma_commit(&done_a);
             }
         }
-        float whole = 0.f;
+        float whole = 0.f, among[4] = {};
         if constexpr (DG) {
+            if (last && warp == kSums) {                         // a token's pairs: read here, behind the next barrier they may be another head's
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 v = *reinterpret_cast<const float4 *>(&colsum[j][lane * 4]), w = *reinterpret_cast<const float4 *>(&rowsum[j][lane * 4]);
+                    among[0] += v.x - w.x; among[1] += v.y - w.y; among[2] += v.z - w.z; among[3] += v.w - w.w;
+                }
+            }
             if (ok) ok = mbar_wait(&bar_s, i & 1);
             if (first) through = 0.f;
             if (ok)
@@ -1067,15 +1074,14 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             ++loads_s;
         }
         if (DG && last && warp == kSums) {
-            float all = lane < 16 ? cross[lane] : 0.f, x[4] = {}, b[4] = {};
+            float all = lane < 16 ? cross[lane] : 0.f, x[4] = {among[0], among[1], among[2], among[3]}, b[4] = {};
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
             all *= ex2_approx(whole);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float4 u = *reinterpret_cast<const float4 *>(&past[j][lane * 4]), v = *reinterpret_cast<const float4 *>(&colsum[j][lane * 4]);
-                const float4 w = *reinterpret_cast<const float4 *>(&rowsum[j][lane * 4]), z = *reinterpret_cast<const float4 *>(&future[j][lane * 4]);
-                x[0] += u.x + (v.x - w.x); x[1] += u.y + (v.y - w.y); x[2] += u.z + (v.z - w.z); x[3] += u.w + (v.w - w.w);
+                const float4 u = *reinterpret_cast<const float4 *>(&past[j][lane * 4]), z = *reinterpret_cast<const float4 *>(&future[j][lane * 4]);
+                x[0] += u.x; x[1] += u.y; x[2] += u.z; x[3] += u.w;
                 b[0] += z.x; b[1] += z.y; b[2] += z.z; b[3] += z.w;
             }
             // sums of x from each token on, of b before each
