@@ -155,7 +155,7 @@ __device__ __forceinline__ void tma_store_read() {
 struct StatesShared {
     uint64_t full[2], full_v[2], ready, done, weights, stored, unused;
     uint32_t tmem;
-    int fail;
+    int fail, loads, loads_v;                                    // fail: the first wait that ran out; loads asked for
     float decay[2];                                              // of a chunk, 2^c_end
     alignas(16) uint32_t w[kQ];                                  // of a chunk's rows: f1 and f2, or EXACT fp32
 };
@@ -213,8 +213,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                                  "r"(s.t0 + place(i + 1) * kQ), "r"(s.batch) : "memory");
         };
         auto load_v = [&](int i) {                               // EXACT
-            mbar_expect_tx(&sh.full_v[i & 1], kSlab);
-            tma_load4(smV + (i & 1) * 3 * kSlab, &tmV, pb * kP, h, s.t0 + place(i) * kQ, s.batch, &sh.full_v[i & 1]);
+            const int st = i & 1;
+            mbar_expect_tx(&sh.full_v[st], kSlab);
+            tma_load4(smV + st * 3 * kSlab, &tmV, pb * kP, h, s.t0 + place(i) * kQ, s.batch, &sh.full_v[st]);
         };
         int loads = 1, loads_v = EXACT ? min(nc, 2) : 0;
         if (lane == 0) {
@@ -252,13 +253,10 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
                 }
             }
         }
-        if (!ok && elect_one()) {                                // leave nothing in flight
-            drain_mmas(&sh.unused);
-            drain_loads(sh.full, EXACT ? 1 : 2, loads);
-            drain_loads(sh.full_v, 2, loads_v);
-            atomicExch(a.status, kErrDecay + 0x10 + *fail);
+        if (lane == 0) {
+            sh.loads = loads;
+            sh.loads_v = loads_v;
         }
-        __syncwarp();
     } else if (warp == 9) {
         const int c0 = uni::segments(a.chunk, s.seq).x + s.idx * (a.seg.seg / kQ);
         Decays d;
@@ -428,6 +426,15 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     }
     tc_fence_before();
     __syncthreads();
+    if (sh.fail) {                                               // a wait of any role ran out: leave nothing in flight
+        if (tid == 0) atomicExch(a.status, kErrDecay + 0x10 + sh.fail);
+        if (warp == 8 && elect_one()) {
+            drain_mmas(&sh.unused);
+            drain_loads(sh.full, EXACT ? 1 : 2, sh.loads);
+            drain_loads(sh.full_v, 2, sh.loads_v);
+        }
+        __syncthreads();
+    }
     if (warp == 0) tmem_dealloc(tmem, EXACT ? 256 : 64);
 }
 
