@@ -54,7 +54,8 @@ struct Decays {
         for (int i = 0; i < 4; ++i) {
             const float g = a.g_dtype == BISSD_F16 ? __half2float(__ushort_as_half((unsigned short)raw[i]))
                                                    : __uint_as_float(a.g_dtype == BISSD_F32 ? raw[i] : raw[i] << 16);
-            v[i] = fmaxf(g * 1.44269504f, -200.f);
+            const float x = g * 1.44269504f;
+            v[i] = x < -200.f ? -200.f : x;                      // what is no number stays none
         }
     }
     // Sums up to and with each token.
