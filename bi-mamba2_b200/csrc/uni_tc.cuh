@@ -6,8 +6,9 @@
 //   decay_chunks   all chunks at once, given the states
 // Heads of v are taken 64 columns at a time: with the same weights, v's parts are heads of their own that share q, k and g.  Head sizes
 // that fill no tile are completed by the loads with zeros.  Log decays count in powers of two and no lower than 2^-200 a token, which
-// fp32 has no number for: -inf never meets +inf.  Factors that reach to a chunk's ends are 2 to the power of a sum that starts there,
-// so that a strong decay elsewhere in the chunk costs them no digits.
+// fp32 has no number for: -inf never meets +inf.  Factors that reach to a chunk's ends are 2 to the power of a sum that starts there, and
+// those between two tokens from sums that start at one of them, or in two parts (Decays), so that a strong decay elsewhere in the chunk
+// costs no digits.
 #pragma once
 #include "tc_tma.cuh"
 #include "uni_plan.cuh"
@@ -73,6 +74,33 @@ struct Decays {
         if (lane > 0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[i] += before;
+        }
+    }
+    // The same for sums that are subtracted from one another: those of the whole numbers, which are exact, and of the rests, at most 64.  In one
+    // they come to 25600 where tokens empty the state, and a step of fp32 is 2^-9 there.
+    __device__ __forceinline__ void prefix(float (&c)[4], float (&rest)[4], int lane) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = rintf(v[i]);
+            c[i] = i ? c[i - 1] + w : w;
+            rest[i] = i ? rest[i - 1] + (v[i] - w) : v[i] - w;
+        }
+        float sum = c[3], sum_r = rest[3];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float u = __shfl_up_sync(0xffffffffu, sum, o), u_r = __shfl_up_sync(0xffffffffu, sum_r, o);
+            if (lane >= o) {
+                sum += u;
+                sum_r += u_r;
+            }
+        }
+        const float before = __shfl_up_sync(0xffffffffu, sum, 1), before_r = __shfl_up_sync(0xffffffffu, sum_r, 1);
+        if (lane > 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                c[i] += before;
+                rest[i] += before_r;
+            }
         }
     }
     // Sums of the tokens behind each.
@@ -466,7 +494,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ uint64_t bar_qk, bar_v, bar_s, done, done_s, unused;
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float cs[kTables][kQ], below[kTables][kQ];   // c_t; 2^(c at the end of s' 32 - c_s)
+    __shared__ __align__(16) float cs[kTables][kQ], cl[kTables][kQ], below[kTables][kQ];   // c_t and its rest; 2^(c at the end of s' 32 - c_s)
     uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + 2 * kSlab, *smS = smV + kSlab;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int part = blockIdx.x % a.parts, m = blockIdx.x / a.parts % a.h.hk, ci = blockIdx.x / (a.parts * a.h.hk);
@@ -489,12 +517,14 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     };
     auto table = [&](int k) {
         if (k >= heads) return;
-        float c[4];
+        float c[4], l[4];
         next.log2(a.h);
-        next.prefix(c, lane);
-        const float end = __shfl_sync(0xffffffffu, c[3], lane | 7);
+        next.prefix(c, l, lane);
+        const float end = __shfl_sync(0xffffffffu, c[3], lane | 7), end_l = __shfl_sync(0xffffffffu, l[3], lane | 7);
         *reinterpret_cast<float4 *>(&cs[warp][lane * 4]) = make_float4(c[0], c[1], c[2], c[3]);
-        *reinterpret_cast<float4 *>(&below[warp][lane * 4]) = make_float4(exp2f(end - c[0]), exp2f(end - c[1]), exp2f(end - c[2]), exp2f(end - c[3]));
+        *reinterpret_cast<float4 *>(&cl[warp][lane * 4]) = make_float4(l[0], l[1], l[2], l[3]);
+        auto w = [&](int k) { return exp2f((end - c[k]) + (end_l - l[k])); };
+        *reinterpret_cast<float4 *>(&below[warp][lane * 4]) = make_float4(w(0), w(1), w(2), w(3));
     };
     ask(warp);
     if (warp == 0) tmem_alloc(&tmem_slot, 256);
@@ -564,8 +594,8 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                 umma_commit(&done_s);
             }
         }
-        const float *c = cs[k % kTables];
-        const float ct = c[t] + a.h.log_scale;
+        const float *c = cs[k % kTables], *l = cl[k % kTables];
+        const float ct = c[t], lt = l[t] + a.h.log_scale;
         {
             uint32_t raw[16];
             tmem_ld16_nowait(tl + u0 * 16, raw);
@@ -577,7 +607,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                 if (u + 1 < u1) tmem_ld16_nowait(tl + (u + 1) * 16, raw);
                 const int cb = u >> 1;
                 if (cb < r32) {
-                    const float rt = exp2f(ct - c[cb * 32 + 31]);
+                    const float rt = exp2f((ct - c[cb * 32 + 31]) + (lt - l[cb * 32 + 31]));
                     const vec::f2 rt2 = vec::pack(rt, rt);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -589,11 +619,11 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                     const int td = t - u * 16;                   // columns up to it; what is behind it may be no number
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float2 f = *reinterpret_cast<const float2 *>(c + u * 16 + j * 2);
+                        const float2 f = *reinterpret_cast<const float2 *>(c + u * 16 + j * 2), fl = *reinterpret_cast<const float2 *>(l + u * 16 + j * 2);
                         float lo, hi;
                         vec::unpack(x[j], lo, hi);
-                        lo *= ex2_approx(ct - f.x);
-                        hi *= ex2_approx(ct - f.y);
+                        lo *= ex2_approx((ct - f.x) + (lt - fl.x));
+                        hi *= ex2_approx((ct - f.y) + (lt - fl.y));
                         x[j] = vec::pack(2 * j <= td ? lo : 0.f, 2 * j + 1 <= td ? hi : 0.f);
                     }
                 }
@@ -641,7 +671,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         tc_fence_after();
         // o = inside + scale e^{c_t} from the state; whole rows leave through the first slab of the weighted pairs
         if (ok) {
-            const float f = exp2f(ct);
+            const float f = exp2f(ct + lt);
             float x[32], y[32];
             tmem_ld32(tl + 128 + half * 32, x);
             tmem_ld32(tl + 192 + half * 32, y);
@@ -741,7 +771,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
     constexpr int kTables = 2, kHelp = 3, kIssue = 7, kSums = 11;   // warps above the diagonal
     extern __shared__ __align__(1024) uint8_t dyn[];
     struct Table {                                               // of a head; two take turns
-        float c[kQ], ws[kQ];                                     // c_t; e^{c_end - c_s}
+        float g[kQ], ws[kQ];                                     // log2 of a token's decay; e^{c_end - c_s}
         uint32_t wv[kQ], wd[kQ];                                 // that and scale e^{c_t} in halves, for v and do
         float above[kQ], beside[3][kQ];                          // weights of blocks of 32 x 32: 2^(c at the end of s' 32 - c_s), scale 2^(c_t - c at the end of the q-th 32)
         float whole[4];                                          // c_end
@@ -772,29 +802,28 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         tma_load2(smG, &tmG, 0, row, &bar_s);
     };
     auto table = [&](Table &to, Decays &next) {                  // one warp
-        float p[4], q[4];
+        float c[4], l[4], q[4];
         next.log2(a.h);
-        next.prefix(p, lane);
-        next.suffix(q, lane);
-        const float end = __shfl_sync(0xffffffffu, p[3], lane | 7);
-        float ends[4];
+        next.prefix(c, l, lane);
+        const float all = __shfl_sync(0xffffffffu, c[3], 31), all_l = __shfl_sync(0xffffffffu, l[3], 31);
+        auto four = [&](float *o, auto f) { *reinterpret_cast<float4 *>(o + lane * 4) = make_float4(f(0), f(1), f(2), f(3)); };
+        four(to.g, [&](int k) { return next.v[k]; });
+        const float end = __shfl_sync(0xffffffffu, c[3], lane | 7), end_l = __shfl_sync(0xffffffffu, l[3], lane | 7);
+        four(to.above, [&](int k) { return ex2_approx((end - c[k]) + (end_l - l[k])); });
 #pragma unroll
-        for (int k = 0; k < 4; ++k) ends[k] = __shfl_sync(0xffffffffu, p[3], 8 * k + 7);
-        auto four = [&](float *o, float x0, float x1, float x2, float x3) { *reinterpret_cast<float4 *>(o + lane * 4) = make_float4(x0, x1, x2, x3); };
-        four(to.c, p[0], p[1], p[2], p[3]);
-        four(to.above, ex2_approx(end - p[0]), ex2_approx(end - p[1]), ex2_approx(end - p[2]), ex2_approx(end - p[3]));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = ex2_approx(q[k]);
-        four(to.ws, q[0], q[1], q[2], q[3]);
+        for (int k = 0; k < 4; ++k) q[k] = ex2_approx((all - c[k]) + (all_l - l[k]));
+        four(to.ws, [&](int k) { return q[k]; });
         *reinterpret_cast<uint4 *>(to.wv + lane * 4) = make_uint4(halves<T>(q[0]), halves<T>(q[1]), halves<T>(q[2]), halves<T>(q[3]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) p[k] += a.h.log_scale;
-        *reinterpret_cast<uint4 *>(to.wd + lane * 4) =
-            make_uint4(halves<T>(ex2_approx(p[0])), halves<T>(ex2_approx(p[1])), halves<T>(ex2_approx(p[2])), halves<T>(ex2_approx(p[3])));
+        for (int k = 0; k < 4; ++k) l[k] += a.h.log_scale;
+        auto wd = [&](int k) { return halves<T>(ex2_approx(c[k] + l[k])); };
+        *reinterpret_cast<uint4 *>(to.wd + lane * 4) = make_uint4(wd(0), wd(1), wd(2), wd(3));
 #pragma unroll
-        for (int b = 0; b < 3; ++b)                              // of use in the blocks behind the b-th
-            four(to.beside[b], ex2_approx(p[0] - ends[b]), ex2_approx(p[1] - ends[b]), ex2_approx(p[2] - ends[b]), ex2_approx(p[3] - ends[b]));
-        if (lane == 0) to.whole[0] = ends[3];
+        for (int b = 0; b < 3; ++b) {                            // of use in the blocks behind the b-th
+            const float from = __shfl_sync(0xffffffffu, end, 8 * b + 7), from_l = __shfl_sync(0xffffffffu, end_l, 8 * b + 7);
+            four(to.beside[b], [&](int k) { return ex2_approx((c[k] - from) + (l[k] - from_l)); });
+        }
+        if (lane == 0) to.whole[0] = all + all_l;
     };
     if (warp == 0) tmem_alloc(&tmem_slot, 512);
     if (tid == 32) {
@@ -897,11 +926,6 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 if (i > 0) from_chunk();                         // of the tile before: here nothing waits for them
             }
         }
-        if (warp == kTables && i + 1 < nv && last) {             // the next head's; the turn before the last one has been read
-            Decays d;
-            d.load(a.h, sg.batch, sg.t0, len, h1, lane);
-            table(tables[(h1 - h0) & 1], d);
-        }
         if (ok && i > 0) put_dv(i - 1, h0 + (i - 1) / a.h.PB, pb == 0 ? a.h.PB - 1 : pb - 1);
         if (ok) ok = mbar_wait(&bar_v[i & 1], (i >> 1) & 1);
         if (ok) {
@@ -926,9 +950,14 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
             uint32_t p[16];
             float of_row = 0.f, of_column = 0.f;                 // for dg: d (q.k) over this row, over column 32 cg + lane
             if (some) {
-                const float cs = tb.c[s] - a.h.log_scale, fs = tb.above[s];
-                const float4 *f4 = reinterpret_cast<const float4 *>(cg == quad ? tb.c + cg * 32 : tb.beside[quad] + cg * 32);
+                const float fs = tb.above[s];
+                const float4 *f4 = reinterpret_cast<const float4 *>(cg == quad ? tb.g + cg * 32 : tb.beside[quad] + cg * 32);
                 vec::f2 sum = vec::pack(0.f, 0.f);
+                float c = -INFINITY;                             // on the diagonal c_t - c_s, summed from s on
+                auto weight = [&](int j, float g) {
+                    c = j == lane ? a.h.log_scale : c + g;
+                    return ex2_approx(c);
+                };
 #pragma unroll
                 for (int j0 = 0; j0 < 32; j0 += 8) {
                     uint32_t d[4];
@@ -937,8 +966,9 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                         const float4 f = f4[j / 4];
                         vec::f2 w0, w1;
                         if (cg == quad) {
-                            w0 = vec::pack(j >= lane ? ex2_approx(f.x - cs) : 0.f, j + 1 >= lane ? ex2_approx(f.y - cs) : 0.f);
-                            w1 = vec::pack(j + 2 >= lane ? ex2_approx(f.z - cs) : 0.f, j + 3 >= lane ? ex2_approx(f.w - cs) : 0.f);
+                            const float e0 = weight(j, f.x), e1 = weight(j + 1, f.y), e2 = weight(j + 2, f.z), e3 = weight(j + 3, f.w);
+                            w0 = vec::pack(e0, e1);
+                            w1 = vec::pack(e2, e3);
                         } else {
                             const vec::f2 fs2 = vec::pack(fs, fs);
                             w0 = vec::mul2(vec::pack(f.x, f.y), fs2);
@@ -1015,6 +1045,11 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 }
                 umma_commit(&done_a);
             }
+        }
+        if (warp == kTables && i + 1 < nv && last) {             // the next head's, under the products; the turn before has been read
+            Decays d;
+            d.load(a.h, sg.batch, sg.t0, len, h1, lane);
+            table(tables[(h1 - h0) & 1], d);
         }
         float whole = 0.f, among[4] = {};
         if constexpr (DG) {
