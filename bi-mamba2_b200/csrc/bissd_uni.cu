@@ -336,10 +336,11 @@ bool tc_tensor(const bissd_tensor &t, long long batch, long long seq, long long 
     auto fits = [](long long stride, long long n) { return n == 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38)); };
     return aligned16(t.ptr) && fits(t.stride_batch, batch) && fits(t.stride_seq, seq) && fits(t.stride_head, heads);
 }
-bool tc_forward_ok(const bissd_decay_args *a) {
+bool tc_inputs(const bissd_decay_args *a) {
     return tc_sizes(a) && tc_tensor(a->q, a->batch, a->seqlen, a->nkheads) && tc_tensor(a->k, a->batch, a->seqlen, a->nkheads) &&
-           tc_tensor(a->v, a->batch, a->seqlen, a->nheads) && aligned16(a->o);
+           tc_tensor(a->v, a->batch, a->seqlen, a->nheads);
 }
+bool tc_forward_ok(const bissd_decay_args *a) { return tc_inputs(a) && aligned16(a->o); }
 
 struct TcSpace {
     int NT, PB;
@@ -523,9 +524,7 @@ TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
     return g;
 }
 bool tc_backward_ok(const bissd_decay_args *a) {
-    return tc_sizes(a) && tc_tensor(a->q, a->batch, a->seqlen, a->nkheads) && tc_tensor(a->k, a->batch, a->seqlen, a->nkheads) &&
-           tc_tensor(a->v, a->batch, a->seqlen, a->nheads) && tc_tensor(a->dout, a->batch, a->seqlen, a->nheads) && aligned16(a->dq) && aligned16(a->dk) &&
-           aligned16(a->dv);
+    return tc_inputs(a) && tc_tensor(a->dout, a->batch, a->seqlen, a->nheads) && aligned16(a->dq) && aligned16(a->dk) && aligned16(a->dv);
 }
 
 int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
@@ -621,6 +620,8 @@ int bissd_decay_forward(const bissd_decay_args *a, void *workspace, size_t works
     size_t need = 0;
     BISSD_DO(bissd_decay_workspace_bytes(a, &need, nullptr));
     BISSD_DO(decay_pointers(a, false));
+    // The backward pass of these inputs would read `saved`, and the CUDA cores, for such an o, do not write it.
+    if (a->saved && tc_inputs(a) && !tc_forward_ok(a)) return BISSD_ERR_ALIGN;
     if (!workspace || workspace_bytes < need) return BISSD_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) % 256 || reinterpret_cast<uintptr_t>(a->saved) % 256) return BISSD_ERR_ALIGN;
     BISSD_DO(check_device());

@@ -286,7 +286,7 @@ typedef struct bissd_decay_args {
     int32_t g_dtype, g_per_head;
     float scale;
     bissd_tensor q, k, v;
-    void *o;                             /* contiguous */
+    void *o;                             /* contiguous; with `saved` and a 16-bit dtype 16-byte aligned, else BISSD_ERR_ALIGN */
     bissd_tensor g;                      /* (batch, seqlen, nheads), or ptr alone with g_per_head (contiguous) */
     const int32_t *cu_seqlens;           /* (nseq + 1) */
     const float *initial_state;          /* (sequences, nheads, kdim, vdim) contiguous, or NULL: zeros */
