@@ -139,7 +139,7 @@ int walk_segment(const bissd_decay_args *a, const Sizes &z) {
     return a->seqlen <= 96 || parts == 1 ? a->seqlen : ceil_div(seg, 16) * 16;
 }
 
-template <class T, bool Y> auto walk_kernel(int ipt) {
+template <class T, int Y> auto walk_kernel(int ipt) {
     return ipt == 4 ? uni::decay_walk<T, 4, Y> : ipt == 8 ? uni::decay_walk<T, 8, Y> : ipt == 16 ? uni::decay_walk<T, 16, Y> : uni::decay_walk<T, 32, Y>;
 }
 int launch_walk(int dtype, const uni::WalkParams &w, cudaStream_t s) {
@@ -149,7 +149,7 @@ int launch_walk(int dtype, const uni::WalkParams &w, cudaStream_t s) {
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     return by_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const auto kernel = w.y ? walk_kernel<T, true>(ipt) : walk_kernel<T, false>(ipt);
+        const auto kernel = !w.y ? walk_kernel<T, uni::kStates>(ipt) : w.others ? walk_kernel<T, uni::kOthers>(ipt) : walk_kernel<T, uni::kOutputs>(ipt);
         BISSD_ALLOW(kernel, smem);
         BISSD_LAUNCH(w.y ? "decay_walk" : "decay_walk_states", launch_pdl(kernel, (int)grid, uni::kWalkThreads, smem, s, w));
         return BISSD_OK;
@@ -212,7 +212,7 @@ struct WalkSpace {                                               // the workspac
     uni::Plan plan;
     uni::PlanOut table{};
     float *states, *decay;
-    float *dstates, *ddecay, *final_, *dqh, *dkh, *flow, *dg_tokens;   // backward
+    float *dstates, *ddecay, *final_, *dqh, *dkh, *into, *from, *dg_tokens;   // backward
 };
 WalkSpace walk_space(const bissd_decay_args *a, Bump &ws, bool backward) {
     const Sizes z = sizes_of(a);
@@ -229,7 +229,8 @@ WalkSpace walk_space(const bissd_decay_args *a, Bump &ws, bool backward) {
         s.final_ = ws.take<float>((size_t)z.sequences * z.H * z.N * z.P);
         s.dqh = ws.take<float>((size_t)z.tokens * z.H * z.N);
         s.dkh = ws.take<float>((size_t)z.tokens * z.H * z.N);
-        s.flow = ws.take<float>((size_t)z.tokens * z.H);
+        s.into = ws.take<float>((size_t)z.tokens * z.H);
+        s.from = ws.take<float>((size_t)z.tokens * z.H);
         if (a->g_per_head) s.dg_tokens = ws.take<float>((size_t)z.tokens * z.H);
     }
     return s;
@@ -285,26 +286,28 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     p.status = reinterpret_cast<int *>(ws.base);
     p.fin = sp.states; p.decay = sp.decay;
     BISSD_DO(launch_walk(a->dtype, p, s));
-    BISSD_DO(launch_chain(chain_params(w, false, a->initial_state, sp.states, sp.decay, a->dfinal_state ? sp.final_ : nullptr), s));
+    BISSD_DO(launch_chain(chain_params(w, false, a->initial_state, sp.states, sp.decay, nullptr), s));
     p = walk_params(w, w.q, w.dout, w.k, true);
     p.a_scale = a->scale; p.fin = sp.dstates; p.decay = sp.ddecay;
     BISSD_DO(launch_walk(a->dtype, p, s));
     BISSD_DO(launch_chain(chain_params(w, true, a->dfinal_state, sp.dstates, sp.ddecay, a->dinitial_state), s));
-    // dv, and for each head dk and dq
+    // dv, and for each head dk and dq without the tokens' own pairs
     p.fin = nullptr; p.decay = nullptr; p.init = sp.dstates;
     p.y = a->dv; p.y_dtype = a->dtype; p.y_batch = (long long)a->seqlen * z.H * z.P;
     BISSD_DO(launch_walk(a->dtype, p, s));
     p = walk_params(w, w.dout, w.q, w.v, true);
     p.a_scale = a->scale; p.init = sp.dstates;
-    p.y = sp.dkh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
+    p.others = 1; p.y = sp.dkh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
     BISSD_DO(launch_walk(a->dtype, p, s));
     p = walk_params(w, w.v, w.k, w.dout, false);
     p.y_scale = a->scale; p.init = sp.states;
-    p.y = sp.dqh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
+    p.fin = a->dg && a->dfinal_state ? sp.final_ : nullptr;
+    p.others = 1; p.y = sp.dqh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
     BISSD_DO(launch_walk(a->dtype, p, s));
     uni::FinishParams f{};
-    f.L = a->seqlen; f.H = z.H; f.hk = z.hk; f.N = z.N; f.tokens = z.tokens; f.q = w.q.v; f.k = w.k.v;
-    f.dqh = sp.dqh; f.dkh = sp.dkh; f.dq = a->dq; f.dk = a->dk; f.flow = sp.flow;
+    f.L = a->seqlen; f.H = z.H; f.hk = z.hk; f.N = z.N; f.P = z.P; f.tokens = z.tokens; f.scale = a->scale;
+    f.q = w.q.v; f.k = w.k.v; f.v = w.v.v; f.dout = w.dout.v; f.bounds = sp.table.bounds; f.nseq = a->nseq;
+    f.dqh = sp.dqh; f.dkh = sp.dkh; f.dq = a->dq; f.dk = a->dk; f.into = sp.into; f.from = sp.from;
     const long long grid = (z.tokens * (z.hk + (a->dg ? z.H : 0)) + 7) / 8;
     if (grid > 0x7fffffffLL || (long long)sp.plan.most * z.H > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     BISSD_DO(by_dtype(a->dtype, [&](auto t) -> int {
@@ -315,7 +318,7 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     uni::DecayGradParams d{};
     d.plan = sp.plan; d.H = z.H; d.per = z.N * z.P; d.g_dtype = a->g_dtype; d.L = a->seqlen;
     d.out_dtype = a->g_per_head ? BISSD_F32 : a->g_dtype;
-    d.flow = sp.flow; d.enter = sp.states; d.denter = sp.dstates; d.final_ = sp.final_; d.dfinal = a->dfinal_state; d.g = w.g;
+    d.into = sp.into; d.from = sp.from; d.enter = sp.states; d.denter = sp.dstates; d.final_ = sp.final_; d.dfinal = a->dfinal_state; d.g = w.g;
     d.dg = a->g_per_head ? sp.dg_tokens : a->dg;
     BISSD_LAUNCH("decay_dg", launch_pdl(uni::decay_dg, sp.plan.most * z.H, 256, 0, s, d));
     if (a->g_per_head)

@@ -2,7 +2,7 @@
 //     S_t = e^{g_t} S_{t-1} + a_t b_t^T,    y_t = y_scale S_t^T r_t
 // walked forwards with (a, b, r) = (k, v, q) gives o and, with the roles of S's two sides exchanged (v, k, dout), dq; walked
 // backwards - the decay of the token after t in e^{g_t}'s place - (q, dout, k) gives dv and (dout, q, v) dk, all four from one
-// kernel.  A thread has one column of S and a part of its rows in registers; the lanes that share a column add their
+// kernel; dq and dk without what a token's own pair adds, e^{g_t} S_{t-1} in S_t's place (decay_finish says why).  A thread has one column of S and a part of its rows in registers; the lanes that share a column add their
 // products up.  Three multiply-adds per element of S and token, two reads of shared memory (16 bytes) for every 12 of them:
 // bound by those reads and the loads' instructions (670 tokens of 24 heads, 112 x 128, fp32: 102 us with outputs, 57 for states alone; the
 // multiply-adds' rate would allow 20).
@@ -28,10 +28,11 @@ struct WalkParams {
     int g_dtype;
     float a_scale, y_scale;
     void *y;                                                     // (tokens, H, J) contiguous, or NULL: states only
+    int others;                                                  // of y: without a token's own pair
     int y_dtype;
     long long y_batch;                                           // elements of a batch row of y
     const float *init;                                           // what enters: (segments, H, ..), or NULL: zeros
-    float *fin;                                                  // what leaves: (segments, H, ..), or NULL
+    float *fin;                                                  // what leaves: (segments, H, ..), or NULL; kOthers: (sequences, H, ..), without the last token's own
     float *decay;                                                // (segments, H): the segment's whole decay, or NULL
     int si, sj;                                                  // strides of S's two sides in init and fin
     int *status;                                                 // cleared, or NULL
@@ -44,9 +45,10 @@ inline size_t walk_smem(int lanes, int ipt) {
     return sizeof(float) * (2 * ((size_t)tile * 2 * lanes * (ipt + 4) + (size_t)tile * cols + 2 * tile) + (size_t)tile * cols);
 }
 
-// Y: outputs are wanted, not the states alone (asked at run time, the question parted the loads of every four elements: 143 us for
-// 114, 670 tokens of 24 heads, 112 x 128).
-template <class T, int IPT, bool Y> __global__ void __launch_bounds__(kWalkThreads, 4) decay_walk(WalkParams a) {
+// Y: outputs are wanted (asked at run time, the question parted the loads of every four elements: 143 us for 114, 670 tokens of 24
+// heads, 112 x 128), with a token's own pair or without it.
+enum { kStates = 0, kOutputs = 1, kOthers = 2 };
+template <class T, int IPT, int Y> __global__ void __launch_bounds__(kWalkThreads, 4) decay_walk(WalkParams a) {
     pdl_begin();
     extern __shared__ __align__(16) float dyn[];
     if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
@@ -89,12 +91,13 @@ template <class T, int IPT, bool Y> __global__ void __launch_bounds__(kWalkThrea
                 const int t = x >> la, i = x & (across - 1), at = t * rowlen + i / IPT * (IPT + 4) + i % IPT;
                 const bool in = t < n && i < a.I;
                 put(as + at, a.a.v.ptr, row(a.a, first + t) + i, in);
-                if (Y) put(rs + at, a.r.v.ptr, row(a.r, first + t) + i, in);
+                if (Y != kStates) put(rs + at, a.r.v.ptr, row(a.r, first + t) + i, in);
             }
 #pragma unroll 4
             for (int x = tid; x < n4 * cols; x += kWalkThreads) {
                 const int t = x >> lc, c = cb * cols + (x & (cols - 1));
-                put(bs + x, a.b.v.ptr, row(a.b, first + t) + c, t < n && c < a.J);
+                const bool own = Y != kOthers || !a.fin || !s.last || first + t < s.t0 + s.len - 1;   // nothing reads what the last token adds
+                put(bs + x, a.b.v.ptr, row(a.b, first + t) + c, t < n && c < a.J && own);
             }
             g = 0.f;
             const int t = first + tid + a.reverse;
@@ -133,21 +136,32 @@ template <class T, int IPT, bool Y> __global__ void __launch_bounds__(kWalkThrea
 #pragma unroll
                 for (int e = 0; e < IPT; e += 4) {
                     const float4 x = a4[e / 4];
-                    st_[e] = st_[e] * d + x.x * b;
-                    st_[e + 1] = st_[e + 1] * d + x.y * b;
-                    st_[e + 2] = st_[e + 2] * d + x.z * b;
-                    st_[e + 3] = st_[e + 3] * d + x.w * b;
-                    if constexpr (Y) {
+                    auto output = [&] {
                         const float4 r = r4[e / 4];
                         sum += r.x * st_[e];
                         sum2 += r.y * st_[e + 1];
                         sum += r.z * st_[e + 2];
                         sum2 += r.w * st_[e + 3];
+                    };
+                    if constexpr (Y == kOthers) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) st_[e + k] *= d;
+                        output();
+                        st_[e] += x.x * b;
+                        st_[e + 1] += x.y * b;
+                        st_[e + 2] += x.z * b;
+                        st_[e + 3] += x.w * b;
+                    } else {
+                        st_[e] = st_[e] * d + x.x * b;
+                        st_[e + 1] = st_[e + 1] * d + x.y * b;
+                        st_[e + 2] = st_[e + 2] * d + x.z * b;
+                        st_[e + 3] = st_[e + 3] * d + x.w * b;
+                        if constexpr (Y == kOutputs) output();
                     }
                 }
                 acc[w] = sum + sum2;
             }
-            if constexpr (Y) {
+            if constexpr (Y != kStates) {
                 for (int o = 1; o < LI; o <<= 1) {
 #pragma unroll
                     for (int w = 0; w < 4; ++w) acc[w] += __shfl_xor_sync(0xffffffffu, acc[w], o);
@@ -160,7 +174,7 @@ template <class T, int IPT, bool Y> __global__ void __launch_bounds__(kWalkThrea
         }
         if (done + tile < s.len) decays(stage ^ 1);
         __syncthreads();                                         // the tile has been read, and ys is written: the next barrier lets it be again
-        if constexpr (Y) {
+        if constexpr (Y != kStates) {
             for (int x = tid; x < n * cols; x += kWalkThreads) {
                 const int t = x >> lc, c = cb * cols + (x & (cols - 1));
                 if (c < a.J)
@@ -169,11 +183,12 @@ template <class T, int IPT, bool Y> __global__ void __launch_bounds__(kWalkThrea
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (a.fin) {
+    if (a.fin && (Y != kOthers || s.last)) {
+        const long long to = Y == kOthers ? s.seq : si;
 #pragma unroll
         for (int e = 0; e < IPT; ++e) {
             const int i = li * IPT + e;
-            if (i < a.I && j < a.J) a.fin[(si * (long long)a.H + h) * S + (long long)i * a.si + (long long)j * a.sj] = st_[e];
+            if (i < a.I && j < a.J) a.fin[(to * (long long)a.H + h) * S + (long long)i * a.si + (long long)j * a.sj] = st_[e];
         }
     }
     if (a.decay && cb == 0 && tid == 0) a.decay[si * (long long)a.H + h] = expf(total);
@@ -248,24 +263,41 @@ template <int VEC> __global__ void __launch_bounds__(256) decay_chain(ChainParam
     }
 }
 
-// What the per-head gradients leave: dq and dk summed over the heads that share them (a warp for a token and head of q), and what a
-// token's decay gets from its own place, flow = q.dq - k.dk (a pair of tokens s < t counts +1 at t and -1 at s; a warp for a token and
-// head).  The second reads again what the first has read: together, one warp's heads waited for one another (89 us, 15 so:
-// 670 tokens, 24 heads of 2, kdim 112).
+// What the per-head gradients leave: dq and dk summed over the heads that share them, with the tokens' own pairs, which the walks leave
+// out: scale sum_h (do_t.v_t) times k_t or q_t (a warp for a token and head of q); and what a token's decay gets from its own place,
+// into = q.dq and from = k.dk (a pair of tokens s < t counts +1 at t and -1 at s; a warp for a token and head).  A token's own pair would be
+// in both of these, and the larger it is beside the others the fewer digits their difference would have.  The second reads again what the first has read: together, one warp's heads waited for one another
+// (89 us, 15 so: 670 tokens, 24 heads of 2, kdim 112).
 struct FinishParams {
-    int L, H, hk, N;
+    int L, H, hk, N, P, nseq;
     long long tokens;
-    View q, k;
-    const float *dqh, *dkh;                                      // (tokens, H, N)
+    float scale;
+    View q, k, v, dout;
+    const int *bounds;                                           // packed: the sequences' tokens are bounds[0] ... bounds[nseq] - 1; or NULL
+    const float *dqh, *dkh;                                      // (tokens, H, N), others' part
     void *dq, *dk;                                               // (tokens, hk, N)
-    float *flow;                                                 // (tokens, H)
+    float *into, *from;                                          // (tokens, H)
 };
 template <class T> __global__ void __launch_bounds__(256) decay_finish(FinishParams a) {
     pdl_begin();
     long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, R = a.H / a.hk;
     if (w < a.tokens * a.hk) {
-        const long long from = w * R * a.N;
+        const long long from = w * R * a.N, tok = w / a.hk, b = tok / a.L, t = tok % a.L;
+        const int m = (int)(w % a.hk);
+        const long long at = b * a.q.sb + t * a.q.sl + m * a.q.sh, kt = b * a.k.sb + t * a.k.sl + m * a.k.sh;
+        const bool in = !a.bounds || (t >= a.bounds[0] && t < a.bounds[a.nseq]);
+        float own = 0.f;
+        if (in) {
+            for (int r = 0; r < R; ++r) {
+                const long long vt = b * a.v.sb + t * a.v.sl + (long long)(m * R + r) * a.v.sh, dt = b * a.dout.sb + t * a.dout.sl + (long long)(m * R + r) * a.dout.sh;
+#pragma unroll 4
+                for (int p = lane; p < a.P; p += 32) own += ld<T>(a.v.ptr, vt + p) * ld<T>(a.dout.ptr, dt + p);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+            own *= a.scale;
+        }
         for (int n = lane; n < a.N; n += 32) {
             float sq = 0.f, sk = 0.f;
 #pragma unroll 4
@@ -273,8 +305,8 @@ template <class T> __global__ void __launch_bounds__(256) decay_finish(FinishPar
                 sq += a.dqh[from + (long long)r * a.N + n];
                 sk += a.dkh[from + (long long)r * a.N + n];
             }
-            st<T>(a.dq, w * a.N + n, sq);
-            st<T>(a.dk, w * a.N + n, sk);
+            st<T>(a.dq, w * a.N + n, in ? fmaf(own, ld<T>(a.k.ptr, kt + n), sq) : sq);
+            st<T>(a.dk, w * a.N + n, in ? fmaf(own, ld<T>(a.q.ptr, at + n), sk) : sk);
         }
         return;
     }
@@ -283,22 +315,34 @@ template <class T> __global__ void __launch_bounds__(256) decay_finish(FinishPar
     const long long tok = w / a.H, b = tok / a.L, t = tok % a.L;
     const int m = (int)(w % a.H) / R;
     const long long at = b * a.q.sb + t * a.q.sl + m * a.q.sh, kt = b * a.k.sb + t * a.k.sl + m * a.k.sh;
-    float f = 0.f;
+    float x = 0.f, y = 0.f;
 #pragma unroll 4
-    for (int n = lane; n < a.N; n += 32) f += ld<T>(a.q.ptr, at + n) * a.dqh[w * a.N + n] - ld<T>(a.k.ptr, kt + n) * a.dkh[w * a.N + n];
+    for (int n = lane; n < a.N; n += 32) {
+        x += ld<T>(a.q.ptr, at + n) * a.dqh[w * a.N + n];
+        y += ld<T>(a.k.ptr, kt + n) * a.dkh[w * a.N + n];
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
-    if (lane == 0) a.flow[w] = f;
+    for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    if (lane == 0) {
+        a.into[w] = x;
+        a.from[w] = y;
+    }
 }
 
 // dg_t: everything that flows from tokens before t (or the initial state) to t and those after (or the final state) = what crosses
-// the segment's right end + flow of the tokens t ... there.  What crosses is a product of two states, so rounding does not pile
-// up over more than one segment.  A block for a (segment, head).
+// the segment's right end + into - from of the tokens t ... there.  What crosses is a product of two states, so rounding does not pile
+// up over more than one segment.  At a sequence's end these are the final state without what its last token adds, which crosses no decay, and
+// the final state's gradient; all that flows from the last token is that part, and is not counted either.  A block for a (segment, head).
+// Off by 3e-7 to 9e-7 of its norm, whether decays are e^-0.005 or e^-12 a token (with own pairs on both sides 6e-7 to 8e-4, and 1e-2 where these are
+// large: 90 and 130 tokens).
 struct DecayGradParams {
     Plan plan;
     int H, per, g_dtype, out_dtype, L;
-    const float *flow, *enter, *denter;                          // states entering each segment from the left, gradients from the right
-    const float *final_, *dfinal;                                // (sequences, H, per); dfinal NULL: zeros
+    const float *into, *from, *enter, *denter;                   // states entering each segment from the left, gradients from the right
+    const float *final_, *dfinal;                                // (sequences, H, per), final_ without the last tokens' own; dfinal NULL: zeros
     View g;
     void *dg;                                                    // (tokens, H)
 };
@@ -329,7 +373,7 @@ __global__ void __launch_bounds__(256) decay_dg(DecayGradParams a) {
     for (int hi = end; hi > s.t0; hi -= 256) {                   // from the right, thread 0 the last token
         const int t = hi - 1 - tid;
         const long long at = ((long long)s.batch * a.L + t) * a.H + h;
-        double v = t >= s.t0 ? (double)a.flow[at] : 0.0;
+        double v = t >= s.t0 ? (double)a.into[at] - (s.last && t == end - 1 ? 0.f : a.from[at]) : 0.0;
         for (int o = 1; o < 32; o <<= 1) {
             const double u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
