@@ -723,8 +723,8 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
 //     dq_t = sum_s d_ts k_s + S (scale e^{c_t} do_t)
 //     dg_t = e^{c_end} S.G  +  sum_{t' >= t} scale e^{c_t'} do_t'.S^T q_t'  +  sum_{s < t} e^{c_end - c_s} v_s.G^T k_s  +  sum_{s < t <= t'} d_t's q_t'.k_s
 // - every pair of places before and from t on: past and future of the chunk, past and its tokens, its tokens and the future, tokens
-// among themselves; the last as sums over rows less sums over columns of the same fp32 products, so that what cancels does so
-// exactly.  Everything is laid out with s along the rows (lanes): p and d then are operands of dv and dk as they lie, and d of dq
+// among themselves; the last as sums over rows less sums over columns of the same fp32 products, without tokens' own pairs, which would be
+// in both and, where decays are strong, nearly all of them.  Everything is laid out with s along the rows (lanes): p and d then are operands of dv and dk as they lie, and d of dq
 // read the other way.  p goes back to tensor memory, d to shared memory.  A block has a chunk and a head of q and k, and walks (its
 // part of) the heads of v that share them, dq and dk adding up in tensor memory; v and do come a tile ahead, the states while the pairs
 // are weighted, and the products of d run under the next tile's first ones, when nobody waits for them.  Ten of the sixteen warps have weights to make, six lie above the
@@ -964,24 +964,28 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
 #pragma unroll
                     for (int j = j0; j < j0 + 8; j += 4) {
                         const float4 f = f4[j / 4];
-                        vec::f2 w0, w1;
+                        const vec::f2 x0 = vec::pack(x[j], x[j + 1]), x1 = vec::pack(x[j + 2], x[j + 3]);
+                        vec::f2 w0, w1, others0 = x0, others1 = x1;
                         if (cg == quad) {
                             const float e0 = weight(j, f.x), e1 = weight(j + 1, f.y), e2 = weight(j + 2, f.z), e3 = weight(j + 3, f.w);
                             w0 = vec::pack(e0, e1);
                             w1 = vec::pack(e2, e3);
+                            if constexpr (DG) {                  // a token's own pair crosses no decay
+                                others0 = vec::pack(j == lane ? 0.f : x[j], j + 1 == lane ? 0.f : x[j + 1]);
+                                others1 = vec::pack(j + 2 == lane ? 0.f : x[j + 2], j + 3 == lane ? 0.f : x[j + 3]);
+                            }
                         } else {
                             const vec::f2 fs2 = vec::pack(fs, fs);
                             w0 = vec::mul2(vec::pack(f.x, f.y), fs2);
                             w1 = vec::mul2(vec::pack(f.z, f.w), fs2);
                         }
-                        const vec::f2 x0 = vec::pack(x[j], x[j + 1]), x1 = vec::pack(x[j + 2], x[j + 3]);
                         const vec::f2 y0 = vec::mul2(vec::pack(y[j], y[j + 1]), w0), y1 = vec::mul2(vec::pack(y[j + 2], y[j + 3]), w1);
                         p[j / 2] = vec::narrow<T>(vec::mul2(x0, w0));
                         p[j / 2 + 1] = vec::narrow<T>(vec::mul2(x1, w1));
                         d[(j - j0) / 2] = vec::narrow<T>(y0);
                         d[(j - j0) / 2 + 1] = vec::narrow<T>(y1);
-                        if constexpr (DG) {                      // a token's own pair is in its row's and its column's sum
-                            const vec::f2 z0 = vec::mul2(x0, y0), z1 = vec::mul2(x1, y1);
+                        if constexpr (DG) {
+                            const vec::f2 z0 = vec::mul2(others0, y0), z1 = vec::mul2(others1, y1);
                             sum = vec::add2(sum, vec::add2(z0, z1));
                             vec::unpack(z0, x[j], x[j + 1]);
                             vec::unpack(z1, x[j + 2], x[j + 3]);
