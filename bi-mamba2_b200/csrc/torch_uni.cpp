@@ -58,6 +58,12 @@ void on_device(const char *who, const char *name, const Tensor &t, c10::Device d
         ks.has(c10::DispatchKey::FuncTorchGradWrapper) || ks.has(c10::DispatchKey::Functionalize) || t.is_conj() || t.is_neg() || t._is_zerotensor())
         bad(who, ": ", name, " must be a plain dense tensor");
 }
+// A tangent would be dropped: nothing here looks at it.
+void refuse_tangents(const char *who, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        if (t->defined() && t->_fw_grad(0).defined())
+            throw std::runtime_error(std::string(who) + ": an input carries a forward-mode tangent, for which no derivative is defined");
+}
 bool wants_grad(std::initializer_list<const Tensor *> ts) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor *t : ts)
@@ -244,6 +250,8 @@ py::object decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, co
             bad(kAttention, ": initial_state must be float32 ", at::IntArrayRef(state_shape(q, v, cfg)), ", not ", initial->scalar_type(), " ",
                 initial->sizes());
     }
+    const Tensor init = value(initial);
+    refuse_tangents(kAttention, {&q, &k, &v, &g, &init});
     const auto dev = q.device();
     on_device(kAttention, "q", q, dev);
     on_device(kAttention, "k", k, dev);
@@ -252,7 +260,6 @@ py::object decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, co
     if (given(initial)) on_device(kAttention, "initial_state", *initial, dev);
     if (given(cu_)) on_device(kAttention, "cu_seqlens", *cu_, dev);
     const c10::cuda::CUDAGuard guard(dev);
-    const Tensor init = value(initial);
     Tensor cu = value(cu_);
     const bool grad = wants_grad({&q, &k, &v, &g, &init});
     if (grad) refuse_mixed_capture(kAttention, {&q, &k, &v, &g, &init});
@@ -285,6 +292,7 @@ Tensor decay_step(const Tensor &state, const Tensor &q_, const Tensor &k_, const
     if (!given(slots_) && state.size(0) < b) bad(who, ": ", b, " requests and only ", state.size(0), " states");
     if (given(slots_) && (slots_->dim() != 1 || slots_->size(0) != b || (slots_->scalar_type() != at::kInt && slots_->scalar_type() != at::kLong)))
         bad(who, ": slots must be int32 or int64 (", b, ")");
+    refuse_tangents(who, {&state, &q_, &k_, &v_, &g_});
     if (wants_grad({&state, &q_, &k_, &v_, &g_})) throw std::runtime_error(std::string(who) + ": no gradient is defined; call it under torch.no_grad()");
     if (state.size(0) == 0 && b > 0) bad(who, ": no state");
     if (state.size(0) > 0x7fffffffLL || b > 0x7fffffffLL / (h * 8)) bad(who, ": too many requests or states");
@@ -461,6 +469,7 @@ py::object block_norm(const Tensor &x, const Tensor &residual, const OptTensor &
             gate_rows = gate.size(0) > 0 && x.numel() > 0 ? x.numel() / d / gate.size(0) : 1;
         }
     }
+    refuse_tangents(kNorm, {&x, &residual, &gate, &scale, &post, &pre});
     const auto dev = x.device();
     on_device(kNorm, "x", x, dev);
     on_device(kNorm, "residual", residual, dev);

@@ -7,7 +7,7 @@
 x is what a block returned, `out` the residual stream after it and `normed` the next block's input: one pass over the rows
 instead of one for each norm, the gate and the sum.  It stands beside the gated RMSNorm inside BiMamba2 (ssd.bi.layernorm_gated) and
 runs on libbissd's kernels (csrc/block_norm.cuh); there is no CPU path.  Wrong arguments raise ValueError, tensors off the GPU
-RuntimeError.
+and forward-mode derivatives RuntimeError.
 """
 from ssd import _cabi
 

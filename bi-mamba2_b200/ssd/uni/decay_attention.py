@@ -8,8 +8,8 @@ keeps a causal path beside its bidirectional one (src/ssd/uni/); these are a dec
   decay_attention         whole sequences, forward and backward, with the state they start from and the one they end in
   decay_attention_step    one token of every request, the states updated in place
 
-Both run on libbissd's kernels (csrc/uni_*.cuh); there is no CPU path.  Wrong arguments raise ValueError, tensors off the GPU
-RuntimeError.
+Both run on libbissd's kernels (csrc/uni_*.cuh); there is no CPU path.  Wrong arguments raise ValueError, tensors off the GPU and
+forward-mode derivatives RuntimeError.
 """
 from ssd import _cabi
 from ssd.bi.ssd_combined import CHECK_STATUS
