@@ -154,7 +154,7 @@ class DecayAttention(nn.Module):
         q, k, v, dt = torch.split(self.in_proj(u), [qk, qk, self.d_inner, self.nheads], dim=-1)
         g = -torch.exp(self.A_log.float()) * F.softplus(dt.float() + self.dt_bias.float())
         heads = lambda t, n: t.unflatten(-1, (n, -1))
-        return heads(q, self.ngroups), heads(k, self.ngroups), heads(v, self.nheads), g.to(v.dtype)
+        return heads(q, self.ngroups), heads(k, self.ngroups), heads(v, self.nheads), g    # log decays stay float32: they add up over tokens
 
     def init_states(self, slots):
         """Empty states for `slots` requests."""
