@@ -218,9 +218,11 @@ class DecayDecoder(nn.Module):
         """x: (batch, seqlen, d_model) -> the normed stream behind the last block, and with return_final_states a list of states."""
         u, residual, finals = self.norm(x), x.float(), []
         for i, block in enumerate(self.blocks):
-            y, state = block.mixer(u, None if initial_states is None else initial_states[i], True, cu_seqlens)
+            y = block.mixer(u, None if initial_states is None else initial_states[i], return_final_states, cu_seqlens)
+            if return_final_states:
+                y, state = y
+                finals.append(state)
             u, residual = reversed(block.join(y, u, residual))
-            finals.append(state)
         return (u, finals) if return_final_states else u
 
     def step(self, x, states, slots=None):
