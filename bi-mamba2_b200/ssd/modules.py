@@ -195,7 +195,10 @@ class Block(nn.Module):
                           gate_activation=self.gate_activation, eps=self.eps)
 
     def forward(self, u, residual, **kwargs):
-        return self.join(self.mixer(u, **kwargs), u, residual)
+        """(stream, next u), and behind them whatever the mixer returns beside its output (DecayAttention: final states, where asked for)."""
+        y = self.mixer(u, **kwargs)
+        y, *rest = y if isinstance(y, (tuple, list)) else (y,)
+        return (*self.join(y, u, residual), *rest)
 
 
 class DecayDecoder(nn.Module):
