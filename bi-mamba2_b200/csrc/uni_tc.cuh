@@ -480,7 +480,6 @@ struct ChunksParams {
     Heads h;
     Plan chunk;
     int vpc, parts;                                              // tiles of v a block, blocks a (chunk, head of q)
-    int tiles_rows;                                              // NT
     void *o;                                                     // (tokens, H, P) contiguous
     int *status;
 };
