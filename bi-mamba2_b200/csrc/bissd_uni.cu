@@ -214,6 +214,13 @@ struct WalkSpace {                                               // the workspac
     float *states, *decay;
     float *dstates, *ddecay, *final_, *dqh, *dkh, *into, *from, *dg_tokens;   // backward
 };
+void gradient_space(const Sizes &z, Bump &ws, WalkSpace &s) {    // of walk_gradients
+    s.final_ = ws.take<float>((size_t)z.sequences * z.H * z.N * z.P);
+    s.dqh = ws.take<float>((size_t)z.tokens * z.H * z.N);
+    s.dkh = ws.take<float>((size_t)z.tokens * z.H * z.N);
+    s.into = ws.take<float>((size_t)z.tokens * z.H);
+    s.from = ws.take<float>((size_t)z.tokens * z.H);
+}
 WalkSpace walk_space(const bissd_decay_args *a, Bump &ws, bool backward) {
     const Sizes z = sizes_of(a);
     WalkSpace s{};
@@ -226,11 +233,7 @@ WalkSpace walk_space(const bissd_decay_args *a, Bump &ws, bool backward) {
     if (backward) {
         s.dstates = ws.take<float>(states);
         s.ddecay = ws.take<float>(decays);
-        s.final_ = ws.take<float>((size_t)z.sequences * z.H * z.N * z.P);
-        s.dqh = ws.take<float>((size_t)z.tokens * z.H * z.N);
-        s.dkh = ws.take<float>((size_t)z.tokens * z.H * z.N);
-        s.into = ws.take<float>((size_t)z.tokens * z.H);
-        s.from = ws.take<float>((size_t)z.tokens * z.H);
+        gradient_space(z, ws, s);
         if (a->g_per_head) s.dg_tokens = ws.take<float>((size_t)z.tokens * z.H);
     }
     return s;
@@ -270,6 +273,52 @@ int walk_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     return launch_walk(a->dtype, p, s);
 }
 
+// dv, and for each head dk and dq without the tokens' own pairs, and from these dq, dk and dg; given the states that enter the segments from
+// the left and the gradients that enter them from the right (NULL: zeros).
+int walk_gradients(const Walks &w, const WalkSpace &sp, const float *states, const float *dstates, const int *bounds, float *dinitial, const int *again,
+                   cudaStream_t s) {
+    const bissd_decay_args *a = w.a;
+    const Sizes &z = w.z;
+    uni::WalkParams p = walk_params(w, w.q, w.dout, w.k, true);
+    p.a_scale = a->scale; p.init = dstates; p.again = again;
+    p.fin = dinitial; p.first_decay = dinitial != nullptr;
+    p.y = a->dv; p.y_dtype = a->dtype; p.y_batch = (long long)a->seqlen * z.H * z.P;
+    BISSD_DO(launch_walk(a->dtype, p, s));
+    p = walk_params(w, w.dout, w.q, w.v, true);
+    p.a_scale = a->scale; p.init = dstates; p.again = again;
+    p.others = 1; p.y = sp.dkh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
+    BISSD_DO(launch_walk(a->dtype, p, s));
+    p = walk_params(w, w.v, w.k, w.dout, false);
+    p.y_scale = a->scale; p.init = states; p.again = again;
+    p.fin = a->dg && a->dfinal_state ? sp.final_ : nullptr;
+    p.others = 1; p.y = sp.dqh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
+    BISSD_DO(launch_walk(a->dtype, p, s));
+    uni::FinishParams f{};
+    f.L = a->seqlen; f.H = z.H; f.hk = z.hk; f.N = z.N; f.P = z.P; f.tokens = z.tokens; f.scale = a->scale;
+    f.q = w.q.v; f.k = w.k.v; f.v = w.v.v; f.dout = w.dout.v; f.bounds = bounds; f.nseq = a->nseq;
+    f.dqh = sp.dqh; f.dkh = sp.dkh; f.dq = a->dq; f.dk = a->dk; f.again = again;
+    if (a->dg) { f.into = sp.into; f.from = sp.from; }
+    const long long all = (z.tokens * (z.hk + (a->dg ? z.H : 0)) + 7) / 8, grid = again ? std::min(all, 8LL * kSms) : all;
+    if (grid > 0x7fffffffLL || (long long)w.plan.most * z.H > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    BISSD_DO(by_dtype(a->dtype, [&](auto t) -> int {
+        BISSD_LAUNCH("decay_finish", launch_pdl(uni::decay_finish<decltype(t)>, (int)grid, 256, 0, s, f));
+        return BISSD_OK;
+    }));
+    if (!a->dg) return BISSD_OK;
+    uni::DecayGradParams d{};
+    d.plan = w.plan; d.H = z.H; d.per = z.N * z.P; d.g_dtype = a->g_dtype; d.L = a->seqlen;
+    d.out_dtype = a->g_per_head ? BISSD_F32 : a->g_dtype;
+    d.into = sp.into; d.from = sp.from; d.enter = states; d.denter = dstates; d.final_ = sp.final_; d.dfinal = a->dfinal_state; d.g = w.g;
+    d.dg = a->g_per_head ? sp.dg_tokens : a->dg; d.again = again;
+    BISSD_LAUNCH("decay_dg", launch_pdl(uni::decay_dg, w.plan.most * z.H, 256, 0, s, d));
+    return BISSD_OK;
+}
+int launch_dg_heads(const bissd_decay_args *a, const float *dg_tokens, const int *bounds, cudaStream_t s) {
+    BISSD_LAUNCH("decay_dg_heads", launch_pdl(uni::decay_dg_heads, (int)a->nheads, 1024, 0, s, dg_tokens, (long long)a->batch * a->seqlen, (int)a->nheads, a->dg,
+                                              (int)a->g_dtype, bounds, (int)a->nseq));
+    return BISSD_OK;
+}
+
 int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     const WalkSpace sp = walk_space(a, ws, true);
     const Walks w = walks_of(a, sp.plan);
@@ -277,9 +326,6 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     Rest rest;
     rest.rows(a->dv, a->dtype, z.H * z.P);
     if (!a->g_per_head) rest.rows(a->dg, a->g_dtype, z.H);
-    rest.rows(sp.dg_tokens, BISSD_F32, z.H);
-    rest.rows(sp.dqh, BISSD_F32, (long long)z.H * z.N);
-    rest.rows(sp.dkh, BISSD_F32, (long long)z.H * z.N);
     BISSD_DO(rest.launch(a, sp.table, nullptr, s));
     // states that enter the segments from the left, gradients that enter them from the right
     uni::WalkParams p = walk_params(w, w.k, w.v, w.q, false);
@@ -291,39 +337,8 @@ int walk_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     p.a_scale = a->scale; p.fin = sp.dstates; p.decay = sp.ddecay;
     BISSD_DO(launch_walk(a->dtype, p, s));
     BISSD_DO(launch_chain(chain_params(w, true, a->dfinal_state, sp.dstates, sp.ddecay, a->dinitial_state), s));
-    // dv, and for each head dk and dq without the tokens' own pairs
-    p.fin = nullptr; p.decay = nullptr; p.init = sp.dstates;
-    p.y = a->dv; p.y_dtype = a->dtype; p.y_batch = (long long)a->seqlen * z.H * z.P;
-    BISSD_DO(launch_walk(a->dtype, p, s));
-    p = walk_params(w, w.dout, w.q, w.v, true);
-    p.a_scale = a->scale; p.init = sp.dstates;
-    p.others = 1; p.y = sp.dkh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
-    BISSD_DO(launch_walk(a->dtype, p, s));
-    p = walk_params(w, w.v, w.k, w.dout, false);
-    p.y_scale = a->scale; p.init = sp.states;
-    p.fin = a->dg && a->dfinal_state ? sp.final_ : nullptr;
-    p.others = 1; p.y = sp.dqh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
-    BISSD_DO(launch_walk(a->dtype, p, s));
-    uni::FinishParams f{};
-    f.L = a->seqlen; f.H = z.H; f.hk = z.hk; f.N = z.N; f.P = z.P; f.tokens = z.tokens; f.scale = a->scale;
-    f.q = w.q.v; f.k = w.k.v; f.v = w.v.v; f.dout = w.dout.v; f.bounds = sp.table.bounds; f.nseq = a->nseq;
-    f.dqh = sp.dqh; f.dkh = sp.dkh; f.dq = a->dq; f.dk = a->dk; f.into = sp.into; f.from = sp.from;
-    const long long grid = (z.tokens * (z.hk + (a->dg ? z.H : 0)) + 7) / 8;
-    if (grid > 0x7fffffffLL || (long long)sp.plan.most * z.H > 0x7fffffffLL) return BISSD_ERR_SHAPE;
-    BISSD_DO(by_dtype(a->dtype, [&](auto t) -> int {
-        BISSD_LAUNCH("decay_finish", launch_pdl(uni::decay_finish<decltype(t)>, (int)grid, 256, 0, s, f));
-        return BISSD_OK;
-    }));
-    if (!a->dg) return BISSD_OK;
-    uni::DecayGradParams d{};
-    d.plan = sp.plan; d.H = z.H; d.per = z.N * z.P; d.g_dtype = a->g_dtype; d.L = a->seqlen;
-    d.out_dtype = a->g_per_head ? BISSD_F32 : a->g_dtype;
-    d.into = sp.into; d.from = sp.from; d.enter = sp.states; d.denter = sp.dstates; d.final_ = sp.final_; d.dfinal = a->dfinal_state; d.g = w.g;
-    d.dg = a->g_per_head ? sp.dg_tokens : a->dg;
-    BISSD_LAUNCH("decay_dg", launch_pdl(uni::decay_dg, sp.plan.most * z.H, 256, 0, s, d));
-    if (a->g_per_head)
-        BISSD_LAUNCH("decay_dg_heads", launch_pdl(uni::decay_dg_heads, z.H, 1024, 0, s, (const float *)sp.dg_tokens, z.tokens, z.H, a->dg, (int)a->g_dtype));
-    return BISSD_OK;
+    BISSD_DO(walk_gradients(w, sp, sp.states, sp.dstates, sp.table.bounds, nullptr, nullptr, s));
+    return a->dg && a->g_per_head ? launch_dg_heads(a, sp.dg_tokens, sp.table.bounds, s) : BISSD_OK;
 }
 
 using tc::make_map2;
@@ -350,6 +365,9 @@ struct TcSpace {
     uni::Plan seg, chunk;
     uni::PlanOut seg_table{}, chunk_table{};
     bool split;                                                  // sequences in several segments, or packed
+    uni::Again again{};                                          // fp16
+    float *dg_tokens;                                            // backward, one decay for each head
+    size_t kept;                                                 // bytes of the workspace that what is done again does not write over
     uint16_t *tiles;                                              // states as 16-bit tiles
     float *states, *decay;
 };
@@ -384,6 +402,13 @@ TcSpace tc_space(const bissd_decay_args *a, Bump &ws, bool backward) {
     t.chunk = plan_of(a, unitc::kQ, ws, &t.chunk_table);
     t.seg = plan_of(a, tc_segment(a, t.PB), ws, &t.seg_table);
     t.split = t.seg.per_seq > 1;
+    if (a->dtype == BISSD_F16) {
+        t.again.H = a->nheads; t.again.seg = t.seg; t.again.per_segment = a->nheads * t.PB;
+        t.again.flags = ws.take<int>(1 + (size_t)(a->nseq > 0 ? a->nseq : a->batch) * a->nheads);
+        t.again.bad = ws.take<int>((size_t)t.seg.most * t.again.per_segment);
+    }
+    if (backward && a->g_per_head) t.dg_tokens = ws.take<float>((size_t)a->batch * a->seqlen * a->nheads);
+    t.kept = ws.used;
     t.tiles = a->saved ? static_cast<uint16_t *>(a->saved) : ws.take<uint16_t>(tc_tile_values(a, t));
     if (t.split && !(a->saved && backward)) {
         t.states = ws.take<float>((size_t)t.seg.most * a->nheads * a->kdim * a->vdim);
@@ -415,20 +440,24 @@ template <class T> auto grads_kernel(int NT, bool dg) {
                     : (dg ? unitc::decay_grads<T, 128, true> : unitc::decay_grads<T, 128, false>);
 }
 // The states that enter the chunks (or the gradients, backwards), as 16-bit tiles; those that enter and leave the sequences in fp32.
-int tc_states(const bissd_decay_args *a, const TcSpace &t, const CUtensorMap &rows, const CUtensorMap &cols, const CUtensorMap &tiles, bool reverse,
-              const float *start, float *end, float *states, float *decay, int *status, bool clear, cudaStream_t s) {
+int tc_states(const bissd_decay_args *a, TcSpace &t, const CUtensorMap &rows, const CUtensorMap &cols, const CUtensorMap &tiles, bool reverse,
+              const float *start, float *end, float *states, float *decay, int *status, bool clear, bool first, cudaStream_t s) {
     unitc::StatesParams p{};
     p.h = tc_heads(a, t.PB);
     p.seg = t.seg; p.chunk = t.chunk; p.reverse = reverse; p.status = status;
     p.clear = clear;
+    p.again = first ? t.again.flags : nullptr;
     const long long grid = (long long)t.seg.most * a->nheads * t.PB;
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    if (end) t.again.bads = t.again.flags ? (int)grid : 0;
     auto launch = [&](const char *name, bool exact) -> int {
         const auto kernel = a->dtype == BISSD_BF16 ? states_kernel<__nv_bfloat16>(t.NT, exact) : states_kernel<__half>(t.NT, exact);
         const size_t smem = unitc::states_smem(t.NT, exact);
+        p.bad = exact ? t.again.bad : nullptr;
         BISSD_ALLOW(kernel, smem);
         BISSD_LAUNCH(name, launch_pdl(kernel, (int)grid, unitc::kStatesThreads, smem, s, p, rows, cols, tiles));
         p.clear = 0;
+        p.again = nullptr;
         return BISSD_OK;
     };
     if (t.split) {
@@ -449,10 +478,19 @@ bool tc_tile_map(CUtensorMap *m, const bissd_decay_args *a, const TcSpace &t, co
     return make_map2(m, a->dtype, tiles, unitc::kP, (unsigned long long)t.chunk.most * a->nheads * t.PB * t.NT, unitc::kP, t.NT);
 }
 
+// Sequences as they are walked again on CUDA cores: one segment each.
+Walks again_walks(const bissd_decay_args *a, const TcSpace &t) {
+    uni::Plan p{};
+    p.packed = a->nseq > 0; p.L = p.seg = a->seqlen; p.per_seq = 1;
+    p.most = a->nseq > 0 ? a->nseq : a->batch;
+    p.bounds = t.chunk_table.bounds;
+    return walks_of(a, p);
+}
+
 constexpr double kChunkStart = 2.0;                              // a block's start and the product q.k, in tiles of v
 
 int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
-    const TcSpace t = tc_space(a, ws, false);
+    TcSpace t = tc_space(a, ws, false);
     int *status = reinterpret_cast<int *>(ws.base);
     if ((long long)t.chunk.most * a->nheads * t.PB * t.NT > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     CUtensorMap q, k, v, tiles;
@@ -465,10 +503,10 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     rest.p.start = a->initial_state;
     rest.p.end = t.split ? nullptr : a->final_state;             // the chain sees to them otherwise
     BISSD_DO(rest.launch(a, t.chunk_table, &t.seg_table, s));
-    BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, a->nseq == 0, s));
+    BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, a->final_state, t.states, t.decay, status, a->nseq == 0, true, s));
     unitc::ChunksParams p{};
     p.h = tc_heads(a, t.PB);
-    p.chunk = t.chunk; p.o = a->o; p.status = status;
+    p.chunk = t.chunk; p.o = a->o; p.status = status; p.again = t.again;
     // blocks a (chunk, head of q): as many as fill two blocks an SM, in the fewest rounds
     const int tiles_v = a->nheads / a->nkheads * t.PB;
     const long long items = (long long)t.chunk.most * a->nkheads, slots = 2 * kSms;
@@ -488,7 +526,14 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     if (grid > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     BISSD_ALLOW(kernel, smem);
     BISSD_LAUNCH("decay_chunks", launch_pdl(kernel, (int)grid, 256, smem, s, p, q, k, v, tiles));
-    return BISSD_OK;
+    if (!t.again.flags) return BISSD_OK;
+    const Walks w = again_walks(a, t);
+    uni::WalkParams f = walk_params(w, w.k, w.v, w.q, false);
+    f.again = t.again.flags;
+    f.init = a->initial_state; f.fin = a->final_state;
+    f.y = a->o; f.y_dtype = a->dtype; f.y_scale = a->scale;
+    f.y_batch = (long long)a->seqlen * w.z.H * w.z.P;
+    return launch_walk(a->dtype, f, s);
 }
 
 struct TcGradSpace {
@@ -496,7 +541,7 @@ struct TcGradSpace {
     uint16_t *grads;                                                 // tiles of the states' gradients
     float *gstates, *gdecay;
     int vpc, parts;
-    float *part, *dg_tokens;
+    float *part;
 };
 TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
     TcGradSpace g{};
@@ -523,7 +568,6 @@ TcGradSpace tc_grad_space(const bissd_decay_args *a, Bump &ws) {
         }
     }
     if (g.parts > 1) g.part = ws.take<float>((size_t)2 * g.parts * tokens * a->nkheads * a->kdim);
-    if (a->g_per_head) g.dg_tokens = ws.take<float>((size_t)tokens * a->nheads);
     return g;
 }
 bool tc_backward_ok(const bissd_decay_args *a) {
@@ -531,8 +575,8 @@ bool tc_backward_ok(const bissd_decay_args *a) {
 }
 
 int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
-    const TcGradSpace g = tc_grad_space(a, ws);
-    const TcSpace &t = g.t;
+    TcGradSpace g = tc_grad_space(a, ws);
+    TcSpace &t = g.t;
     int *status = reinterpret_cast<int *>(ws.base);
     if ((long long)t.chunk.most * a->nheads * t.PB * t.NT > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     CUtensorMap q, k, v, dout, tiles, grads;
@@ -545,21 +589,21 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     rest.rows(a->dq, a->dtype, a->nkheads * a->kdim);
     rest.rows(a->dk, a->dtype, a->nkheads * a->kdim);
     if (!a->g_per_head) rest.rows(a->dg, a->g_dtype, a->nheads);
-    rest.rows(g.dg_tokens, BISSD_F32, a->nheads);
     rest.p.start = a->dfinal_state;
     rest.p.end = t.split ? nullptr : a->dinitial_state;
     rest.p.parts = g.part; rest.p.n_parts = g.part ? 2 * g.parts : 0; rest.p.part_row = (long long)a->nkheads * a->kdim;
     BISSD_DO(rest.launch(a, t.chunk_table, &t.seg_table, s));
-    if (!a->saved) BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, a->nseq == 0, s));
-    BISSD_DO(tc_states(a, t, q, dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, a->saved && a->nseq == 0, s));
+    if (!a->saved) BISSD_DO(tc_states(a, t, k, v, tiles, false, a->initial_state, nullptr, t.states, t.decay, status, a->nseq == 0, true, s));
+    BISSD_DO(tc_states(a, t, q, dout, grads, true, a->dfinal_state, a->dinitial_state, g.gstates, g.gdecay, status, a->saved && a->nseq == 0,
+                       a->saved != nullptr, s));
     unitc::GradsParams p{};
     p.h = tc_heads(a, t.PB);
     p.chunk = t.chunk; p.vpc = g.vpc; p.parts = g.parts;
     p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
     p.part = g.part; p.tokens = (long long)a->batch * a->seqlen;
-    p.dg = a->dg ? (a->g_per_head ? g.dg_tokens : a->dg) : nullptr;
+    p.dg = a->dg ? (a->g_per_head ? t.dg_tokens : a->dg) : nullptr;
     p.dg_dtype = a->g_per_head ? BISSD_F32 : a->g_dtype;
-    p.status = status;
+    p.status = status; p.again = t.again;
     const bool dg = p.dg != nullptr;
     const auto kernel = a->dtype == BISSD_BF16 ? grads_kernel<__nv_bfloat16>(t.NT, dg) : grads_kernel<__half>(t.NT, dg);
     const size_t smem = unitc::grads_smem(t.NT);
@@ -579,10 +623,15 @@ int tc_backward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
         });
         if (rc != BISSD_OK) return rc;
     }
-    if (a->dg && a->g_per_head)
-        BISSD_LAUNCH("decay_dg_heads", launch_pdl(uni::decay_dg_heads, (int)a->nheads, 1024, 0, s, (const float *)g.dg_tokens, p.tokens, (int)a->nheads, a->dg,
-                                                  (int)a->g_dtype));
-    return BISSD_OK;
+    if (t.again.flags) {
+        Bump over{ws.base, t.kept};
+        const Walks w = again_walks(a, t);
+        WalkSpace sp{};
+        gradient_space(w.z, over, sp);
+        sp.dg_tokens = t.dg_tokens;
+        BISSD_DO(walk_gradients(w, sp, a->initial_state, a->dfinal_state, t.chunk_table.bounds, a->dinitial_state, t.again.flags, s));
+    }
+    return a->dg && a->g_per_head ? launch_dg_heads(a, t.dg_tokens, t.chunk_table.bounds, s) : BISSD_OK;
 }
 
 }  // namespace
@@ -613,7 +662,15 @@ int bissd_decay_workspace_bytes(const bissd_decay_args *a, size_t *fwd_bytes, si
     if (bwd_bytes) {
         Bump b{nullptr}, c{nullptr};
         walk_space(a, b, true);
-        if (tc_sizes(a)) tc_grad_space(a, c);
+        if (tc_sizes(a)) {
+            const size_t kept = tc_grad_space(a, c).t.kept;
+            if (a->dtype == BISSD_F16) {
+                Bump over{nullptr, kept};
+                WalkSpace sp{};
+                gradient_space(sizes_of(a), over, sp);
+                c.used = std::max(c.used, over.used);
+            }
+        }
         *bwd_bytes = std::max(b.used, c.used);
     }
     return BISSD_OK;

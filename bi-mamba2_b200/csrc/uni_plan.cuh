@@ -11,6 +11,7 @@ struct Plan {
     int packed, L, seg, per_seq, most;                           // most: segments there can be (all of them where not packed)
     const int4 *table;                                           // packed: first token, tokens, sequence, 2 * index + last
     const int *first;                                            // packed: (nseq + 1) first segment of each sequence
+    const int *bounds;                                           // packed, each sequence one segment: (nseq + 1) boundaries, no table; or NULL
 };
 struct Segment {
     int batch, t0, len, seq, idx;                                // len 0: there is no such segment
@@ -19,7 +20,9 @@ struct Segment {
 
 __device__ __forceinline__ Segment segment(const Plan &p, int i) {
     Segment s;
-    if (p.packed) {
+    if (p.bounds) {
+        s.batch = s.idx = 0; s.t0 = p.bounds[i]; s.len = p.bounds[i + 1] - s.t0; s.seq = i; s.last = true;
+    } else if (p.packed) {
         const int4 e = __ldg(p.table + i);
         s.batch = 0; s.t0 = e.x; s.len = e.y; s.seq = e.z; s.idx = e.w >> 1; s.last = e.w & 1;
     } else {
@@ -35,6 +38,25 @@ __device__ __forceinline__ Segment segment(const Plan &p, int i) {
 __device__ __forceinline__ int2 segments(const Plan &p, int seq) {
     if (!p.packed) return make_int2(seq * p.per_seq, p.per_seq);
     return make_int2(p.first[seq], p.first[seq + 1] - p.first[seq]);
+}
+
+// Calls in fp16 on the tensor cores whose products leave the type's range somewhere: heads of sequences that are to be done again, on CUDA
+// cores in fp32.  flags[0]: any of them; flags[1 + sequence H + head].  Cleared in a call's first kernel that goes by sequences, set in later
+// ones, read in those behind; `bad`: by blocks of decay_states, whether the state that leaves the library left the range.
+struct Again {
+    int *flags, *bad;
+    int H, bads, per_segment;                                    // bads: blocks, per_segment of them to a segment of `seg`
+    Plan seg;
+};
+__device__ __forceinline__ bool again(const int *flags, int H, int seq, int h) { return flags[0] && flags[1 + (long long)seq * H + h]; }
+// Every gradient of heads that share q and k is done again where one of them is: R heads, R = 1 for outputs.
+__device__ __forceinline__ void do_again(const Again &a, int seq, int h, int R) {
+    a.flags[0] = 1;
+    for (int r = 0; r < R; ++r) a.flags[1 + (long long)seq * a.H + h / R * R + r] = 1;
+}
+__device__ __forceinline__ void do_again_states(const Again &a, int R, int threads) {   // what decay_states found; all blocks of a launch
+    for (int i = blockIdx.x * threads + threadIdx.x; i < a.bads; i += gridDim.x * threads)
+        if (a.bad[i]) do_again(a, segment(a.seg, i / a.per_segment).seq, i % a.per_segment / (a.per_segment / a.H), R);
 }
 
 struct PlanOut {                                                 // one table for each segment length

@@ -9,6 +9,10 @@
 // fp32 has no number for: -inf never meets +inf.  Factors that reach to a chunk's ends are 2 to the power of a sum that starts there, and
 // those between two tokens from sums that start at one of them, or in two parts (Decays), so that a strong decay elsewhere in the chunk
 // costs no digits.
+// Products take operands of T: states, pairs and weighted rows are rounded to it.  In fp16 they may be out of its range where inputs and
+// outputs are not.  An operand that is no number leaves no number in every sum that it enters, so the kernels look at their fp32 sums alone,
+// and heads of sequences where one is none are done again by uni_walk.cuh's kernels, which leave at once where there are none (3.6 us a
+// launch: a forward pass has one, a backward pass five; 8 x 2048 tokens of 24 heads, both passes, 265 us before, 293 so).
 #pragma once
 #include "tc_tma.cuh"
 #include "uni_plan.cuh"
@@ -175,6 +179,8 @@ struct StatesParams {
     float *fin, *decay;                                          // decay: (segments, H) the segment's whole decay, or NULL
     int *status;
     int clear;                                                   // the status, by the first block: any wait of another takes far longer to run out
+    int *again;                                                  // fp16: flags of what is to be done again, cleared; or NULL
+    int *bad;                                                    // fp16, EXACT: by blocks, whether what leaves is out of fp16's range; or NULL
 };
 // The thread's tile stores so far have read their shared memory.
 __device__ __forceinline__ void tma_store_read() {
@@ -184,7 +190,7 @@ __device__ __forceinline__ void tma_store_read() {
 struct StatesShared {
     uint64_t full[2], full_v[2], ready, done, weights, stored, unused;
     uint32_t tmem;
-    int fail, loads, loads_v;                                    // fail: the first wait that ran out; loads asked for
+    int fail, loads, loads_v, bad;                               // fail: the first wait that ran out; loads asked for
     float decay[2];                                              // of a chunk, 2^c_end
     alignas(16) uint32_t w[kQ];                                  // of a chunk's rows: f1 and f2, or EXACT fp32
 };
@@ -195,6 +201,7 @@ template <class T, int NT, bool EXACT> __global__ void __launch_bounds__(kStates
 decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
     if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+    if (a.again && blockIdx.x == 0 && threadIdx.x == 0) a.again[0] = 0;
     constexpr int kSlabs = NT / 64;
     extern __shared__ __align__(1024) uint8_t dyn[];
     // two stages of k, two of weighted rows, S.  EXACT: one of k, v's rows, two parts, v's rows, S
@@ -203,7 +210,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pb = blockIdx.x % a.h.PB, h = blockIdx.x / a.h.PB % a.h.H, si = blockIdx.x / (a.h.PB * a.h.H), hq = h * a.h.hk / a.h.H;
     const Segment s = uni::segment(a.seg, si);
+    if (a.bad && tid == 0 && s.len == 0) a.bad[blockIdx.x] = 0;
     if (s.len == 0) return;                                      // packed: fewer segments than there could be
+    if (a.again && tid == 0 && pb == 0 && s.idx == 0) a.again[1 + (long long)s.seq * a.h.H + h] = 0;
     if (smem_u32(dyn) & 1023) {                                  // the swizzled tiles' alignment, which nothing else here sees to
         if (tid == 0) atomicExch(a.status, kErrDecay + 4);
         return;
@@ -222,7 +231,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         mbar_init(&sh.done, 1);
         mbar_init(&sh.weights, 1);
         mbar_init(&sh.stored, 1);
-        sh.fail = 0;
+        sh.fail = sh.bad = 0;
         fence_mbar_init();
     }
     tc_fence_before();
@@ -451,6 +460,12 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
             for (int j = 0; j < 32; ++j)
                 if (col + j < a.h.P) a.fin[at + j] = S[j];
+            if (a.bad) {                                         // a row times a weight above 1, in a part of 16 bits
+                float none = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) none = fmaf(S[j], 0.f, none);
+                if (none != 0.f) sh.bad = 1;
+            }
         }
     }
     tc_fence_before();
@@ -464,6 +479,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         }
         __syncthreads();
     }
+    if (a.bad && tid == 0) a.bad[blockIdx.x] = sh.bad;
     if (warp == 0) tmem_dealloc(tmem, EXACT ? 256 : 64);
 }
 
@@ -482,6 +498,7 @@ struct ChunksParams {
     int vpc, parts;                                              // tiles of v a block, blocks a (chunk, head of q)
     void *o;                                                     // (tokens, H, P) contiguous
     int *status;
+    uni::Again again;                                            // fp16
 };
 inline size_t chunks_smem(int NT) { return 1024 + (size_t)(NT / 64) * kSlab + 2 * (size_t)kSlab + (size_t)kSlab + (size_t)NT * 128; }
 
@@ -489,6 +506,8 @@ template <class T, int NT> __global__ void __launch_bounds__(256, 2)
 decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
              const __grid_constant__ CUtensorMap tmS) {
     pdl_begin();
+    constexpr bool kNarrow = std::is_same<T, __half>::value;     // what lies between inputs and outputs may be out of T's range
+    if constexpr (kNarrow) uni::do_again_states(a.again, 1, 256);
     constexpr int kSlabs = NT / 64, kTables = 8;                 // heads whose tables are made at a time, one a warp
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ uint64_t bar_qk, bar_v, bar_s, done, done_s, unused;
@@ -671,16 +690,20 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         // o = inside + scale e^{c_t} from the state; whole rows leave through the first slab of the weighted pairs
         if (ok) {
             const float f = exp2f(ct + lt);
-            float x[32], y[32];
+            float x[32], y[32], none = 0.f;
             tmem_ld32(tl + 128 + half * 32, x);
             tmem_ld32(tl + 192 + half * 32, y);
 #pragma unroll
             for (int j = 0; j < 32; j += 8) {
                 float e[8];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) e[q] = fmaf(y[j + q], f, x[j + q]);
+                for (int q = 0; q < 8; ++q) {
+                    e[q] = fmaf(y[j + q], f, x[j + q]);
+                    if constexpr (kNarrow) none = fmaf(e[q], 0.f, none);
+                }
                 *reinterpret_cast<uint4 *>(smK + t * 128 + (((half * 4 + (j >> 3)) ^ (t & 7)) << 4)) = pack8<T>(e);
             }
+            if (kNarrow && none != 0.f && t < s.len) uni::do_again(a.again, s.seq, h, 1);
         }
         tc_fence_before();
         ok = __syncthreads_and(ok);
@@ -740,6 +763,7 @@ struct GradsParams {
     void *dg;                                                    // DG: (tokens, H)
     int dg_dtype;
     int *status;
+    uni::Again again;                                            // fp16
 };
 inline size_t grads_smem(int NT) { return 1024 + 2 * (size_t)(NT / 64) * kSlab + 4 * (size_t)kSlab + 3 * (size_t)kSlab + 2 * (size_t)NT * 128; }
 
@@ -766,6 +790,8 @@ template <class T, int NT, bool DG> __global__ void __launch_bounds__(512, 1)
 decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmG) {
     pdl_begin();
+    constexpr bool kNarrow = std::is_same<T, __half>::value;     // what lies between inputs and outputs may be out of T's range
+    if constexpr (kNarrow) uni::do_again_states(a.again, a.h.H / a.h.hk, 512);
     constexpr int kSlabs = NT / 64, kT = 512;
     constexpr int kTables = 2, kHelp = 3, kIssue = 7, kSums = 11;   // warps above the diagonal
     extern __shared__ __align__(1024) uint8_t dyn[];
@@ -1085,7 +1111,7 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         tc_fence_after();
         if (ok) {                                                // row s (or t), columns 16 cg ... of v's 64
             float own[16], far[16], o[16];
-            vec::f2 f = vec::pack(0.f, 0.f), p = f;
+            vec::f2 f = vec::pack(0.f, 0.f), p = f, none = f;
             tmem_ld16(tl + cOwn + cg * 16, own);
             tmem_ld16(tl + cFar + cg * 16, far);
             if constexpr (DG) tmem_ld16(tl + cOut + cg * 16, o);
@@ -1103,10 +1129,13 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                         f = vec::fma2(vec::widen<T>(vs[k]), far2, f);
                         p = vec::fma2(vec::widen<T>(ds[k]), vec::pack(o[j + 2 * k], o[j + 2 * k + 1]), p);
                     }
-                    to[k] = vec::narrow<T>(vec::fma2(w, far2, vec::pack(own[j + 2 * k], own[j + 2 * k + 1])));
+                    const vec::f2 sum = vec::fma2(w, far2, vec::pack(own[j + 2 * k], own[j + 2 * k + 1]));
+                    if constexpr (kNarrow) none = vec::fma2(sum, vec::pack(0.f, 0.f), none);
+                    to[k] = vec::narrow<T>(sum);
                 }
                 *reinterpret_cast<uint4 *>(sV + at) = make_uint4(to[0], to[1], to[2], to[3]);   // dv, where this thread alone has read v
             }
+            if (kNarrow && both(none) != 0.f && s < len) uni::do_again(a.again, sg.seq, h, R);
             if constexpr (DG) {
                 future[cg][s] = both(f) + (first ? 0.f : future[cg][s]);
                 past[cg][s] = both(p) + (first ? 0.f : past[cg][s]);
@@ -1167,6 +1196,12 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
                 float x[16];
                 tmem_ld16(at + j0, x);
                 const int n = cg * kCols + j0;
+                if constexpr (kNarrow) {
+                    float none = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) none = fmaf(x[j], 0.f, none);
+                    if (none != 0.f && s < len) uni::do_again(a.again, sg.seq, h0, R);
+                }
                 if (a.parts > 1) {
                     float *o = a.part + (((long long)(what * a.parts + part) * a.tokens + token + s) * a.h.hk + m) * a.h.N + n;
 #pragma unroll

@@ -35,6 +35,8 @@ struct WalkParams {
     float *fin;                                                  // what leaves: (segments, H, ..), or NULL; kOthers: (sequences, H, ..), without the last token's own
     float *decay;                                                // (segments, H): the segment's whole decay, or NULL
     int si, sj;                                                  // strides of S's two sides in init and fin
+    int first_decay;                                             // backwards, a whole sequence a segment: fin is one decay further back
+    const int *again;                                            // flags of what is to be done, or NULL: everything
     int *status;                                                 // cleared, or NULL
 };
 
@@ -57,8 +59,9 @@ template <class T, int IPT, int Y> __global__ void __launch_bounds__(kWalkThread
     float *ys = dyn + 2 * stage_len;
     const int jb = (a.J + cols - 1) / cols;
     const int cb = blockIdx.x % jb, h = blockIdx.x / jb % a.H, si = blockIdx.x / (jb * a.H);
+    if (a.again && !a.again[0]) return;
     const Segment s = segment(a.plan, si);
-    if (s.len == 0) return;
+    if (s.len == 0 || (a.again && !again(a.again, a.H, s.seq, h))) return;
     const int tid = threadIdx.x, li = tid % LI, jc = tid / LI, j = cb * cols + jc, hq = h * a.hk / a.H;
     const long long S = (long long)a.I * a.J;
     float st_[IPT];
@@ -185,6 +188,11 @@ template <class T, int IPT, int Y> __global__ void __launch_bounds__(kWalkThread
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (a.fin && (Y != kOthers || s.last)) {
         const long long to = Y == kOthers ? s.seq : si;
+        if (a.first_decay) {
+            const float d = expf(ld_any(a.g.ptr, a.g_dtype, (long long)s.batch * a.g.sb + (long long)s.t0 * a.g.sl + (long long)h * a.g.sh));
+#pragma unroll
+            for (int e = 0; e < IPT; ++e) st_[e] *= d;
+        }
 #pragma unroll
         for (int e = 0; e < IPT; ++e) {
             const int i = li * IPT + e;
@@ -277,58 +285,78 @@ struct FinishParams {
     const float *dqh, *dkh;                                      // (tokens, H, N), others' part
     void *dq, *dk;                                               // (tokens, hk, N)
     float *into, *from;                                          // (tokens, H)
+    const int *again;                                            // as in WalkParams
 };
 template <class T> __global__ void __launch_bounds__(256) decay_finish(FinishParams a) {
     pdl_begin();
-    long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (a.again && !a.again[0]) return;
     const int lane = threadIdx.x & 31, R = a.H / a.hk;
-    if (w < a.tokens * a.hk) {
-        const long long from = w * R * a.N, tok = w / a.hk, b = tok / a.L, t = tok % a.L;
-        const int m = (int)(w % a.hk);
-        const long long at = b * a.q.sb + t * a.q.sl + m * a.q.sh, kt = b * a.k.sb + t * a.k.sl + m * a.k.sh;
+    const long long sums = a.tokens * a.hk, all = sums + (a.into ? a.tokens * a.H : 0);
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < all; i += (long long)gridDim.x * 8) {
+        const long long w = i < sums ? i : i - sums, tok = i < sums ? w / a.hk : w / a.H, b = tok / a.L, t = tok % a.L;
+        const int m = i < sums ? (int)(w % a.hk) : (int)(w % a.H) / R;
         const bool in = !a.bounds || (t >= a.bounds[0] && t < a.bounds[a.nseq]);
-        float own = 0.f;
-        if (in) {
-            for (int r = 0; r < R; ++r) {
-                const long long vt = b * a.v.sb + t * a.v.sl + (long long)(m * R + r) * a.v.sh, dt = b * a.dout.sb + t * a.dout.sl + (long long)(m * R + r) * a.dout.sh;
-#pragma unroll 4
-                for (int p = lane; p < a.P; p += 32) own += ld<T>(a.v.ptr, vt + p) * ld<T>(a.dout.ptr, dt + p);
+        if (a.again) {
+            if (!in) continue;
+            int seq = (int)b;
+            if (a.bounds) {                                      // the last sequence that begins at t or before it and is not behind it
+                int lo = 0, hi = a.nseq;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if (a.bounds[mid] <= t) lo = mid;
+                    else hi = mid;
+                }
+                seq = lo;
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
-            own *= a.scale;
+            if (!again(a.again, a.H, seq, m * R)) continue;
         }
+        const long long at = b * a.q.sb + t * a.q.sl + m * a.q.sh, kt = b * a.k.sb + t * a.k.sl + m * a.k.sh;
+        if (i < sums) {
+            const long long from = w * R * a.N;
+            float own = 0.f;
+            if (in) {
+                for (int r = 0; r < R; ++r) {
+                    const long long vt = b * a.v.sb + t * a.v.sl + (long long)(m * R + r) * a.v.sh,
+                                    dt = b * a.dout.sb + t * a.dout.sl + (long long)(m * R + r) * a.dout.sh;
+#pragma unroll 4
+                    for (int p = lane; p < a.P; p += 32) own += ld<T>(a.v.ptr, vt + p) * ld<T>(a.dout.ptr, dt + p);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+                own *= a.scale;
+            }
+            for (int n = lane; n < a.N; n += 32) {
+                float sq = 0.f, sk = 0.f;
+                if (in) {
+#pragma unroll 4
+                    for (int r = 0; r < R; ++r) {
+                        sq += a.dqh[from + (long long)r * a.N + n];
+                        sk += a.dkh[from + (long long)r * a.N + n];
+                    }
+                    sq = fmaf(own, ld<T>(a.k.ptr, kt + n), sq);
+                    sk = fmaf(own, ld<T>(a.q.ptr, at + n), sk);
+                }
+                st<T>(a.dq, w * a.N + n, sq);
+                st<T>(a.dk, w * a.N + n, sk);
+            }
+            continue;
+        }
+        if (!in) continue;                                       // of no use to anyone
+        float x = 0.f, y = 0.f;
+#pragma unroll 4
         for (int n = lane; n < a.N; n += 32) {
-            float sq = 0.f, sk = 0.f;
-#pragma unroll 4
-            for (int r = 0; r < R; ++r) {
-                sq += a.dqh[from + (long long)r * a.N + n];
-                sk += a.dkh[from + (long long)r * a.N + n];
-            }
-            st<T>(a.dq, w * a.N + n, in ? fmaf(own, ld<T>(a.k.ptr, kt + n), sq) : sq);
-            st<T>(a.dk, w * a.N + n, in ? fmaf(own, ld<T>(a.q.ptr, at + n), sk) : sk);
+            x += ld<T>(a.q.ptr, at + n) * a.dqh[w * a.N + n];
+            y += ld<T>(a.k.ptr, kt + n) * a.dkh[w * a.N + n];
         }
-        return;
-    }
-    w -= a.tokens * a.hk;
-    if (w >= a.tokens * a.H) return;
-    const long long tok = w / a.H, b = tok / a.L, t = tok % a.L;
-    const int m = (int)(w % a.H) / R;
-    const long long at = b * a.q.sb + t * a.q.sl + m * a.q.sh, kt = b * a.k.sb + t * a.k.sl + m * a.k.sh;
-    float x = 0.f, y = 0.f;
-#pragma unroll 4
-    for (int n = lane; n < a.N; n += 32) {
-        x += ld<T>(a.q.ptr, at + n) * a.dqh[w * a.N + n];
-        y += ld<T>(a.k.ptr, kt + n) * a.dkh[w * a.N + n];
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o);
-        y += __shfl_xor_sync(0xffffffffu, y, o);
-    }
-    if (lane == 0) {
-        a.into[w] = x;
-        a.from[w] = y;
+        for (int o = 16; o > 0; o >>= 1) {
+            x += __shfl_xor_sync(0xffffffffu, x, o);
+            y += __shfl_xor_sync(0xffffffffu, y, o);
+        }
+        if (lane == 0) {
+            a.into[w] = x;
+            a.from[w] = y;
+        }
     }
 }
 
@@ -345,13 +373,15 @@ struct DecayGradParams {
     const float *final_, *dfinal;                                // (sequences, H, per), final_ without the last tokens' own; dfinal NULL: zeros
     View g;
     void *dg;                                                    // (tokens, H)
+    const int *again;                                            // as in WalkParams
 };
 __global__ void __launch_bounds__(256) decay_dg(DecayGradParams a) {
     pdl_begin();
     __shared__ double part[8], carry;
     const int h = blockIdx.x % a.H, si = blockIdx.x / a.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (a.again && !a.again[0]) return;
     const Segment s = segment(a.plan, si);
-    if (s.len == 0) return;
+    if (s.len == 0 || (a.again && !again(a.again, a.H, s.seq, h))) return;
     const int end = s.t0 + s.len;
     double cross = 0.0;
     if (!s.last || a.dfinal) {
@@ -389,12 +419,15 @@ __global__ void __launch_bounds__(256) decay_dg(DecayGradParams a) {
     }
 }
 
-// One decay for each head: the sum of its tokens' gradients, in a fixed order.
-__global__ void __launch_bounds__(1024) decay_dg_heads(const float *dg, long long tokens, int H, void *out, int dtype) {
+// One decay for each head: the sum of its tokens' gradients, in a fixed order.  bounds: of packed sequences, or NULL.
+__global__ void __launch_bounds__(1024) decay_dg_heads(const float *dg, long long tokens, int H, void *out, int dtype, const int *bounds, int nseq) {
     pdl_begin();
     __shared__ double part[32];
     double v = 0.0;
-    for (long long t = threadIdx.x; t < tokens; t += 1024) v += dg[t * H + blockIdx.x];
+    const int first = bounds ? bounds[0] : 0;
+    const long long end = bounds ? bounds[nseq] : tokens;
+    for (long long t = threadIdx.x; t < end; t += 1024)
+        if (t >= first) v += dg[t * H + blockIdx.x];
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();

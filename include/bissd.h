@@ -278,7 +278,9 @@ int bissd_layer_params_out(const bissd_layer_params *args, void *stream);
  * tokens cu_seqlens[i] ... cu_seqlens[i + 1] - 1 (device memory; what lies outside 0 ... seqlen or runs backwards is
  * taken as the nearest that does not).  Tokens of no sequence get zeros in o, dq, dk, dv and dg.
  * Log decays are meant to be <= 0; -inf empties the state.  kdim and vdim from 1 to 256.
- * The states are fp32 wherever they leave the library, and there as exact as fp32 sums of the inputs' products. */
+ * The states are fp32 wherever they leave the library, and there as exact as fp32 sums of the inputs' products.
+ * 16-bit operands of products between inputs and outputs: heads of sequences where fp16 has no number for one of them are computed again in
+ * fp32, in the same call. */
 typedef struct bissd_decay_args {
     int32_t batch, seqlen, nheads, nkheads, kdim, vdim;
     int32_t nseq;                        /* 0: each row of the batch is a sequence */
