@@ -155,6 +155,23 @@ int launch_walk(int dtype, const uni::WalkParams &w, cudaStream_t s) {
         return BISSD_OK;
     });
 }
+// out: a forward pass's, or dv; dk and dq NULL in a forward pass.
+int launch_walks_again(uni::WalkParams out, const uni::WalkParams *dk, const uni::WalkParams *dq, cudaStream_t s) {
+    uni::WalkParams w[3] = {out, dk ? *dk : out, dq ? *dq : out};
+    size_t smem = 0;
+    long long blocks[3] = {}, all = 0;
+    for (int i = 0; i < (dk ? 3 : 1); ++i) {
+        w[i].lanes = 1;
+        while (w[i].lanes * uni::kAgainRows < w[i].I) w[i].lanes *= 2;
+        smem = std::max(smem, uni::walk_smem(w[i].lanes, uni::kAgainRows));
+        all += blocks[i] = (long long)w[i].plan.most * w[i].H * ceil_div(w[i].J, uni::kWalkThreads / w[i].lanes);
+    }
+    if (all > 0x7fffffffLL) return BISSD_ERR_SHAPE;
+    BISSD_ALLOW(uni::decay_walks_again<__half>, smem);
+    BISSD_LAUNCH("decay_walks_again", launch_pdl(uni::decay_walks_again<__half>, (int)std::min<long long>(all, 4 * kSms), uni::kWalkThreads, smem, s, w[0], w[1], w[2],
+                                                 (int)blocks[0], (int)blocks[1], (int)all));
+    return BISSD_OK;
+}
 int launch_chain(const uni::ChainParams &c, cudaStream_t s) {
     const bool quads = c.per % 4 == 0 && aligned16(c.start) && aligned16(c.states) && aligned16(c.end);
     const long long grid = (long long)c.nseq * c.H * ceil_div(c.per, quads ? 1024 : 256);
@@ -279,26 +296,29 @@ int walk_gradients(const Walks &w, const WalkSpace &sp, const float *states, con
                    cudaStream_t s) {
     const bissd_decay_args *a = w.a;
     const Sizes &z = w.z;
-    uni::WalkParams p = walk_params(w, w.q, w.dout, w.k, true);
-    p.a_scale = a->scale; p.init = dstates; p.again = again;
-    p.fin = dinitial; p.first_decay = dinitial != nullptr;
-    p.y = a->dv; p.y_dtype = a->dtype; p.y_batch = (long long)a->seqlen * z.H * z.P;
-    BISSD_DO(launch_walk(a->dtype, p, s));
-    p = walk_params(w, w.dout, w.q, w.v, true);
-    p.a_scale = a->scale; p.init = dstates; p.again = again;
-    p.others = 1; p.y = sp.dkh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
-    BISSD_DO(launch_walk(a->dtype, p, s));
-    p = walk_params(w, w.v, w.k, w.dout, false);
-    p.y_scale = a->scale; p.init = states; p.again = again;
-    p.fin = a->dg && a->dfinal_state ? sp.final_ : nullptr;
-    p.others = 1; p.y = sp.dqh; p.y_dtype = BISSD_F32; p.y_batch = (long long)a->seqlen * z.H * z.N;
-    BISSD_DO(launch_walk(a->dtype, p, s));
+    uni::WalkParams dv = walk_params(w, w.q, w.dout, w.k, true), dk = walk_params(w, w.dout, w.q, w.v, true), dq = walk_params(w, w.v, w.k, w.dout, false);
+    dv.a_scale = dk.a_scale = dq.y_scale = a->scale;
+    dv.init = dk.init = dstates;
+    dq.init = states;
+    dv.again = dk.again = dq.again = again;
+    dv.y = a->dv; dv.y_dtype = a->dtype; dv.y_batch = (long long)a->seqlen * z.H * z.P;
+    dk.y = sp.dkh; dq.y = sp.dqh;
+    dk.others = dq.others = 1;
+    dk.y_dtype = dq.y_dtype = BISSD_F32;
+    dk.y_batch = dq.y_batch = (long long)a->seqlen * z.H * z.N;
+    dv.fin = dinitial; dv.first_decay = dinitial != nullptr;
+    dq.fin = a->dg && a->dfinal_state ? sp.final_ : nullptr;
+    if (again) {
+        BISSD_DO(launch_walks_again(dv, &dk, &dq, s));
+    } else {
+        for (const uni::WalkParams *p : {&dv, &dk, &dq}) BISSD_DO(launch_walk(a->dtype, *p, s));
+    }
     uni::FinishParams f{};
     f.L = a->seqlen; f.H = z.H; f.hk = z.hk; f.N = z.N; f.P = z.P; f.tokens = z.tokens; f.scale = a->scale;
     f.q = w.q.v; f.k = w.k.v; f.v = w.v.v; f.dout = w.dout.v; f.bounds = bounds; f.nseq = a->nseq;
     f.dqh = sp.dqh; f.dkh = sp.dkh; f.dq = a->dq; f.dk = a->dk; f.again = again;
     if (a->dg) { f.into = sp.into; f.from = sp.from; }
-    const long long all = (z.tokens * (z.hk + (a->dg ? z.H : 0)) + 7) / 8, grid = again ? std::min(all, 8LL * kSms) : all;
+    const long long all = (z.tokens * (z.hk + (a->dg ? z.H : 0)) + 7) / 8, grid = again ? std::min<long long>(all, kSms) : all;
     if (grid > 0x7fffffffLL || (long long)w.plan.most * z.H > 0x7fffffffLL) return BISSD_ERR_SHAPE;
     BISSD_DO(by_dtype(a->dtype, [&](auto t) -> int {
         BISSD_LAUNCH("decay_finish", launch_pdl(uni::decay_finish<decltype(t)>, (int)grid, 256, 0, s, f));
@@ -533,7 +553,7 @@ int tc_forward(const bissd_decay_args *a, Bump &ws, cudaStream_t s) {
     f.init = a->initial_state; f.fin = a->final_state;
     f.y = a->o; f.y_dtype = a->dtype; f.y_scale = a->scale;
     f.y_batch = (long long)a->seqlen * w.z.H * w.z.P;
-    return launch_walk(a->dtype, f, s);
+    return launch_walks_again(f, nullptr, nullptr, s);
 }
 
 struct TcGradSpace {

@@ -11,8 +11,8 @@
 // costs no digits.
 // Products take operands of T: states, pairs and weighted rows are rounded to it.  In fp16 they may be out of its range where inputs and
 // outputs are not.  An operand that is no number leaves no number in every sum that it enters, so the kernels look at their fp32 sums alone,
-// and heads of sequences where one is none are done again by uni_walk.cuh's kernels, which leave at once where there are none (3.6 us a
-// launch: a forward pass has one, a backward pass five; 8 x 2048 tokens of 24 heads, both passes, 265 us before, 293 so).
+// and heads of sequences where one is none are done again by uni_walk.cuh's kernels, which leave at once where there are none
+// (one more launch forward, three backward; with the looking 265 -> 286 us for both passes of 8 x 2048 tokens of 24 heads).
 #pragma once
 #include "tc_tma.cuh"
 #include "uni_plan.cuh"

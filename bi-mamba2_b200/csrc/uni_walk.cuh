@@ -50,16 +50,13 @@ inline size_t walk_smem(int lanes, int ipt) {
 // Y: outputs are wanted (asked at run time, the question parted the loads of every four elements: 143 us for 114, 670 tokens of 24
 // heads, 112 x 128), with a token's own pair or without it.
 enum { kStates = 0, kOutputs = 1, kOthers = 2 };
-template <class T, int IPT, int Y> __global__ void __launch_bounds__(kWalkThreads, 4) decay_walk(WalkParams a) {
-    pdl_begin();
+template <class T, int IPT, int Y> __device__ __forceinline__ void walk(const WalkParams &a, int block) {
     extern __shared__ __align__(16) float dyn[];
-    if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
     const int LI = a.lanes, cols = kWalkThreads / LI, tile = walk_tile(LI), rowlen = LI * (IPT + 4);
     const int stage_len = tile * (2 * rowlen + cols + 2);
     float *ys = dyn + 2 * stage_len;
     const int jb = (a.J + cols - 1) / cols;
-    const int cb = blockIdx.x % jb, h = blockIdx.x / jb % a.H, si = blockIdx.x / (jb * a.H);
-    if (a.again && !a.again[0]) return;
+    const int cb = block % jb, h = block / jb % a.H, si = block / (jb * a.H);
     const Segment s = segment(a.plan, si);
     if (s.len == 0 || (a.again && !again(a.again, a.H, s.seq, h))) return;
     const int tid = threadIdx.x, li = tid % LI, jc = tid / LI, j = cb * cols + jc, hq = h * a.hk / a.H;
@@ -200,6 +197,28 @@ template <class T, int IPT, int Y> __global__ void __launch_bounds__(kWalkThread
         }
     }
     if (a.decay && cb == 0 && tid == 0) a.decay[si * (long long)a.H + h] = expf(total);
+}
+
+template <class T, int IPT, int Y> __global__ void __launch_bounds__(kWalkThreads, 4) decay_walk(WalkParams a) {
+    pdl_begin();
+    if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+    walk<T, IPT, Y>(a, blockIdx.x);
+}
+// What is done again: the walk of a forward pass, or the three of a backward pass at once.  Mostly there is nothing to do, and then a launch costs
+// its latency and the blocks it starts: no more than are resident, which take the walks' blocks in turn.  Eight rows a thread.
+constexpr int kAgainRows = 8;
+template <class T> __global__ void __launch_bounds__(kWalkThreads, 4)
+decay_walks_again(const __grid_constant__ WalkParams out, const __grid_constant__ WalkParams dk, const __grid_constant__ WalkParams dq, int out_blocks, int dk_blocks,
+                  int blocks) {
+    pdl_begin();
+    if (!out.again[0]) return;
+    for (int x = blockIdx.x; x < blocks; x += gridDim.x) {
+        const int block = x - out_blocks;
+        if (block < 0) walk<T, kAgainRows, kOutputs>(out, x);
+        else if (block < dk_blocks) walk<T, kAgainRows, kOthers>(dk, block);
+        else walk<T, kAgainRows, kOthers>(dq, block - dk_blocks);
+        __syncthreads();                                         // shared memory has been read
+    }
 }
 
 // The states that enter the segments, from each segment's own sum (in its place): forwards run = D run + own, written before it is
