@@ -490,7 +490,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 // column factor, both counted from the block's last column and at most 1; on the diagonal it is one 2^x an element.  A warp has
 // 32 rows and half of the columns up to the diagonal, in units of 16.
 // Two blocks an SM: one's loads and element-wise work run under the other's MMAs.  Bound by memory where rows are long: 512 chunks of
-// 32 heads, 128 x 64 states, 1.05 GB in 210 us (4.8 TB/s).  Stores from registers, without the way through shared memory, took 244
+// 32 heads, 128 x 64 states, 1.05 GB in 216 us (4.7 TB/s).  Stores from registers, without the way through shared memory, took 244
 // us, 512 threads a block 264.
 struct ChunksParams {
     Heads h;
@@ -751,7 +751,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
 // part of) the heads of v that share them, dq and dk adding up in tensor memory; v and do come a tile ahead, the states while the pairs
 // are weighted, and the products of d run under the next tile's first ones, when nobody waits for them.  Ten of the sixteen warps have weights to make, six lie above the
 // diagonal: one of these makes the next head's tables, one sums dg, one issues the products, and together they weight v.  A tile's
-// products (3300 cycles, most from shared memory) and its arithmetic (7000) take turns: 128 chunks of 24 heads, 128 x 64 states, 161 us on 128
+// products (3300 cycles, most from shared memory) and its arithmetic (7000) take turns: 128 chunks of 24 heads, 128 x 64 states, 164 us on 128
 // SMs.  The loops of products are not unrolled: a shorter body ran 180 -> 170 us.
 struct GradsParams {
     Heads h;
