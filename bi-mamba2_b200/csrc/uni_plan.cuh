@@ -55,8 +55,8 @@ __device__ __forceinline__ void do_again(const Again &a, int seq, int h, int R) 
     for (int r = 0; r < R; ++r) a.flags[1 + (long long)seq * a.H + h / R * R + r] = 1;
 }
 __device__ __forceinline__ void do_again_states(const Again &a, int R, int threads) {   // what decay_states found; all blocks of a launch
-    for (int i = blockIdx.x * threads + threadIdx.x; i < a.bads; i += gridDim.x * threads)
-        if (a.bad[i]) do_again(a, segment(a.seg, i / a.per_segment).seq, i % a.per_segment / (a.per_segment / a.H), R);
+    for (long long i = (long long)blockIdx.x * threads + threadIdx.x; i < a.bads; i += (long long)gridDim.x * threads)
+        if (a.bad[i]) do_again(a, segment(a.seg, (int)i / a.per_segment).seq, (int)i % a.per_segment / (a.per_segment / a.H), R);
 }
 
 struct PlanOut {                                                 // one table for each segment length
