@@ -41,10 +41,11 @@ def decay_attention(q, k, v, g, scale=None, initial_state=None, return_final_sta
     On the tensor cores (16-bit types, kdim up to 128, head sizes that are multiples of 8, scale > 0) the state that enters a chunk of 128
     tokens of a sequence, the products scale * q.k of its pairs, rows of v weighted by decays and their gradients' like are rounded to the tensors'
     type on the way.  In float16 a head of a sequence for which any of these, or an input, is out of range (65504) is computed again on the CUDA
-    cores, in float32 throughout and many times slower; gradients lose bits where the type has few (below 2^-14).  In bfloat16 a value of v, in the
-    backward pass also of q, k or a gradient, that is not finite reaches all 128 tokens of its chunk, also those before it; other sequences never.
-    The states handed in and out are float32 throughout.  How a call is split over the GPU follows its sizes: the last bits of a row may depend
-    on the number of rows.
+    cores, in float32 throughout and many times slower; those below 2^-14, where float16 has fewer bits, are off by up to 2^-25 each (small q and k
+    beside a large v, a small scale, small gradients: float32 tensors, of which nothing is rounded on the way, are the choice there).  In
+    bfloat16 a value of v, in the backward pass also of q, k or a gradient, that is not finite reaches all 128 tokens of its chunk, also those
+    before it; other sequences never.  The states handed in and out are float32 throughout.  How a call is split over the GPU follows its
+    sizes: the last bits of a row may depend on the number of rows.
 
     A call has at most 2^23 - 1 tokens.
 
