@@ -20,9 +20,7 @@ struct Segment {
 
 __device__ __forceinline__ Segment segment(const Plan &p, int i) {
     Segment s;
-    if (p.bounds) {
-        s.batch = s.idx = 0; s.t0 = p.bounds[i]; s.len = p.bounds[i + 1] - s.t0; s.seq = i; s.last = true;
-    } else if (p.packed) {
+    if (p.packed) {
         const int4 e = __ldg(p.table + i);
         s.batch = 0; s.t0 = e.x; s.len = e.y; s.seq = e.z; s.idx = e.w >> 1; s.last = e.w & 1;
     } else {
@@ -32,6 +30,13 @@ __device__ __forceinline__ Segment segment(const Plan &p, int i) {
         s.len = min(p.seg, p.L - s.t0);
         s.last = s.idx == p.per_seq - 1;
     }
+    return s;
+}
+// The same where a plan may have bounds.
+__device__ __forceinline__ Segment segment_or_sequence(const Plan &p, int i) {
+    if (!p.bounds) return segment(p, i);
+    Segment s;
+    s.batch = s.idx = 0; s.t0 = p.bounds[i]; s.len = p.bounds[i + 1] - s.t0; s.seq = i; s.last = true;
     return s;
 }
 // The segments of a sequence: first and how many.

@@ -7,8 +7,7 @@
 // Heads of v are taken 64 columns at a time: with the same weights, v's parts are heads of their own that share q, k and g.  Head sizes
 // that fill no tile are completed by the loads with zeros.  Log decays count in powers of two and no lower than 2^-200 a token, which
 // fp32 has no number for: -inf never meets +inf.  Factors that reach to a chunk's ends are 2 to the power of a sum that starts there, and
-// those between two tokens from sums that start at one of them, or in two parts (Decays), so that a strong decay elsewhere in the chunk
-// costs no digits.
+// and those between two tokens of sums over what lies between them, so that a strong decay elsewhere in the chunk costs no digits.
 // Products take operands of T: states, pairs and weighted rows are rounded to it.  In fp16 they may be out of its range where inputs and
 // outputs are not.  An operand that is no number leaves no number in every sum that it enters, so the kernels look at their fp32 sums alone,
 // and heads of sequences where one is none are done again by uni_walk.cuh's kernels, which leave at once where there are none
@@ -63,63 +62,38 @@ struct Decays {
             v[i] = x < -200.f ? -200.f : x;                      // what is no number stays none
         }
     }
-    // Sums up to and with each token.
-    __device__ __forceinline__ void prefix(float (&c)[4], int lane) const {
+    // Sums up to and with each token, from the first of its W lanes on.  What is needed between two tokens is made of sums over what lies
+    // between them, not of one such sum less another: where tokens empty the state one over a chunk comes to 25600, and a step of fp32 is 2^-9 there.
+    // (Sums of 32 tokens are subtracted where they are at most 64.)
+    template <int W = 32> __device__ __forceinline__ void prefix(float (&c)[4], int lane) const {
         c[0] = v[0];
 #pragma unroll
         for (int i = 1; i < 4; ++i) c[i] = c[i - 1] + v[i];
-        float mine = c[3], sum = mine;
+        float sum = c[3];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
+        for (int o = 1; o < W; o <<= 1) {
             const float u = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += u;
+            if ((lane & (W - 1)) >= o) sum += u;
         }
         const float before = __shfl_up_sync(0xffffffffu, sum, 1);
-        if (lane > 0) {
+        if (lane & (W - 1)) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[i] += before;
         }
     }
-    // The same for sums that are subtracted from one another: those of the whole numbers, which are exact, and of the rests, at most 64.  In one
-    // they come to 25600 where tokens empty the state, and a step of fp32 is 2^-9 there.
-    __device__ __forceinline__ void prefix(float (&c)[4], float (&rest)[4], int lane) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float w = rintf(v[i]);
-            c[i] = i ? c[i - 1] + w : w;
-            rest[i] = i ? rest[i - 1] + (v[i] - w) : v[i] - w;
-        }
-        float sum = c[3], sum_r = rest[3];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float u = __shfl_up_sync(0xffffffffu, sum, o), u_r = __shfl_up_sync(0xffffffffu, sum_r, o);
-            if (lane >= o) {
-                sum += u;
-                sum_r += u_r;
-            }
-        }
-        const float before = __shfl_up_sync(0xffffffffu, sum, 1), before_r = __shfl_up_sync(0xffffffffu, sum_r, 1);
-        if (lane > 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[i] += before;
-                rest[i] += before_r;
-            }
-        }
-    }
-    // Sums of the tokens behind each.
-    __device__ __forceinline__ void suffix(float (&c)[4], int lane) const {
+    // Sums of the tokens behind each, up to the last of its W lanes.
+    template <int W = 32> __device__ __forceinline__ void suffix(float (&c)[4], int lane) const {
         c[3] = 0.f;
 #pragma unroll
         for (int i = 2; i >= 0; --i) c[i] = c[i + 1] + v[i + 1];
         float sum = c[0] + v[0];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
+        for (int o = 1; o < W; o <<= 1) {
             const float u = __shfl_down_sync(0xffffffffu, sum, o);
-            if (lane + o < 32) sum += u;
+            if ((lane & (W - 1)) + o < W) sum += u;
         }
         const float behind = __shfl_down_sync(0xffffffffu, sum, 1);
-        if (lane < 31) {
+        if ((lane & (W - 1)) < W - 1) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[i] += behind;
         }
@@ -201,7 +175,8 @@ template <class T, int NT, bool EXACT> __global__ void __launch_bounds__(kStates
 decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmTiles) {
     pdl_begin();
     if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
-    if (a.again && blockIdx.x == 0 && threadIdx.x == 0) a.again[0] = 0;
+    constexpr bool kNarrow = std::is_same<T, __half>::value;     // what lies between inputs and outputs may be out of T's range
+    if (kNarrow && a.again && blockIdx.x == 0 && threadIdx.x == 0) a.again[0] = 0;
     constexpr int kSlabs = NT / 64;
     extern __shared__ __align__(1024) uint8_t dyn[];
     // two stages of k, two of weighted rows, S.  EXACT: one of k, v's rows, two parts, v's rows, S
@@ -210,9 +185,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pb = blockIdx.x % a.h.PB, h = blockIdx.x / a.h.PB % a.h.H, si = blockIdx.x / (a.h.PB * a.h.H), hq = h * a.h.hk / a.h.H;
     const Segment s = uni::segment(a.seg, si);
-    if (a.bad && tid == 0 && s.len == 0) a.bad[blockIdx.x] = 0;
+    if (kNarrow && a.bad && tid == 0 && s.len == 0) a.bad[blockIdx.x] = 0;
     if (s.len == 0) return;                                      // packed: fewer segments than there could be
-    if (a.again && tid == 0 && pb == 0 && s.idx == 0) a.again[1 + (long long)s.seq * a.h.H + h] = 0;
+    if (kNarrow && a.again && tid == 0 && pb == 0 && s.idx == 0) a.again[1 + (long long)s.seq * a.h.H + h] = 0;
     if (smem_u32(dyn) & 1023) {                                  // the swizzled tiles' alignment, which nothing else here sees to
         if (tid == 0) atomicExch(a.status, kErrDecay + 4);
         return;
@@ -460,7 +435,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 #pragma unroll
             for (int j = 0; j < 32; ++j)
                 if (col + j < a.h.P) a.fin[at + j] = S[j];
-            if (a.bad) {                                         // a row times a weight above 1, in a part of 16 bits
+            if (kNarrow && a.bad) {                              // a row times a weight above 1, in a part of 16 bits
                 float none = 0.f;
 #pragma unroll
                 for (int j = 0; j < 32; ++j) none = fmaf(S[j], 0.f, none);
@@ -479,7 +454,7 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
         }
         __syncthreads();
     }
-    if (a.bad && tid == 0) a.bad[blockIdx.x] = sh.bad;
+    if (kNarrow && a.bad && tid == 0) a.bad[blockIdx.x] = sh.bad;
     if (warp == 0) tmem_dealloc(tmem, EXACT ? 256 : 64);
 }
 
@@ -487,7 +462,9 @@ decay_states(StatesParams a, const __grid_constant__ CUtensorMap tmK, const __gr
 // A block has one chunk of one head of q and k, and walks `vpc` of the tiles of v that share them: Q, K and their product stay, in
 // shared and tensor memory, and per tile come v's rows and the state.  The product, weighted by the decays and rounded to T (it
 // meets v's T), takes K's place in shared memory.  Where a block of 32 x 32 lies below the diagonal, the weight is a row factor times a
-// column factor, both counted from the block's last column and at most 1; on the diagonal it is one 2^x an element.  A warp has
+// column factor, both counted from the block's last column and at most 1; on the diagonal it is one 2^x an element, of the difference of two
+// sums over 32 tokens at most, or where these are above 64 of a sum that starts at the row's token and takes in a token a column (a chain:
+// 234 us for 211 if always so).  A warp has
 // 32 rows and half of the columns up to the diagonal, in units of 16.
 // Two blocks an SM: one's loads and element-wise work run under the other's MMAs.  Bound by memory where rows are long: 512 chunks of
 // 32 heads, 128 x 64 states, 1.05 GB in 216 us (4.7 TB/s).  Stores from registers, without the way through shared memory, took 244
@@ -512,7 +489,8 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     extern __shared__ __align__(1024) uint8_t dyn[];
     __shared__ uint64_t bar_qk, bar_v, bar_s, done, done_s, unused;
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float cs[kTables][kQ], cl[kTables][kQ], below[kTables][kQ];   // c_t and its rest; 2^(c at the end of s' 32 - c_s)
+    __shared__ __align__(16) float gs[kTables][kQ], upto[kTables][kQ], below[kTables][kQ];   // log2 decays; their sums in t's 32 up to t; 2^(sum in s' 32 behind s)
+    __shared__ float between[kTables][4][4];                     // [1 + b][q]: sums of the 32s behind the b-th and before the q-th
     uint8_t *smQ = smem_align1024(dyn), *smK = smQ + kSlabs * kSlab, *smV = smK + 2 * kSlab, *smS = smV + kSlab;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int part = blockIdx.x % a.parts, m = blockIdx.x / a.parts % a.h.hk, ci = blockIdx.x / (a.parts * a.h.hk);
@@ -535,14 +513,20 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
     };
     auto table = [&](int k) {
         if (k >= heads) return;
-        float c[4], l[4];
+        float c[4], w[4];
         next.log2(a.h);
-        next.prefix(c, l, lane);
-        const float end = __shfl_sync(0xffffffffu, c[3], lane | 7), end_l = __shfl_sync(0xffffffffu, l[3], lane | 7);
-        *reinterpret_cast<float4 *>(&cs[warp][lane * 4]) = make_float4(c[0], c[1], c[2], c[3]);
-        *reinterpret_cast<float4 *>(&cl[warp][lane * 4]) = make_float4(l[0], l[1], l[2], l[3]);
-        auto w = [&](int k) { return exp2f((end - c[k]) + (end_l - l[k])); };
-        *reinterpret_cast<float4 *>(&below[warp][lane * 4]) = make_float4(w(0), w(1), w(2), w(3));
+        next.prefix<8>(c, lane);
+        next.suffix<8>(w, lane);
+        float sum = 0.f;
+#pragma unroll
+        for (int b = 0; b < 3; ++b) {
+            const float of = __shfl_sync(0xffffffffu, c[3], 8 * b + 7);
+            sum += b >= lane >> 2 && b < (lane & 3) ? of : 0.f;
+        }
+        if (lane < 16) between[warp][lane >> 2][lane & 3] = sum;
+        *reinterpret_cast<float4 *>(&gs[warp][lane * 4]) = make_float4(next.v[0], next.v[1], next.v[2], next.v[3]);
+        *reinterpret_cast<float4 *>(&upto[warp][lane * 4]) = make_float4(c[0], c[1], c[2], c[3]);
+        *reinterpret_cast<float4 *>(&below[warp][lane * 4]) = make_float4(exp2f(w[0]), exp2f(w[1]), exp2f(w[2]), exp2f(w[3]));
     };
     ask(warp);
     if (warp == 0) tmem_alloc(&tmem_slot, 256);
@@ -612,8 +596,9 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                 umma_commit(&done_s);
             }
         }
-        const float *c = cs[k % kTables], *l = cl[k % kTables];
-        const float ct = c[t], lt = l[t] + a.h.log_scale;
+        const float *g = gs[k % kTables], *c = upto[k % kTables];
+        const float ct = c[t] + a.h.log_scale;
+        const bool strong = fabsf(c[r32 * 32 + 31]) > 64.f;      // differences of sums lack digits
         {
             uint32_t raw[16];
             tmem_ld16_nowait(tl + u0 * 16, raw);
@@ -625,7 +610,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                 if (u + 1 < u1) tmem_ld16_nowait(tl + (u + 1) * 16, raw);
                 const int cb = u >> 1;
                 if (cb < r32) {
-                    const float rt = exp2f((ct - c[cb * 32 + 31]) + (lt - l[cb * 32 + 31]));
+                    const float rt = exp2f(ct + between[k % kTables][1 + cb][r32]);
                     const vec::f2 rt2 = vec::pack(rt, rt);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -635,14 +620,32 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
                     }
                 } else {
                     const int td = t - u * 16;                   // columns up to it; what is behind it may be no number
+                    if (!strong) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 f = *reinterpret_cast<const float2 *>(c + u * 16 + j * 2), fl = *reinterpret_cast<const float2 *>(l + u * 16 + j * 2);
-                        float lo, hi;
-                        vec::unpack(x[j], lo, hi);
-                        lo *= ex2_approx((ct - f.x) + (lt - fl.x));
-                        hi *= ex2_approx((ct - f.y) + (lt - fl.y));
-                        x[j] = vec::pack(2 * j <= td ? lo : 0.f, 2 * j + 1 <= td ? hi : 0.f);
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 f = *reinterpret_cast<const float2 *>(c + u * 16 + j * 2);
+                            float lo, hi;
+                            vec::unpack(x[j], lo, hi);
+                            lo *= ex2_approx(ct - f.x);
+                            hi *= ex2_approx(ct - f.y);
+                            x[j] = vec::pack(2 * j <= td ? lo : 0.f, 2 * j + 1 <= td ? hi : 0.f);
+                        }
+                    } else {
+                        float e = td > 15 ? a.h.log_scale : -INFINITY;   // from the unit's end
+                        for (int x = u * 16 + 16; x <= t; ++x) e += g[x];
+#pragma unroll
+                        for (int j = 7; j >= 0; --j) {
+                            const float2 f = *reinterpret_cast<const float2 *>(g + u * 16 + j * 2);
+                            float lo, hi;
+                            vec::unpack(x[j], lo, hi);
+                            if (2 * j + 1 == td) e = a.h.log_scale;
+                            hi *= ex2_approx(e);
+                            e += f.y;
+                            if (2 * j == td) e = a.h.log_scale;
+                            lo *= ex2_approx(e);
+                            e += f.x;
+                            x[j] = vec::pack(2 * j <= td ? lo : 0.f, 2 * j + 1 <= td ? hi : 0.f);
+                        }
                     }
                 }
 #pragma unroll
@@ -689,7 +692,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
         tc_fence_after();
         // o = inside + scale e^{c_t} from the state; whole rows leave through the first slab of the weighted pairs
         if (ok) {
-            const float f = exp2f(ct + lt);
+            const float f = exp2f(ct + between[k % kTables][0][r32]);
             float x[32], y[32], none = 0.f;
             tmem_ld32(tl + 128 + half * 32, x);
             tmem_ld32(tl + 192 + half * 32, y);
@@ -751,7 +754,7 @@ decay_chunks(ChunksParams a, const __grid_constant__ CUtensorMap tmQ, const __gr
 // part of) the heads of v that share them, dq and dk adding up in tensor memory; v and do come a tile ahead, the states while the pairs
 // are weighted, and the products of d run under the next tile's first ones, when nobody waits for them.  Ten of the sixteen warps have weights to make, six lie above the
 // diagonal: one of these makes the next head's tables, one sums dg, one issues the products, and together they weight v.  A tile's
-// products (3300 cycles, most from shared memory) and its arithmetic (7000) take turns: 128 chunks of 24 heads, 128 x 64 states, 164 us on 128
+// products (3300 cycles, most from shared memory) and its arithmetic (7000) take turns: 128 chunks of 24 heads, 128 x 64 states, 162 us on 128
 // SMs.  The loops of products are not unrolled: a shorter body ran 180 -> 170 us.
 struct GradsParams {
     Heads h;
@@ -827,28 +830,32 @@ decay_grads(GradsParams a, const __grid_constant__ CUtensorMap tmQ, const __grid
         tma_load2(smG, &tmG, 0, row, &bar_s);
     };
     auto table = [&](Table &to, Decays &next) {                  // one warp
-        float c[4], l[4], q[4];
+        float c[4], q[4];
         next.log2(a.h);
-        next.prefix(c, l, lane);
-        const float all = __shfl_sync(0xffffffffu, c[3], 31), all_l = __shfl_sync(0xffffffffu, l[3], 31);
+        next.prefix<8>(c, lane);
+        next.suffix<8>(q, lane);
+        const int own = lane >> 3;                               // 32 tokens of four
+        float sums[4];                                           // theirs
+#pragma unroll
+        for (int b = 0; b < 4; ++b) sums[b] = __shfl_sync(0xffffffffu, c[3], 8 * b + 7);
         auto four = [&](float *o, auto f) { *reinterpret_cast<float4 *>(o + lane * 4) = make_float4(f(0), f(1), f(2), f(3)); };
         four(to.g, [&](int k) { return next.v[k]; });
-        const float end = __shfl_sync(0xffffffffu, c[3], lane | 7), end_l = __shfl_sync(0xffffffffu, l[3], lane | 7);
-        four(to.above, [&](int k) { return ex2_approx((end - c[k]) + (end_l - l[k])); });
+        four(to.above, [&](int k) { return ex2_approx(q[k]); });
+        float rest = 0.f, head = a.h.log_scale;                  // behind the lane's 32 tokens, and before them
 #pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = ex2_approx((all - c[k]) + (all_l - l[k]));
+        for (int b = 1; b < 4; ++b) rest += b > own ? sums[b] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = ex2_approx(q[k] + rest);
         four(to.ws, [&](int k) { return q[k]; });
         *reinterpret_cast<uint4 *>(to.wv + lane * 4) = make_uint4(halves<T>(q[0]), halves<T>(q[1]), halves<T>(q[2]), halves<T>(q[3]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) l[k] += a.h.log_scale;
-        auto wd = [&](int k) { return halves<T>(ex2_approx(c[k] + l[k])); };
-        *reinterpret_cast<uint4 *>(to.wd + lane * 4) = make_uint4(wd(0), wd(1), wd(2), wd(3));
-#pragma unroll
-        for (int b = 0; b < 3; ++b) {                            // of use in the blocks behind the b-th
-            const float from = __shfl_sync(0xffffffffu, end, 8 * b + 7), from_l = __shfl_sync(0xffffffffu, end_l, 8 * b + 7);
-            four(to.beside[b], [&](int k) { return ex2_approx((c[k] - from) + (l[k] - from_l)); });
+        for (int b = 2; b >= 0; --b) {                           // of use in the blocks behind the b-th
+            four(to.beside[b], [&](int k) { return ex2_approx(c[k] + head); });
+            head += b < own ? sums[b] : 0.f;
         }
-        if (lane == 0) to.whole[0] = all + all_l;
+        auto wd = [&](int k) { return halves<T>(ex2_approx(c[k] + head)); };
+        *reinterpret_cast<uint4 *>(to.wd + lane * 4) = make_uint4(wd(0), wd(1), wd(2), wd(3));
+        if (lane == 0) to.whole[0] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     };
     if (warp == 0) tmem_alloc(&tmem_slot, 512);
     if (tid == 32) {

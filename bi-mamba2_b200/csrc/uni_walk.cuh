@@ -57,7 +57,7 @@ template <class T, int IPT, int Y> __device__ __forceinline__ void walk(const Wa
     float *ys = dyn + 2 * stage_len;
     const int jb = (a.J + cols - 1) / cols;
     const int cb = block % jb, h = block / jb % a.H, si = block / (jb * a.H);
-    const Segment s = segment(a.plan, si);
+    const Segment s = segment_or_sequence(a.plan, si);
     if (s.len == 0 || (a.again && !again(a.again, a.H, s.seq, h))) return;
     const int tid = threadIdx.x, li = tid % LI, jc = tid / LI, j = cb * cols + jc, hq = h * a.hk / a.H;
     const long long S = (long long)a.I * a.J;
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(256) decay_dg(DecayGradParams a) {
     __shared__ double part[8], carry;
     const int h = blockIdx.x % a.H, si = blockIdx.x / a.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (a.again && !a.again[0]) return;
-    const Segment s = segment(a.plan, si);
+    const Segment s = segment_or_sequence(a.plan, si);
     if (s.len == 0 || (a.again && !again(a.again, a.H, s.seq, h))) return;
     const int end = s.t0 + s.len;
     double cross = 0.0;
